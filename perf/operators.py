@@ -160,7 +160,7 @@ def _plain(state):
     w, scale = state["head"][0].float(), state["head"][1]
     x = state["x"].float()
     largest = x.abs().amax(1, keepdim=True)
-    s = torch.where(largest > 0, largest / 127, 1.0)
+    s = (largest / torch.full_like(largest, 127)).clamp_min(2.0 ** -126)       # (by a number torch multiplies with its rounded inverse)
     q = (x * (1 / s)).round()
     return _pieces(case["m"], 2048, lambda i, j: _of_logits(((q[i:j] @ w.T) * s[i:j]) * scale, tokens[i:j], top))
 
@@ -199,7 +199,7 @@ def exact(case, seed):
         else:
             # the row's scale is a 32-bit number, and so is the inverse that its values are multiplied by before they are rounded
             x = state["x"][i: i + 512].float()
-            s = x.abs().max(dim=1, keepdim=True).values / 127
+            s = (x.abs().max(dim=1, keepdim=True).values.double() / 127).float()
             s[s == 0] = 1
             z = (torch.round(x * torch.reciprocal(s)).double() @ head.T) * s.double() * state["head"][1].double()
         lp = torch.log_softmax(z, dim=1)
