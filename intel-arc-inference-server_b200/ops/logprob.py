@@ -1,0 +1,154 @@
+"""Log probabilities of given tokens, with each row's entropy and top alternatives (``csrc/logprob.cu``, ``csrc/score_head.cu``).
+
+A row's logits z, its token t, S = sum exp(z - max z):
+
+    log p(t) = z_t - max z - ln S        H = - sum p ln p        the ``top`` largest z, of equal ones the lower id first
+
+``token_logprobs`` takes logits that are there (a decode or verify step's, ``Engine.logits``); ``score`` and ``score_i8`` take rows
+behind the final norm and the lm_head, and keep no logits.  All sums are fp32.
+
+A token outside the vocabulary (-1: no token) has log probability NaN; its row's other results are as ever.  A row without a finite
+logit (every id banned) has log probabilities of -inf and entropy 0.  A NaN or +inf among a row's logits makes its numbers NaN.
+Alternatives beyond the vocabulary have id -1 and log probability -inf.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import lib as K
+
+MAX_TOP = 32           # alternatives a row can have
+SLAB_ELEMS = 80 << 20  # logits that ``score`` with alternatives keeps at a time
+
+
+@dataclass
+class Logprobs:
+    """Results of ``m`` rows: ``logprob``, ``entropy`` fp32 ``[m]``; ``top_ids`` int32 and ``top_logprobs`` fp32 ``[m][top]``."""
+    logprob: torch.Tensor
+    entropy: torch.Tensor
+    top_ids: torch.Tensor
+    top_logprobs: torch.Tensor
+
+    @staticmethod
+    def empty(m: int, top: int, device) -> "Logprobs":
+        f = lambda *s: torch.empty(s, dtype=torch.float32, device=device)           # noqa: E731
+        return Logprobs(f(m), f(m), torch.empty(m, top, dtype=torch.int32, device=device), f(m, top))
+
+    def rows(self, begin: int, end: int) -> "Logprobs":
+        return Logprobs(self.logprob[begin:end], self.entropy[begin:end], self.top_ids[begin:end], self.top_logprobs[begin:end])
+
+
+def _results(m: int, top: Optional[int], out: Optional[Logprobs], device) -> Logprobs:
+    if out is None:
+        top = top or 0
+        if not 0 <= top <= MAX_TOP:
+            raise ValueError(f"log probabilities of at most {MAX_TOP} alternatives, not {top}")
+        return Logprobs.empty(m, top, device)
+    n = out.top_ids.shape[-1]
+    if top is not None and top != n or not 0 <= n <= MAX_TOP:
+        raise ValueError(f"results for {n} alternatives, {top} asked (at most {MAX_TOP})")
+    for t, shape, dtype in ((out.logprob, (m,), torch.float32), (out.entropy, (m,), torch.float32), (out.top_ids, (m, n), torch.int32),
+                            (out.top_logprobs, (m, n), torch.float32)):
+        if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+            raise ValueError(f"results of {m} rows and {n} alternatives are contiguous fp32 / int32 tensors of {device}")
+    return out
+
+
+def _check_tokens(tokens: torch.Tensor, m: int, device):
+    if tokens.dtype != torch.int32 or tokens.shape != (m,) or tokens.device != device or not tokens.is_contiguous():
+        raise ValueError(f"tokens: {m} contiguous int32 ids on {device}")
+
+
+def _rows_of(t: torch.Tensor, dtype, what: str, align: int = 1):
+    if t.dim() != 2 or t.dtype != dtype or t.device.type != "cuda" or t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"{what}: rows of {dtype} on a CUDA device, one element after another")
+    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        raise ValueError(f"{what}: rows that do not overlap")
+    if align > 1 and (t.data_ptr() % align or t.shape[0] > 1 and t.stride(0) * t.element_size() % align):
+        raise ValueError(f"{what}: rows begin at multiples of {align} bytes")
+
+
+def _ld(t: torch.Tensor, align: int = 1) -> int:
+    """Elements from row to row; a lone row's stride says nothing."""
+    if t.shape[0] > 1:
+        return t.stride(0)
+    step = max(1, align // t.element_size())
+    return (t.shape[1] + step - 1) // step * step
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
+    """Rows of fp32 ``logits`` ``[m][vocabulary]`` (any row stride), one int32 token each.  ``out``: results to write, whose width is
+    then ``top``."""
+    _rows_of(logits, torch.float32, "logits")
+    m, n = logits.shape
+    dev = logits.device
+    if n < 1:
+        raise ValueError("logits of an empty vocabulary")
+    _check_tokens(tokens, m, dev)
+    out = _results(m, top, out, dev)
+    if m:
+        with torch.cuda.device(dev):
+            K._check(K.lib().b2_logprob_rows(K._p(logits), ctypes.c_longlong(_ld(logits)), m, n, K._p(tokens), out.top_ids.shape[1], K._p(out.logprob),
+                                             K._p(out.entropy), K._p(out.top_ids), K._p(out.top_logprobs), K._stream()), "logprob_rows")
+    return out
+
+
+def _score(x, w, i8: bool, x_scale, w_scale, tokens, out: Logprobs):
+    m, k = x.shape
+    n = w.shape[0]
+    ldz = (n + 3) // 4 * 4
+    step = max(1, min(m, max(256, SLAB_ELEMS // ldz // 256 * 256)))
+    z = torch.empty(step, ldz, dtype=torch.float32, device=x.device)
+    for i in range(0, m, step):
+        c = min(step, m - i)
+        xs = None if x_scale is None else x_scale[i:]
+        K._check(K.lib().b2_score_logits(K._p(x[i:]), ctypes.c_longlong(_ld(x, 16)), K._p(w), ctypes.c_longlong(_ld(w, 16)), int(i8), K._p(xs), K._p(w_scale),
+                                         c, n, k, K._p(z), ctypes.c_longlong(ldz), K._stream()), "score_logits")
+        token_logprobs(z[:c, :n], tokens[i: i + c], out=out.rows(i, i + c))
+    return out
+
+
+def _check_head(x, w, dtype):
+    _rows_of(w, dtype, "head", 16)
+    if w.device != x.device or w.shape[1] != x.shape[1] or w.shape[0] < 1:
+        raise ValueError(f"head {tuple(w.shape)} on {w.device} against rows {tuple(x.shape)} on {x.device}")
+    if x.shape[1] * w.element_size() < 128:
+        raise ValueError(f"rows of {x.shape[1]} columns: 128 bytes of the head's type at least")
+
+
+def score(x: torch.Tensor, head: torch.Tensor, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
+    """Rows ``x`` ``[m][k]`` against the lm_head ``[vocabulary][k]``, both bf16 with rows at multiples of 16 bytes: ``token_logprobs`` of
+    ``x @ head.T`` in fp32."""
+    _rows_of(x, torch.bfloat16, "rows", 16)
+    _check_head(x, head, torch.bfloat16)
+    _check_tokens(tokens, x.shape[0], x.device)
+    out = _results(x.shape[0], top, out, x.device)
+    if x.shape[0]:
+        with torch.cuda.device(x.device):
+            _score(x, head, False, None, None, tokens, out)
+    return out
+
+
+def score_i8(x: torch.Tensor, head: tuple, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
+    """Rows ``x`` ``[m][k]`` bf16 against an int8 lm_head (``[vocabulary][k]``, fp32 scale per row), rows of both at multiples of 16
+    bytes: rows are quantised per token (s = max|x| / 127, q = rint(x / s), as the int8 prompt pass does) and logits are (q . w) s s_w."""
+    w8, scale = head
+    _rows_of(x, torch.bfloat16, "rows", 16)
+    _check_head(x, w8, torch.int8)
+    m, k = x.shape
+    if scale.dtype != torch.float32 or scale.shape != (w8.shape[0],) or scale.device != x.device or not scale.is_contiguous():
+        raise ValueError(f"scales of the head: {w8.shape[0]} contiguous fp32 numbers on {x.device}")
+    _check_tokens(tokens, m, x.device)
+    out = _results(m, top, out, x.device)
+    if m:
+        with torch.cuda.device(x.device):
+            q = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
+            s = torch.empty(m, dtype=torch.float32, device=x.device)
+            K._check(K.lib().b2_score_quant(K._p(x), ctypes.c_longlong(_ld(x, 16)), m, k, K._p(q), ctypes.c_longlong(q.shape[1]), K._p(s), K._stream()),
+                     "score_quant")
+            _score(q[:, :k], w8, True, s, scale, tokens, out)
+    return out
