@@ -13,7 +13,9 @@ Alternatives beyond the vocabulary have id -1 and log probability -inf.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 from dataclasses import dataclass
 from typing import Optional
 
@@ -25,16 +27,28 @@ MAX_TOP = 32           # alternatives a row can have
 SLAB_ELEMS = 80 << 20  # logits that ``score`` with alternatives keeps at a time
 
 
-@dataclass
+@dataclass(frozen=True)
 class Logprobs:
-    """Results of ``m`` rows: ``logprob``, ``entropy`` fp32 ``[m]``; ``top_ids`` int32 and ``top_logprobs`` fp32 ``[m][top]``."""
+    """Results of ``m`` rows: ``logprob``, ``entropy`` fp32 ``[m]``; ``top_ids`` int32 and ``top_logprobs`` fp32 ``[m][top]``, contiguous, on
+    one device."""
     logprob: torch.Tensor
     entropy: torch.Tensor
     top_ids: torch.Tensor
     top_logprobs: torch.Tensor
 
+    def __post_init__(self):
+        m, n, dev = self.logprob.shape[0], self.top_ids.shape[-1], self.logprob.device
+        if n > MAX_TOP:
+            raise ValueError(f"log probabilities of at most {MAX_TOP} alternatives, not {n}")
+        for t, shape, dtype in ((self.logprob, (m,), torch.float32), (self.entropy, (m,), torch.float32), (self.top_ids, (m, n), torch.int32),
+                                (self.top_logprobs, (m, n), torch.float32)):
+            if t.shape != shape or t.dtype != dtype or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"results of {m} rows and {n} alternatives are contiguous fp32 / int32 tensors of {dev}")
+
     @staticmethod
     def empty(m: int, top: int, device) -> "Logprobs":
+        if not 0 <= top <= MAX_TOP:
+            raise ValueError(f"log probabilities of at most {MAX_TOP} alternatives, not {top}")
         f = lambda *s: torch.empty(s, dtype=torch.float32, device=device)           # noqa: E731
         return Logprobs(f(m), f(m), torch.empty(m, top, dtype=torch.int32, device=device), f(m, top))
 
@@ -44,17 +58,10 @@ class Logprobs:
 
 def _results(m: int, top: Optional[int], out: Optional[Logprobs], device) -> Logprobs:
     if out is None:
-        top = top or 0
-        if not 0 <= top <= MAX_TOP:
-            raise ValueError(f"log probabilities of at most {MAX_TOP} alternatives, not {top}")
-        return Logprobs.empty(m, top, device)
-    n = out.top_ids.shape[-1]
-    if top is not None and top != n or not 0 <= n <= MAX_TOP:
-        raise ValueError(f"results for {n} alternatives, {top} asked (at most {MAX_TOP})")
-    for t, shape, dtype in ((out.logprob, (m,), torch.float32), (out.entropy, (m,), torch.float32), (out.top_ids, (m, n), torch.int32),
-                            (out.top_logprobs, (m, n), torch.float32)):
-        if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
-            raise ValueError(f"results of {m} rows and {n} alternatives are contiguous fp32 / int32 tensors of {device}")
+        return Logprobs.empty(m, top or 0, device)
+    got = out.top_ids.shape
+    if got[0] != m or top is not None and top != got[1] or out.logprob.device != device:
+        raise ValueError(f"results of {got[0]} rows and {got[1]} alternatives on {out.logprob.device}: {m} and {top} asked on {device}")
     return out
 
 
@@ -80,6 +87,25 @@ def _ld(t: torch.Tensor, align: int = 1) -> int:
     return (t.shape[1] + step - 1) // step * step
 
 
+@functools.lru_cache(maxsize=None)
+def _entry(name: str, kinds: str):
+    """An entry point of the library with its argument types (p: pointer, l: 64 bits, i: 32 bits), so that a call of a few microseconds
+    wraps no numbers one by one."""
+    fn = getattr(K.lib(), name)
+    fn.argtypes = [{"p": ctypes.c_void_p, "l": ctypes.c_longlong, "i": ctypes.c_int}[c] for c in kinds]
+    return fn
+
+
+def _on(device):
+    """The device made the current one where it is not."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device) -> int:
+    """The device's current stream, without the object around it (2.3 us of a call of 10)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
     """Rows of fp32 ``logits`` ``[m][vocabulary]`` (any row stride), one int32 token each.  ``out``: results to write, whose width is
     then ``top``."""
@@ -91,9 +117,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int
     _check_tokens(tokens, m, dev)
     out = _results(m, top, out, dev)
     if m:
-        with torch.cuda.device(dev):
-            K._check(K.lib().b2_logprob_rows(K._p(logits), ctypes.c_longlong(_ld(logits)), m, n, K._p(tokens), out.top_ids.shape[1], K._p(out.logprob),
-                                             K._p(out.entropy), K._p(out.top_ids), K._p(out.top_logprobs), K._stream()), "logprob_rows")
+        with _on(dev):
+            K._check(_entry("b2_logprob_rows", "pliipippppp")(
+                logits.data_ptr(), _ld(logits), m, n, tokens.data_ptr(), out.top_ids.shape[1], out.logprob.data_ptr(), out.entropy.data_ptr(),
+                out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), _stream(dev)), "logprob_rows")
     return out
 
 
@@ -105,9 +132,9 @@ def _score(x, w, i8: bool, x_scale, w_scale, tokens, out: Logprobs):
     z = torch.empty(step, ldz, dtype=torch.float32, device=x.device)
     for i in range(0, m, step):
         c = min(step, m - i)
-        xs = None if x_scale is None else x_scale[i:]
-        K._check(K.lib().b2_score_logits(K._p(x[i:]), ctypes.c_longlong(_ld(x, 16)), K._p(w), ctypes.c_longlong(_ld(w, 16)), int(i8), K._p(xs), K._p(w_scale),
-                                         c, n, k, K._p(z), ctypes.c_longlong(ldz), K._stream()), "score_logits")
+        K._check(_entry("b2_score_logits", "plplippiiiplp")(
+            x[i:].data_ptr(), _ld(x, 16), w.data_ptr(), _ld(w, 16), int(i8), None if x_scale is None else x_scale[i:].data_ptr(),
+            None if w_scale is None else w_scale.data_ptr(), c, n, k, z.data_ptr(), ldz, _stream(x.device)), "score_logits")
         token_logprobs(z[:c, :n], tokens[i: i + c], out=out.rows(i, i + c))
     return out
 
@@ -128,7 +155,7 @@ def score(x: torch.Tensor, head: torch.Tensor, tokens: torch.Tensor, top: Option
     _check_tokens(tokens, x.shape[0], x.device)
     out = _results(x.shape[0], top, out, x.device)
     if x.shape[0]:
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             _score(x, head, False, None, None, tokens, out)
     return out
 
@@ -145,10 +172,10 @@ def score_i8(x: torch.Tensor, head: tuple, tokens: torch.Tensor, top: Optional[i
     _check_tokens(tokens, m, x.device)
     out = _results(m, top, out, x.device)
     if m:
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             q = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
             s = torch.empty(m, dtype=torch.float32, device=x.device)
-            K._check(K.lib().b2_score_quant(K._p(x), ctypes.c_longlong(_ld(x, 16)), m, k, K._p(q), ctypes.c_longlong(q.shape[1]), K._p(s), K._stream()),
+            K._check(_entry("b2_score_quant", "pliiplpp")(x.data_ptr(), _ld(x, 16), m, k, q.data_ptr(), q.shape[1], s.data_ptr(), _stream(x.device)),
                      "score_quant")
             _score(q[:, :k], w8, True, s, scale, tokens, out)
     return out

@@ -95,14 +95,19 @@ def test_refusals():
         LP.score(torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(8, 64, dtype=torch.bfloat16), t)
     with pytest.raises(ValueError, match="CUDA"):
         LP.score_i8(torch.zeros(2, 64, dtype=torch.bfloat16), (torch.zeros(8, 64, dtype=torch.int8), torch.ones(8)), t)
-    with pytest.raises(ValueError, match="at most"):
-        LP._results(2, LP.MAX_TOP + 1, None, z.device)
-    with pytest.raises(ValueError, match="at most"):
-        LP._results(2, -1, None, z.device)
-    with pytest.raises(ValueError, match="asked"):
-        LP._results(2, 3, LP.Logprobs.empty(2, 4, "cpu"), z.device)
-    with pytest.raises(ValueError, match="contiguous"):
-        LP._results(3, None, LP.Logprobs.empty(2, 4, "cpu"), z.device)
+    for top in (LP.MAX_TOP + 1, -1):
+        with pytest.raises(ValueError, match="at most"):
+            LP.Logprobs.empty(2, top, "cpu")
+    out = LP.Logprobs.empty(2, 4, "cpu")
+    for m, top in ((2, 3), (3, 4), (3, None)):
+        with pytest.raises(ValueError, match="asked"):
+            LP._results(m, top, out, z.device)
+    f = torch.zeros(2, 4)
+    for wrong in ((out.logprob[:1], out.entropy, out.top_ids, f), (out.logprob, out.entropy.double(), out.top_ids, f), (out.logprob, out.entropy, out.top_ids.long(), f),
+                  (out.logprob, out.entropy, out.top_ids, f[:, :3]), (out.logprob, out.entropy, out.top_ids, torch.zeros(4, 2).T),
+                  (out.logprob, out.entropy, torch.zeros(2, 33, dtype=torch.int32), torch.zeros(2, 33))):
+        with pytest.raises(ValueError, match="contiguous|at most"):
+            LP.Logprobs(*wrong)
     for bad in (t.long(), t[:1], torch.zeros(4, dtype=torch.int32)[::2], torch.zeros(2)):
         with pytest.raises(ValueError, match="int32"):
             LP._check_tokens(bad, 2, z.device)
