@@ -56,29 +56,6 @@ __device__ __forceinline__ LogStat join_lanes(const LogStat& a) {
   return r;
 }
 
-// Sixteen more logits of a thread, whose largest is `largest`.
-__device__ __forceinline__ void add_terms(LogStat& s, const float (&v)[4 * kVecs], float largest) {
-  const bool record = largest > s.m;
-  if (record) {      // the old maximum becomes a term like others
-    if (s.m > -INFINITY) {
-      const float d = below(s.m, largest), f = ex2(d * kLog2e), n = 1.f + s.s;
-      s.t = f * fmaf(d, n, s.t);
-      s.s = n * f;
-    }
-    s.m = largest;
-  }
-  const float m = fmaxf(s.m, -3.402823466e38f);
-  float less = 0.f, equal = record ? -1.f : 0.f;      // of the maximum's own terms one is not counted
-#pragma unroll
-  for (int i = 0; i < 4 * kVecs; ++i) {
-    const float d = max_nan(v[i] - m, -200.f), e = ex2(d * kLog2e), one = d == 0.f ? 1.f : 0.f;
-    less += e - one;
-    equal += one;
-    s.t = fmaf(d, e, s.t);
-  }
-  s.s += less + equal;
-}
-
 // The largest 32 keys of two lists, each sorted across the lanes, the largest first; so is the result.
 __device__ __forceinline__ unsigned long long merge_lists(unsigned long long a, unsigned long long b, int lane) {
   unsigned long long k = max(a, __shfl_xor_sync(0xffffffffu, b, 31));

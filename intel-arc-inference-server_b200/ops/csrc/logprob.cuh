@@ -29,11 +29,28 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // a finite number counts as the lowest one, so that -inf minus it is -inf.
 __device__ __forceinline__ float below(float z, float m) { return max_nan(z - fmaxf(m, -3.402823466e38f), -200.f); }
 
-// The term of z, which is not the maximum s.m itself.
-__device__ __forceinline__ void add_term(LogStat& s, float z) {
-  const float d = below(z, s.m), e = ex2(d * kLog2e);
-  s.s += e;
-  s.t = fmaf(d, e, s.t);
+// N more logits, the largest of them `largest`.
+template <int N>
+__device__ __forceinline__ void add_terms(LogStat& s, const float (&v)[N], float largest) {
+  const bool record = largest > s.m;
+  if (record) {      // the old maximum becomes a term like others
+    if (s.m > -INFINITY) {
+      const float d = below(s.m, largest), f = ex2(d * kLog2e), n = 1.f + s.s;
+      s.t = f * fmaf(d, n, s.t);
+      s.s = n * f;
+    }
+    s.m = largest;
+  }
+  const float m = fmaxf(s.m, -3.402823466e38f);
+  float less = 0.f, equal = record ? -1.f : 0.f;      // of the maximum's own terms one is not counted
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float d = max_nan(v[i] - m, -200.f), e = ex2(d * kLog2e), one = d == 0.f ? 1.f : 0.f;
+    less += e - one;
+    equal += one;
+    s.t = fmaf(d, e, s.t);
+  }
+  s.s += less + equal;
 }
 
 // a and b together.

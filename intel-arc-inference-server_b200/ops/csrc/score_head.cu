@@ -1,9 +1,12 @@
-// A prompt's rows through the head: z = x W^T (bf16), or (q . w) s_row s_column (int8), on tcgen05, two SMs on one 256 x 256 tile.
+// A prompt's rows through the head: z = x W^T (bf16), or (q . w) s_row s_column (int8), on tcgen05, two SMs on one 256 x 256 tile.  The
+// logits of a tile leave tensor memory for registers and go no further: what stays of 256 logits of a row are their maximum and two sums
+// (LogStat, 16 bytes in place of 1024), and the token's logit where it is among them.  A second kernel joins a row's tiles in order.
+// With alternatives the logits themselves are stored, for logprob.cu.
 //
 // Structure, per cluster of two CTAs (192 threads each):
 //   warp 0    copies by TMA: this CTA's 128 rows of x and 128 of the tile's 256 rows of W, 128 bytes of k a stage, six stages
 //   warp 1    even CTA: tcgen05.mma.cta_group::2, M = 256, N = 256; two accumulators in tensor memory
-//   warps 2-5 this CTA's 128 rows of the accumulator: logits to memory
+//   warps 2-5 this CTA's 128 rows of the accumulator, a thread per row: sums, or logits to memory
 // Tiles are walked rows first, so that the clusters that run together share the rows of W in L2.
 #include "common.cuh"
 #include "logprob.cuh"
@@ -21,8 +24,11 @@ constexpr int kSmem = kStages * kStage + 1024 + 256;    // + alignment, barriers
 struct ScoreParams {
   int m, n, kb;             // kb: stages of k
   const float *x_scale, *w_scale;      // int8: per row of x, per row of W
-  float* z;                 // [m][ldz]
+  float* z;                 // [m][ldz] logits
   long long ldz;
+  const int* tokens;        // sums: [m]
+  float4* part;             // [column of tiles][m]: maximum and sums of a row's 256 logits
+  float* token_z;           // [m] logit of the row's token, where it has one
 };
 
 __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -33,10 +39,12 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       : "memory");
 }
 
-template <bool I8>
+// SUMS: maxima and sums; else logits.
+template <bool I8, bool SUMS>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const ScoreParams p) {
   extern __shared__ uint8_t smem_raw[];
+  __shared__ float scales[2][I8 ? BN : 1];      // of the columns of a tile and of the next
   const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = smem + kStages * kStage;
   const uint32_t full0 = bars, empty0 = full0 + 8 * kStages, done0 = empty0 + 8 * kStages, read0 = done0 + 16, slot = read0 + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
@@ -119,23 +127,51 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
     const int quarter = warp & 3;      // of the lanes of tensor memory, this warp's
     int i = 0;
     bool ok = true;
-    for (int t = first; t < tiles && ok; t += pairs, ++i) {
-      const int a = i & 1, row = (t % tiles_m) * 2 * BM + rank * BM + quarter * 32 + lane, col0 = (t / tiles_m) * BN;
-      ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * a, (i >> 1) & 1, ERR_GEMM_TMEM_FULL_WAIT));
-      if (!ok) break;
+    for (int t = first; t < tiles; t += pairs, ++i) {      // (to the end also after a wait that ran out: the warps meet at a barrier)
+      const int a = i & 1, row0 = (t % tiles_m) * 2 * BM + rank * BM + quarter * 32, row = row0 + lane, nt = t / tiles_m, col0 = nt * BN;
+      if (I8) {      // (written while others may still read the tile before: two buffers)
+        const int j = threadIdx.x - 64;
+        scales[a][j] = p.w_scale[min(col0 + j, p.n - 1)];
+        scales[a][j + 128] = p.w_scale[min(col0 + j + 128, p.n - 1)];
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+      }
+      const bool there = row < p.m;
+      const float xs = I8 && there ? p.x_scale[row] : 1.f;
+      const int token = SUMS && there ? p.tokens[row] : -1;
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * a, (i >> 1) & 1, ERR_GEMM_TMEM_FULL_WAIT));
+      if (!ok) continue;
       tc_fence_after();
-      const float xs = I8 && row < p.m ? p.x_scale[row] : 1.f;
+      LogStat s{-INFINITY, 0.f, 0.f};
 #pragma unroll 1
-      for (int c = 0; c < BN / 32; ++c) {
+      for (int c = 0; c < BN / 32 && row0 < p.m; ++c) {
         uint32_t v[32];
         B2_TMEM_LD_32(tmem + a * BN + c * 32 + ((uint32_t)(quarter * 32) << 16), v);
         tmem_ld_wait();
         const int n0 = col0 + c * 32;
+        if (n0 >= p.n) break;
         if (I8) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint((float)(int)v[j] * xs * p.w_scale[min(n0 + j, p.n - 1)]);
+          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint((float)(int)v[j] * xs * scales[a][c * 32 + j]);
         }
-        if (row < p.m) {
+        if (SUMS) {
+          float z[32], largest = -INFINITY;
+#pragma unroll
+          for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(v[j]);
+          if (n0 + 32 > p.n) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (n0 + j >= p.n) z[j] = -INFINITY;
+          }
+#pragma unroll
+          for (int j = 0; j < 32; ++j) largest = fmaxf(largest, z[j]);
+          add_terms(s, z, largest);
+          if (token >= n0 && token < min(n0 + 32, p.n)) {
+            float mine = z[0];
+#pragma unroll
+            for (int j = 1; j < 32; ++j) mine = token == n0 + j ? z[j] : mine;
+            p.token_z[row] = mine;
+          }
+        } else if (there) {
           float* dst = p.z + row * p.ldz + n0;
           if (n0 + 32 <= p.n) {
 #pragma unroll
@@ -147,6 +183,7 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
           }
         }
       }
+      if (SUMS && there) p.part[(long long)nt * p.m + row] = make_float4(s.m, s.s, s.t, 0.f);
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(map_rank0(read0 + 8 * a));
@@ -160,6 +197,36 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+  }
+}
+
+// ------------------------------------------------------------------ a row's tiles together
+// A CTA takes 32 rows: warp w joins tiles w, w + 32, ... of all of them (a lane a row, so that a warp reads whole lines), then the warps'
+// results are joined in the order of the warps.
+__global__ void __launch_bounds__(1024) score_join_kernel(const float4* __restrict__ part, const float* __restrict__ token_z, const int* __restrict__ tokens, int m,
+                                                          int n, float* __restrict__ logprob, float* __restrict__ entropy) {
+  __shared__ LogStat sh[32][33];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 32 + lane, tiles = (n + BN - 1) / BN;
+  pdl_wait();
+  LogStat s{-INFINITY, 0.f, 0.f};
+  if (row < m)
+#pragma unroll 4
+    for (int t = warp; t < tiles; t += 32) {
+      const float4 q = part[(long long)t * m + row];
+      s = join(s, LogStat{q.x, q.y, q.z});
+    }
+  sh[warp][lane] = s;
+  __syncthreads();
+#pragma unroll
+  for (int half = 16; half > 0; half >>= 1) {
+    if (warp < half) sh[warp][lane] = s = join(s, sh[warp + half][lane]);
+    __syncthreads();
+  }
+  if (warp == 0 && row < m) {
+    const LogNorm norm = log_norm(s);
+    const int t = tokens[row];
+    logprob[row] = t >= 0 && t < n ? log_prob(norm, token_z[row]) : NAN;
+    entropy[row] = norm.entropy;
   }
 }
 
@@ -240,38 +307,55 @@ int sm_count() {
   return n[dev & 63];
 }
 
-template <bool I8>
-int launch(const CUtensorMap& mx, const CUtensorMap& mw, const ScoreParams& p, cudaStream_t st) {
+template <bool I8, bool SUMS>
+int launch(const CUtensorMap& mx, const CUtensorMap& mw, const ScoreParams& p, int tiles, cudaStream_t st) {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(score_kernel<I8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(score_kernel<I8, SUMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return (int)e;
     configured[dev & 63] = true;
   }
-  const long long tiles = (long long)((p.m + 2 * BM - 1) / (2 * BM)) * ((p.n + BN - 1) / BN);
-  if (tiles > 0x3fffffff) return -2;
-  const int pairs = (int)min(tiles, (long long)(sm_count() / 2));
-  score_kernel<I8><<<2 * pairs, kThreads, kSmem, st>>>(mx, mw, p);
+  score_kernel<I8, SUMS><<<2 * min(tiles, sm_count() / 2), kThreads, kSmem, st>>>(mx, mw, p);
   return (int)cudaGetLastError();
+}
+
+int run(const void* x, long long ldx, const void* w, long long ldw, bool i8, int k, ScoreParams& p, bool sums, cudaStream_t st) {
+  const int size = i8 ? 1 : 2;
+  const long long tiles = (long long)((p.m + 2 * BM - 1) / (2 * BM)) * ((p.n + BN - 1) / BN);
+  if (p.m < 1 || p.n < 1 || (long long)k * size < kStageRow || ldx < k || ldw < k || tiles > 0x3fffffff || (i8 && (!p.x_scale || !p.w_scale))) return -1;
+  if (((uintptr_t)x | (uintptr_t)w | (unsigned long long)(ldx * size) | (unsigned long long)(ldw * size)) & 15) return -3;
+  p.kb = (int)(((long long)k * size + kStageRow - 1) / kStageRow);
+  CUtensorMap mx, mw;
+  int rc = make_map(&mx, x, i8, p.m, k, ldx);
+  if (!rc) rc = make_map(&mw, w, i8, p.n, k, ldw);
+  if (rc) return rc;
+  if (sums) return i8 ? launch<true, true>(mx, mw, p, (int)tiles, st) : launch<false, true>(mx, mw, p, (int)tiles, st);
+  return i8 ? launch<true, false>(mx, mw, p, (int)tiles, st) : launch<false, false>(mx, mw, p, (int)tiles, st);
 }
 
 }  // namespace
 
-// Logits z [m][ldz] (ldz a multiple of 4) of rows x [m][k] against the head w [n][k], both bf16, or int8 with scales.  Rows of x and w are
-// ldx and ldw elements apart, multiples of 16 bytes.
+// Rows x [m][k] against the head w [n][k], both bf16, or int8 with scales; rows are ldx and ldw elements apart, multiples of 16 bytes, of
+// 128 bytes at least.
+// Logits z [m][ldz], ldz a multiple of 4.
 extern "C" int b2_score_logits(const void* x, long long ldx, const void* w, long long ldw, int i8, const float* x_scale, const float* w_scale, int m, int n,
                                int k, float* z, long long ldz, void* stream) {
-  const int size = i8 ? 1 : 2;
-  if (m < 1 || n < 1 || k < 1 || ldx < k || ldw < k || ldz < n) return -1;
-  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)z | (unsigned long long)(ldx * size) | (unsigned long long)(ldw * size) | (unsigned long long)(ldz * 4)) & 15) return -3;
-  ScoreParams p{m, n, (int)(((long long)k * size + kStageRow - 1) / kStageRow), x_scale, w_scale, z, ldz};
-  CUtensorMap mx, mw;
-  int rc = make_map(&mx, x, i8 != 0, m, k, ldx);
-  if (!rc) rc = make_map(&mw, w, i8 != 0, n, k, ldw);
+  if (ldz < n || (((uintptr_t)z | (unsigned long long)(ldz * 4)) & 15)) return -2;
+  ScoreParams p{m, n, 0, x_scale, w_scale, z, ldz, nullptr, nullptr, nullptr};
+  return run(x, ldx, w, ldw, i8 != 0, k, p, false, (cudaStream_t)stream);
+}
+// Log probabilities of the rows' tokens and entropies.  work: b2_score_work(m, n) floats, 16-byte aligned, of this call alone.
+extern "C" long long b2_score_work(int m, int n) { return ((long long)((n + BN - 1) / BN) * 4 + 1) * m; }
+extern "C" int b2_score_tokens(const void* x, long long ldx, const void* w, long long ldw, int i8, const float* x_scale, const float* w_scale, int m, int n,
+                               int k, const int* tokens, float* work, float* logprob, float* entropy, void* stream) {
+  if ((uintptr_t)work & 15) return -2;
+  float* token_z = work + (long long)((n + BN - 1) / BN) * 4 * m;
+  ScoreParams p{m, n, 0, x_scale, w_scale, nullptr, 0, tokens, (float4*)work, token_z};
+  const int rc = run(x, ldx, w, ldw, i8 != 0, k, p, true, (cudaStream_t)stream);
   if (rc) return rc;
-  return i8 ? launch<true>(mx, mw, p, (cudaStream_t)stream) : launch<false>(mx, mw, p, (cudaStream_t)stream);
+  return b2_launch(score_join_kernel, dim3((m + 31) / 32), dim3(1024), 0, (cudaStream_t)stream, true, (const float4*)work, token_z, tokens, m, n, logprob, entropy);
 }
 
 // Rows x [m][k] bf16 (16-byte aligned, ldx a multiple of 8) as int8 q [m][ldq] (16-byte aligned, ldq a multiple of 16) and scales.

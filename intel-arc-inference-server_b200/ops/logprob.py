@@ -88,10 +88,11 @@ def _ld(t: torch.Tensor, align: int = 1) -> int:
 
 
 @functools.lru_cache(maxsize=None)
-def _entry(name: str, kinds: str):
+def _entry(name: str, kinds: str, result=ctypes.c_int):
     """An entry point of the library with its argument types (p: pointer, l: 64 bits, i: 32 bits), so that a call of a few microseconds
     wraps no numbers one by one."""
     fn = getattr(K.lib(), name)
+    fn.restype = result
     fn.argtypes = [{"p": ctypes.c_void_p, "l": ctypes.c_longlong, "i": ctypes.c_int}[c] for c in kinds]
     return fn
 
@@ -127,14 +128,22 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int
 def _score(x, w, i8: bool, x_scale, w_scale, tokens, out: Logprobs):
     m, k = x.shape
     n = w.shape[0]
+    ws = None if w_scale is None else w_scale.data_ptr()
+    if not out.top_ids.shape[1]:
+        work = torch.empty(_entry("b2_score_work", "ii", ctypes.c_longlong)(m, n), dtype=torch.float32, device=x.device)
+        K._check(_entry("b2_score_tokens", "plplippiiippppp")(
+            x.data_ptr(), _ld(x, 16), w.data_ptr(), _ld(w, 16), int(i8), None if x_scale is None else x_scale.data_ptr(), ws, m, n, k, tokens.data_ptr(),
+            work.data_ptr(), out.logprob.data_ptr(), out.entropy.data_ptr(), _stream(x.device)), "score_tokens")
+        K.launch_count += 1      # the rows' tiles joined
+        return out
     ldz = (n + 3) // 4 * 4
     step = max(1, min(m, max(256, SLAB_ELEMS // ldz // 256 * 256)))
     z = torch.empty(step, ldz, dtype=torch.float32, device=x.device)
     for i in range(0, m, step):
         c = min(step, m - i)
         K._check(_entry("b2_score_logits", "plplippiiiplp")(
-            x[i:].data_ptr(), _ld(x, 16), w.data_ptr(), _ld(w, 16), int(i8), None if x_scale is None else x_scale[i:].data_ptr(),
-            None if w_scale is None else w_scale.data_ptr(), c, n, k, z.data_ptr(), ldz, _stream(x.device)), "score_logits")
+            x[i:].data_ptr(), _ld(x, 16), w.data_ptr(), _ld(w, 16), int(i8), None if x_scale is None else x_scale[i:].data_ptr(), ws, c, n, k, z.data_ptr(),
+            ldz, _stream(x.device)), "score_logits")
         token_logprobs(z[:c, :n], tokens[i: i + c], out=out.rows(i, i + c))
     return out
 
