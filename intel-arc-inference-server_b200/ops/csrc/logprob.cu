@@ -7,8 +7,11 @@
 // in every run.
 //
 // Alternatives: the top-th largest of the threads' maxima is a bound that at least `top` logits of the CTA reach, so only the logits of the
-// threads whose maximum reaches it can matter: about `top` threads of a CTA.  Those few are read again, and what reaches the bound is put
-// in order.  The pass itself does nothing for the alternatives.
+// threads whose maximum reaches it can matter: about `top` threads of a CTA, and of their logits those of the tiles (in up to eight groups)
+// whose own maximum does.  Those few are read again, and what reaches the bound is put in order.  The pass itself does nothing for the
+// alternatives but to keep eight maxima a thread.
+// Bound by the logits' bytes with many rows (500 x 151936: 57 us with 10 alternatives, 52 without, 46 at the measured copy rate), by its own
+// chain of reductions with few (1 x 151936: 7.2 and 3.9 us).  Alternatives kept in sorted lists during the pass: 108 us and 8.9.
 #include "common.cuh"
 #include "logprob.cuh"
 #include "pair.cuh"
@@ -20,6 +23,7 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kVecs = 4;                              // 16-byte vectors of a thread and tile
 constexpr int kTile = kThreads * kVecs;               // vectors
+constexpr int kGroups = 8;                            // of a CTA's tiles
 constexpr int kParts = 16;                            // CTAs that share a row, at most
 
 struct RowsParams {
@@ -32,76 +36,11 @@ struct RowsParams {
   float* top_logprobs;
 };
 
-__device__ __forceinline__ float order_value(uint32_t o) {      // of logit_order
-  return __uint_as_float(o == 1u ? 0x7fffffffu : (o & 0x80000000u) ? (o ^ 0x80000000u) : ~o);
-}
-
-// The stats of `width` lanes (a power of two) in all of them: the maximum first, then plain sums of what each lane is to it.
-template <int width>
-__device__ __forceinline__ LogStat join_lanes(const LogStat& a) {
-  float m = a.m;
-#pragma unroll
-  for (int o = width / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  const bool none = a.m == -INFINITY, best = a.m == m;
-  const float d = below(a.m, m), f = ex2(d * kLog2e), n = 1.f + a.s;
-  LogStat r{m, none || best ? a.s : n * f, none || best ? a.t : f * fmaf(d, n, a.t)};
-  float count = best && !none ? 1.f : 0.f;      // lanes with a term of the maximum beside their sums
-#pragma unroll
-  for (int o = width / 2; o > 0; o >>= 1) {
-    r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
-    r.t += __shfl_xor_sync(0xffffffffu, r.t, o);
-    count += __shfl_xor_sync(0xffffffffu, count, o);
-  }
-  r.s += fmaxf(count - 1.f, 0.f);
-  return r;
-}
-
-// The largest 32 keys of two lists, each sorted across the lanes, the largest first; so is the result.
-__device__ __forceinline__ unsigned long long merge_lists(unsigned long long a, unsigned long long b, int lane) {
-  unsigned long long k = max(a, __shfl_xor_sync(0xffffffffu, b, 31));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
-    k = (lane & o) ? min(k, other) : max(k, other);
-  }
-  return k;
-}
-
-// One more key for a sorted list.
-__device__ __forceinline__ void insert(unsigned long long& list, unsigned long long key, int lane) {
-  const int at = __popc(__ballot_sync(0xffffffffu, list > key));
-  const unsigned long long before = __shfl_up_sync(0xffffffffu, list, 1);
-  list = lane < at ? list : lane == at ? key : before;
-}
-
-// The lanes' numbers, none of them NaN, the largest first.
-__device__ __forceinline__ float sort_lanes(float x, int lane) {
-#pragma unroll
-  for (int size = 2; size <= 32; size *= 2)
-#pragma unroll
-    for (int o = size / 2; o > 0; o >>= 1) {
-      const float other = __shfl_xor_sync(0xffffffffu, x, o);
-      const bool low = (lane & o) == 0, falling = (lane & size) == 0;
-      x = low == falling ? fmaxf(x, other) : fminf(x, other);
-    }
-  return x;
-}
-// The largest 32 of two lists of numbers, as merge_lists.
-__device__ __forceinline__ float merge_floats(float a, float b, int lane) {
-  float x = fmaxf(a, __shfl_xor_sync(0xffffffffu, b, 31));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float other = __shfl_xor_sync(0xffffffffu, x, o);
-    x = (lane & o) ? fminf(x, other) : fmaxf(x, other);
-  }
-  return x;
-}
-
 struct Shared {
   LogStat stat[kWarps], parts[kParts];
   unsigned long long list[kWarps][32], part_list[kParts][32];
-  float best[kWarps][32];
-  int chosen, threads[kThreads];
+  float best[kWarps][32], group[kGroups][kThreads];
+  int count, chosen[kGroups * kThreads];      // group * kThreads + thread
 };
 
 __device__ __forceinline__ uint32_t map_cluster(uint32_t addr, int rank) {      // a CTA's copy of a shared-memory word
@@ -111,7 +50,7 @@ __device__ __forceinline__ uint32_t map_cluster(uint32_t addr, int rank) {      
 }
 
 template <bool TOP>
-__global__ void __launch_bounds__(kThreads, 5) logprob_rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(kThreads, 4) logprob_rows_kernel(const RowsParams p) {
   __shared__ Shared sh;
   const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (p.parts > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // the first CTA is there: waited for below
@@ -119,34 +58,48 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_rows_kernel(const RowsPar
   const float* z = p.z + row * p.ld;
   const int shift = (int)((uintptr_t)z >> 2) & 3;        // logits before the row in its first 16 bytes
   const int vecs = (p.n + shift + 3) / 4, tiles = (vecs + kTile - 1) / kTile;
-  const auto load = [&](int tile, float (&v)[4 * kVecs]) {
+  const auto load = [&](int vec, float* v) {
+    const int j = vec * 4 - shift;
+    if (j >= 0 && j + 4 <= p.n) {
+      const float4 q = __ldcs(reinterpret_cast<const float4*>(z + j));
+      v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      const int vec = tile * kTile + i * kThreads + threadIdx.x, j = vec * 4 - shift;
-      if (j >= 0 && j + 4 <= p.n) {
-        const float4 q = __ldcs(reinterpret_cast<const float4*>(z + j));
-        v[4 * i] = q.x; v[4 * i + 1] = q.y; v[4 * i + 2] = q.z; v[4 * i + 3] = q.w;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[4 * i + e] = j + e >= 0 && j + e < p.n ? z[j + e] : -INFINITY;
-      }
+      for (int e = 0; e < 4; ++e) v[e] = j + e >= 0 && j + e < p.n ? z[j + e] : -INFINITY;
     }
   };
+  const int mine = (tiles - part + p.parts - 1) / p.parts, per = (mine + kGroups - 1) / kGroups;      // this CTA's tiles, and those of a group
   LogStat s{-INFINITY, 0.f, 0.f};
-  for (int tile = part; tile < tiles; tile += p.parts) {
+  float in_group = -INFINITY;
+  float next[4 * kVecs];      // the next tile's, on their way while a tile is added up (500 rows of 151936, us: 56 -> 52)
+  const auto fetch = [&](int i) {
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) load((part + i * p.parts) * kTile + k * kThreads + threadIdx.x, next + 4 * k);
+  };
+  if (mine > 0) fetch(0);
+  for (int i = 0, left = per, group = 0; i < mine; ++i) {
     float v[4 * kVecs];
-    load(tile, v);
+#pragma unroll
+    for (int k = 0; k < 4 * kVecs; ++k) v[k] = next[k];
+    if (i + 1 < mine) fetch(i + 1);
     float largest = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 4 * kVecs; ++i) largest = fmaxf(largest, v[i]);
+    for (int k = 0; k < 4 * kVecs; ++k) largest = fmaxf(largest, v[k]);
     add_terms(s, v, largest);
+    if (TOP) {
+      in_group = fmaxf(in_group, largest);
+      if (--left == 0 || i == mine - 1) {
+        sh.group[group++][threadIdx.x] = in_group;
+        in_group = -INFINITY;
+        left = per;
+      }
+    }
   }
 
   unsigned long long list = 0;
   if (TOP) {
-    const float mine = s.m;
-    if (threadIdx.x == 0) sh.chosen = 0;
-    float best = sort_lanes(mine, lane);
+    if (threadIdx.x == 0) sh.count = 0;
+    float best = sort_lanes(s.m, lane);
     sh.best[warp][lane] = best;
     __syncthreads();
 #pragma unroll
@@ -158,36 +111,29 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_rows_kernel(const RowsPar
       __syncthreads();
     }
     const float bound = sh.best[0][p.top - 1];
-    const bool choose = mine >= bound && mine > -INFINITY;
-    const uint32_t mask = __ballot_sync(0xffffffffu, choose);
-    int at = 0;
-    if (lane == 0 && mask) at = atomicAdd(&sh.chosen, __popc(mask));      // (whatever their order, the same logits come out)
-    at = __shfl_sync(0xffffffffu, at, 0) + __popc(mask & ((1u << lane) - 1));
-    if (choose) sh.threads[at] = threadIdx.x;
+    if (s.m >= bound && s.m > -INFINITY)
+      for (int g = 0; g * per < mine; ++g) {
+        const float x = sh.group[g][threadIdx.x];
+        if (x >= bound && x > -INFINITY) sh.chosen[atomicAdd(&sh.count, 1)] = g * kThreads + threadIdx.x;      // (whatever their order, the same logits come out)
+      }
     __syncthreads();
-    // the chosen threads' vectors, dealt out to the warps one by one
-    const int each = (tiles - part + p.parts - 1) / p.parts * kVecs, items = sh.chosen * each;
+    // their vectors, dealt out to the warps one by one
+    const int each = per * kVecs, items = sh.count * each;
     unsigned long long last = 0;
     for (int base = 0; base < items; base += kThreads) {
       const int q = base + lane * kWarps + warp;
       int id = p.n;
-      float v[4];
+      float v[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       if (q < items) {
-        const int thread = sh.threads[q / each], i = q % each, vec = (part + i / kVecs * p.parts) * kTile + i % kVecs * kThreads + thread;
-        id = vec * 4 - shift;
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = id + e >= 0 && id + e < p.n ? z[id + e] : -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const unsigned long long key = v[e] >= bound && v[e] > -INFINITY ? logit_key(v[e], id + e) : 0;
-        uint32_t more = __ballot_sync(0xffffffffu, key > last);
-        while (more) {
-          insert(list, __shfl_sync(0xffffffffu, key, __ffs(more) - 1), lane);
-          last = __shfl_sync(0xffffffffu, list, p.top - 1);
-          more = __ballot_sync(0xffffffffu, key > last) & (more & (more - 1));
+        const int what = sh.chosen[q / each], k = q % each, i = what / kThreads * per + k / kVecs;
+        if (i < mine) {
+          const int vec = (part + i * p.parts) * kTile + k % kVecs * kThreads + what % kThreads;
+          load(vec, v);
+          id = vec * 4 - shift;
         }
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) offer(list, last, v[e] >= bound && v[e] > -INFINITY ? logit_key(v[e], id + e) : 0, p.top, lane);
     }
   }
 
@@ -242,22 +188,7 @@ __global__ void __launch_bounds__(kThreads, 5) logprob_rows_kernel(const RowsPar
     p.entropy[row] = norm.entropy;
   }
   if (TOP) {
-    // Fewer than `top` logits above -inf: banned ids follow, the lowest first, then those without a number.
-    int have = __popc(__ballot_sync(0xffffffffu, list != 0));
-    for (int kind = 0; kind < 2 && have < p.top; ++kind) {
-      for (int j0 = 0; j0 < p.n && have < p.top; j0 += 32) {
-        const int j = j0 + lane;
-        const float x = j < p.n ? z[j] : 0.f;
-        const bool take = j < p.n && (kind == 0 ? x == -INFINITY : x != x);
-        const uint32_t mask = __ballot_sync(0xffffffffu, take);
-        const int nth = lane - have;      // this lane's place is the nth of them
-        if (nth >= 0 && nth < __popc(mask)) {
-          const int from = __fns(mask, 0, nth + 1);
-          list = logit_key(kind == 0 ? -INFINITY : __int_as_float(0x7fffffff), j0 + from);
-        }
-        have += __popc(mask);
-      }
-    }
+    list = fill_list(list, z, p.n, p.top, lane);
     if (lane < p.top) {
       p.top_ids[(long long)row * p.top + lane] = list ? (int)key_id(list) : -1;
       p.top_logprobs[(long long)row * p.top + lane] = list ? log_prob(norm, order_value((uint32_t)(list >> 32))) : -INFINITY;
@@ -305,8 +236,8 @@ extern "C" int b2_logprob_rows(const float* z, long long ld, int m, int n, const
                                int* top_ids, float* top_logprobs, void* stream) {
   if (m < 1 || n < 1 || n > 0x7fff0000 || ld < n || top < 0 || top > kMaxTop || ((uintptr_t)z & 3)) return -1;
   // CTAs of a row: as many as it has tiles, and as leave four to an SM; sixteen, whose joining costs most, where there are two to an SM.
-  // Rows of 151936, 10 alternatives, 1 / 2 / 4 / 8 / 16 CTAs a row, us: 8 rows 27.4 / 16.5 / 11.2 / 8.1 / 7.9, 32 rows 27.6 / 16.6 / 11.5 / 9.7 / 14.3,
-  // 100 rows 41.8 / 26.8 / 19.0 / 23.0 / 34.2, 200 rows 49.7 / 32.6 / 37.9 / 39.2 / 63.6, 500 rows 65.8 / 67.5 / 78.4 / 94.8 / 153.4.
+  // Rows of 151936, 10 alternatives, us with 1 / 2 / 4 / 8 / 16 CTAs a row (an earlier form): 8 rows 27.4 / 16.5 / 11.2 / 8.1 / 7.9, 32 rows 27.6 / 16.6 /
+  // 11.5 / 9.7 / 14.3, 100 rows 41.8 / 26.8 / 19.0 / 23.0 / 34.2, 200 rows 49.7 / 32.6 / 37.9 / 39.2 / 63.6, 500 rows 65.8 / 67.5 / 78.4 / 94.8 / 153.4.
   const int tiles = ((n + 6) / 4 + kTile - 1) / kTile, sms = sm_count();
   int parts = 1;
   while (parts < kParts && 2 * parts <= tiles && 2ll * parts * m <= (2 * parts == kParts ? 2 : 4) * sms) parts *= 2;

@@ -85,4 +85,96 @@ __device__ __forceinline__ uint32_t logit_order(float z) {
 __device__ __forceinline__ unsigned long long logit_key(float z, int id) { return ((unsigned long long)logit_order(z) << 32) | (uint32_t)~id; }
 __device__ __forceinline__ uint32_t key_id(unsigned long long key) { return ~(uint32_t)key; }
 
+__device__ __forceinline__ float order_value(uint32_t o) {      // of logit_order
+  return __uint_as_float(o == 1u ? 0x7fffffffu : (o & 0x80000000u) ? (o ^ 0x80000000u) : ~o);
+}
+
+// The stats of `width` lanes (a power of two) in all of them: the maximum first, then plain sums of what each lane is to it.
+template <int width>
+__device__ __forceinline__ LogStat join_lanes(const LogStat& a) {
+  float m = a.m;
+#pragma unroll
+  for (int o = width / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const bool none = a.m == -INFINITY, best = a.m == m;
+  const float d = below(a.m, m), f = ex2(d * kLog2e), n = 1.f + a.s;
+  LogStat r{m, none || best ? a.s : n * f, none || best ? a.t : f * fmaf(d, n, a.t)};
+  float count = best && !none ? 1.f : 0.f;      // lanes with a term of the maximum beside their sums
+#pragma unroll
+  for (int o = width / 2; o > 0; o >>= 1) {
+    r.s += __shfl_xor_sync(0xffffffffu, r.s, o);
+    r.t += __shfl_xor_sync(0xffffffffu, r.t, o);
+    count += __shfl_xor_sync(0xffffffffu, count, o);
+  }
+  r.s += fmaxf(count - 1.f, 0.f);
+  return r;
+}
+
+// The largest 32 keys of two lists, each sorted across the lanes, the largest first; so is the result.
+__device__ __forceinline__ unsigned long long merge_lists(unsigned long long a, unsigned long long b, int lane) {
+  unsigned long long k = max(a, __shfl_xor_sync(0xffffffffu, b, 31));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long other = __shfl_xor_sync(0xffffffffu, k, o);
+    k = (lane & o) ? min(k, other) : max(k, other);
+  }
+  return k;
+}
+
+// One more key for a sorted list.
+__device__ __forceinline__ void insert(unsigned long long& list, unsigned long long key, int lane) {
+  const int at = __popc(__ballot_sync(0xffffffffu, list > key));
+  const unsigned long long before = __shfl_up_sync(0xffffffffu, list, 1);
+  list = lane < at ? list : lane == at ? key : before;
+}
+
+// The lanes' numbers, none of them NaN, the largest first.
+__device__ __forceinline__ float sort_lanes(float x, int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+    for (int o = size / 2; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, x, o);
+      const bool low = (lane & o) == 0, falling = (lane & size) == 0;
+      x = low == falling ? fmaxf(x, other) : fminf(x, other);
+    }
+  return x;
+}
+// The largest 32 of two lists of numbers, as merge_lists.
+__device__ __forceinline__ float merge_floats(float a, float b, int lane) {
+  float x = fmaxf(a, __shfl_xor_sync(0xffffffffu, b, 31));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float other = __shfl_xor_sync(0xffffffffu, x, o);
+    x = (lane & o) ? fminf(x, other) : fmaxf(x, other);
+  }
+  return x;
+}
+
+// A list with fewer than `top` logits above -inf: banned ids follow, the lowest first, then those without a number.
+__device__ __forceinline__ unsigned long long fill_list(unsigned long long list, const float* z, int n, int top, int lane) {
+  int have = __popc(__ballot_sync(0xffffffffu, list != 0));
+  for (int kind = 0; kind < 2 && have < top; ++kind) {
+    for (int j0 = 0; j0 < n && have < top; j0 += 32) {
+      const int j = j0 + lane;
+      const float x = j < n ? z[j] : 0.f;
+      const bool take = j < n && (kind == 0 ? x == -INFINITY : x != x);
+      const uint32_t mask = __ballot_sync(0xffffffffu, take);
+      const int nth = lane - have;      // this lane's place is the nth of them
+      if (nth >= 0 && nth < __popc(mask)) list = logit_key(kind == 0 ? -INFINITY : __int_as_float(0x7fffffff), j0 + __fns(mask, 0, nth + 1));
+      have += __popc(mask);
+    }
+  }
+  return list;
+}
+
+// A logit per lane into a sorted list of which the first `top` count; last: the top-th key.
+__device__ __forceinline__ void offer(unsigned long long& list, unsigned long long& last, unsigned long long key, int top, int lane) {
+  uint32_t more = __ballot_sync(0xffffffffu, key > last);
+  while (more) {
+    insert(list, __shfl_sync(0xffffffffu, key, __ffs(more) - 1), lane);
+    last = __shfl_sync(0xffffffffu, list, top - 1);
+    more = __ballot_sync(0xffffffffu, key > last) & (more & (more - 1));
+  }
+}
+
 }  // namespace b2

@@ -1,13 +1,18 @@
-// A prompt's rows through the head: z = x W^T (bf16), or (q . w) s_row s_column (int8), on tcgen05, two SMs on one 256 x 256 tile.  The
-// logits of a tile leave tensor memory for registers and go no further: what stays of 256 logits of a row are their maximum and two sums
-// (LogStat, 16 bytes in place of 1024), and the token's logit where it is among them.  A second kernel joins a row's tiles in order.
-// With alternatives the logits themselves are stored, for logprob.cu.
+// A prompt's rows through the head: z = x W^T (bf16), or (q . w) s_row s_column (int8), on tcgen05.  The logits of a tile leave tensor memory
+// for registers: what stays of a row's logits there are their maximum and two sums (LogStat), and the token's logit where it is among
+// them.  A second kernel joins a row's parts in order.  With alternatives the logits are stored too, beside the largest of every 32; the
+// second kernel reads these maxima and only those logits whose maximum reaches the top-th largest of a few (as in logprob.cu).
 //
-// Structure, per cluster of two CTAs (192 threads each):
-//   warp 0    copies by TMA: this CTA's 128 rows of x and 128 of the tile's 256 rows of W, 128 bytes of k a stage, six stages
-//   warp 1    even CTA: tcgen05.mma.cta_group::2, M = 256, N = 256; two accumulators in tensor memory
-//   warps 2-5 this CTA's 128 rows of the accumulator, a thread per row: sums, or logits to memory
-// Tiles are walked rows first, so that the clusters that run together share the rows of W in L2.
+// Two forms.  PAIR: a cluster of two CTAs on a 256 x 256 tile (tcgen05 cta_group::2), which asks least of the L2.  Else a CTA by itself on 128 x
+// 256, for up to 128 rows, where the head's bytes are what counts and the multiplication has to keep out of their way, and for 257 to 384,
+// of which pairs would multiply 512.  Pairs / CTAs by themselves, us, 151936 x 5120: 64 rows 297 / 271, 256 rows 324 / 352, 300 rows
+// 528 / 466, 512 rows 565 / 618.
+//   warp 0    copies by TMA: 128 rows of x and the CTA's rows of the tile of W (128 or 256), 128 bytes of k a stage
+//   warp 1    tcgen05.mma (PAIR: of the even CTA), N = 256; two accumulators in tensor memory
+//   warps 2-5 the CTA's 128 rows of the accumulator, a thread per row
+// More than 512 rows: tiles are walked rows first, so that the clusters that run together share the rows of W in L2.  Up to 512 rows whole
+// tiles would leave SMs idle at the end (102400 columns: 400 tiles for 74 clusters): every cluster gets a range of columns of its own,
+// equal but for 32, whose last tile is as narrow as it has to be; a thread's sums go on through the range.
 #include "common.cuh"
 #include "logprob.cuh"
 #include "pair.cuh"
@@ -18,17 +23,28 @@ namespace {
 
 constexpr int BM = 128, BN = 256, kStageRow = 128;      // rows of a CTA, columns of a tile, bytes of k a stage
 constexpr int kThreads = 192;
-constexpr int kHalf = 128 * kStageRow, kStage = 2 * kHalf, kStages = 6;
-constexpr int kSmem = kStages * kStage + 1024 + 256;    // + alignment, barriers
+constexpr int kGrain = 32, kChunk = 32;        // columns that ranges are cut at, columns of a maximum
+constexpr int kRangeRows = 512;      // up to these many rows ranges
+
+template <bool PAIR>
+struct Form {
+  static constexpr int ROWS = PAIR ? 2 * BM : BM;                   // of a tile
+  static constexpr int X_BYTES = BM * kStageRow, W_BYTES = (PAIR ? BN / 2 : BN) * kStageRow, STAGE = X_BYTES + W_BYTES;
+  static constexpr int STAGES = PAIR ? 6 : 4;
+  static constexpr int SMEM = STAGES * STAGE + 1024 + 256;          // + alignment, barriers
+};
 
 struct ScoreParams {
   int m, n, kb;             // kb: stages of k
+  int ranges;               // of columns, for each row of tiles; 0: tiles in turn
   const float *x_scale, *w_scale;      // int8: per row of x, per row of W
-  float* z;                 // [m][ldz] logits
-  long long ldz;
-  const int* tokens;        // sums: [m]
-  float4* part;             // [column of tiles][m]: maximum and sums of a row's 256 logits
+  const int* tokens;        // [m]
+  float4* part;             // [range, or column of tiles][m]: maximum and sums of a row's logits
   float* token_z;           // [m] logit of the row's token, where it has one
+  float* z;                 // alternatives: logits [m][ldz], and the largest of every kChunk [m][ldc]
+  long long ldz;
+  float* largest;
+  int ldc;
 };
 
 __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -39,37 +55,68 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t d_tmem, uint64_t a_desc, u
       : "memory");
 }
 
-// SUMS: maxima and sums; else logits.
-template <bool I8, bool SUMS>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
-score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const ScoreParams p) {
+// The tiles of a cluster, one after another: row of tiles mt, columns [col0, end) of which the tile has `width`, a multiple of 32; part: where
+// its sums go.
+struct Tile {
+  int mt, col0, end, width, part;
+};
+template <bool PAIR>
+__device__ __forceinline__ bool tile_at(const ScoreParams& p, int i, Tile& t) {
+  const int first = PAIR ? blockIdx.x >> 1 : blockIdx.x, tiles_m = (p.m + Form<PAIR>::ROWS - 1) / Form<PAIR>::ROWS;
+  if (p.ranges) {
+    const long long grains = (p.n + kGrain - 1) / kGrain;
+    t.mt = first % tiles_m;
+    t.part = first / tiles_m;
+    t.col0 = (int)(t.part * grains / p.ranges) * kGrain + i * BN;
+    t.end = min(p.n, (int)((t.part + 1) * grains / p.ranges) * kGrain);
+    t.width = min(BN, (t.end - t.col0 + kGrain - 1) / kGrain * kGrain);
+    return t.col0 < t.end;
+  }
+  const int at = first + i * (PAIR ? gridDim.x >> 1 : gridDim.x);
+  t.mt = at % tiles_m;
+  t.part = at / tiles_m;
+  t.col0 = t.part * BN;
+  t.end = p.n;
+  t.width = BN;
+  return t.col0 < p.n;
+}
+
+// ALT: logits and their maxima are stored.  map_g: W in boxes of 16 (PAIR) or 32 rows, for narrow tiles.
+template <bool I8, bool ALT, bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_g, const ScoreParams p) {
+  using F = Form<PAIR>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float scales[2][I8 ? BN : 1];      // of the columns of a tile and of the next
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = smem + kStages * kStage;
-  const uint32_t full0 = bars, empty0 = full0 + 8 * kStages, done0 = empty0 + 8 * kStages, read0 = done0 + 16, slot = read0 + 16;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = (int)cluster_rank();
-  const int tiles_m = (p.m + 2 * BM - 1) / (2 * BM), tiles = tiles_m * ((p.n + BN - 1) / BN);
-  const int first = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = smem + F::STAGES * F::STAGE;
+  const uint32_t full0 = bars, empty0 = full0 + 8 * F::STAGES, done0 = empty0 + 8 * F::STAGES, read0 = done0 + 16, slot = read0 + 16;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = PAIR ? (int)cluster_rank() : 0;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(full0 + 8 * i, 1);      // used in the even CTA: both CTAs' bytes
+    for (int i = 0; i < F::STAGES; ++i) {
+      mbar_init(full0 + 8 * i, 1);      // PAIR: used in the even CTA, both CTAs' bytes
       mbar_init(empty0 + 8 * i, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(done0 + 8 * i, 1);
-      mbar_init(read0 + 8 * i, 8);      // used in the even CTA: both CTAs' four warps
+      mbar_init(read0 + 8 * i, PAIR ? 8 : 4);      // PAIR: used in the even CTA, both CTAs' four warps
     }
     mbar_fence_init();
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(slot) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(slot, 512);
+      tmem_relinquish();
+    }
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();      // both CTAs' barriers are there before anything arrives on them
+  if (PAIR) cluster_sync_all();      // both CTAs' barriers are there before anything arrives on them
   tc_fence_after();
+  pdl_wait();
   uint32_t tmem;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(tmem) : "r"(slot));
 
@@ -79,154 +126,261 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
       prefetch_tmap(&map_w);
       int s = 0, round = 0, issued = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += pairs) {
-        const int row0 = (t % tiles_m) * 2 * BM + rank * BM, col0 = (t / tiles_m) * BN + rank * (BN / 2);
+      Tile t;
+      for (int i = 0; ok && tile_at<PAIR>(p, i, t); ++i) {
+        const int row0 = t.mt * F::ROWS + rank * BM, mine = PAIR ? t.width / 2 : t.width, col0 = t.col0 + rank * mine;
         for (int kb = 0; kb < p.kb; ++kb) {
           if (round > 0) ok = mbar_wait_lone(empty0 + 8 * s, (round - 1) & 1, ERR_GEMM_EMPTY_WAIT);
           if (!ok) break;
-          const uint32_t at = smem + s * kStage, bar = map_rank0(full0 + 8 * s);
-          if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * kStage);
-          tma_load_2d_pair(at, &map_x, kb * (I8 ? kStageRow : kStageRow / 2), row0, bar);
-          tma_load_2d_pair(at + kHalf, &map_w, kb * (I8 ? kStageRow : kStageRow / 2), col0, bar);
+          const uint32_t at = smem + s * F::STAGE;
+          const int k = kb * (I8 ? kStageRow : kStageRow / 2);
+          const uint32_t bytes = F::X_BYTES + mine * kStageRow;
+          if (PAIR) {
+            const uint32_t bar = map_rank0(full0 + 8 * s);
+            if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * bytes);
+            tma_load_2d_pair(at, &map_x, k, row0, bar);
+            if (t.width == BN) tma_load_2d_pair(at + F::X_BYTES, &map_w, k, col0, bar);
+            else
+              for (int j = 0; j < mine; j += kGrain / 2) tma_load_2d_pair(at + F::X_BYTES + j * kStageRow, &map_g, k, col0 + j, bar);
+          } else {
+            const uint32_t bar = full0 + 8 * s;
+            mbar_expect_tx(bar, bytes);
+            tma_load_2d(at, &map_x, k, row0, bar);
+            if (t.width == BN) tma_load_2d(at + F::X_BYTES, &map_w, k, col0, bar);
+            else
+              for (int j = 0; j < mine; j += kGrain) tma_load_2d(at + F::X_BYTES + j * kStageRow, &map_g, k, col0 + j, bar);
+          }
           ++issued;
-          if (++s == kStages) { s = 0; ++round; }
+          if (++s == F::STAGES) { s = 0; ++round; }
         }
       }
-      // After a wait that ran out the even CTA waits (bounded) for the bytes both have asked for; the odd one meets it at the cluster
+      // After a wait that ran out the (even) CTA waits (bounded) for the bytes that were asked for; the odd one meets it at the cluster
       // barrier below.
       if (!ok && rank == 0)
-        for (int i = max(0, issued - kStages); i < issued; ++i) mbar_wait(full0 + 8 * (i % kStages), (i / kStages) & 1, ERR_GEMM_FULL_WAIT);
+        for (int i = max(0, issued - F::STAGES); i < issued; ++i) mbar_wait(full0 + 8 * (i % F::STAGES), (i / F::STAGES) & 1, ERR_GEMM_FULL_WAIT);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = I8 ? make_idesc(2, 1, 2 * BM, BN) : make_idesc(1, 1, 2 * BM, BN);
-      int s = 0, par = 0, i = 0;
+      int s = 0, par = 0;
       bool ok = true;
-      for (int t = first; t < tiles && ok; t += pairs, ++i) {
+      Tile t;
+      const auto wait = [](uint32_t bar, uint32_t parity, unsigned code) {
+        return PAIR ? mbar_wait_cluster(bar, parity, code) : mbar_wait_lone(bar, parity, code);
+      };
+      const auto commit = [](uint32_t bar) {
+        if (PAIR) tc_commit_pair(bar);
+        else tc_commit(bar);
+      };
+      for (int i = 0; ok && tile_at<PAIR>(p, i, t); ++i) {
         const int a = i & 1;
-        if (i >= 2) ok = mbar_wait_cluster(read0 + 8 * a, ((i >> 1) - 1) & 1, ERR_GEMM_TMEM_EMPTY_WAIT);
+        const uint32_t idesc = I8 ? make_idesc(2, 1, F::ROWS, t.width) : make_idesc(1, 1, F::ROWS, t.width);
+        if (i >= 2) ok = wait(read0 + 8 * a, ((i >> 1) - 1) & 1, ERR_GEMM_TMEM_EMPTY_WAIT);
         if (!ok) break;
         tc_fence_after();
         for (int kb = 0; kb < p.kb; ++kb) {
-          ok = mbar_wait_cluster(full0 + 8 * s, par, ERR_GEMM_FULL_WAIT);
+          ok = wait(full0 + 8 * s, par, ERR_GEMM_FULL_WAIT);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t da = make_desc_sw128(smem + s * kStage), db = make_desc_sw128(smem + s * kStage + kHalf);
+          const uint64_t da = make_desc_sw128(smem + s * F::STAGE), db = make_desc_sw128(smem + s * F::STAGE + F::X_BYTES);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {      // 32 bytes of k each
-            if (I8) umma_i8_pair(tmem + a * BN, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
-            else umma_f16_pair(tmem + a * BN, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+            if (PAIR && I8) umma_i8_pair(tmem + a * BN, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+            else if (PAIR) umma_f16_pair(tmem + a * BN, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+            else if (I8) umma_i8(tmem + a * BN, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
+            else umma_f16(tmem + a * BN, da + 2 * k, db + 2 * k, idesc, (kb | k) != 0);
           }
-          tc_commit_pair(empty0 + 8 * s);
-          if (++s == kStages) { s = 0; par ^= 1; }
+          commit(empty0 + 8 * s);
+          if (++s == F::STAGES) { s = 0; par ^= 1; }
         }
-        if (ok) tc_commit_pair(done0 + 8 * a);
+        if (ok) commit(done0 + 8 * a);
       }
     }
   } else {
     const int quarter = warp & 3;      // of the lanes of tensor memory, this warp's
-    int i = 0;
     bool ok = true;
-    for (int t = first; t < tiles; t += pairs, ++i) {      // (to the end also after a wait that ran out: the warps meet at a barrier)
-      const int a = i & 1, row0 = (t % tiles_m) * 2 * BM + rank * BM + quarter * 32, row = row0 + lane, nt = t / tiles_m, col0 = nt * BN;
+    Tile t;
+    LogStat s{-INFINITY, 0.f, 0.f};
+    for (int i = 0; tile_at<PAIR>(p, i, t); ++i) {      // (to the end also after a wait that ran out: the warps meet at a barrier)
+      const int a = i & 1, row0 = t.mt * F::ROWS + rank * BM + quarter * 32, row = row0 + lane;
       if (I8) {      // (written while others may still read the tile before: two buffers)
         const int j = threadIdx.x - 64;
-        scales[a][j] = p.w_scale[min(col0 + j, p.n - 1)];
-        scales[a][j + 128] = p.w_scale[min(col0 + j + 128, p.n - 1)];
+        scales[a][j] = p.w_scale[min(t.col0 + j, p.n - 1)];
+        scales[a][j + 128] = p.w_scale[min(t.col0 + j + 128, p.n - 1)];
         asm volatile("bar.sync 1, 128;" ::: "memory");
       }
       const bool there = row < p.m;
       const float xs = I8 && there ? p.x_scale[row] : 1.f;
-      const int token = SUMS && there ? p.tokens[row] : -1;
+      const int token = there ? p.tokens[row] : -1;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait(done0 + 8 * a, (i >> 1) & 1, ERR_GEMM_TMEM_FULL_WAIT));
       if (!ok) continue;
       tc_fence_after();
-      LogStat s{-INFINITY, 0.f, 0.f};
+      if (!p.ranges) s = LogStat{-INFINITY, 0.f, 0.f};
 #pragma unroll 1
-      for (int c = 0; c < BN / 32 && row0 < p.m; ++c) {
+      for (int c = 0; c < BN && row0 < p.m; c += kChunk) {
+        const int n0 = t.col0 + c;
+        if (n0 >= t.end) break;
         uint32_t v[32];
-        B2_TMEM_LD_32(tmem + a * BN + c * 32 + ((uint32_t)(quarter * 32) << 16), v);
+        B2_TMEM_LD_32(tmem + a * BN + c + ((uint32_t)(quarter * 32) << 16), v);
         tmem_ld_wait();
-        const int n0 = col0 + c * 32;
-        if (n0 >= p.n) break;
-        if (I8) {
+        float z[32], largest = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = __float_as_uint((float)(int)v[j] * xs * scales[a][c * 32 + j]);
+        for (int j = 0; j < 32; ++j) z[j] = I8 ? (float)(int)v[j] * xs * scales[a][c + j] : __uint_as_float(v[j]);
+        if (n0 + 32 > t.end) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (n0 + j >= t.end) z[j] = -INFINITY;
         }
-        if (SUMS) {
-          float z[32], largest = -INFINITY;
 #pragma unroll
-          for (int j = 0; j < 32; ++j) z[j] = __uint_as_float(v[j]);
-          if (n0 + 32 > p.n) {
+        for (int j = 0; j < 32; ++j) largest = fmaxf(largest, z[j]);
+        add_terms(s, z, largest);
+        if (token >= n0 && token < min(n0 + 32, t.end)) {
+          float mine = z[0];
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (n0 + j >= p.n) z[j] = -INFINITY;
-          }
+          for (int j = 1; j < 32; ++j) mine = token == n0 + j ? z[j] : mine;
+          p.token_z[row] = mine;
+        }
+        if (ALT && there) {
+          p.largest[(long long)row * p.ldc + n0 / kChunk] = largest;
+          float4* dst = reinterpret_cast<float4*>(p.z + row * p.ldz + n0);      // (to the end of the buffer's row: it is a multiple of 32)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) largest = fmaxf(largest, z[j]);
-          add_terms(s, z, largest);
-          if (token >= n0 && token < min(n0 + 32, p.n)) {
-            float mine = z[0];
-#pragma unroll
-            for (int j = 1; j < 32; ++j) mine = token == n0 + j ? z[j] : mine;
-            p.token_z[row] = mine;
-          }
-        } else if (there) {
-          float* dst = p.z + row * p.ldz + n0;
-          if (n0 + 32 <= p.n) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(dst + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (n0 + j < p.n) dst[j] = __uint_as_float(v[j]);
-          }
+          for (int j = 0; j < 8; ++j) dst[j] = make_float4(z[4 * j], z[4 * j + 1], z[4 * j + 2], z[4 * j + 3]);
         }
       }
-      if (SUMS && there) p.part[(long long)nt * p.m + row] = make_float4(s.m, s.s, s.t, 0.f);
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(map_rank0(read0 + 8 * a));
+      if (lane == 0) {
+        if (PAIR) mbar_arrive_cluster(map_rank0(read0 + 8 * a));
+        else mbar_arrive(read0 + 8 * a);
+      }
+      if (there && (!p.ranges || t.col0 + BN >= t.end)) p.part[(long long)t.part * p.m + row] = make_float4(s.m, s.s, s.t, 0.f);
     }
   }
 
-  // every thread of both CTAs arrives here on every path
+  // every thread arrives here on every path
   tc_fence_before();
   __syncthreads();
-  cluster_sync_all();
+  if (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    else tmem_dealloc(tmem, 512);
   }
 }
 
 // ------------------------------------------------------------------ a row's tiles together
-// A CTA takes 32 rows: warp w joins tiles w, w + 32, ... of all of them (a lane a row, so that a warp reads whole lines), then the warps'
-// results are joined in the order of the warps.
-__global__ void __launch_bounds__(1024) score_join_kernel(const float4* __restrict__ part, const float* __restrict__ token_z, const int* __restrict__ tokens, int m,
-                                                          int n, float* __restrict__ logprob, float* __restrict__ entropy) {
-  __shared__ LogStat sh[32][33];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * 32 + lane, tiles = (n + BN - 1) / BN;
+// A CTA takes eight rows: a warp reads four parts of all of them at a time (whole lines), then the lanes' and the warps' results are joined,
+// always in the same order.
+constexpr int kJoinRows = 8, kJoinWarps = 16;
+__global__ void __launch_bounds__(32 * kJoinWarps) score_join_kernel(const float4* __restrict__ part, int parts, const float* __restrict__ token_z,
+                                                                     const int* __restrict__ tokens, int m, int n, float* __restrict__ logprob,
+                                                                     float* __restrict__ entropy) {
+  __shared__ LogStat sh[kJoinWarps][kJoinRows];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * kJoinRows + lane % kJoinRows;
   pdl_wait();
   LogStat s{-INFINITY, 0.f, 0.f};
   if (row < m)
 #pragma unroll 4
-    for (int t = warp; t < tiles; t += 32) {
+    for (int t = warp * 4 + lane / kJoinRows; t < parts; t += 4 * kJoinWarps) {
       const float4 q = part[(long long)t * m + row];
       s = join(s, LogStat{q.x, q.y, q.z});
     }
-  sh[warp][lane] = s;
-  __syncthreads();
 #pragma unroll
-  for (int half = 16; half > 0; half >>= 1) {
-    if (warp < half) sh[warp][lane] = s = join(s, sh[warp + half][lane]);
-    __syncthreads();
-  }
-  if (warp == 0 && row < m) {
-    const LogNorm norm = log_norm(s);
+  for (int o = 16; o >= kJoinRows; o >>= 1)
+    s = join(s, LogStat{__shfl_down_sync(0xffffffffu, s.m, o), __shfl_down_sync(0xffffffffu, s.s, o), __shfl_down_sync(0xffffffffu, s.t, o)});
+  if (lane < kJoinRows) sh[warp][lane] = s;
+  __syncthreads();
+  if (threadIdx.x < kJoinRows && row < m) {
+    LogStat all = sh[0][threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < kJoinWarps; ++w) all = join(all, sh[w][threadIdx.x]);
+    const LogNorm norm = log_norm(all);
     const int t = tokens[row];
     logprob[row] = t >= 0 && t < n ? log_prob(norm, token_z[row]) : NAN;
     entropy[row] = norm.entropy;
+  }
+}
+
+// A CTA takes a row: its parts joined, and the alternatives from the maxima of its chunks and the few chunks that matter.
+constexpr int kAltThreads = 256, kAltWarps = kAltThreads / 32, kAltChunks = 1024;
+__global__ void __launch_bounds__(kAltThreads) score_alternatives_kernel(const float4* __restrict__ part, int parts, const float* __restrict__ token_z,
+                                                                         const int* __restrict__ tokens, int m, int n, const float* __restrict__ z, long long ldz,
+                                                                         const float* __restrict__ largest, int ldc, int top, float* __restrict__ logprob,
+                                                                         float* __restrict__ entropy, int* __restrict__ top_ids, float* __restrict__ top_logprobs) {
+  __shared__ LogStat stat[kAltWarps];
+  __shared__ float best_of[kAltWarps][32];
+  __shared__ unsigned long long lists[kAltWarps][32];
+  __shared__ int count, chosen[kAltChunks];
+  const int row = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, chunks = (n + kChunk - 1) / kChunk;
+  pdl_wait();
+  z += row * ldz;
+  largest += (long long)row * ldc;
+  float best = -INFINITY;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < chunks; i += kAltThreads) best = fmaxf(best, largest[i]);
+  LogStat s{-INFINITY, 0.f, 0.f};
+#pragma unroll 4
+  for (int t = threadIdx.x; t < parts; t += kAltThreads) {
+    const float4 q = part[(long long)t * m + row];
+    s = join(s, LogStat{q.x, q.y, q.z});
+  }
+  const float mine = best;
+  best = sort_lanes(best, lane);
+  best_of[warp][lane] = best;
+  s = join_lanes<32>(s);
+  if (lane == 0) stat[warp] = s;
+  if (threadIdx.x == 0) count = 0;
+  __syncthreads();
+#pragma unroll
+  for (int half = kAltWarps / 2; half > 0; half >>= 1) {
+    if (warp < half) best_of[warp][lane] = best = merge_floats(best, best_of[warp + half][lane], lane);
+    __syncthreads();
+  }
+  // the top-th largest of the threads' maxima: as many logits reach it
+  const float bound = best_of[0][top - 1];
+  if (mine >= bound && mine > -INFINITY)
+#pragma unroll 8
+    for (int i = threadIdx.x; i < chunks; i += kAltThreads) {
+      const float x = largest[i];
+      if (x >= bound && x > -INFINITY) {
+        const int at = atomicAdd(&count, 1);      // (whatever their order, the same logits come out)
+        if (at < kAltChunks) chosen[at] = i;
+      }
+    }
+  __syncthreads();
+  unsigned long long list = 0, last = 0;
+  const bool listed = count <= kAltChunks;      // else (rows of ties) all chunks are looked at again
+  constexpr int kAhead = 4;
+  const int all = listed ? count : chunks;
+  for (int c0 = warp; c0 < all; c0 += kAhead * kAltWarps) {
+    float x[kAhead];
+    int id[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int c = c0 + j * kAltWarps;
+      id[j] = c < all ? (listed ? chosen[c] : c) * kChunk + lane : n;
+      x[j] = id[j] < n ? z[id[j]] : -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) offer(list, last, x[j] >= bound && x[j] > -INFINITY ? logit_key(x[j], id[j]) : 0, top, lane);
+  }
+  lists[warp][lane] = list;
+  __syncthreads();
+#pragma unroll
+  for (int half = kAltWarps / 2; half > 0; half >>= 1) {
+    if (warp < half) lists[warp][lane] = list = merge_lists(list, lists[warp + half][lane], lane);
+    __syncthreads();
+  }
+  if (warp) return;
+  list = fill_list(list, z, n, top, lane);
+  const LogNorm norm = log_norm(join_lanes<kAltWarps>(stat[lane % kAltWarps]));
+  if (lane == 0) {
+    const int t = tokens[row];
+    logprob[row] = t >= 0 && t < n ? log_prob(norm, token_z[row]) : NAN;
+    entropy[row] = norm.entropy;
+  }
+  if (lane < top) {
+    top_ids[(long long)row * top + lane] = list ? (int)key_id(list) : -1;
+    top_logprobs[(long long)row * top + lane] = list ? log_prob(norm, order_value((uint32_t)(list >> 32))) : -INFINITY;
   }
 }
 
@@ -236,6 +390,7 @@ __global__ void __launch_bounds__(1024) score_join_kernel(const float4* __restri
 __global__ void __launch_bounds__(256) quant_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int k, int8_t* __restrict__ q, long long ldq,
                                                     float* __restrict__ scale) {
   __shared__ float part[8];
+  pdl_wait();
   const uint4* row = reinterpret_cast<const uint4*>(x + blockIdx.x * ldx);
   const int vecs = k / 8, tail = k % 8;
   const __nv_bfloat16* end = x + blockIdx.x * ldx + vecs * 8;
@@ -287,13 +442,13 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// 128 rows x 128 bytes of a matrix [rows][cols], rows ld elements apart; what lies outside reads as zeros
-int make_map(CUtensorMap* map, const void* ptr, bool i8, int rows, int cols, long long ld) {
+// box_rows rows x 128 bytes of a matrix [rows][cols], rows ld elements apart; what lies outside reads as zeros
+int make_map(CUtensorMap* map, const void* ptr, bool i8, int rows, int cols, long long ld, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return -100;
   const int size = i8 ? 1 : 2;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * size};
-  const cuuint32_t box[2] = {(cuuint32_t)(kStageRow / size), 128}, step[2] = {1, 1};
+  const cuuint32_t box[2] = {(cuuint32_t)(kStageRow / size), (cuuint32_t)box_rows}, step[2] = {1, 1};
   const CUresult r = fn(map, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, step,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -101 - (int)r;
@@ -307,62 +462,114 @@ int sm_count() {
   return n[dev & 63];
 }
 
-template <bool I8, bool SUMS>
-int launch(const CUtensorMap& mx, const CUtensorMap& mw, const ScoreParams& p, int tiles, cudaStream_t st) {
+// How a product is laid out: CTAs by themselves or pairs, ranges of columns or tiles in turn, parts of a row.
+struct Layout {
+  bool pair;
+  int ranges, parts, clusters;
+};
+int layout_of(int m, int n, Layout& l) {
+  if (m < 1 || n < 1 || n > 0x7fff0000) return -1;
+  l.pair = m > 3 * BM || (m > BM && m <= 2 * BM);
+  const int tiles_m = (m - 1) / (l.pair ? 2 * BM : BM) + 1, tiles_n = (n + BN - 1) / BN, at_once = l.pair ? sm_count() / 2 : sm_count();
+  l.ranges = m <= kRangeRows ? min(max(1, at_once / tiles_m), (n + kGrain - 1) / kGrain) : 0;
+  l.parts = l.ranges ? l.ranges : tiles_n;
+  if ((long long)tiles_m * l.parts > 0x3fffffff) return -1;
+  l.clusters = l.ranges ? tiles_m * l.ranges : min(tiles_m * tiles_n, at_once);
+  return 0;
+}
+
+template <bool I8, bool ALT, bool PAIR>
+int launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mg, const ScoreParams& p, int clusters, cudaStream_t st) {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(score_kernel<I8, SUMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    const cudaError_t e = cudaFuncSetAttribute(score_kernel<I8, ALT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<PAIR>::SMEM);
     if (e != cudaSuccess) return (int)e;
     configured[dev & 63] = true;
   }
-  score_kernel<I8, SUMS><<<2 * min(tiles, sm_count() / 2), kThreads, kSmem, st>>>(mx, mw, p);
-  return (int)cudaGetLastError();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(PAIR ? 2 * clusters : clusters);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Form<PAIR>::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = PAIR ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, score_kernel<I8, ALT, PAIR>, mx, mw, mg, p);
+}
+template <bool I8, bool ALT>
+int launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mg, const ScoreParams& p, const Layout& l, cudaStream_t st) {
+  return l.pair ? launch<I8, ALT, true>(mx, mw, mg, p, l.clusters, st) : launch<I8, ALT, false>(mx, mw, mg, p, l.clusters, st);
 }
 
-int run(const void* x, long long ldx, const void* w, long long ldw, bool i8, int k, ScoreParams& p, bool sums, cudaStream_t st) {
-  const int size = i8 ? 1 : 2;
-  const long long tiles = (long long)((p.m + 2 * BM - 1) / (2 * BM)) * ((p.n + BN - 1) / BN);
-  if (p.m < 1 || p.n < 1 || (long long)k * size < kStageRow || ldx < k || ldw < k || tiles > 0x3fffffff || (i8 && (!p.x_scale || !p.w_scale))) return -1;
-  if (((uintptr_t)x | (uintptr_t)w | (unsigned long long)(ldx * size) | (unsigned long long)(ldw * size)) & 15) return -3;
-  p.kb = (int)(((long long)k * size + kStageRow - 1) / kStageRow);
-  CUtensorMap mx, mw;
-  int rc = make_map(&mx, x, i8, p.m, k, ldx);
-  if (!rc) rc = make_map(&mw, w, i8, p.n, k, ldw);
-  if (rc) return rc;
-  if (sums) return i8 ? launch<true, true>(mx, mw, p, (int)tiles, st) : launch<false, true>(mx, mw, p, (int)tiles, st);
-  return i8 ? launch<true, false>(mx, mw, p, (int)tiles, st) : launch<false, false>(mx, mw, p, (int)tiles, st);
+// The workspace of a call, in floats from its beginning: sums, tokens' logits; alternatives: logits and their maxima; int8: rows and scales.
+struct Room {
+  long long token_z, z, largest, scale, q, all;
+  int chunks, ldq;
+};
+Room room_of(const Layout& l, int m, int n, int k, int top, bool i8) {
+  const auto lines = [](long long floats) { return (floats + 31) / 32 * 32; };
+  Room r;
+  r.chunks = (n + kChunk - 1) / kChunk;
+  r.ldq = (k + 15) / 16 * 16;
+  r.token_z = 4ll * l.parts * m;
+  r.z = lines(r.token_z + m);
+  r.largest = r.z + (top ? (long long)r.chunks * kChunk * m : 0);
+  r.scale = lines(r.largest + (top ? (long long)r.chunks * m : 0));
+  r.q = lines(r.scale + (i8 ? m : 0));
+  r.all = r.q + (i8 ? (long long)r.ldq / 4 * m : 0);
+  return r;
 }
-
 }  // namespace
 
-// Rows x [m][k] against the head w [n][k], both bf16, or int8 with scales; rows are ldx and ldw elements apart, multiples of 16 bytes, of
-// 128 bytes at least.
-// Logits z [m][ldz], ldz a multiple of 4.
-extern "C" int b2_score_logits(const void* x, long long ldx, const void* w, long long ldw, int i8, const float* x_scale, const float* w_scale, int m, int n,
-                               int k, float* z, long long ldz, void* stream) {
-  if (ldz < n || (((uintptr_t)z | (unsigned long long)(ldz * 4)) & 15)) return -2;
-  ScoreParams p{m, n, 0, x_scale, w_scale, z, ldz, nullptr, nullptr, nullptr};
-  return run(x, ldx, w, ldw, i8 != 0, k, p, false, (cudaStream_t)stream);
+// Floats of workspace for m rows of k against n columns (-1: sizes that are refused): `work`, of one call at a time, 16-byte aligned.
+extern "C" long long b2_score_work(int m, int n, int k, int top, int i8) {
+  Layout l;
+  return layout_of(m, n, l) || k < 1 || k > 0x7fffff00 ? -1 : room_of(l, m, n, k, top, i8 != 0).all;
 }
-// Log probabilities of the rows' tokens and entropies.  work: b2_score_work(m, n) floats, 16-byte aligned, of this call alone.
-extern "C" long long b2_score_work(int m, int n) { return ((long long)((n + BN - 1) / BN) * 4 + 1) * m; }
-extern "C" int b2_score_tokens(const void* x, long long ldx, const void* w, long long ldw, int i8, const float* x_scale, const float* w_scale, int m, int n,
-                               int k, const int* tokens, float* work, float* logprob, float* entropy, void* stream) {
-  if ((uintptr_t)work & 15) return -2;
-  float* token_z = work + (long long)((n + BN - 1) / BN) * 4 * m;
-  ScoreParams p{m, n, 0, x_scale, w_scale, nullptr, 0, tokens, (float4*)work, token_z};
-  const int rc = run(x, ldx, w, ldw, i8 != 0, k, p, true, (cudaStream_t)stream);
+// Log probabilities of the tokens of bf16 rows x [m][k] against the head w [n][k], entropies and alternatives.  The head is bf16, or int8 (w_scale: of its
+// rows), for which the rows are quantised too.  Rows are ldx and ldw elements apart, multiples of 16 bytes, and those of the head of 128 bytes at least.
+extern "C" int b2_score(const void* x, long long ldx, const void* w, long long ldw, const float* w_scale, int m, int n, int k, const int* tokens, int top,
+                        float* work, float* logprob, float* entropy, int* top_ids, float* top_logprobs, void* stream) {
+  const bool i8 = w_scale != nullptr;
+  const int size = i8 ? 1 : 2;
+  Layout l;
+  if (layout_of(m, n, l) || (long long)k * size < kStageRow || k > 0x7fffff00 || ldx < k || ldw < k || top < 0 || top > kMaxTop) return -1;
+  if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)work | (unsigned long long)(ldx * 2) | (unsigned long long)(ldw * size)) & 15) return -3;
+  const Room r = room_of(l, m, n, k, top, i8);
+  cudaStream_t st = (cudaStream_t)stream;
+  ScoreParams p{};
+  p.m = m; p.n = n; p.kb = (int)(((long long)k * size + kStageRow - 1) / kStageRow);
+  p.ranges = l.ranges;
+  p.x_scale = work + r.scale; p.w_scale = w_scale; p.tokens = tokens;
+  p.part = (float4*)work; p.token_z = work + r.token_z;
+  p.z = work + r.z; p.ldz = (long long)r.chunks * kChunk;
+  p.largest = work + r.largest; p.ldc = r.chunks;
+  void* q = work + r.q;
+  CUtensorMap mx, mw, mg;
+  int rc = i8 ? make_map(&mx, q, true, m, k, r.ldq, BM) : make_map(&mx, x, false, m, k, ldx, BM);
+  if (!rc) rc = make_map(&mw, w, i8, n, k, ldw, l.pair ? BN / 2 : BN);
+  mg = mw;
+  if (!rc && l.ranges) rc = make_map(&mg, w, i8, n, k, ldw, l.pair ? kGrain / 2 : kGrain);
   if (rc) return rc;
-  return b2_launch(score_join_kernel, dim3((m + 31) / 32), dim3(1024), 0, (cudaStream_t)stream, true, (const float4*)work, token_z, tokens, m, n, logprob, entropy);
-}
-
-// Rows x [m][k] bf16 (16-byte aligned, ldx a multiple of 8) as int8 q [m][ldq] (16-byte aligned, ldq a multiple of 16) and scales.
-extern "C" int b2_score_quant(const void* x, long long ldx, int m, int k, void* q, long long ldq, float* scale, void* stream) {
-  if (m < 1 || k < 1 || ldx < k || ldq < k || ((uintptr_t)x | (uintptr_t)q | (unsigned long long)(ldx * 2) | (unsigned long long)ldq) & 15) return -1;
-  quant_kernel<<<m, 256, 0, (cudaStream_t)stream>>>((const __nv_bfloat16*)x, ldx, k, (int8_t*)q, ldq, scale);
-  return (int)cudaGetLastError();
+  if (i8) {
+    rc = b2_launch(quant_kernel, dim3(m), dim3(256), 0, st, true, (const __nv_bfloat16*)x, ldx, k, (int8_t*)q, (long long)r.ldq, work + r.scale);
+    if (rc) return rc;
+  }
+  if (top) rc = i8 ? launch<true, true>(mx, mw, mg, p, l, st) : launch<false, true>(mx, mw, mg, p, l, st);
+  else rc = i8 ? launch<true, false>(mx, mw, mg, p, l, st) : launch<false, false>(mx, mw, mg, p, l, st);
+  if (rc) return rc;
+  if (top)
+    return b2_launch(score_alternatives_kernel, dim3(m), dim3(kAltThreads), 0, st, true, p.part, l.parts, p.token_z, tokens, m, n, p.z, p.ldz, p.largest, p.ldc,
+                     top, logprob, entropy, top_ids, top_logprobs);
+  return b2_launch(score_join_kernel, dim3((m + kJoinRows - 1) / kJoinRows), dim3(32 * kJoinWarps), 0, st, true, p.part, l.parts, p.token_z, tokens, m, n,
+                   logprob, entropy);
 }
 
 B2_DEFINE_STATUS(score)

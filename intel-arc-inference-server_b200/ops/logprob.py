@@ -24,7 +24,7 @@ import torch
 from . import lib as K
 
 MAX_TOP = 32           # alternatives a row can have
-SLAB_ELEMS = 80 << 20  # logits that ``score`` with alternatives keeps at a time
+SLAB_ELEMS = 160 << 20 # logits that ``score`` with alternatives keeps at a time
 
 
 @dataclass(frozen=True)
@@ -70,21 +70,19 @@ def _check_tokens(tokens: torch.Tensor, m: int, device):
         raise ValueError(f"tokens: {m} contiguous int32 ids on {device}")
 
 
-def _rows_of(t: torch.Tensor, dtype, what: str, align: int = 1):
-    if t.dim() != 2 or t.dtype != dtype or t.device.type != "cuda" or t.shape[1] > 1 and t.stride(1) != 1:
+def _rows_of(t: torch.Tensor, dtype, what: str, align: int = 4):
+    m, n = t.shape if t.dim() == 2 else (0, 0)
+    if t.dim() != 2 or t.dtype != dtype or not t.is_cuda or n > 1 and t.stride(1) != 1:
         raise ValueError(f"{what}: rows of {dtype} on a CUDA device, one element after another")
-    if t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+    if m > 1 and t.stride(0) < n:
         raise ValueError(f"{what}: rows that do not overlap")
-    if align > 1 and (t.data_ptr() % align or t.shape[0] > 1 and t.stride(0) * t.element_size() % align):
+    if t.data_ptr() % align or m > 1 and t.stride(0) * t.element_size() % align:
         raise ValueError(f"{what}: rows begin at multiples of {align} bytes")
 
 
-def _ld(t: torch.Tensor, align: int = 1) -> int:
-    """Elements from row to row; a lone row's stride says nothing."""
-    if t.shape[0] > 1:
-        return t.stride(0)
-    step = max(1, align // t.element_size())
-    return (t.shape[1] + step - 1) // step * step
+def _ld(t: torch.Tensor) -> int:
+    """Elements from row to row; a lone row's stride says nothing: a multiple of 16 bytes that holds it."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 @functools.lru_cache(maxsize=None)
@@ -125,26 +123,23 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int
     return out
 
 
-def _score(x, w, i8: bool, x_scale, w_scale, tokens, out: Logprobs):
+def _score(x, w, w_scale, tokens, out: Logprobs) -> Logprobs:
     m, k = x.shape
-    n = w.shape[0]
-    ws = None if w_scale is None else w_scale.data_ptr()
-    if not out.top_ids.shape[1]:
-        work = torch.empty(_entry("b2_score_work", "ii", ctypes.c_longlong)(m, n), dtype=torch.float32, device=x.device)
-        K._check(_entry("b2_score_tokens", "plplippiiippppp")(
-            x.data_ptr(), _ld(x, 16), w.data_ptr(), _ld(w, 16), int(i8), None if x_scale is None else x_scale.data_ptr(), ws, m, n, k, tokens.data_ptr(),
-            work.data_ptr(), out.logprob.data_ptr(), out.entropy.data_ptr(), _stream(x.device)), "score_tokens")
-        K.launch_count += 1      # the rows' tiles joined
-        return out
-    ldz = (n + 3) // 4 * 4
-    step = max(1, min(m, max(256, SLAB_ELEMS // ldz // 256 * 256)))
-    z = torch.empty(step, ldz, dtype=torch.float32, device=x.device)
-    for i in range(0, m, step):
-        c = min(step, m - i)
-        K._check(_entry("b2_score_logits", "plplippiiiplp")(
-            x[i:].data_ptr(), _ld(x, 16), w.data_ptr(), _ld(w, 16), int(i8), None if x_scale is None else x_scale[i:].data_ptr(), ws, c, n, k, z.data_ptr(),
-            ldz, _stream(x.device)), "score_logits")
-        token_logprobs(z[:c, :n], tokens[i: i + c], out=out.rows(i, i + c))
+    n, top, i8 = w.shape[0], out.top_ids.shape[1], w_scale is not None
+    dev, ldx, ldw = x.device, _ld(x), _ld(w)
+    room, run = _entry("b2_score_work", "iiiii", ctypes.c_longlong), _entry("b2_score", "plplpiiipipppppp")
+    step = m if not top else min(m, max(256, SLAB_ELEMS // n // 256 * 256))
+    need = room(step, n, k, top, i8)
+    if m % step:
+        need = max(need, room(m % step, n, k, top, i8))
+    with _on(dev):
+        work = torch.empty(need, dtype=torch.float32, device=dev)
+        for i in range(0, m, step):
+            c = min(step, m - i)
+            o = out if c == m else out.rows(i, i + c)
+            K._check(run(x.data_ptr() + 2 * i * ldx, ldx, w.data_ptr(), ldw, w_scale.data_ptr() if i8 else None, c, n, k, tokens.data_ptr() + 4 * i, top,
+                         work.data_ptr(), o.logprob.data_ptr(), o.entropy.data_ptr(), o.top_ids.data_ptr(), o.top_logprobs.data_ptr(), _stream(dev)), "score")
+            K.launch_count += 2 if i8 else 1      # rows quantised; a row's parts joined
     return out
 
 
@@ -161,12 +156,10 @@ def score(x: torch.Tensor, head: torch.Tensor, tokens: torch.Tensor, top: Option
     ``x @ head.T`` in fp32."""
     _rows_of(x, torch.bfloat16, "rows", 16)
     _check_head(x, head, torch.bfloat16)
-    _check_tokens(tokens, x.shape[0], x.device)
-    out = _results(x.shape[0], top, out, x.device)
-    if x.shape[0]:
-        with _on(x.device):
-            _score(x, head, False, None, None, tokens, out)
-    return out
+    m, dev = x.shape[0], x.device
+    _check_tokens(tokens, m, dev)
+    out = _results(m, top, out, dev)
+    return _score(x, head, None, tokens, out) if m else out
 
 
 def score_i8(x: torch.Tensor, head: tuple, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
@@ -175,16 +168,9 @@ def score_i8(x: torch.Tensor, head: tuple, tokens: torch.Tensor, top: Optional[i
     w8, scale = head
     _rows_of(x, torch.bfloat16, "rows", 16)
     _check_head(x, w8, torch.int8)
-    m, k = x.shape
-    if scale.dtype != torch.float32 or scale.shape != (w8.shape[0],) or scale.device != x.device or not scale.is_contiguous():
-        raise ValueError(f"scales of the head: {w8.shape[0]} contiguous fp32 numbers on {x.device}")
-    _check_tokens(tokens, m, x.device)
-    out = _results(m, top, out, x.device)
-    if m:
-        with _on(x.device):
-            q = torch.empty(m, (k + 15) // 16 * 16, dtype=torch.int8, device=x.device)
-            s = torch.empty(m, dtype=torch.float32, device=x.device)
-            K._check(_entry("b2_score_quant", "pliiplpp")(x.data_ptr(), _ld(x, 16), m, k, q.data_ptr(), q.shape[1], s.data_ptr(), _stream(x.device)),
-                     "score_quant")
-            _score(q[:, :k], w8, True, s, scale, tokens, out)
-    return out
+    m, dev = x.shape[0], x.device
+    if scale.dtype != torch.float32 or scale.shape != (w8.shape[0],) or scale.device != dev or not scale.is_contiguous():
+        raise ValueError(f"scales of the head: {w8.shape[0]} contiguous fp32 numbers on {dev}")
+    _check_tokens(tokens, m, dev)
+    out = _results(m, top, out, dev)
+    return _score(x, w8, scale, tokens, out) if m else out

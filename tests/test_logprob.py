@@ -266,7 +266,7 @@ def grid(shape, seed, steps, scale):
 
 
 @gpu
-@pytest.mark.parametrize("m", [1, 3, 127, 129, 256, 257, 700])
+@pytest.mark.parametrize("m", [1, 3, 127, 128, 129, 256, 257, 512, 513, 700])
 @pytest.mark.parametrize("n,k,top", [(1, 64, 0), (5, 72, 8), (255, 64, 0), (257, 200, 3), (1000, 512, 0), (2051, 136, 32), (20000, 384, 0)])
 def test_score(m, n, k, top):
     x, w = grid((m, k), m + n, 12, 1 / 16), grid((n, k), m + n + 1, 20, 1 / 64)
@@ -278,7 +278,7 @@ def test_score(m, n, k, top):
 
 
 @gpu
-@pytest.mark.parametrize("m", [1, 130, 300])
+@pytest.mark.parametrize("m", [1, 100, 130, 300, 600])
 @pytest.mark.parametrize("n,k,top", [(3, 128, 2), (257, 200, 0), (1000, 512, 5), (20003, 144, 0)])
 def test_score_i8(m, n, k, top):
     g = torch.Generator(device="cuda").manual_seed(m + n)
