@@ -22,6 +22,7 @@ from typing import Dict, List, Optional
 import torch
 
 from ..ops import lib as K
+from ..ops import logprob as LP
 from .config import ModelConfig, SandwichBlock
 from .oracle import rope_tables
 from .weights import ModelWeights, LayerWeights, QLinear
@@ -690,10 +691,10 @@ class DecoderModel:
                                 **ll.experts(scratch, spec.ffn, lw.moe, m))
         return resid
 
-    def listed_logits(self, final, sel, n: int, scratch, logits):
-        """Head of rows ``sel[:n]`` (None: rows 0..n - 1) of what ``listed_walk`` returned into ``logits[:n]``."""
+    def listed_rows(self, final, sel, n: int, scratch):
+        """What the head reads of rows ``sel[:n]`` (None: rows 0..n - 1) of what ``listed_walk`` returned."""
         from ..ops import latent as L
-        ll, cfg, b = self.listed, self.cfg, self.buf
+        ll, cfg = self.listed, self.cfg
         if self.streams is None:
             x = scratch.get("head_x", n, ll.wp)
             L.layer_norm_rows(final, sel, self.w.final_norm, cfg.rms_eps, n, cfg.hidden, x)
@@ -702,6 +703,13 @@ class DecoderModel:
         else:                   # rows by index, the same kernel as an embedding
             x = scratch.get("head_x", n, ll.wp)
             L.embed_rows(final, sel, n, scratch.get("head_x32", n, ll.wp, torch.float32), x, self.buf.flag)
+        return x
+
+    def listed_logits(self, final, sel, n: int, scratch, logits):
+        """Head of rows ``sel[:n]`` (None: rows 0..n - 1) of what ``listed_walk`` returned into ``logits[:n]``."""
+        from ..ops import latent as L
+        ll, cfg, b = self.listed, self.cfg, self.buf
+        x = self.listed_rows(final, sel, n, scratch)
         if ll.f32:
             L.linear_f32(x, self.w.lm_head, logits, n)
             L.row_argmax(logits, n, cfg.vocab, b.cand_val, b.cand_idx)
@@ -747,6 +755,28 @@ class DecoderModel:
                                self.tp.mcap)
         else:
             K.argmax_finish(b.cand_val, b.cand_idx, b.ncand, m, ctrl, advance)
+
+    def score_rows(self, x, tokens, out, int8: bool = False):
+        """Log probabilities of a prompt's rows ``x`` behind the final norm, any number of them (``ops.logprob.Logprobs``).  The head is the one
+        that decodes: bf16 without stored logits; of an int8 head the 8-bit product where the prompt pass is one too (``int8``), else --
+        and in 32-bit -- the logits of a step's rows at a time (``buf.logits``)."""
+        b, cfg = self.buf, self.cfg
+        f32 = self.listed is not None and self.listed.f32
+        if not f32 and not self.int8_head:
+            LP.score(x, self.w.lm_head, tokens, out=out)
+        elif not f32 and int8:
+            LP.score_i8(x, self.w.lm_head_i8, tokens, out=out)
+        else:
+            from ..ops import latent as L
+            for c0 in range(0, x.shape[0], b.max_rows):
+                part = x[c0: c0 + b.max_rows]
+                n = part.shape[0]
+                if f32:
+                    L.linear_f32(part, self.w.lm_head, b.logits, n)
+                else:
+                    w8, sc = self.w.lm_head_i8
+                    K.head_gemv(w8, part, b.logits, n, self.head_rows, cfg.hidden, b.cand_val, b.cand_idx, wscale=sc)
+                LP.token_logprobs(b.logits[:n], tokens[c0: c0 + n], out=out.rows(c0, c0 + n))
 
     def _head_nccl(self, m: int, ctrl, advance: bool):
         """Comparison path of the vocabulary-parallel arg-max: local arg-max, NCCL all-gather, torch merge."""

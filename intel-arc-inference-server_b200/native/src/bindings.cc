@@ -388,7 +388,10 @@ PYBIND11_MODULE(b200host, m) {
       .def_readonly("temperature", &ChatRequest::temperature)
       .def_readonly("top_k", &ChatRequest::top_k)
       .def_readonly("top_p", &ChatRequest::top_p)
-      .def_readonly("repetition_penalty", &ChatRequest::repetition_penalty);
+      .def_readonly("repetition_penalty", &ChatRequest::repetition_penalty)
+      .def_readonly("logprobs", &ChatRequest::logprobs)
+      .def_readonly("echo", &ChatRequest::echo)
+      .def_readonly("score_only", &ChatRequest::score_only);
   m.def("parse_request", &parse_request, py::arg("body"), py::arg("chat"));
   m.def("error_body", &error_body);
   m.def("models_response", &models_response);
@@ -396,16 +399,20 @@ PYBIND11_MODULE(b200host, m) {
         [](const ChatRequest& req, const std::string& id, int64_t created, const std::string& model,
            const std::string& content, const std::string& reasoning, const py::list& calls,
            const std::string& finish_reason, int prompt_tokens, int completion_tokens, int cached_tokens,
-           const std::vector<uint32_t>& token_ids) {
+           const std::vector<uint32_t>& token_ids, const py::object& logprobs) {
           std::vector<ToolCall> cs;
           for (auto c : calls) cs.push_back(call_from_py(c.cast<py::dict>()));
           Usage u{prompt_tokens, completion_tokens, cached_tokens};
-          return completion_response(req, id, created, model, content, reasoning, cs, finish_reason, u, token_ids);
-        });
+          return completion_response(req, id, created, model, content, reasoning, cs, finish_reason, u, token_ids, from_py(logprobs));
+        },
+        py::arg("req"), py::arg("id"), py::arg("created"), py::arg("model"), py::arg("content"), py::arg("reasoning"), py::arg("calls"),
+        py::arg("finish_reason"), py::arg("prompt_tokens"), py::arg("completion_tokens"), py::arg("cached_tokens"), py::arg("token_ids"),
+        py::arg("logprobs") = py::none());
   m.def("stream_frame",
         [](const ChatRequest& req, const std::string& id, int64_t created, const std::string& model,
            const std::string& kind, const std::string& text, const py::object& call, uint32_t call_index,
-           const std::string& finish_reason, const py::object& usage, const std::vector<uint32_t>& token_ids) {
+           const std::string& finish_reason, const py::object& usage, const std::vector<uint32_t>& token_ids,
+           const py::object& logprobs) {
           static const std::map<std::string, int> kinds{{"role", 0}, {"content", 1}, {"reasoning", 2},
                                                         {"call", 3},  {"finish", 4},  {"usage", 5}};
           ToolCall tc;
@@ -418,11 +425,11 @@ PYBIND11_MODULE(b200host, m) {
             u = Usage{t[0].cast<int>(), t[1].cast<int>(), t[2].cast<int>()};
           }
           return stream_frame(req, id, created, model, kinds.at(kind), text, has_call ? &tc : nullptr, call_index,
-                              finish_reason, has_usage ? &u : nullptr, token_ids.empty() ? nullptr : &token_ids);
+                              finish_reason, has_usage ? &u : nullptr, token_ids.empty() ? nullptr : &token_ids, from_py(logprobs));
         },
         py::arg("req"), py::arg("id"), py::arg("created"), py::arg("model"), py::arg("kind"), py::arg("text") = "",
         py::arg("call") = py::none(), py::arg("call_index") = 0, py::arg("finish_reason") = "",
-        py::arg("usage") = py::none(), py::arg("token_ids") = std::vector<uint32_t>());
+        py::arg("usage") = py::none(), py::arg("token_ids") = std::vector<uint32_t>(), py::arg("logprobs") = py::none());
   py::class_<StopMatcher>(m, "StopMatcher")
       .def(py::init<std::vector<std::string>>())
       .def("push",

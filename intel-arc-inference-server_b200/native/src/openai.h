@@ -4,7 +4,7 @@
 // max_tokens (or max_completion_tokens), min_tokens, ignore_eos, stream,
 // stream_options.include_usage, stop (string or list), return_token_ids, seed, temperature
 // (absent = greedy), top_k, top_p, repetition_penalty, tools, chat_template_kwargs,
-// reasoning_effort; responses carry reasoning_content, tool_calls, finish_reason in
+// reasoning_effort, and (beyond the reference) logprobs / top_logprobs and, for completions, echo with max_tokens 0; responses carry reasoning_content, tool_calls, finish_reason in
 // {stop, length, tool_calls} and usage.prompt_tokens_details.cached_tokens.  A malformed request
 // raises BadRequest, which the server answers with an OpenAI error body and status 400.
 #pragma once
@@ -43,7 +43,12 @@ struct ChatRequest {
   int top_k = 0;
   double top_p = 1.0;
   double repetition_penalty = 1.0;
+  int logprobs = -1;           // alternatives reported with every token's log probability; -1: no log probabilities
+  bool echo = false;           // completions: the prompt comes back ahead of what is generated
+  bool score_only = false;     // max_tokens 0 beside echo: nothing is generated
 };
+
+constexpr int kMaxLogprobs = 20;
 
 inline std::string error_body(const std::string& message, const std::string& type, int code) {
   Json e = Json::object();
@@ -97,7 +102,10 @@ inline ChatRequest parse_request(const std::string& body, bool chat) {
     } else if (p->is_array() && p->size() == 1 && (*p)[0].is_string()) r.prompt = (*p)[0].as_string();
     else throw BadRequest("prompt must be a string or a list of token ids");
   }
-  r.max_tokens = (int)num("max_tokens", 1, 1e9, 0);
+  if (!chat) r.echo = boolean("echo", false);
+  const Json* mt = j.find("max_tokens");
+  r.score_only = r.echo && mt && mt->is_number() && mt->as_double() == 0.0;
+  r.max_tokens = r.score_only ? 1 : (int)num("max_tokens", 1, 1e9, 0);
   if (r.max_tokens == 0) r.max_tokens = (int)num("max_completion_tokens", 1, 1e9, 0);
   r.min_tokens = (int)num("min_tokens", 0, 1e9, 0);
   r.ignore_eos = boolean("ignore_eos", false);
@@ -131,6 +139,21 @@ inline ChatRequest parse_request(const std::string& body, bool chat) {
   r.top_p = num("top_p", 0.0, 1.0, 1.0);
   if (r.top_p <= 0.0) throw BadRequest("top_p must be in (0, 1]");
   r.repetition_penalty = num("repetition_penalty", 0.01, 100.0, 1.0);
+  const auto alternatives = [&](const char* k) {
+    const Json* v = j.find(k);
+    if (!v || v->is_null()) return 0;
+    if (!v->is_int() || v->as_int() < 0 || v->as_int() > kMaxLogprobs)
+      throw BadRequest(std::string(k) + " must be an integer from 0 to " + std::to_string(kMaxLogprobs));
+    return (int)v->as_int();
+  };
+  // chat: a truth value, and how many alternatives beside it; completions: the number (or a truth value, without alternatives)
+  if (const Json* lp = j.find("logprobs")) {
+    if (chat || lp->is_bool()) {
+      if (boolean("logprobs", false)) r.logprobs = chat ? alternatives("top_logprobs") : 0;
+    } else if (!lp->is_null()) {
+      r.logprobs = alternatives("logprobs");
+    }
+  }
   if (const Json* t = j.find("tools")) {
     if (t->is_array() && t->size() > 0) r.tools = *t;
     else if (!t->is_null() && !t->is_array()) throw BadRequest("tools must be an array");
@@ -181,7 +204,7 @@ inline std::string completion_response(const ChatRequest& req, const std::string
                                        const std::string& model, const std::string& content,
                                        const std::string& reasoning, const std::vector<ToolCall>& calls,
                                        const std::string& finish_reason, const Usage& usage,
-                                       const std::vector<uint32_t>& token_ids) {
+                                       const std::vector<uint32_t>& token_ids, const Json& logprobs = Json()) {
   Json j = Json::object();
   j["id"] = id;
   j["object"] = req.chat ? "chat.completion" : "text_completion";
@@ -204,6 +227,7 @@ inline std::string completion_response(const ChatRequest& req, const std::string
     for (uint32_t t : token_ids) ids.push_back(Json(t));
     choice["token_ids"] = ids;
   }
+  if (!logprobs.is_null()) choice["logprobs"] = logprobs;
   choice["finish_reason"] = finish_reason;
   Json choices = Json::array();
   choices.push_back(choice);
@@ -217,7 +241,7 @@ inline std::string completion_response(const ChatRequest& req, const std::string
 inline std::string stream_frame(const ChatRequest& req, const std::string& id, int64_t created,
                                 const std::string& model, int kind, const std::string& text,
                                 const ToolCall* call, uint32_t call_index, const std::string& finish_reason,
-                                const Usage* usage, const std::vector<uint32_t>* token_ids) {
+                                const Usage* usage, const std::vector<uint32_t>* token_ids, const Json& logprobs = Json()) {
   Json j = Json::object();
   j["id"] = id;
   j["object"] = req.chat ? "chat.completion.chunk" : "text_completion";
@@ -244,6 +268,7 @@ inline std::string stream_frame(const ChatRequest& req, const std::string& id, i
       for (uint32_t t : *token_ids) ids.push_back(Json(t));
       choice["token_ids"] = ids;
     }
+    if (!logprobs.is_null()) choice["logprobs"] = logprobs;
     choice["finish_reason"] = kind == 4 ? Json(finish_reason) : Json();
     choices.push_back(choice);
   }

@@ -129,11 +129,18 @@ def _score(x, w, w_scale, tokens, out: Logprobs) -> Logprobs:
     dev, ldx, ldw = x.device, _ld(x), _ld(w)
     room, run = _entry("b2_score_work", "iiiii", ctypes.c_longlong), _entry("b2_score", "plplpiiipipppppp")
     step = m if not top else min(m, max(256, SLAB_ELEMS // n // 256 * 256))
-    need = room(step, n, k, top, i8)
-    if m % step:
-        need = max(need, room(m % step, n, k, top, i8))
     with _on(dev):
-        work = torch.empty(need, dtype=torch.float32, device=dev)
+        while True:
+            need = room(step, n, k, top, i8)
+            if m % step:
+                need = max(need, room(m % step, n, k, top, i8))
+            try:
+                work = torch.empty(need, dtype=torch.float32, device=dev)
+                break
+            except torch.OutOfMemoryError:
+                if step <= 256 or not top:
+                    raise
+                step = max(256, step // 512 * 256)      # fewer logits at a time
         for i in range(0, m, step):
             c = min(step, m - i)
             o = out if c == m else out.rows(i, i + c)

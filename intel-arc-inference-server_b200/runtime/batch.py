@@ -242,7 +242,7 @@ class BatchRunner:
                     for r in rows:
                         out[r].copy_(lg[i])
 
-    def prefill(self, slot: int, ids: List[int], chunk: Optional[int] = None) -> int:
+    def prefill(self, slot: int, ids: List[int], chunk: Optional[int] = None, scores=None) -> int:
         """``Engine.prefill``: portions of at most ``chunk`` tokens; the last row's logits go to ``buf.logits[0]``."""
         eng, m = self.eng, self.eng.model
         chunk = min(chunk or self.max_tokens, self.max_tokens)
@@ -250,6 +250,8 @@ class BatchRunner:
             part = ids[c0: c0 + chunk]
             last = c0 + chunk >= len(ids)
             final, sel = self._walk([(slot, part)], [(0, len(part) - 1)] if last else [])
+            if scores is not None:
+                m.score_rows(m.listed_rows(final, None, len(part), self.scratch), *scores.take(len(part)))
         m.listed_logits(final, sel, 1, self.scratch, m.buf.logits)
         K.argmax_finish(m.buf.cand_val, m.buf.cand_idx, m.buf.ncand, 1, eng.ctrl, False)
         return eng._read_out(1)[0]

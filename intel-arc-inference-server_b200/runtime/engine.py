@@ -21,9 +21,11 @@ from ..models.config import ModelConfig
 from ..models.decoder import DecoderModel, KVCache, attn_splits
 from ..models.weights import ModelWeights
 from ..ops import lib as K
+from ..ops import logprob as LP
 from ..utils.graphs import capture
 from ..utils.staging import Staged
 from .kv_pool import KvPool
+from .scoring import PromptScores, ScoreBuffer, TokenScore
 
 PAGE = 16
 
@@ -366,14 +368,28 @@ class Engine:
             self._batch = BatchRunner(self)
         return self._batch
 
-    def prefill(self, slot: int, ids: Sequence[int], chunk: Optional[int] = None) -> int:
-        """Ingest ``ids`` after the slot's current length; returns the greedy next token."""
+    @property
+    def can_score(self) -> bool:
+        """``prefill`` takes ``scores``: one GPU holds the whole model."""
+        return self.tp is None and self.model.nccl is None and type(self).prefill is Engine.prefill
+
+    def prompt_scores(self, ids: Sequence[int], top: int = 0) -> PromptScores:
+        """What ``prefill`` fills with the log probabilities of a prompt's tokens as it goes (the ``scores`` of every portion)."""
+        return PromptScores(ids, top, self.device)
+
+    def prefill(self, slot: int, ids: Sequence[int], chunk: Optional[int] = None, scores: Optional[PromptScores] = None) -> int:
+        """Ingest ``ids`` after the slot's current length; returns the greedy next token.  ``scores``: the next ``len(ids)`` tokens of this
+        prompt get their log probabilities."""
         self.require_ok()
         ids = list(ids)
+        if scores is not None:
+            if not self.can_score:
+                raise ValueError("log probabilities of a prompt are not available for a model spread over several GPUs")
+            scores.expect(ids)
         if self.mixed_batches and len(ids) > self.max_rows:
             self.last_prefill_row = 0
             self._snap = None
-            return self._batch_runner().prefill(slot, ids, chunk)
+            return self._batch_runner().prefill(slot, ids, chunk, scores)
         if self._use_tc_prefill(len(ids)):
             if self._prefill is None:
                 if self.tp is not None:
@@ -386,7 +402,7 @@ class Engine:
                     from .prefill import PrefillRunner
                     self._prefill = PrefillRunner(self)
             self.last_prefill_row = 0      # row of model.buf.logits that holds the prompt's last position
-            tok = self._prefill.run(slot, ids, chunk)
+            tok = self._prefill.run(slot, ids, chunk) if scores is None else self._prefill.run(slot, ids, chunk, scores)
             self.check_failed("prompt pass")
             return tok
         start = self.seq_len[slot]
@@ -396,6 +412,9 @@ class Engine:
             rows = [Row(slot, start + c0 + i, t) for i, t in enumerate(part)]
             last = c0 + self.max_rows >= len(ids)
             out = self.forward_rows(rows, advance=False, read=last)
+            if scores is not None:      # the step left all rows' logits
+                tokens, res = scores.take(len(part))
+                LP.token_logprobs(self.logits(len(part)), tokens, out=res)
             hook = getattr(self, "on_chunk_hidden", None)
             if hook is not None:
                 hook(None, slot, part, start + c0, self.model.buf.resid[: len(part)])
@@ -416,6 +435,22 @@ class Engine:
             raise ValueError(f"prefill backend {self.prefill_backend!r} needs head_dim 128 (and a bf16 KV cache under "
                              "tensor parallelism)")
         return ok
+
+    def score(self, ids: Sequence[int], top: int = 0, slot: int = 0) -> List[TokenScore]:
+        """Log probability, entropy and top alternatives of every token of ``ids`` behind the ones before it (the first one's are those
+        of no prediction: NaN and nothing).  The slot starts afresh and holds ``ids`` afterwards."""
+        self.reset(slot)
+        scores = self.prompt_scores(ids, top)
+        self.prefill(slot, ids, scores=scores)
+        return scores.read()
+
+    def logprobs(self, tokens: Sequence[int], top: int = 0, logits: Optional[torch.Tensor] = None) -> List[TokenScore]:
+        """Log probability of one token per row, entropy and top alternatives, of ``logits`` or of the last step's rows (-1: a row without a
+        token)."""
+        lg = self.logits(len(tokens)) if logits is None else logits
+        buf = ScoreBuffer(len(tokens), top, self.device)
+        LP.token_logprobs(lg, torch.tensor(tokens, dtype=torch.int32).to(self.device), out=buf.out)
+        return buf.read()
 
     def decode_begin(self, slots: Sequence[int], tokens: Sequence[int]):
         """Arm plain decode: one row per slot, starting with ``tokens`` at each slot's current length."""

@@ -218,7 +218,13 @@ class PrefillRunner:
             pr.end()
 
     # ------------------------------------------------------------------ one chunk
-    def chunk(self, slot: int, ids: List[int], pos0: int):
+    def _score(self, scores, resid):
+        """Log probabilities of the tokens behind these residual rows."""
+        m, c, x = self.eng.model, resid.shape[0], self.x[: resid.shape[0]]
+        K.resid_norm(1, c, self.cfg.hidden, m.w.final_norm, self.cfg.rms_eps, resid, x, resid_in=resid, splits=0)
+        m.score_rows(x, *scores.take(c), int8=self.backend == "int8")
+
+    def chunk(self, slot: int, ids: List[int], pos0: int, scores=None):
         eng, cfg, m = self.eng, self.cfg, self.eng.model
         c, h = len(ids), cfg.hidden
         eng._ensure_pages(slot, pos0 + c)
@@ -231,6 +237,8 @@ class PrefillRunner:
         bt_row = eng.block_table[slot]
         for li, lw in enumerate(m.w.layers):
             self.layer(lw, li, slot, c, pos0, resid, x)
+        if scores is not None:      # (before a draft head takes the buffers)
+            self._score(scores, resid)
         hook = getattr(eng, "on_chunk_hidden", None)
         if hook is not None:      # draft heads ingest the prompt from the trunk's hidden states
             hook(self, slot, ids, pos0, resid)
@@ -238,7 +246,7 @@ class PrefillRunner:
         return resid
 
     # ------------------------------------------------------------------ int8 KV cache: layer-major pass
-    def _run_int8_kv(self, slot: int, ids: List[int], chunk: int):
+    def _run_int8_kv(self, slot: int, ids: List[int], chunk: int, scores=None):
         """Prompt pass into an int8 KV cache.  The attention kernel reads bf16 pages, so the walk is LAYER-major:
         all chunks go through layer l against a one-layer bf16 scratch (identity page table, positions of the
         whole sequence), then the layer's new rows are quantised into the int8 cache and the scratch is reused
@@ -294,14 +302,17 @@ class PrefillRunner:
                     finally:
                         self.resid = keep
             K.kv_convert(k16[0], v16[0], tab16[0], k8, v8, ks, vs, tab8, start, n, cfg.n_kv_heads, cfg.head_dim, True)
+        if scores is not None:
+            for c0 in range(0, n, chunk):
+                self._score(scores, resid_all[c0: c0 + chunk])
         eng.seq_len[slot] = total
         return resid_all[n - 1: n]
 
-    def run(self, slot: int, ids: List[int], chunk: Optional[int] = None) -> int:
+    def run(self, slot: int, ids: List[int], chunk: Optional[int] = None, scores=None) -> int:
         eng, cfg, m = self.eng, self.cfg, self.eng.model
         chunk = min(chunk or self.max_chunk, self.max_chunk)
         if eng.kv.kv_int8:
-            last_row = self._run_int8_kv(slot, ids, chunk)
+            last_row = self._run_int8_kv(slot, ids, chunk, scores)
             b = m.buf
             b.resid[0].copy_(last_row[0])
             return self._head_of_row0()
@@ -309,7 +320,7 @@ class PrefillRunner:
         resid = None
         n = len(ids)
         for c0 in range(0, n, chunk):
-            resid = self.chunk(slot, ids[c0: c0 + chunk], start + c0)
+            resid = self.chunk(slot, ids[c0: c0 + chunk], start + c0, scores)
         last = (n - 1) % chunk
         m.buf.resid[0].copy_(resid[last])
         tok = self._head_of_row0()

@@ -366,8 +366,11 @@ class SpecAdapter:
         fn = getattr(self.inner, "sample", None)
         return fn(*args, **kw) if fn is not None else None
 
-    def prefill(self, slot, ids):
-        tok = self.inner.prefill(slot, ids)
+    def logprobs(self, items, top=0): return self.inner.logprobs(items, top)
+    def prompt_scores(self, ids, top=0): return self.inner.prompt_scores(ids, top)
+
+    def prefill(self, slot, ids, scores=None):
+        tok = self.inner.prefill(slot, ids) if scores is None else self.inner.prefill(slot, ids, scores)
         n = self.e.seq_len[slot]
         self.hid[slot] = self.head.last_prompt_hidden(slot).view(1, -1)
         self.base[slot] = n - 1

@@ -45,8 +45,8 @@ class EngineAdapter(EngineIface):
         """After a step failed on a bounded wait: clear the device status and release the engine's latch."""
         self.e.reset_failure()
 
-    def prefill(self, slot, ids):
-        tok = self.e.prefill(slot, list(ids))
+    def prefill(self, slot, ids, scores=None):
+        tok = self.e.prefill(slot, list(ids)) if scores is None else self.e.prefill(slot, list(ids), scores=scores)
         r = self.e.last_prefill_row
         self._rows_of = {slot: range(r, r + 1)}
         self._logits_host = self._logits_dev = None
@@ -88,6 +88,20 @@ class EngineAdapter(EngineIface):
         if self._logits_host is None:
             self._logits_host = self._device_logits().float().cpu().numpy()
         return self._logits_host[self._rows_of[slot][row]]
+
+    def logprobs(self, items, top=0):
+        """``EngineIface.logprobs`` on the device: one launch over the step's rows, one read.  ``None``: sharded logits."""
+        if not self.e.can_score:
+            return None
+        lg = self._device_logits()
+        want = [-1] * lg.shape[0]
+        for slot, row, token in items:
+            want[self._rows_of[slot][row]] = int(token)
+        got = self.e.logprobs(want, top, lg)
+        return [got[self._rows_of[slot][row]] for slot, row, _ in items]
+
+    def prompt_scores(self, ids, top=0):
+        return self.e.prompt_scores(ids, top) if self.e.can_score else None
 
     def logits_shard(self, slot, row=0):
         """(first vocabulary id, fp32 values) of the part of the row's logits that this rank holds: the whole row

@@ -26,6 +26,7 @@ import numpy as np
 from ..native import host as H
 from .chat_template import ChatTemplate
 from .iface import EngineIface, TokIface
+from .logprobs import Entry, chat_block, host_logprob, text_block
 
 
 @dataclass
@@ -73,6 +74,10 @@ class Session:
     klen: object = None                # DraftLengthPolicy of this request
     copy: object = None                # LookupPolicy (spec = dflash-lookup): copy steps inside a block drafter
     copy_step: bool = False            # the drafts of the step in flight came from the copy proposer
+    scores: object = None              # echoed prompts: what the prompt pass fills with the prompt's log probabilities
+    entries: List[Entry] = field(default_factory=list)     # log probabilities of the response's tokens
+    told: int = 0                      # of them, those that frames have carried
+    text_at: int = 0                   # completions: where the next told token's text begins
 
 
 class Server:
@@ -172,6 +177,11 @@ class Server:
             s.parser = H.OutputStream(thinking, req.tools, tool_format) if chat else None
         s.stopper = H.StopMatcher(list(req.stop))
         req.max_tokens = max_new
+        if req.echo and req.logprobs >= 0:
+            make = getattr(self.engine, "prompt_scores", None)
+            s.scores = make(ids, req.logprobs) if make is not None else None
+            if s.scores is None:
+                return self._error(hid, 400, "log probabilities of the prompt are not available on this server")
         preferred = self.prefix.preferred_slot(ids) if self.prefix else -1
         want_rows = 1 + (self.o.spec_max if self.o.spec != "off" else 0)
         if not self.sched.submit(hid, len(ids), max_new, preferred, want_rows):
@@ -193,7 +203,7 @@ class Server:
         while acts:
             a = acts.pop(0)
             # a prompt chunk and the decode rows of the same tick run as one batch where the engine can
-            b = acts.pop(0) if mixed and a["kind"] == "prefill" and acts and acts[0]["kind"] == "decode" else None
+            b = acts.pop(0) if mixed and a["kind"] == "prefill" and acts and acts[0]["kind"] == "decode" and not self._scored(a["slot"]) else None
             try:
                 self._act(a) if b is None else self._mixed(a, b)
             except Exception as e:  # noqa: BLE001   (whatever a request trips over fails that request, not the server)
@@ -202,6 +212,10 @@ class Server:
                     s = self.by_slot.get(slot)
                     if s is not None and not s.finished:
                         self._fail(s, e)
+
+    def _scored(self, slot: int) -> bool:
+        s = self.by_slot.get(slot)
+        return s is not None and s.scores is not None
 
     def _act(self, a):
         if True:
@@ -214,7 +228,9 @@ class Server:
                 s = self.sessions[a["req"]]
                 s.slot = a["slot"]
                 self.by_slot[s.slot] = s
-                cached = self.prefix.begin(s.slot, s.prompt_ids, self.o.prefix_split_last) if self.prefix else 0
+                # a prompt whose tokens are scored goes through the model from its first token on
+                known = s.prompt_ids if s.scores is None else []
+                cached = self.prefix.begin(s.slot, known, self.o.prefix_split_last) if self.prefix else 0
                 if not self.prefix:
                     self.engine.reset(s.slot)
                 s.cached_tokens = cached
@@ -228,7 +244,8 @@ class Server:
     def _prefill(self, a):
         s = self.by_slot[a["slot"]]
         try:
-            tok = self.engine.prefill(s.slot, s.prompt_ids[a["begin"]: a["end"]])
+            more = {} if s.scores is None else {"scores": s.scores}
+            tok = self.engine.prefill(s.slot, s.prompt_ids[a["begin"]: a["end"]], **more)
         except Exception as e:  # noqa: BLE001
             self._fail(s, e)
             return self._recover_engine()
@@ -254,10 +271,36 @@ class Server:
         if a["last"]:
             if self.prefix:
                 self.prefix.after_prefill(s.slot, s.prompt_ids)
+            if s.req.echo:
+                self._echo(s)
+            if s.req.score_only:
+                return self._end(s, "length")
             if not s.req.greedy:
                 tok = self._sample(s)
             s.t_first = time.time()
-            self._emit_token(s, tok)       # the first token goes out before the first decode step
+            score = self._logprobs([(s, 0, tok)])[0]
+            self._emit_token(s, tok, score)       # the first token goes out before the first decode step
+
+    def _echo(self, s: Session):
+        """The prompt ahead of the completion: its text as it is, its tokens' log probabilities where they are asked for."""
+        if s.scores is not None:
+            scores, s.scores = s.scores.read(), None
+            s.entries += [Entry(t, e if i else None) for i, (t, e) in enumerate(zip(s.prompt_ids, scores))]
+        text = s.req.prompt or self.tok.decode(s.prompt_ids)
+        self._deliver(s, [{"kind": "content", "text": text}])
+
+    def _logprobs(self, items):
+        """Scores of (session, row of its slot in the last pass, token), ``None`` for sessions that want none: one call of the engine for all."""
+        want = [(s.slot, row, tok) for s, row, tok in items if s.req.logprobs >= 0]
+        if not want:
+            return [None] * len(items)
+        top = max(s.req.logprobs for s, _, _ in items)
+        on_device = getattr(self.engine, "logprobs", None)
+        got = on_device(want, top) if on_device is not None else None
+        if got is None:
+            got = [host_logprob(np.asarray(self.engine.logits(slot, row))[: self.engine.vocab_size], tok, top) for slot, row, tok in want]
+        got = iter(got)
+        return [next(got) if s.req.logprobs >= 0 else None for s, _, _ in items]
 
     def _sample(self, s: Session, logits=None, row: int = 0) -> int:
         """The request's next token from its logits row: on the device when the engine has a sampler (only the
@@ -318,6 +361,7 @@ class Server:
         return rows, s_q
 
     def _decode_done(self, rows, res, s_q):
+        done, items = [], []
         for slot, toks in rows.items():
             s = self.by_slot[slot]
             out = res[slot]
@@ -338,20 +382,21 @@ class Server:
                                                    s.req.top_k, s.req.top_p, seed)
             else:
                 acc, nxt = 0, (self._sample(s) if host_rule else out[0])
+            done.append((s, drafts, acc, len(items)))
+            items += [(s, i, t) for i, t in enumerate(drafts[:acc] + [nxt])]
+        scores = self._logprobs(items)      # before rejected rows are taken back: a recurrent model runs rows again for that
+        for s, drafts, acc, first in done:
             self._observe_drafts(s, len(drafts), acc)
             if acc < len(drafts):       # rejected rows leave the cache
-                self.engine.truncate(slot, self.engine.length(slot) - (len(drafts) - acc))
+                self.engine.truncate(s.slot, self.engine.length(s.slot) - (len(drafts) - acc))
             emitted = 0
-            for t in drafts[:acc]:
+            for i in range(first, first + acc + 1):
                 if s.finished:
                     break
-                self._emit_token(s, t)
+                self._emit_token(s, items[i][2], scores[i])
                 emitted += 1
             if not s.finished:
-                self._emit_token(s, nxt)
-                emitted += 1
-            if not s.finished:
-                self.sched.tokens(slot, emitted, False)
+                self.sched.tokens(s.slot, emitted, False)
 
     def _step_costs(self):
         if self.o.spec_costs is not None:
@@ -423,7 +468,7 @@ class Server:
         return list(self._lookup(s).propose(min(k, room), 2))
 
     # ------------------------------------------------------------------ output
-    def _emit_token(self, s: Session, tok: int):
+    def _emit_token(self, s: Session, tok: int, score=None):
         """``tok`` was produced: record it, stream its text, decide whether the request ends."""
         r = s.req
         is_eos = tok in self.engine.eos_ids
@@ -432,6 +477,8 @@ class Server:
             s.pending = None
             return self._end(s, "stop")
         s.out_ids.append(tok)
+        if score is not None:
+            s.entries.append(Entry(tok, score))
         if s.lookup is not None:
             s.lookup.append(tok)
         s.pending = tok
@@ -469,8 +516,18 @@ class Server:
             if r.stream:
                 self.http.send_event(s.http_id, H.stream_frame(
                     r, s.rid, s.created, self.o.model_name, d["kind"], d.get("text", ""),
-                    d if d["kind"] == "call" else None, d.get("index", 0), "", None, ids))
+                    d if d["kind"] == "call" else None, d.get("index", 0), "", None, ids, self._tell(s)))
                 ids = []
+
+    def _tell(self, s: Session):
+        """Log probabilities of the tokens that no frame has carried yet, in the endpoint's form; ``None`` where none are asked for."""
+        if s.req.logprobs < 0 or s.told == len(s.entries):
+            return None
+        new, s.told = s.entries[s.told:], len(s.entries)
+        if s.req.chat:
+            return chat_block(self.tok, new)
+        block, s.text_at = text_block(self.tok, new, s.req.logprobs, s.text_at)
+        return block
 
     def _end(self, s: Session, reason: str, flush: bool = True):
         """Ends generation.  ``flush``: text still held by the detokeniser and the stop matcher is
@@ -515,14 +572,14 @@ class Server:
                 if not s.stream_started:
                     self._deliver(s, [])
                 self.http.send_event(s.http_id, H.stream_frame(r, s.rid, s.created, self.o.model_name, "finish", "",
-                                                               None, 0, s.finish_reason))
+                                                               None, 0, s.finish_reason, None, [], self._tell(s)))
                 if r.include_usage:
                     self.http.send_event(s.http_id, H.stream_frame(r, s.rid, s.created, self.o.model_name, "usage", "",
                                                                    None, 0, "", usage))
                 self.http.end_stream(s.http_id)
             else:
                 body = H.completion_response(r, s.rid, s.created, self.o.model_name, s.content, s.reasoning, s.calls,
-                                             s.finish_reason, usage[0], usage[1], usage[2], s.out_ids)
+                                             s.finish_reason, usage[0], usage[1], usage[2], s.out_ids, self._tell(s))
                 self.http.respond(s.http_id, 200, "application/json", body)
         else:
             self.http.respond(s.http_id, 499, "application/json", "{}")

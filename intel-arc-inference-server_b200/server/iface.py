@@ -22,8 +22,9 @@ class EngineIface:
     def reset(self, slot: int) -> None: ...
     def length(self, slot: int) -> int: ...
     def truncate(self, slot: int, length: int) -> None: ...
-    def prefill(self, slot: int, ids: Sequence[int]) -> int:
-        """Ingest ``ids`` after the slot's current length; returns the greedy next token."""
+    def prefill(self, slot: int, ids: Sequence[int], scores=None) -> int:
+        """Ingest ``ids`` after the slot's current length; returns the greedy next token.  ``scores``: of ``prompt_scores``, only given to
+        engines that have it."""
     def step(self, rows: Dict[int, List[int]]) -> Dict[int, List[int]]:
         """For every slot, run its row tokens at consecutive positions (the first is the pending token,
         the rest are drafts); returns the arg-max after each row."""
@@ -31,6 +32,12 @@ class EngineIface:
         """``prefill(slot, ids)`` and ``step(rows)`` as one batch; returns (token, step result)."""
     def logits(self, slot: int, row: int = 0) -> np.ndarray:
         """fp32 logits of ``row`` of ``slot`` from the last prefill / step (for host sampling)."""
+    def logprobs(self, items, top: int = 0):
+        """Log probability and top alternatives (``.logprob``, ``.top``) of (slot, row, token) items of the last prefill / step; ``None``: the
+        caller takes them from ``logits``."""
+    def prompt_scores(self, ids: Sequence[int], top: int = 0):
+        """Something ``prefill`` fills with the log probabilities of a prompt ingested from its first token on, portion by portion; its
+        ``read()`` gives one per token (the first one's is NaN).  ``None``: not available."""
     def kv_form(self) -> str:
         return "bf16"
 
@@ -74,9 +81,14 @@ class MockEngine(EngineIface):
         v[(tok + 1) % self.vocab_size] = 4.0
         return v
 
-    def prefill(self, slot, ids):
+    def prompt_scores(self, ids, top=0):
+        return MockScores(self, ids, top)
+
+    def prefill(self, slot, ids, scores=None):
         if len(self.seqs[slot]) + len(ids) > self.max_len:
             raise ValueError("prompt exceeds max_len")
+        if scores is not None:
+            scores.ingest(self.seqs[slot], ids)
         self.seqs[slot].extend(ids)
         self.prefilled_tokens += len(ids)
         t = self._next(self.seqs[slot])
@@ -111,10 +123,32 @@ class MockEngine(EngineIface):
         return self._logits[slot][row]
 
 
+class MockScores:
+    """``prompt_scores`` of the stand-in: what its logits rows say of every next token."""
+
+    def __init__(self, engine, ids, top):
+        self.e, self.ids, self.top, self.got = engine, list(ids), top, []
+
+    def ingest(self, before, ids):
+        from .logprobs import host_logprob
+        assert list(before) == self.ids[: len(self.got)] and list(ids) == self.ids[len(self.got): len(self.got) + len(ids)]
+        for i in range(len(ids)):
+            at = len(self.got) + 1
+            self.got.append(host_logprob(self.e._row(self.e._next(self.ids[:at])), self.ids[at] if at < len(self.ids) else -1, self.top))
+
+    def read(self):
+        from .logprobs import Score
+        assert len(self.got) == len(self.ids)
+        return [Score(float("nan"), [])] + self.got[:-1]
+
+
 class TokIface:
     def encode(self, text: str) -> List[int]: ...
     def decode(self, ids: Sequence[int]) -> str: ...
     def streamer(self): ...
+    def token_bytes(self, i: int) -> bytes:
+        """The bytes a token stands for (part of a character, if it is one)."""
+        return self.decode([i]).encode("utf-8")
 
 
 class ByteTok(TokIface):
@@ -127,6 +161,9 @@ class ByteTok(TokIface):
 
     def decode(self, ids):
         return bytes((i - 3) % 256 for i in ids if i >= 3).decode("utf-8", "replace")
+
+    def token_bytes(self, i):
+        return bytes([(i - 3) % 256]) if i >= 3 else b""
 
     def streamer(self):
         tok = self
@@ -172,6 +209,9 @@ class NativeTok(TokIface):
 
     def streamer(self):
         return self.H.Streamer(self.tok, True)
+
+    def token_bytes(self, i):
+        return bytes(self.tok.token_bytes(int(i)))
 
     def token_to_id(self, s):
         return self.tok.token_to_id(s)
