@@ -24,6 +24,7 @@ namespace {
 constexpr int BM = 128, BN = 256, kStageRow = 128;      // rows of a CTA, columns of a tile, bytes of k a stage
 constexpr int kThreads = 192;
 constexpr int kGrain = 32, kChunk = 32;        // columns that ranges are cut at, columns of a maximum
+constexpr int kMostI8 = 1 << 17;       // columns of 127 x 127 that an int32 sum holds
 constexpr int kRangeRows = 512;      // up to these many rows ranges
 
 template <bool PAIR>
@@ -531,7 +532,7 @@ Room room_of(const Layout& l, int m, int n, int k, int top, bool i8) {
 // Floats of workspace for m rows of k against n columns (-1: sizes that are refused): `work`, of one call at a time, 16-byte aligned.
 extern "C" long long b2_score_work(int m, int n, int k, int top, int i8) {
   Layout l;
-  return layout_of(m, n, l) || k < 1 || k > 0x7fffff00 ? -1 : room_of(l, m, n, k, top, i8 != 0).all;
+  return layout_of(m, n, l) || k < 1 || k > (i8 ? kMostI8 : 0x7fffff00) ? -1 : room_of(l, m, n, k, top, i8 != 0).all;
 }
 // Log probabilities of the tokens of bf16 rows x [m][k] against the head w [n][k], entropies and alternatives.  The head is bf16, or int8 (w_scale: of its
 // rows), for which the rows are quantised too.  Rows are ldx and ldw elements apart, multiples of 16 bytes, and those of the head of 128 bytes at least.
@@ -540,7 +541,7 @@ extern "C" int b2_score(const void* x, long long ldx, const void* w, long long l
   const bool i8 = w_scale != nullptr;
   const int size = i8 ? 1 : 2;
   Layout l;
-  if (layout_of(m, n, l) || (long long)k * size < kStageRow || k > 0x7fffff00 || ldx < k || ldw < k || top < 0 || top > kMaxTop) return -1;
+  if (layout_of(m, n, l) || (long long)k * size < kStageRow || k > (i8 ? kMostI8 : 0x7fffff00) || ldx < k || ldw < k || top < 0 || top > kMaxTop) return -1;
   if (((uintptr_t)x | (uintptr_t)w | (uintptr_t)work | (unsigned long long)(ldx * 2) | (unsigned long long)(ldw * size)) & 15) return -3;
   const Room r = room_of(l, m, n, k, top, i8);
   cudaStream_t st = (cudaStream_t)stream;

@@ -13,7 +13,6 @@ Alternatives beyond the vocabulary have id -1 and log probability -inf.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from dataclasses import dataclass
@@ -24,7 +23,9 @@ import torch
 from . import lib as K
 
 MAX_TOP = 32           # alternatives a row can have
-SLAB_ELEMS = 160 << 20 # logits that ``score`` with alternatives keeps at a time
+SLAB_ELEMS = 160 << 20 # logits that ``score`` with alternatives keeps at a time (fewer where there is no room for them)
+SLAB_ROWS = 32768      # rows whose sums it keeps at a time
+MAX_I8_COLUMNS = 1 << 17
 
 
 @dataclass(frozen=True)
@@ -50,10 +51,17 @@ class Logprobs:
         if not 0 <= top <= MAX_TOP:
             raise ValueError(f"log probabilities of at most {MAX_TOP} alternatives, not {top}")
         f = lambda *s: torch.empty(s, dtype=torch.float32, device=device)           # noqa: E731
-        return Logprobs(f(m), f(m), torch.empty(m, top, dtype=torch.int32, device=device), f(m, top))
+        return Logprobs._of(f(m), f(m), torch.empty((m, top), dtype=torch.int32, device=device), f(m, top))
 
     def rows(self, begin: int, end: int) -> "Logprobs":
-        return Logprobs(self.logprob[begin:end], self.entropy[begin:end], self.top_ids[begin:end], self.top_logprobs[begin:end])
+        return Logprobs._of(self.logprob[begin:end], self.entropy[begin:end], self.top_ids[begin:end], self.top_logprobs[begin:end])
+
+    @staticmethod
+    def _of(logprob, entropy, top_ids, top_logprobs) -> "Logprobs":
+        """Tensors that need no check."""
+        out = object.__new__(Logprobs)
+        out.__dict__.update(logprob=logprob, entropy=entropy, top_ids=top_ids, top_logprobs=top_logprobs)
+        return out
 
 
 def _results(m: int, top: Optional[int], out: Optional[Logprobs], device) -> Logprobs:
@@ -70,19 +78,20 @@ def _check_tokens(tokens: torch.Tensor, m: int, device):
         raise ValueError(f"tokens: {m} contiguous int32 ids on {device}")
 
 
-def _rows_of(t: torch.Tensor, dtype, what: str, align: int = 4):
-    m, n = t.shape if t.dim() == 2 else (0, 0)
-    if t.dim() != 2 or t.dtype != dtype or not t.is_cuda or n > 1 and t.stride(1) != 1:
-        raise ValueError(f"{what}: rows of {dtype} on a CUDA device, one element after another")
-    if m > 1 and t.stride(0) < n:
+def _rows_of(t: torch.Tensor, dtype, what: str, align: int = 4) -> tuple:
+    """(rows, columns, elements from row to row) of a matrix."""
+    if t.dim() != 2 or t.dtype != dtype or not t.is_cuda:
+        raise ValueError(f"{what}: rows of {dtype} on a CUDA device")
+    (m, n), (ld, step) = t.shape, t.stride()
+    if n > 1 and step != 1:
+        raise ValueError(f"{what}: one element after another")
+    if m < 2:
+        ld = (n + 15) // 16 * 16      # (a lone row's stride says nothing: a multiple of 16 bytes that holds it)
+    elif ld < n:
         raise ValueError(f"{what}: rows that do not overlap")
-    if t.data_ptr() % align or m > 1 and t.stride(0) * t.element_size() % align:
+    if t.data_ptr() % align or ld * t.element_size() % align:
         raise ValueError(f"{what}: rows begin at multiples of {align} bytes")
-
-
-def _ld(t: torch.Tensor) -> int:
-    """Elements from row to row; a lone row's stride says nothing: a multiple of 16 bytes that holds it."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+    return m, n, ld
 
 
 @functools.lru_cache(maxsize=None)
@@ -95,9 +104,9 @@ def _entry(name: str, kinds: str, result=ctypes.c_int):
     return fn
 
 
-def _on(device):
-    """The device made the current one where it is not."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _elsewhere(device) -> bool:
+    """Another device is the current one."""
+    return device.index != torch.cuda.current_device()
 
 
 def _stream(device) -> int:
@@ -108,76 +117,71 @@ def _stream(device) -> int:
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
     """Rows of fp32 ``logits`` ``[m][vocabulary]`` (any row stride), one int32 token each.  ``out``: results to write, whose width is
     then ``top``."""
-    _rows_of(logits, torch.float32, "logits")
-    m, n = logits.shape
+    m, n, ld = _rows_of(logits, torch.float32, "logits")
     dev = logits.device
     if n < 1:
         raise ValueError("logits of an empty vocabulary")
     _check_tokens(tokens, m, dev)
     out = _results(m, top, out, dev)
-    if m:
-        with _on(dev):
-            K._check(_entry("b2_logprob_rows", "pliipippppp")(
-                logits.data_ptr(), _ld(logits), m, n, tokens.data_ptr(), out.top_ids.shape[1], out.logprob.data_ptr(), out.entropy.data_ptr(),
-                out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), _stream(dev)), "logprob_rows")
+    if not m:
+        return out
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return token_logprobs(logits, tokens, top, out)
+    K._check(_entry("b2_logprob_rows", "pliipippppp")(
+        logits.data_ptr(), ld, m, n, tokens.data_ptr(), out.top_ids.shape[1], out.logprob.data_ptr(), out.entropy.data_ptr(),
+        out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), _stream(dev)), "logprob_rows")
     return out
 
 
-def _score(x, w, w_scale, tokens, out: Logprobs) -> Logprobs:
-    m, k = x.shape
-    n, top, i8 = w.shape[0], out.top_ids.shape[1], w_scale is not None
-    dev, ldx, ldw = x.device, _ld(x), _ld(w)
+def _score(x, w, w_scale, tokens, top: Optional[int], out: Optional[Logprobs]) -> Logprobs:
+    i8, dev = w_scale is not None, x.device
+    m, k, ldx = _rows_of(x, torch.bfloat16, "rows", 16)
+    n, kw, ldw = _rows_of(w, torch.int8 if i8 else torch.bfloat16, "head", 16)
+    if kw != k or n < 1 or w.device != dev:
+        raise ValueError(f"head {tuple(w.shape)} on {w.device} against rows {tuple(x.shape)} on {dev}")
+    if k * w.element_size() < 128 or i8 and k > MAX_I8_COLUMNS:
+        raise ValueError(f"rows of {k} columns: 128 bytes of the head's type at least" + (f", {MAX_I8_COLUMNS} at most" if i8 else ""))
+    _check_tokens(tokens, m, dev)
+    out = _results(m, top, out, dev)
+    if not m:
+        return out
+    top = out.top_ids.shape[1]
     room, run = _entry("b2_score_work", "iiiii", ctypes.c_longlong), _entry("b2_score", "plplpiiipipppppp")
-    step = m if not top else min(m, max(256, SLAB_ELEMS // n // 256 * 256))
-    with _on(dev):
-        while True:
-            need = room(step, n, k, top, i8)
-            if m % step:
-                need = max(need, room(m % step, n, k, top, i8))
-            try:
-                work = torch.empty(need, dtype=torch.float32, device=dev)
-                break
-            except torch.OutOfMemoryError:
-                if step <= 256 or not top:
-                    raise
-                step = max(256, step // 512 * 256)      # fewer logits at a time
-        for i in range(0, m, step):
-            c = min(step, m - i)
-            o = out if c == m else out.rows(i, i + c)
-            K._check(run(x.data_ptr() + 2 * i * ldx, ldx, w.data_ptr(), ldw, w_scale.data_ptr() if i8 else None, c, n, k, tokens.data_ptr() + 4 * i, top,
-                         work.data_ptr(), o.logprob.data_ptr(), o.entropy.data_ptr(), o.top_ids.data_ptr(), o.top_logprobs.data_ptr(), _stream(dev)), "score")
-            K.launch_count += 2 if i8 else 1      # rows quantised; a row's parts joined
+    step = min(m, SLAB_ROWS if not top else max(256, SLAB_ELEMS // n // 256 * 256))
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return _score(x, w, w_scale, tokens, None, out)
+    while True:
+        need = room(step, n, k, top, i8)
+        if m % step:
+            need = max(need, room(m % step, n, k, top, i8))
+        try:
+            work = torch.empty(need, dtype=torch.float32, device=dev)
+            break
+        except torch.OutOfMemoryError:
+            if step <= 256 or not top:
+                raise
+            step = max(256, step // 512 * 256)      # fewer logits at a time
+    for i in range(0, m, step):
+        c = min(step, m - i)
+        o = out if c == m else out.rows(i, i + c)
+        K._check(run(x.data_ptr() + 2 * i * ldx, ldx, w.data_ptr(), ldw, w_scale.data_ptr() if i8 else None, c, n, k, tokens.data_ptr() + 4 * i, top,
+                     work.data_ptr(), o.logprob.data_ptr(), o.entropy.data_ptr(), o.top_ids.data_ptr(), o.top_logprobs.data_ptr(), _stream(dev)), "score")
+        K.launch_count += 2 if i8 else 1      # rows quantised; a row's parts joined
     return out
-
-
-def _check_head(x, w, dtype):
-    _rows_of(w, dtype, "head", 16)
-    if w.device != x.device or w.shape[1] != x.shape[1] or w.shape[0] < 1:
-        raise ValueError(f"head {tuple(w.shape)} on {w.device} against rows {tuple(x.shape)} on {x.device}")
-    if x.shape[1] * w.element_size() < 128:
-        raise ValueError(f"rows of {x.shape[1]} columns: 128 bytes of the head's type at least")
 
 
 def score(x: torch.Tensor, head: torch.Tensor, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
     """Rows ``x`` ``[m][k]`` against the lm_head ``[vocabulary][k]``, both bf16 with rows at multiples of 16 bytes: ``token_logprobs`` of
     ``x @ head.T`` in fp32."""
-    _rows_of(x, torch.bfloat16, "rows", 16)
-    _check_head(x, head, torch.bfloat16)
-    m, dev = x.shape[0], x.device
-    _check_tokens(tokens, m, dev)
-    out = _results(m, top, out, dev)
-    return _score(x, head, None, tokens, out) if m else out
+    return _score(x, head, None, tokens, top, out)
 
 
 def score_i8(x: torch.Tensor, head: tuple, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
     """Rows ``x`` ``[m][k]`` bf16 against an int8 lm_head (``[vocabulary][k]``, fp32 scale per row), rows of both at multiples of 16
     bytes: rows are quantised per token (s = max|x| / 127, q = rint(x / s), as the int8 prompt pass does) and logits are (q . w) s s_w."""
     w8, scale = head
-    _rows_of(x, torch.bfloat16, "rows", 16)
-    _check_head(x, w8, torch.int8)
-    m, dev = x.shape[0], x.device
-    if scale.dtype != torch.float32 or scale.shape != (w8.shape[0],) or scale.device != dev or not scale.is_contiguous():
-        raise ValueError(f"scales of the head: {w8.shape[0]} contiguous fp32 numbers on {dev}")
-    _check_tokens(tokens, m, dev)
-    out = _results(m, top, out, dev)
-    return _score(x, w8, scale, tokens, out) if m else out
+    if scale.dtype != torch.float32 or scale.shape != (w8.shape[0],) or scale.device != x.device or not scale.is_contiguous():
+        raise ValueError(f"scales of the head: {w8.shape[0]} contiguous fp32 numbers on {x.device}")
+    return _score(x, w8, scale, tokens, top, out)

@@ -93,12 +93,16 @@ class EngineAdapter(EngineIface):
         """``EngineIface.logprobs`` on the device: one launch over the step's rows, one read.  ``None``: sharded logits."""
         if not self.e.can_score:
             return None
+        at = [self._rows_of[slot][row] for slot, row, _ in items]
         lg = self._device_logits()
+        if len(set(at)) < len(at):      # a row that is asked about twice
+            got = self.e.logprobs([int(t) for _, _, t in items], top, lg[at])
+            return got
         want = [-1] * lg.shape[0]
-        for slot, row, token in items:
-            want[self._rows_of[slot][row]] = int(token)
+        for i, (_, _, token) in zip(at, items):
+            want[i] = int(token)
         got = self.e.logprobs(want, top, lg)
-        return [got[self._rows_of[slot][row]] for slot, row, _ in items]
+        return [got[i] for i in at]
 
     def prompt_scores(self, ids, top=0):
         return self.e.prompt_scores(ids, top) if self.e.can_score else None

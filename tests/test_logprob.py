@@ -132,7 +132,9 @@ def test_refusals_of_shapes_and_strides():
                  lambda: LP.score(torch.zeros(2, 72, dtype=torch.bfloat16, device="cuda")[:, 1:65], w, t), lambda: LP.score(x, w, t, out=LP.Logprobs.empty(3, 0, "cuda")),
                  lambda: LP.score_i8(x, (w8, ws), t), lambda: LP.score_i8(torch.zeros(2, 128, dtype=torch.bfloat16, device="cuda"), (w8, ws[:3]), t),
                  lambda: LP.score_i8(torch.zeros(2, 128, dtype=torch.bfloat16, device="cuda"), (w8, ws.half()), t),
-                 lambda: LP.score_i8(torch.zeros(2, 128, dtype=torch.bfloat16, device="cuda"), (w8.float(), ws), t)):
+                 lambda: LP.score_i8(torch.zeros(2, 128, dtype=torch.bfloat16, device="cuda"), (w8.float(), ws), t),
+                 lambda: LP.score_i8(torch.zeros(2, LP.MAX_I8_COLUMNS + 16, dtype=torch.bfloat16, device="cuda"),
+                                     (torch.zeros(8, LP.MAX_I8_COLUMNS + 16, dtype=torch.int8, device="cuda"), ws), t)):
         with pytest.raises(ValueError):
             call()
 
@@ -359,6 +361,54 @@ def test_score_of_rows_and_heads_without_numbers(top):
     tiny = torch.full((2, k), 2.0 ** -133, dtype=torch.bfloat16, device="cuda")      # the smallest bf16: a scale without an inverse in fp32
     out = LP.score_i8(tiny, (w8, ws), t[:2].contiguous(), top)
     close(out.entropy, torch.full((2,), math.log(n), device="cuda"), 300 * U)
+
+
+@gpu
+@pytest.mark.parametrize("n", [3000, 40000])
+def test_score_of_ties(n):
+    """Rows whose logits are all alike, or of two values: more chunks reach the bound than are noted."""
+    x, w = grid((5, 128), 21, 12, 1 / 16), torch.zeros(n, 128, dtype=torch.bfloat16, device="cuda")
+    w[:, 0] = (torch.arange(n, device="cuda") % 3 == 1).bfloat16()
+    x[:, 0] = torch.tensor([1.0, 0.0, -1.0, 2.0, -0.5], device="cuda")
+    t = torch.tensor([0, 1, 2, n - 1, -1], dtype=torch.int32, device="cuda")
+    for top in (1, 32):
+        check(LP.score(x, w, t, top), x.double() @ w.double().T, t, top)
+
+
+@gpu
+def test_score_of_ragged_columns():
+    """Rows of columns that no 16 bytes hold: a matrix cut out of a wider one."""
+    for k in (129, 135, 200, 257):
+        x, w = grid((70, 272), 22, 12, 1 / 16)[:, :k], grid((900, 272), 23, 20, 1 / 64)[:, :k]
+        t = torch.randint(0, 900, (70,), device="cuda", dtype=torch.int32)
+        check(LP.score(x, w, t, 3), x.double() @ w.double().T, t, 3)
+        w8, ws = (w * 64).to(torch.int8), torch.full((900,), 1 / 64, device="cuda")
+        w8 = torch.nn.functional.pad(w8, (0, 272 - k), value=3)[:, :k]      # beside the columns: something that must not count
+        largest = x.float().abs().amax(1, keepdim=True)
+        s = largest / torch.full_like(largest, 127)
+        z = ((x.float() * (1 / s)).round().double() @ w8.double().T).float() * s * ws
+        check(LP.score_i8(x, (w8, ws), t, 3), z, t, 3)
+
+
+@gpu
+def test_score_with_little_room(monkeypatch):
+    """No room for the logits of all rows: fewer at a time."""
+    x, w = grid((700, 128), 24, 12, 1 / 16), grid((999, 128), 25, 20, 1 / 64)
+    t = torch.randint(0, 999, (700,), device="cuda", dtype=torch.int32)
+    want, sizes, real = LP.score(x, w, t, 4), [], torch.empty
+
+    def empty(*a, **kw):
+        if a and isinstance(a[0], int) and a[0] > 400 * 1000:
+            sizes.append(a[0])
+            raise torch.OutOfMemoryError("no room")
+        return real(*a, **kw)
+    out = LP.Logprobs.empty(700, 4, "cuda")
+    monkeypatch.setattr(torch, "empty", empty)
+    LP.score(x, w, t, out=out)
+    monkeypatch.undo()
+    assert len(sizes) >= 1
+    for a, b in zip(vars(out).values(), vars(want).values()):
+        assert torch.equal(a, b) or float((a - b).abs().max()) <= 1e-5
 
 
 @gpu

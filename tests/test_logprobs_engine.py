@@ -185,6 +185,9 @@ def test_rows_of_steps(name):
     items = [(0, 0, 5), (0, 2, 9), (1, 0, 11)]
     for (slot, row, tok), s in zip(items, ad.logprobs(items, 1)):
         assert abs(s.logprob - float(lp[row if slot == 0 else 3, tok])) <= 2e-5
+    twice = ad.logprobs([(0, 1, 5), (1, 0, 11), (0, 1, 6)], 0)      # a row asked about twice
+    for (row, tok), s in zip(((1, 5), (3, 11), (1, 6)), twice):
+        assert abs(s.logprob - float(lp[row, tok])) <= 2e-5
     if eng.mixed_batches:      # a prompt's portion beside decode rows
         eng.reset(1)
         tok, res = ad.step_mixed(1, b, {0: [7]})
