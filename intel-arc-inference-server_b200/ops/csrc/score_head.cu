@@ -13,6 +13,11 @@
 // More than 512 rows: tiles are walked rows first, so that the clusters that run together share the rows of W in L2.  Up to 512 rows whole
 // tiles would leave SMs idle at the end (102400 columns: 400 tiles for 74 clusters): every cluster gets a range of columns of its own,
 // equal but for 32, whose last tile is as narrow as it has to be; a thread's sums go on through the range.
+//
+// More than about 300 rows are bound by the multiplication: 4096 rows x 151936 x 5120 take 3.6 ms in a short run (1.78 PFLOP/s) and 4.1 under
+// the power cap, int8 1.86 and 2.2 ms; halving the copies of x changes nothing, four warps more for the sums cost 5 %.  Fewer rows are
+// bound by the head's bytes: 77 rows x 102400 x 2048 72 us (5.8 TB/s), 64 rows x 151936 x 5120 260 us with the join (6.0 TB/s).  With
+// the logits stored and read again by logprob.cu (with alternatives it was so once) 900 rows x 151936 x 5120 took 1.41 ms, now 1.23.
 #include "common.cuh"
 #include "logprob.cuh"
 #include "pair.cuh"
@@ -555,9 +560,12 @@ extern "C" int b2_score(const void* x, long long ldx, const void* w, long long l
   void* q = work + r.q;
   CUtensorMap mx, mw, mg;
   int rc = i8 ? make_map(&mx, q, true, m, k, r.ldq, BM) : make_map(&mx, x, false, m, k, ldx, BM);
-  if (!rc) rc = make_map(&mw, w, i8, n, k, ldw, l.pair ? BN / 2 : BN);
-  mg = mw;
+  // (a map is a microsecond of the host's: ranges that are narrower than a tile have no whole ones)
+  const bool narrow = l.ranges && ((n + kGrain - 1) / kGrain + l.ranges - 1) / l.ranges < BN / kGrain;
+  if (!rc && !narrow) rc = make_map(&mw, w, i8, n, k, ldw, l.pair ? BN / 2 : BN);
   if (!rc && l.ranges) rc = make_map(&mg, w, i8, n, k, ldw, l.pair ? kGrain / 2 : kGrain);
+  if (narrow) mw = mg;
+  if (!l.ranges) mg = mw;
   if (rc) return rc;
   if (i8) {
     rc = b2_launch(quant_kernel, dim3(m), dim3(256), 0, st, true, (const __nv_bfloat16*)x, ldx, k, (int8_t*)q, (long long)r.ldq, work + r.scale);
