@@ -244,6 +244,5 @@ extern "C" int b2_logprob_rows(const float* z, long long ld, int m, int n, const
   const RowsParams p{z, ld, n, top, parts, tokens, logprob, entropy, top_ids, top_logprobs};
   return top ? launch<true>(p, m, (cudaStream_t)stream) : launch<false>(p, m, (cudaStream_t)stream);
 }
-extern "C" int b2_logprob_max_top() { return kMaxTop; }
 
 B2_DEFINE_STATUS(logprob)

@@ -13,7 +13,7 @@ struct LogStat {
   float m, s, t;
 };
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -153,15 +153,20 @@ __device__ __forceinline__ float merge_floats(float a, float b, int lane) {
 // A list with fewer than `top` logits above -inf: banned ids follow, the lowest first, then those without a number.
 __device__ __forceinline__ unsigned long long fill_list(unsigned long long list, const float* z, int n, int top, int lane) {
   int have = __popc(__ballot_sync(0xffffffffu, list != 0));
+  constexpr int kAhead = 8;
   for (int kind = 0; kind < 2 && have < top; ++kind) {
-    for (int j0 = 0; j0 < n && have < top; j0 += 32) {
-      const int j = j0 + lane;
-      const float x = j < n ? z[j] : 0.f;
-      const bool take = j < n && (kind == 0 ? x == -INFINITY : x != x);
-      const uint32_t mask = __ballot_sync(0xffffffffu, take);
-      const int nth = lane - have;      // this lane's place is the nth of them
-      if (nth >= 0 && nth < __popc(mask)) list = logit_key(kind == 0 ? -INFINITY : __int_as_float(0x7fffffff), j0 + __fns(mask, 0, nth + 1));
-      have += __popc(mask);
+    for (int j0 = 0; j0 < n && have < top; j0 += 32 * kAhead) {
+      float x[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) x[i] = j0 + 32 * i + lane < n ? z[j0 + 32 * i + lane] : 0.f;
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int first = j0 + 32 * i;
+        const uint32_t mask = __ballot_sync(0xffffffffu, first + lane < n && (kind == 0 ? x[i] == -INFINITY : x[i] != x[i]));
+        const int nth = lane - have;      // this lane's place is the nth of them
+        if (nth >= 0 && nth < __popc(mask)) list = logit_key(kind == 0 ? -INFINITY : __int_as_float(0x7fffffff), first + __fns(mask, 0, nth + 1));
+        have += __popc(mask);
+      }
     }
   }
   return list;

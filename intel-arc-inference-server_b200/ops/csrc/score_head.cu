@@ -274,12 +274,13 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
 }
 
 // ------------------------------------------------------------------ a row's tiles together
-// A CTA takes eight rows: a warp reads four parts of all of them at a time (whole lines), then the lanes' and the warps' results are joined,
+// (Here and below: no __restrict__ on what the kernel before wrote.  These kernels are launched while it still runs, and a read-only load is for
+// memory that nothing writes from a kernel's launch on.)  A CTA takes eight rows: a warp reads four parts of all of them at a time (whole lines), then the lanes' and the warps' results are joined,
 // always in the same order.
 constexpr int kJoinRows = 8, kJoinWarps = 16;
-__global__ void __launch_bounds__(32 * kJoinWarps) score_join_kernel(const float4* __restrict__ part, int parts, const float* __restrict__ token_z,
-                                                                     const int* __restrict__ tokens, int m, int n, float* __restrict__ logprob,
-                                                                     float* __restrict__ entropy) {
+__global__ void __launch_bounds__(32 * kJoinWarps) score_join_kernel(const float4* part, int parts, const float* token_z,
+                                                                     const int* tokens, int m, int n, float* logprob,
+                                                                     float* entropy) {
   __shared__ LogStat sh[kJoinWarps][kJoinRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = blockIdx.x * kJoinRows + lane % kJoinRows;
   pdl_wait();
@@ -308,10 +309,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) score_join_kernel(const float
 
 // A CTA takes a row: its parts joined, and the alternatives from the maxima of its chunks and the few chunks that matter.
 constexpr int kAltThreads = 256, kAltWarps = kAltThreads / 32, kAltChunks = 1024;
-__global__ void __launch_bounds__(kAltThreads) score_alternatives_kernel(const float4* __restrict__ part, int parts, const float* __restrict__ token_z,
-                                                                         const int* __restrict__ tokens, int m, int n, const float* __restrict__ z, long long ldz,
-                                                                         const float* __restrict__ largest, int ldc, int top, float* __restrict__ logprob,
-                                                                         float* __restrict__ entropy, int* __restrict__ top_ids, float* __restrict__ top_logprobs) {
+__global__ void __launch_bounds__(kAltThreads) score_alternatives_kernel(const float4* part, int parts, const float* token_z,
+                                                                         const int* tokens, int m, int n, const float* z, long long ldz,
+                                                                         const float* largest, int ldc, int top, float* logprob,
+                                                                         float* entropy, int* top_ids, float* top_logprobs) {
   __shared__ LogStat stat[kAltWarps];
   __shared__ float best_of[kAltWarps][32];
   __shared__ unsigned long long lists[kAltWarps][32];
@@ -393,8 +394,8 @@ __global__ void __launch_bounds__(kAltThreads) score_alternatives_kernel(const f
 // ------------------------------------------------------------------ rows as int8 with a scale per row
 // s = max|x| / 127, q = rint(x (1 / s)): 8 bits a value, off by at most s / 2.  A row with a NaN or an infinity has the scale NaN, and so
 // have its logits; no scale is below 2^-126, whose inverse is finite.  One CTA per row, 16 bytes a thread and step.
-__global__ void __launch_bounds__(256) quant_kernel(const __nv_bfloat16* __restrict__ x, long long ldx, int k, int8_t* __restrict__ q, long long ldq,
-                                                    float* __restrict__ scale) {
+__global__ void __launch_bounds__(256) quant_kernel(const __nv_bfloat16* x, long long ldx, int k, int8_t* q, long long ldq,
+                                                    float* scale) {
   __shared__ float part[8];
   pdl_wait();
   const uint4* row = reinterpret_cast<const uint4*>(x + blockIdx.x * ldx);
@@ -402,7 +403,7 @@ __global__ void __launch_bounds__(256) quant_kernel(const __nv_bfloat16* __restr
   const __nv_bfloat16* end = x + blockIdx.x * ldx + vecs * 8;
   float largest = 0.f;
   for (int i = threadIdx.x; i < vecs; i += 256) {
-    const uint4 v = __ldg(row + i);
+    const uint4 v = row[i];
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) largest = max_nan(largest, max_nan(fabsf(bf16_lo(w[j])), fabsf(bf16_hi(w[j]))));
@@ -419,7 +420,7 @@ __global__ void __launch_bounds__(256) quant_kernel(const __nv_bfloat16* __restr
   const float s = fmaxf(largest / 127.f, 1.17549435e-38f), inv = finite ? 1.f / s : 0.f;
   int8_t* out = q + blockIdx.x * ldq;
   for (int i = threadIdx.x; i < vecs; i += 256) {
-    const uint4 v = __ldg(row + i);
+    const uint4 v = row[i];
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
     uint32_t o[2] = {0, 0};
 #pragma unroll

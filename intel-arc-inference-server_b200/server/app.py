@@ -26,7 +26,7 @@ import numpy as np
 from ..native import host as H
 from .chat_template import ChatTemplate
 from .iface import EngineIface, TokIface
-from .logprobs import Entry, chat_block, host_logprob, text_block
+from .logprobs import Entry, Score, chat_block, host_logprob, text_block
 
 
 @dataclass
@@ -300,7 +300,7 @@ class Server:
         if got is None:
             got = [host_logprob(np.asarray(self.engine.logits(slot, row))[: self.engine.vocab_size], tok, top) for slot, row, tok in want]
         got = iter(got)
-        return [next(got) if s.req.logprobs >= 0 else None for s, _, _ in items]
+        return [Score(g.logprob, g.top[: s.req.logprobs]) if s.req.logprobs >= 0 and (g := next(got)) else None for s, _, _ in items]
 
     def _sample(self, s: Session, logits=None, row: int = 0) -> int:
         """The request's next token from its logits row: on the device when the engine has a sampler (only the
@@ -519,9 +519,10 @@ class Server:
                     d if d["kind"] == "call" else None, d.get("index", 0), "", None, ids, self._tell(s)))
                 ids = []
 
-    def _tell(self, s: Session):
-        """Log probabilities of the tokens that no frame has carried yet, in the endpoint's form; ``None`` where none are asked for."""
-        if s.req.logprobs < 0 or s.told == len(s.entries):
+    def _tell(self, s: Session, whole: bool = False):
+        """Log probabilities of the tokens that no frame has carried yet, in the endpoint's form; ``None`` where none are asked for, and in
+        frames (not in a ``whole`` response) where there are none."""
+        if s.req.logprobs < 0 or s.told == len(s.entries) and not whole:
             return None
         new, s.told = s.entries[s.told:], len(s.entries)
         if s.req.chat:
@@ -579,7 +580,7 @@ class Server:
                 self.http.end_stream(s.http_id)
             else:
                 body = H.completion_response(r, s.rid, s.created, self.o.model_name, s.content, s.reasoning, s.calls,
-                                             s.finish_reason, usage[0], usage[1], usage[2], s.out_ids, self._tell(s))
+                                             s.finish_reason, usage[0], usage[1], usage[2], s.out_ids, self._tell(s, whole=True))
                 self.http.respond(s.http_id, 200, "application/json", body)
         else:
             self.http.respond(s.http_id, 499, "application/json", "{}")

@@ -188,9 +188,12 @@ def test_rows_that_leave_nothing():
     z[13] = INF
     t[14], t[15] = -1, n
     check(LP.token_logprobs(z, t, top), z, t, top)
-    wide = torch.full((3, 200000), -INF, device="cuda")
+    wide = torch.full((6, 200000), -INF, device="cuda")
     wide[1, 199999], wide[2, 77777] = 1.0, NAN
-    tw = torch.tensor([5, 199999, 3], dtype=torch.int32, device="cuda")
+    wide[3] = NAN                                 # no number at all; three banned ids far in; numbers, a banned id and the rest NaN
+    wide[4] = NAN; wide[4, [1000, 1001, 199990]] = -INF
+    wide[5] = NAN; wide[5, 150000:150004] = 1.0; wide[5, 7] = -INF
+    tw = torch.tensor([5, 199999, 3, 0, 1000, 7], dtype=torch.int32, device="cuda")
     check(LP.token_logprobs(wide, tw, 32), wide, tw, 32)
 
 

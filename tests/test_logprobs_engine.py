@@ -207,7 +207,7 @@ def post(port, body):
     return r.status, json.loads(data)
 
 
-@pytest.mark.parametrize("spec,prefix", [("off", False), ("lookup", True), ("mtp", False)])
+@pytest.mark.parametrize("spec,prefix", [("off", False), ("lookup", True), ("mtp", False), ("dflash", True)])
 def test_generated_text_scored_again(spec, prefix):
     """Tokens that were generated with log probabilities, then scored as an echoed prompt: decode steps and the prompt pass, two kernels and two
     heads, say the same to rounding of the activations (bf16, as above)."""
@@ -221,7 +221,7 @@ def test_generated_text_scored_again(spec, prefix):
     cfg = dataclasses.replace(preset("small-dense"), mtp_layers=1, vocab=259, name="small-dense-bytes")
     eng = Engine(random_weights(cfg, device="cuda", seed=8), max_seqs=2, max_len=1024, extra_kv_layers=2)
     adapter = EngineAdapter(eng, eos_ids=())
-    if spec == "mtp":
+    if spec in ("mtp", "dflash"):
         adapter = SpecAdapter(adapter, spec, 3)
     store = PrefixStore(eng, host_gb=0.05, block_tokens=64) if prefix else None
     srv = Server(adapter, ByteTok(), ChatTemplate(), ServerOptions(model_name=cfg.name, spec=spec, spec_max=3), prefix=store).start()

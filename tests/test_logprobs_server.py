@@ -185,6 +185,24 @@ def test_engine_scores_are_used(server):
     assert eng.calls == 3
 
 
+def test_sessions_of_a_step_get_what_they_asked_for(server):
+    from types import SimpleNamespace as N
+    srv, eng = server(engine=Plain)
+    eng._logits = {0: [eng._row(7), eng._row(9)], 1: [eng._row(8)]}
+    of = lambda slot, n: N(slot=slot, req=N(logprobs=n))      # noqa: E731
+    a, b, c = of(0, 1), of(1, 5), of(0, -1)
+    got = srv._logprobs([(a, 1, 9), (c, 0, 7), (b, 0, 8), (a, 0, 3)])
+    assert [g and len(g.top) for g in got] == [1, None, 5, 1] and got[0].top[0][0] == 9 and got[2].top[0][0] == 8
+    assert close(got[0].logprob, BEST) and close(got[3].logprob, REST)
+    assert srv._logprobs([(c, 0, 1)]) == [None]
+
+
+def test_a_response_without_tokens(server):
+    srv, _ = server({enc("ab"): [2]})
+    ch = post(srv.port, "/v1/completions", {"prompt": "ab", "logprobs": 1})[1]["choices"][0]
+    assert ch["text"] == "" and ch["logprobs"] == {"tokens": [], "token_logprobs": [], "top_logprobs": [], "text_offset": []}
+
+
 class Prefix:
     """Hands out half of a prompt as cached."""
     asked = None
