@@ -406,6 +406,11 @@ __device__ __forceinline__ void store_row_vec(uint8_t* xr, int T, int row, int v
     return (int)cudaMemcpyToSymbol(b2::g_host_flag, &pinned_word, sizeof(pinned_word));     \
   }
 
+static inline bool b2_no_pdl() {      // measurement switch: plain stream order
+  static const bool off = getenv("B2_NO_PDL") != nullptr;
+  return off;
+}
+
 template <typename... KArgs, typename... Args>
 static inline int b2_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                             bool pdl, Args... args) {
@@ -418,7 +423,6 @@ static inline int b2_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, siz
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  static const bool no_pdl = getenv("B2_NO_PDL") != nullptr;  // measurement switch: plain stream order
-  cfg.numAttrs = (pdl && !no_pdl) ? 1 : 0;
+  cfg.numAttrs = (pdl && !b2_no_pdl()) ? 1 : 0;
   return (int)cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
 }
