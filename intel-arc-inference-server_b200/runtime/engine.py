@@ -439,9 +439,10 @@ class Engine:
     def score(self, ids: Sequence[int], top: int = 0, slot: int = 0) -> List[TokenScore]:
         """Log probability, entropy and top alternatives of every token of ``ids`` behind the ones before it (the first one's are those
         of no prediction: NaN and nothing).  The slot starts afresh and holds ``ids`` afterwards."""
-        self.reset(slot)
         scores = self.prompt_scores(ids, top)
-        self.prefill(slot, ids, scores=scores)
+        self.reset(slot)
+        if scores.ids:
+            self.prefill(slot, ids, scores=scores)
         return scores.read()
 
     def logprobs(self, tokens: Sequence[int], top: int = 0, logits: Optional[torch.Tensor] = None) -> List[TokenScore]:

@@ -179,7 +179,10 @@ class Server:
         req.max_tokens = max_new
         if req.echo and req.logprobs >= 0:
             make = getattr(self.engine, "prompt_scores", None)
-            s.scores = make(ids, req.logprobs) if make is not None else None
+            try:
+                s.scores = make(ids, req.logprobs) if make is not None else None
+            except Exception as e:  # noqa: BLE001   (no room for the results, ids that are none: this request's matter)
+                return self._error(hid, 400, f"cannot score the prompt: {e}")
             if s.scores is None:
                 return self._error(hid, 400, "log probabilities of the prompt are not available on this server")
         preferred = self.prefix.preferred_slot(ids) if self.prefix else -1

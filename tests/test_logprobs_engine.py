@@ -164,7 +164,9 @@ def test_portions_and_refusals():
         eng.prefill(0, ids[1:80], scores=scores)
     with pytest.raises(ValueError, match="at most"):
         eng.prompt_scores(ids, 33)
-    assert eng.score([5], 2) == eng.score([5], 2) or math.isnan(eng.score([5], 2)[0].logprob)
+    assert math.isnan(eng.score([5], 2)[0].logprob) and len(eng.score([5], 2)) == 1 and eng.score([], 2) == []
+    with pytest.raises((ValueError, RuntimeError, OverflowError)):
+        eng.prompt_scores([5, 1 << 32])
 
 
 # ------------------------------------------------------------------ steps

@@ -144,6 +144,18 @@ def test_requests_that_are_refused(server):
     assert st == 200 and all(close(x, BEST) for x in body["choices"][0]["logprobs"]["token_logprobs"])
 
 
+class Full(MockEngine):
+    def prompt_scores(self, ids, top=0):
+        raise RuntimeError("no room")
+
+
+def test_scores_that_cannot_be_made_fail_their_request(server):
+    srv, _ = server(engine=Full)
+    st, body = post(srv.port, "/v1/completions", {"prompt": "xyz", "echo": True, "logprobs": 1, "max_tokens": 1})
+    assert st == 400 and "no room" in body["error"]["message"]
+    assert post(srv.port, "/v1/completions", {"prompt": "xyz", "max_tokens": 1})[0] == 200
+
+
 def test_fields_of_requests():
     one = lambda chat, **kw: H.parse_request(json.dumps({"messages": MSGS, "prompt": "p", **kw}), chat)      # noqa: E731
     assert one(True).logprobs == -1 and one(False).logprobs == -1 and not one(False).echo
