@@ -87,10 +87,17 @@ __device__ __forceinline__ bool tile_at(const ScoreParams& p, int i, Tile& t) {
   return t.col0 < p.n;
 }
 
-// ALT: logits and their maxima are stored.  map_g: W in boxes of 16 (PAIR) or 32 rows, for narrow tiles.
+// Rows of x that a CTA fetches of a block of 128 that begins at row0: those that there are, in eights.  (Rows outside the matrix cost a copy more than
+// rows inside: with boxes of 128 for all, 1 row x 102400 x 2048 took 100 us, 16 rows 87, 77 rows 76; with these 74 to 76.)  What the rest
+// of the block holds then goes to rows of the accumulator that nobody reads.
+__device__ __forceinline__ int rows_at(const ScoreParams& p, int row0) { return min(BM, max(0, (p.m - row0 + 7) / 8 * 8)); }
+
+// ALT: logits and their maxima are stored.  map_e: the rows behind the last whole block of 128 of x; map_g: W in boxes of 16 (PAIR) or 32
+// rows, for narrow tiles.
 template <bool I8, bool ALT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
-score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_g, const ScoreParams p) {
+score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_e, const __grid_constant__ CUtensorMap map_w,
+             const __grid_constant__ CUtensorMap map_g, const ScoreParams p) {
   using F = Form<PAIR>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float scales[2][I8 ? BN : 1];      // of the columns of a tile and of the next
@@ -135,23 +142,25 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
       Tile t;
       for (int i = 0; ok && tile_at<PAIR>(p, i, t); ++i) {
         const int row0 = t.mt * F::ROWS + rank * BM, mine = PAIR ? t.width / 2 : t.width, col0 = t.col0 + rank * mine;
+        const int rows = rows_at(p, row0);
+        const CUtensorMap* const map = rows == BM ? &map_x : &map_e;
+        const uint32_t bytes = PAIR ? (rows + rows_at(p, row0 + BM) + 2 * mine) * kStageRow : (rows + mine) * kStageRow;      // (of the even CTA: both CTAs')
         for (int kb = 0; kb < p.kb; ++kb) {
           if (round > 0) ok = mbar_wait_lone(empty0 + 8 * s, (round - 1) & 1, ERR_GEMM_EMPTY_WAIT);
           if (!ok) break;
           const uint32_t at = smem + s * F::STAGE;
           const int k = kb * (I8 ? kStageRow : kStageRow / 2);
-          const uint32_t bytes = F::X_BYTES + mine * kStageRow;
           if (PAIR) {
             const uint32_t bar = map_rank0(full0 + 8 * s);
-            if (rank == 0) mbar_expect_tx(full0 + 8 * s, 2 * bytes);
-            tma_load_2d_pair(at, &map_x, k, row0, bar);
+            if (rank == 0) mbar_expect_tx(full0 + 8 * s, bytes);
+            if (rows) tma_load_2d_pair(at, map, k, row0, bar);
             if (t.width == BN) tma_load_2d_pair(at + F::X_BYTES, &map_w, k, col0, bar);
             else
               for (int j = 0; j < mine; j += kGrain / 2) tma_load_2d_pair(at + F::X_BYTES + j * kStageRow, &map_g, k, col0 + j, bar);
           } else {
             const uint32_t bar = full0 + 8 * s;
             mbar_expect_tx(bar, bytes);
-            tma_load_2d(at, &map_x, k, row0, bar);
+            tma_load_2d(at, map, k, row0, bar);
             if (t.width == BN) tma_load_2d(at + F::X_BYTES, &map_w, k, col0, bar);
             else
               for (int j = 0; j < mine; j += kGrain) tma_load_2d(at + F::X_BYTES + j * kStageRow, &map_g, k, col0 + j, bar);
@@ -486,7 +495,7 @@ int layout_of(int m, int n, Layout& l) {
 }
 
 template <bool I8, bool ALT, bool PAIR>
-int launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mg, const ScoreParams& p, int clusters, cudaStream_t st) {
+int launch(const CUtensorMap& mx, const CUtensorMap& me, const CUtensorMap& mw, const CUtensorMap& mg, const ScoreParams& p, int clusters, cudaStream_t st) {
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -513,11 +522,11 @@ int launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mg, 
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  return (int)cudaLaunchKernelEx(&cfg, score_kernel<I8, ALT, PAIR>, mx, mw, mg, p);
+  return (int)cudaLaunchKernelEx(&cfg, score_kernel<I8, ALT, PAIR>, mx, me, mw, mg, p);
 }
 template <bool I8, bool ALT>
-int launch(const CUtensorMap& mx, const CUtensorMap& mw, const CUtensorMap& mg, const ScoreParams& p, const Layout& l, cudaStream_t st) {
-  return l.pair ? launch<I8, ALT, true>(mx, mw, mg, p, l.clusters, st) : launch<I8, ALT, false>(mx, mw, mg, p, l.clusters, st);
+int launch(const CUtensorMap& mx, const CUtensorMap& me, const CUtensorMap& mw, const CUtensorMap& mg, const ScoreParams& p, const Layout& l, cudaStream_t st) {
+  return l.pair ? launch<I8, ALT, true>(mx, me, mw, mg, p, l.clusters, st) : launch<I8, ALT, false>(mx, me, mw, mg, p, l.clusters, st);
 }
 
 // The workspace of a call, in floats from its beginning: sums, tokens' logits; alternatives: logits and their maxima; int8: rows and scales.
@@ -564,9 +573,13 @@ extern "C" int b2_score(const void* x, long long ldx, const void* w, long long l
   p.z = work + r.z; p.ldz = (long long)r.chunks * kChunk;
   p.largest = work + r.largest; p.ldc = r.chunks;
   void* q = work + r.q;
-  CUtensorMap mx, mw, mg;
-  int rc = i8 ? make_map(&mx, q, true, m, k, r.ldq, BM) : make_map(&mx, x, false, m, k, ldx, BM);
-  // (a map is a microsecond of the host's: ranges that are narrower than a tile have no whole ones)
+  // (a map is a microsecond of the host's: none is made that no block of x, or no tile in ranges that are narrower than one, would use)
+  CUtensorMap mx, me, mw, mg;
+  const auto map_of_x = [&](CUtensorMap* to, int box) { return i8 ? make_map(to, q, true, m, k, r.ldq, box) : make_map(to, x, false, m, k, ldx, box); };
+  int rc = m >= BM ? map_of_x(&mx, BM) : 0;
+  if (!rc && m % BM) rc = map_of_x(&me, (m % BM + 7) / 8 * 8);
+  if (m < BM) mx = me;
+  if (m % BM == 0) me = mx;
   const bool narrow = l.ranges && ((n + kGrain - 1) / kGrain + l.ranges - 1) / l.ranges < BN / kGrain;
   if (!rc && !narrow) rc = make_map(&mw, w, i8, n, k, ldw, l.pair ? BN / 2 : BN);
   if (!rc && l.ranges) rc = make_map(&mg, w, i8, n, k, ldw, l.pair ? kGrain / 2 : kGrain);
@@ -577,8 +590,8 @@ extern "C" int b2_score(const void* x, long long ldx, const void* w, long long l
     rc = b2_launch(quant_kernel, dim3(m), dim3(256), 0, st, true, (const __nv_bfloat16*)x, ldx, k, (int8_t*)q, (long long)r.ldq, work + r.scale);
     if (rc) return rc;
   }
-  if (top) rc = i8 ? launch<true, true>(mx, mw, mg, p, l, st) : launch<false, true>(mx, mw, mg, p, l, st);
-  else rc = i8 ? launch<true, false>(mx, mw, mg, p, l, st) : launch<false, false>(mx, mw, mg, p, l, st);
+  if (top) rc = i8 ? launch<true, true>(mx, me, mw, mg, p, l, st) : launch<false, true>(mx, me, mw, mg, p, l, st);
+  else rc = i8 ? launch<true, false>(mx, me, mw, mg, p, l, st) : launch<false, false>(mx, me, mw, mg, p, l, st);
   if (rc) return rc;
   if (top)
     return b2_launch(score_alternatives_kernel, dim3(m), dim3(kAltThreads), 0, st, true, p.part, l.parts, p.token_z, tokens, m, n, p.z, p.ldz, p.largest, p.ldc,
