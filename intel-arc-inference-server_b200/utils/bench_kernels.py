@@ -2,6 +2,7 @@
 
     python -m b200serve.utils.bench_kernels gemv            # W4A16 weight-streaming kernel, 27B shapes
     python -m b200serve.utils.bench_kernels gemm            # tcgen05 GEMMs, 27B prefill shapes
+    python -m b200serve.utils.bench_kernels logprob         # log probabilities: rows of logits, rows through both heads
 
 Weights rotate through enough copies to exceed the 126 MB L2 between launches, so
 every launch streams from HBM.  Fractions are of the measured peaks in
@@ -113,6 +114,33 @@ def bench_gemm():
     K.check_status()
 
 
+def bench_logprob():
+    """Rows of 151,936 logits in a graph (small calls are shorter than the host's part of them), and prompts through the 27B shape's heads."""
+    from ..ops import logprob as LP
+    hbm, tflops, src = peaks()
+    for m in (1, 8, 64, 200, 500):
+        z, t = torch.randn(m, 151936, device="cuda") * 2.5, torch.zeros(m, dtype=torch.int32, device="cuda")
+        for top in (0, 10):
+            out, g = LP.Logprobs.empty(m, top, "cuda"), torch.cuda.CUDAGraph()
+            LP.token_logprobs(z, t, out=out)
+            with torch.cuda.graph(g):
+                for _ in range(10):
+                    LP.token_logprobs(z, t, out=out)
+            us = time_ms(g.replay) * 100
+            print(f"token_logprobs {m} x 151936, {top} alternatives: {us:.1f} us, {z.numel() * 4 / us / 1e3 / hbm:.2f} of {src} copy")
+    n, k = 151936, 5120
+    head = torch.empty(n, k, dtype=torch.bfloat16, device="cuda").normal_(0, 0.02)
+    w8, ws = (head.float() * 1500).round_().clamp_(-127, 127).to(torch.int8), torch.full((n,), 1 / 1500, device="cuda")
+    for m in (1, 64, 300, 1024, 4096):
+        x, t = torch.randn(m, k, device="cuda").to(torch.bfloat16), torch.zeros(m, dtype=torch.int32, device="cuda")
+        for name, call, size in (("bf16", lambda top: LP.score(x, head, t, top), 2), ("int8", lambda top: LP.score_i8(x, (w8, ws), t, top), 1)):
+            floor = max((m + n) * k * size / hbm / 1e3, 2 * m * n * k * size / 2 / tflops / 1e6)
+            for top in (0, 5):
+                us = time_ms(lambda: call(top), iters=10) * 1e3
+                print(f"score {name} {m} x {n} x {k}, {top} alternatives: {us:.0f} us, {floor / us:.2f} of its floor ({src} copy, product)")
+    K.check_status()
+
+
 if __name__ == "__main__":
     what = sys.argv[1] if len(sys.argv) > 1 else "gemv"
     if what == "gemv-one":      # one shape, one M, few launches: the target of an ncu capture
@@ -176,4 +204,4 @@ if __name__ == "__main__":
     elif what == "gemv-graph":  # back-to-back launches inside a CUDA graph
         bench_gemv((1, 4, 8), graph=True)
     else:
-        {"gemv": bench_gemv, "gemm": bench_gemm}[what]()
+        {"gemv": bench_gemv, "gemm": bench_gemm, "logprob": bench_logprob}[what]()
