@@ -39,6 +39,7 @@ struct Form {
   static constexpr int STAGES = PAIR ? 6 : 4;
   static constexpr int SMEM = STAGES * STAGE + 1024 + 256;          // + alignment, barriers
 };
+constexpr int kOutBytes = BM * kChunk * 4;      // alternatives: the warps' 32 x 32 logits on their way out
 
 struct ScoreParams {
   int m, n, kb;             // kb: stages of k
@@ -47,9 +48,7 @@ struct ScoreParams {
   const int* tokens;        // [m]
   float4* part;             // [range, or column of tiles][m]: maximum and sums of a row's logits
   float* token_z;           // [m] logit of the row's token, where it has one
-  float* z;                 // alternatives: logits [m][ldz], and the largest of every kChunk [m][ldc]
-  long long ldz;
-  float* largest;
+  float* largest;           // alternatives: the largest of every kChunk logits [m][ldc]
   int ldc;
 };
 
@@ -92,16 +91,16 @@ __device__ __forceinline__ bool tile_at(const ScoreParams& p, int i, Tile& t) {
 // of the block holds then goes to rows of the accumulator that nobody reads.
 __device__ __forceinline__ int rows_at(const ScoreParams& p, int row0) { return min(BM, max(0, (p.m - row0 + 7) / 8 * 8)); }
 
-// ALT: logits and their maxima are stored.  map_e: the rows behind the last whole block of 128 of x; map_g: W in boxes of 16 (PAIR) or 32
+// ALT: logits (map_z, 32 x 32 at a time) and their maxima are stored.  map_e: the rows behind the last whole block of 128 of x; map_g: W in boxes of 16 (PAIR) or 32
 // rows, for narrow tiles.
 template <bool I8, bool ALT, bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
 score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_e, const __grid_constant__ CUtensorMap map_w,
-             const __grid_constant__ CUtensorMap map_g, const ScoreParams p) {
+             const __grid_constant__ CUtensorMap map_g, const __grid_constant__ CUtensorMap map_z, const ScoreParams p) {
   using F = Form<PAIR>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ float scales[2][I8 ? BN : 1];      // of the columns of a tile and of the next
-  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = smem + F::STAGES * F::STAGE;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023u) & ~1023u, bars = smem + F::STAGES * F::STAGE + (ALT ? kOutBytes : 0);
   const uint32_t full0 = bars, empty0 = full0 + 8 * F::STAGES, done0 = empty0 + 8 * F::STAGES, read0 = done0 + 16, slot = read0 + 16;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = PAIR ? (int)cluster_rank() : 0;
 
@@ -212,6 +211,7 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
     }
   } else {
     const int quarter = warp & 3;      // of the lanes of tensor memory, this warp's
+    const uint32_t out = smem + F::STAGES * F::STAGE + quarter * (kOutBytes / 4);      // (a multiple of 1024; the barriers are behind it)
     bool ok = true;
     Tile t;
     LogStat s{-INFINITY, 0.f, 0.f};
@@ -254,11 +254,23 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
           for (int j = 1; j < 32; ++j) mine = token == n0 + j ? z[j] : mine;
           p.token_z[row] = mine;
         }
-        if (ALT && there) {
-          p.largest[(long long)row * p.ldc + n0 / kChunk] = largest;
-          float4* dst = reinterpret_cast<float4*>(p.z + row * p.ldz + n0);      // (to the end of the buffer's row: it is a multiple of 32)
+        if (ALT) {
+          // Through shared memory (a row's 128 bytes in the order of the 128-byte swizzle) and out as one copy, which leaves out rows that are not
+          // there: stored by the threads, 16 bytes of 32 rows at a time, the logits took 1024 int8 rows x 151936 x 5120 from 626 to 903 us.
+          if (there) p.largest[(long long)row * p.ldc + n0 / kChunk] = largest;
+          if (lane == 0) tma_store_wait_read0();
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j) dst[j] = make_float4(z[4 * j], z[4 * j + 1], z[4 * j + 2], z[4 * j + 3]);
+          for (int j = 0; j < 8; ++j)
+            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(out + lane * 128 + ((j ^ (lane & 7)) << 4)), "f"(z[4 * j]), "f"(z[4 * j + 1]),
+                         "f"(z[4 * j + 2]), "f"(z[4 * j + 3])
+                         : "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_2d(&map_z, out, n0, row0);
+            tma_store_commit();
+          }
         }
       }
       tc_fence_before();
@@ -269,6 +281,7 @@ score_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ 
       }
       if (there && (!p.ranges || t.col0 + BN >= t.end)) p.part[(long long)t.part * p.m + row] = make_float4(s.m, s.s, s.t, 0.f);
     }
+    if (ALT && lane == 0) tma_store_wait0();
   }
 
   // every thread arrives here on every path
@@ -458,14 +471,14 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-// box_rows rows x 128 bytes of a matrix [rows][cols], rows ld elements apart; what lies outside reads as zeros
-int make_map(CUtensorMap* map, const void* ptr, bool i8, int rows, int cols, long long ld, int box_rows) {
+// box_rows rows x 128 bytes of a matrix [rows][cols] of elements of 1 (int8), 2 (bf16) or 4 (fp32) bytes, rows ld elements apart; what lies outside
+// reads as zeros and is not written
+int make_map(CUtensorMap* map, const void* ptr, int size, int rows, long long cols, long long ld, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return -100;
-  const int size = i8 ? 1 : 2;
   const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld * size};
   const cuuint32_t box[2] = {(cuuint32_t)(kStageRow / size), (cuuint32_t)box_rows}, step[2] = {1, 1};
-  const CUresult r = fn(map, i8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), dims, strides, box, step,
+  const CUresult r = fn(map, size == 1 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : size == 2 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(ptr), dims, strides, box, step,
                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? 0 : -101 - (int)r;
 }
@@ -495,19 +508,20 @@ int layout_of(int m, int n, Layout& l) {
 }
 
 template <bool I8, bool ALT, bool PAIR>
-int launch(const CUtensorMap& mx, const CUtensorMap& me, const CUtensorMap& mw, const CUtensorMap& mg, const ScoreParams& p, int clusters, cudaStream_t st) {
+int launch(const CUtensorMap& mx, const CUtensorMap& me, const CUtensorMap& mw, const CUtensorMap& mg, const CUtensorMap& mz, const ScoreParams& p, int clusters, cudaStream_t st) {
+  constexpr int kSmem = Form<PAIR>::SMEM + (ALT ? kOutBytes : 0);
   static bool configured[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (!configured[dev & 63]) {
-    const cudaError_t e = cudaFuncSetAttribute(score_kernel<I8, ALT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Form<PAIR>::SMEM);
+    const cudaError_t e = cudaFuncSetAttribute(score_kernel<I8, ALT, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return (int)e;
     configured[dev & 63] = true;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(PAIR ? 2 * clusters : clusters);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Form<PAIR>::SMEM;
+  cfg.dynamicSmemBytes = kSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   cfg.attrs = attr;
@@ -522,11 +536,11 @@ int launch(const CUtensorMap& mx, const CUtensorMap& me, const CUtensorMap& mw, 
     attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
     ++cfg.numAttrs;
   }
-  return (int)cudaLaunchKernelEx(&cfg, score_kernel<I8, ALT, PAIR>, mx, me, mw, mg, p);
+  return (int)cudaLaunchKernelEx(&cfg, score_kernel<I8, ALT, PAIR>, mx, me, mw, mg, mz, p);
 }
 template <bool I8, bool ALT>
-int launch(const CUtensorMap& mx, const CUtensorMap& me, const CUtensorMap& mw, const CUtensorMap& mg, const ScoreParams& p, const Layout& l, cudaStream_t st) {
-  return l.pair ? launch<I8, ALT, true>(mx, me, mw, mg, p, l.clusters, st) : launch<I8, ALT, false>(mx, me, mw, mg, p, l.clusters, st);
+int launch(const CUtensorMap& mx, const CUtensorMap& me, const CUtensorMap& mw, const CUtensorMap& mg, const CUtensorMap& mz, const ScoreParams& p, const Layout& l, cudaStream_t st) {
+  return l.pair ? launch<I8, ALT, true>(mx, me, mw, mg, mz, p, l.clusters, st) : launch<I8, ALT, false>(mx, me, mw, mg, mz, p, l.clusters, st);
 }
 
 // The workspace of a call, in floats from its beginning: sums, tokens' logits; alternatives: logits and their maxima; int8: rows and scales.
@@ -570,31 +584,33 @@ extern "C" int b2_score(const void* x, long long ldx, const void* w, long long l
   p.ranges = l.ranges;
   p.x_scale = work + r.scale; p.w_scale = w_scale; p.tokens = tokens;
   p.part = (float4*)work; p.token_z = work + r.token_z;
-  p.z = work + r.z; p.ldz = (long long)r.chunks * kChunk;
   p.largest = work + r.largest; p.ldc = r.chunks;
   void* q = work + r.q;
   // (a map is a microsecond of the host's: none is made that no block of x, or no tile in ranges that are narrower than one, would use)
-  CUtensorMap mx, me, mw, mg;
-  const auto map_of_x = [&](CUtensorMap* to, int box) { return i8 ? make_map(to, q, true, m, k, r.ldq, box) : make_map(to, x, false, m, k, ldx, box); };
+  CUtensorMap mx, me, mw, mg, mz;
+  const auto map_of_x = [&](CUtensorMap* to, int box) { return i8 ? make_map(to, q, 1, m, k, r.ldq, box) : make_map(to, x, 2, m, k, ldx, box); };
   int rc = m >= BM ? map_of_x(&mx, BM) : 0;
   if (!rc && m % BM) rc = map_of_x(&me, (m % BM + 7) / 8 * 8);
   if (m < BM) mx = me;
   if (m % BM == 0) me = mx;
   const bool narrow = l.ranges && ((n + kGrain - 1) / kGrain + l.ranges - 1) / l.ranges < BN / kGrain;
-  if (!rc && !narrow) rc = make_map(&mw, w, i8, n, k, ldw, l.pair ? BN / 2 : BN);
-  if (!rc && l.ranges) rc = make_map(&mg, w, i8, n, k, ldw, l.pair ? kGrain / 2 : kGrain);
+  if (!rc && !narrow) rc = make_map(&mw, w, size, n, k, ldw, l.pair ? BN / 2 : BN);
+  if (!rc && l.ranges) rc = make_map(&mg, w, size, n, k, ldw, l.pair ? kGrain / 2 : kGrain);
   if (narrow) mw = mg;
   if (!l.ranges) mg = mw;
+  mz = mw;
+  const long long ldz = (long long)r.chunks * kChunk;
+  if (!rc && top) rc = make_map(&mz, work + r.z, 4, m, ldz, ldz, 32);
   if (rc) return rc;
   if (i8) {
     rc = b2_launch(quant_kernel, dim3(m), dim3(256), 0, st, true, (const __nv_bfloat16*)x, ldx, k, (int8_t*)q, (long long)r.ldq, work + r.scale);
     if (rc) return rc;
   }
-  if (top) rc = i8 ? launch<true, true>(mx, me, mw, mg, p, l, st) : launch<false, true>(mx, me, mw, mg, p, l, st);
-  else rc = i8 ? launch<true, false>(mx, me, mw, mg, p, l, st) : launch<false, false>(mx, me, mw, mg, p, l, st);
+  if (top) rc = i8 ? launch<true, true>(mx, me, mw, mg, mz, p, l, st) : launch<false, true>(mx, me, mw, mg, mz, p, l, st);
+  else rc = i8 ? launch<true, false>(mx, me, mw, mg, mz, p, l, st) : launch<false, false>(mx, me, mw, mg, mz, p, l, st);
   if (rc) return rc;
   if (top)
-    return b2_launch(score_alternatives_kernel, dim3(m), dim3(kAltThreads), 0, st, true, p.part, l.parts, p.token_z, tokens, m, n, p.z, p.ldz, p.largest, p.ldc,
+    return b2_launch(score_alternatives_kernel, dim3(m), dim3(kAltThreads), 0, st, true, p.part, l.parts, p.token_z, tokens, m, n, work + r.z, ldz, p.largest, p.ldc,
                      top, logprob, entropy, top_ids, top_logprobs);
   return b2_launch(score_join_kernel, dim3((m + kJoinRows - 1) / kJoinRows), dim3(32 * kJoinWarps), 0, st, true, p.part, l.parts, p.token_z, tokens, m, n,
                    logprob, entropy);
