@@ -17,7 +17,7 @@
 // More than about 300 rows are bound by the multiplication: 4096 rows x 151936 x 5120 take 3.6 ms in a short run (1.78 PFLOP/s) and 4.1 under
 // the power cap, int8 1.86 and 2.2 ms; halving the copies of x changes nothing, four warps more for the sums cost 5 %.  Fewer rows are
 // bound by the head's bytes: 77 rows x 102400 x 2048 72 us (5.8 TB/s), 64 rows x 151936 x 5120 260 us with the join (6.0 TB/s).  With
-// the logits stored and read again by logprob.cu (with alternatives it was so once) 900 rows x 151936 x 5120 took 1.41 ms, now 1.23.
+// the logits stored and read again by logprob.cu (with alternatives it was so once) 900 rows x 151936 x 5120 took 1.41 ms, now 1.20.
 #include "common.cuh"
 #include "logprob.cuh"
 #include "pair.cuh"

@@ -74,24 +74,25 @@ def _results(m: int, top: Optional[int], out: Optional[Logprobs], device) -> Log
 
 
 def _check_tokens(tokens: torch.Tensor, m: int, device):
-    if tokens.dtype != torch.int32 or tokens.shape != (m,) or tokens.device != device or not tokens.is_contiguous():
+    if tokens.dtype is not torch.int32 or tokens.shape != (m,) or tokens.device != device or m > 1 and tokens.stride(0) != 1:
         raise ValueError(f"tokens: {m} contiguous int32 ids on {device}")
 
 
 def _rows_of(t: torch.Tensor, dtype, what: str, align: int = 4) -> tuple:
-    """(rows, columns, elements from row to row) of a matrix."""
-    if t.dim() != 2 or t.dtype != dtype or not t.is_cuda:
+    """(rows, columns, elements from row to row, address) of a matrix."""
+    shape = t.shape
+    if len(shape) != 2 or t.dtype is not dtype or not t.is_cuda:
         raise ValueError(f"{what}: rows of {dtype} on a CUDA device")
-    (m, n), (ld, step) = t.shape, t.stride()
+    (m, n), (ld, step), at = shape, t.stride(), t.data_ptr()
     if n > 1 and step != 1:
         raise ValueError(f"{what}: one element after another")
     if m < 2:
         ld = (n + 15) // 16 * 16      # (a lone row's stride says nothing: a multiple of 16 bytes that holds it)
     elif ld < n:
         raise ValueError(f"{what}: rows that do not overlap")
-    if t.data_ptr() % align or ld * t.element_size() % align:
+    if at % align or ld * dtype.itemsize % align:
         raise ValueError(f"{what}: rows begin at multiples of {align} bytes")
-    return m, n, ld
+    return m, n, ld, at
 
 
 @functools.lru_cache(maxsize=None)
@@ -106,7 +107,7 @@ def _entry(name: str, kinds: str, result=ctypes.c_int):
 
 def _elsewhere(device) -> bool:
     """Another device is the current one."""
-    return device.index != torch.cuda.current_device()
+    return device.index != torch._C._cuda_getDevice()
 
 
 def _stream(device) -> int:
@@ -117,7 +118,7 @@ def _stream(device) -> int:
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
     """Rows of fp32 ``logits`` ``[m][vocabulary]`` (any row stride), one int32 token each.  ``out``: results to write, whose width is
     then ``top``."""
-    m, n, ld = _rows_of(logits, torch.float32, "logits")
+    m, n, ld, at = _rows_of(logits, torch.float32, "logits")
     dev = logits.device
     if n < 1:
         raise ValueError("logits of an empty vocabulary")
@@ -129,18 +130,18 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int
         with torch.cuda.device(dev):
             return token_logprobs(logits, tokens, top, out)
     K._check(_entry("b2_logprob_rows", "pliipippppp")(
-        logits.data_ptr(), ld, m, n, tokens.data_ptr(), out.top_ids.shape[1], out.logprob.data_ptr(), out.entropy.data_ptr(),
+        at, ld, m, n, tokens.data_ptr(), out.top_ids.shape[1], out.logprob.data_ptr(), out.entropy.data_ptr(),
         out.top_ids.data_ptr(), out.top_logprobs.data_ptr(), _stream(dev)), "logprob_rows")
     return out
 
 
 def _score(x, w, w_scale, tokens, top: Optional[int], out: Optional[Logprobs]) -> Logprobs:
     i8, dev = w_scale is not None, x.device
-    m, k, ldx = _rows_of(x, torch.bfloat16, "rows", 16)
-    n, kw, ldw = _rows_of(w, torch.int8 if i8 else torch.bfloat16, "head", 16)
+    m, k, ldx, px = _rows_of(x, torch.bfloat16, "rows", 16)
+    n, kw, ldw, pw = _rows_of(w, torch.int8 if i8 else torch.bfloat16, "head", 16)
     if kw != k or n < 1 or w.device != dev:
         raise ValueError(f"head {tuple(w.shape)} on {w.device} against rows {tuple(x.shape)} on {dev}")
-    if k * w.element_size() < 128 or i8 and k > MAX_I8_COLUMNS:
+    if k * (1 if i8 else 2) < 128 or i8 and k > MAX_I8_COLUMNS:
         raise ValueError(f"rows of {k} columns: 128 bytes of the head's type at least" + (f", {MAX_I8_COLUMNS} at most" if i8 else ""))
     _check_tokens(tokens, m, dev)
     out = _results(m, top, out, dev)
@@ -163,11 +164,12 @@ def _score(x, w, w_scale, tokens, top: Optional[int], out: Optional[Logprobs]) -
             if step <= 256 or not top:
                 raise
             step = max(256, step // 512 * 256)      # fewer logits at a time
+    ps, pt, pwork, stream = w_scale.data_ptr() if i8 else None, tokens.data_ptr(), work.data_ptr(), _stream(dev)
     for i in range(0, m, step):
         c = min(step, m - i)
         o = out if c == m else out.rows(i, i + c)
-        K._check(run(x.data_ptr() + 2 * i * ldx, ldx, w.data_ptr(), ldw, w_scale.data_ptr() if i8 else None, c, n, k, tokens.data_ptr() + 4 * i, top,
-                     work.data_ptr(), o.logprob.data_ptr(), o.entropy.data_ptr(), o.top_ids.data_ptr(), o.top_logprobs.data_ptr(), _stream(dev)), "score")
+        K._check(run(px + 2 * i * ldx, ldx, pw, ldw, ps, c, n, k, pt + 4 * i, top, pwork, o.logprob.data_ptr(), o.entropy.data_ptr(),
+                     o.top_ids.data_ptr(), o.top_logprobs.data_ptr(), stream), "score")
         K.launch_count += 2 if i8 else 1      # rows quantised; a row's parts joined
     return out
 
@@ -182,6 +184,6 @@ def score_i8(x: torch.Tensor, head: tuple, tokens: torch.Tensor, top: Optional[i
     """Rows ``x`` ``[m][k]`` bf16 against an int8 lm_head (``[vocabulary][k]``, fp32 scale per row), rows of both at multiples of 16
     bytes: rows are quantised per token (s = max|x| / 127, q = rint(x / s), as the int8 prompt pass does) and logits are (q . w) s s_w."""
     w8, scale = head
-    if scale.dtype != torch.float32 or scale.shape != (w8.shape[0],) or scale.device != x.device or not scale.is_contiguous():
+    if scale.dtype is not torch.float32 or scale.shape != (w8.shape[0],) or scale.device != x.device or not scale.is_contiguous():
         raise ValueError(f"scales of the head: {w8.shape[0]} contiguous fp32 numbers on {x.device}")
     return _score(x, w8, scale, tokens, top, out)
