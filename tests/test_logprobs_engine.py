@@ -244,3 +244,29 @@ def test_generated_text_scored_again(spec, prefix):
         assert b["usage"]["prompt_tokens_details"]["cached_tokens"] == 0
     finally:
         srv.stop()
+
+
+def test_scored_prompt_beside_decode_rows_of_a_mixed_batch_engine():
+    """A model whose prompt portions share batches with decode rows: a scored prompt has its own, and says what the engine says alone."""
+    import threading
+    from b200serve.server.adapter import EngineAdapter
+    from b200serve.server.app import Server, ServerOptions
+    from b200serve.server.chat_template import ChatTemplate
+    from b200serve.server.iface import ByteTok
+    eng = engine("napadra-mini")
+    ids = prompt(eng.cfg, 180, 6)
+    alone = eng.score(ids, 2)
+    eng.reset()
+    srv = Server(EngineAdapter(eng, eos_ids=()), ByteTok(), ChatTemplate(), ServerOptions(prefill_chunk=100)).start()
+    try:
+        other = threading.Thread(target=post, args=(srv.port, {"prompt": prompt(eng.cfg, 90, 7), "max_tokens": 200, "ignore_eos": True, "logprobs": 1}))
+        other.start()
+        st, body = post(srv.port, {"prompt": ids, "max_tokens": 0, "echo": True, "logprobs": 2})
+        other.join()
+        assert st == 200
+        got = body["choices"][0]["logprobs"]["token_logprobs"]
+        assert len(got) == len(ids) and got[0] is None
+        # other portions, so other tiles: rounding of activations, as above
+        assert max(abs(x - y.logprob) for x, y in zip(got[1:], alone[1:])) < 0.1
+    finally:
+        srv.stop()

@@ -215,6 +215,31 @@ def test_a_response_without_tokens(server):
     assert ch["text"] == "" and ch["logprobs"] == {"tokens": [], "token_logprobs": [], "top_logprobs": [], "text_offset": []}
 
 
+class Mixed(MockEngine):
+    """Prompt portions and decode rows as one batch, which notes nothing of a prompt's scores."""
+    mixed_batches = True
+    slow = 0.002
+
+    def step(self, rows):
+        import time
+        time.sleep(self.slow)
+        return super().step(rows)
+
+
+def test_scored_prompts_beside_decode_rows(server):
+    import threading
+    srv, eng = server(engine=Mixed, prefill_chunk=4)
+    busy = threading.Thread(target=post, args=(srv.port, "/v1/completions", {"prompt": "go on", "max_tokens": 150, "ignore_eos": True}))
+    busy.start()
+    text = "a prompt in many portions"
+    got = [post(srv.port, "/v1/completions", {"prompt": text, "max_tokens": 2, "echo": True, "logprobs": 1, "ignore_eos": True})[1]["choices"][0]["logprobs"]
+           for _ in range(2)]
+    busy.join()
+    alone = post(srv.port, "/v1/completions", {"prompt": text, "max_tokens": 2, "echo": True, "logprobs": 1, "ignore_eos": True})[1]["choices"][0]["logprobs"]
+    assert got == [alone, alone] and len(alone["tokens"]) == len(text) + 2
+    assert post(srv.port, "/v1/completions", {"prompt": text, "max_tokens": 2})[0] == 200
+
+
 class Prefix:
     """Hands out half of a prompt as cached."""
     asked = None
