@@ -26,7 +26,7 @@ import numpy as np
 from ..native import host as H
 from .chat_template import ChatTemplate
 from .iface import EngineIface, TokIface
-from .logprobs import Entry, Score, chat_block, host_logprob, text_block
+from .logprobs import Entry, Place, Score, chat_block, host_logprob, text_block
 
 
 @dataclass
@@ -77,7 +77,7 @@ class Session:
     scores: object = None              # echoed prompts: what the prompt pass fills with the prompt's log probabilities
     entries: List[Entry] = field(default_factory=list)     # log probabilities of the response's tokens
     told: int = 0                      # of them, those that frames have carried
-    text_at: int = 0                   # completions: where the next told token's text begins
+    place: Place = field(default_factory=Place)            # the end of the response's text, token by token
 
 
 class Server:
@@ -286,10 +286,12 @@ class Server:
 
     def _echo(self, s: Session):
         """The prompt ahead of the completion: its text as it is, its tokens' log probabilities where they are asked for."""
+        text = s.req.prompt or self.tok.decode(s.prompt_ids)
         if s.scores is not None:
             scores, s.scores = s.scores.read(), None
-            s.entries += [Entry(t, e if i else None) for i, (t, e) in enumerate(zip(s.prompt_ids, scores))]
-        text = s.req.prompt or self.tok.decode(s.prompt_ids)
+            raw = self.tok.token_bytes if s.req.prompt else self.tok.text_bytes      # special tokens stand in a prompt's own text
+            s.entries += [Entry(t, e if i else None, s.place.add(raw(t))) for i, (t, e) in enumerate(zip(s.prompt_ids, scores))]
+        s.place = Place(len(text))
         self._deliver(s, [{"kind": "content", "text": text}])
 
     def _logprobs(self, items):
@@ -481,7 +483,7 @@ class Server:
             return self._end(s, "stop")
         s.out_ids.append(tok)
         if score is not None:
-            s.entries.append(Entry(tok, score))
+            s.entries.append(Entry(tok, score, s.place.add(self.tok.text_bytes(tok))))
         if s.lookup is not None:
             s.lookup.append(tok)
         s.pending = tok
@@ -530,8 +532,7 @@ class Server:
         new, s.told = s.entries[s.told:], len(s.entries)
         if s.req.chat:
             return chat_block(self.tok, new)
-        block, s.text_at = text_block(self.tok, new, s.req.logprobs, s.text_at)
-        return block
+        return text_block(self.tok, new, s.req.logprobs, 0)[0]
 
     def _end(self, s: Session, reason: str, flush: bool = True):
         """Ends generation.  ``flush``: text still held by the detokeniser and the stop matcher is

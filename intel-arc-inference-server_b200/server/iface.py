@@ -149,6 +149,9 @@ class TokIface:
     def token_bytes(self, i: int) -> bytes:
         """The bytes a token stands for (part of a character, if it is one)."""
         return self.decode([i]).encode("utf-8")
+    def text_bytes(self, i: int) -> bytes:
+        """The bytes that ``decode`` and ``streamer`` add to a text for a token: none for the special ones."""
+        return self.token_bytes(i)
 
 
 class ByteTok(TokIface):
@@ -212,6 +215,9 @@ class NativeTok(TokIface):
 
     def token_bytes(self, i):
         return bytes(self.tok.token_bytes(int(i)))
+
+    def text_bytes(self, i):
+        return b"" if self.tok.is_special(int(i)) else self.token_bytes(i)
 
     def token_to_id(self, s):
         return self.tok.token_to_id(s)

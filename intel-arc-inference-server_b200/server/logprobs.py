@@ -2,6 +2,7 @@
 logits but no kernel over them (sharded vocabularies, stand-ins)."""
 from __future__ import annotations
 
+import codecs
 import math
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
@@ -29,9 +30,38 @@ def host_logprob(logits: np.ndarray, token: int, top: int) -> Score:
 
 
 class Entry(NamedTuple):
-    """A token of a response with its score (None: the first token of an echoed prompt, which nothing predicts)."""
+    """A token of a response with its score (None: the first token of an echoed prompt, which nothing predicts), and where its text begins
+    in the response's (None: behind the entries before it)."""
     token: int
     score: Optional[Score]
+    at: Optional[int] = None
+
+
+class Place:
+    """Counts the characters of a text whose bytes come token by token, a character often in parts."""
+
+    def __init__(self, at: int = 0):
+        self.at = at            # characters that have ended
+        self.held = b""         # the beginning of one that has not
+
+    def add(self, raw: bytes) -> int:
+        """Characters of the text before the first of these bytes; one that they go on with counts from where it begins, at the next place."""
+        if self.held and raw and not _goes_on(self.held, raw[:1]):
+            self.at += len(_text(self.held))      # it never ends: the text has replacement characters there
+            self.held = b""
+        at = self.at
+        dec = codecs.getincrementaldecoder("utf-8")("replace")
+        self.at += len(dec.decode(self.held + raw))
+        self.held = dec.getstate()[0]
+        return at
+
+
+def _goes_on(held: bytes, byte: bytes) -> bool:
+    try:
+        codecs.getincrementaldecoder("utf-8")("strict").decode(held + byte)
+        return True
+    except UnicodeDecodeError:
+        return False
 
 
 def number(x: float):
@@ -54,10 +84,12 @@ def text_block(tok, entries: Sequence[Entry], top: int, offset: int) -> Tuple[di
     """``choices[0].logprobs`` of completions for tokens whose text begins at ``offset``, and the offset behind them.  Alternatives whose texts are
     the same keep the likelier one's number; the token itself is always among them."""
     out = {"tokens": [], "token_logprobs": [], "top_logprobs": [] if top else None, "text_offset": []}
+    place = Place(offset)
     for e in entries:
         text = _text(tok.token_bytes(e.token))
+        at = place.add(tok.text_bytes(e.token))
         out["tokens"].append(text)
-        out["text_offset"].append(offset)
+        out["text_offset"].append(at if e.at is None else e.at)
         out["token_logprobs"].append(None if e.score is None else number(e.score.logprob))
         if top:
             best = None
@@ -67,5 +99,4 @@ def text_block(tok, entries: Sequence[Entry], top: int, offset: int) -> Tuple[di
                     best.setdefault(_text(tok.token_bytes(i)), number(lp))
                 best.setdefault(text, number(e.score.logprob))
             out["top_logprobs"].append(best)
-        offset += len(text)
-    return out, offset
+    return out, place.at
