@@ -72,6 +72,14 @@ def _text(raw: bytes) -> str:
     return raw.decode("utf-8", "replace")
 
 
+def _name(raw: bytes) -> str:
+    """A token's text, or its bytes where they are no text by themselves (part of a character): two tokens' are never one replacement character."""
+    try:
+        return raw.decode("utf-8")
+    except UnicodeDecodeError:
+        return "bytes:" + "".join(f"\\x{b:02x}" for b in raw)
+
+
 def chat_block(tok, entries: Sequence[Entry]) -> dict:
     """``choices[0].logprobs`` of chat completions."""
     def one(token, lp):
@@ -82,11 +90,11 @@ def chat_block(tok, entries: Sequence[Entry]) -> dict:
 
 def text_block(tok, entries: Sequence[Entry], top: int, offset: int) -> Tuple[dict, int]:
     """``choices[0].logprobs`` of completions for tokens whose text begins at ``offset``, and the offset behind them.  Alternatives whose texts are
-    the same keep the likelier one's number; the token itself is always among them."""
+    the same keep the likelier one's number; the token itself is always among them, with its own."""
     out = {"tokens": [], "token_logprobs": [], "top_logprobs": [] if top else None, "text_offset": []}
     place = Place(offset)
     for e in entries:
-        text = _text(tok.token_bytes(e.token))
+        text = _name(tok.token_bytes(e.token))
         at = place.add(tok.text_bytes(e.token))
         out["tokens"].append(text)
         out["text_offset"].append(at if e.at is None else e.at)
@@ -96,7 +104,7 @@ def text_block(tok, entries: Sequence[Entry], top: int, offset: int) -> Tuple[di
             if e.score is not None:
                 best = {}
                 for i, lp in e.score.top:
-                    best.setdefault(_text(tok.token_bytes(i)), number(lp))
-                best.setdefault(text, number(e.score.logprob))
+                    best.setdefault(_name(tok.token_bytes(i)), number(lp))
+                best[text] = number(e.score.logprob)
             out["top_logprobs"].append(best)
     return out, place.at

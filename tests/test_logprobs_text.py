@@ -152,3 +152,23 @@ def test_blocks_that_begin_somewhere():
     assert block["text_offset"] == [4, 4, 5] and at == 6
     block, _ = text_block(ByteTok(), [Entry(enc("x")[0], None, 9), Entry(enc("y")[0], None, 3)], 0, 0)
     assert block["text_offset"] == [9, 3]
+
+
+def test_alternatives_that_are_parts_of_characters():
+    """Tokens that are no text by themselves are told apart, and the token itself keeps its own number."""
+    a, b, c = enc("é日")[:3]
+    block, _ = text_block(TOK, [Entry(a, Score(-3.0, [(b, -0.5), (c, -1.0)])), Entry(b, Score(-3.25, [(c, -0.5)]))], 2, 0)
+    assert block["tokens"] == ["bytes:\\xc3", "bytes:\\xa9"]
+    assert block["top_logprobs"] == [{"bytes:\\xc3": -3.0, "bytes:\\xa9": -0.5, "bytes:\\xe6": -1.0}, {"bytes:\\xa9": -3.25, "bytes:\\xe6": -0.5}]
+    # an alternative of the same text (ids 0 and 1 have none): the token's own number
+    block, _ = text_block(TOK, [Entry(1, Score(-4.0, [(0, -0.25), (a, -2.0)]))], 2, 0)
+    assert block["top_logprobs"] == [{"": -4.0, "bytes:\\xc3": -2.0}]
+
+
+@pytest.mark.parametrize("stream", [False, True])
+def test_every_token_is_among_its_alternatives(serve, stream):
+    srv = serve({enc("go "): list(enc("日é"))})
+    out, lp = complete(srv, stream, prompt="go ", max_tokens=5, logprobs=2)
+    assert out == "日é" and len(lp["tokens"]) == 5
+    for token, number, top in zip(lp["tokens"], lp["token_logprobs"], lp["top_logprobs"]):
+        assert len(top) == 2 and top[token] == number == max(top.values())
