@@ -282,6 +282,8 @@ class Server:
                 tok = self._sample(s)
             s.t_first = time.time()
             score = self._logprobs([(s, 0, tok)])[0]
+            if s.finished:
+                return
             self._emit_token(s, tok, score)       # the first token goes out before the first decode step
 
     def _echo(self, s: Session):
@@ -295,15 +297,21 @@ class Server:
         self._deliver(s, [{"kind": "content", "text": text}])
 
     def _logprobs(self, items):
-        """Scores of (session, row of its slot in the last pass, token), ``None`` for sessions that want none: one call of the engine for all."""
+        """Scores of (session, row of its slot in the last pass, token), ``None`` for sessions that want none: one call of the engine for all.
+        Where it fails, the sessions that asked fail, and the others of the step go on."""
         want = [(s.slot, row, tok) for s, row, tok in items if s.req.logprobs >= 0]
         if not want:
             return [None] * len(items)
         top = max(s.req.logprobs for s, _, _ in items)
-        on_device = getattr(self.engine, "logprobs", None)
-        got = on_device(want, top) if on_device is not None else None
-        if got is None:
-            got = [host_logprob(np.asarray(self.engine.logits(slot, row))[: self.engine.vocab_size], tok, top) for slot, row, tok in want]
+        try:
+            on_device = getattr(self.engine, "logprobs", None)
+            got = on_device(want, top) if on_device is not None else None
+            if got is None:
+                got = [host_logprob(np.asarray(self.engine.logits(slot, row))[: self.engine.vocab_size], tok, top) for slot, row, tok in want]
+        except Exception as e:  # noqa: BLE001
+            for s in {id(s): s for s, _, _ in items if s.req.logprobs >= 0}.values():
+                self._fail(s, e)
+            return [None] * len(items)
         got = iter(got)
         return [Score(g.logprob, g.top[: s.req.logprobs]) if s.req.logprobs >= 0 and (g := next(got)) else None for s, _, _ in items]
 
