@@ -370,11 +370,16 @@ class Engine:
 
     @property
     def can_score(self) -> bool:
-        """``prefill`` takes ``scores``: one GPU holds the whole model."""
+        """``prefill`` takes ``scores``, and the last step's logits are whole rows: one GPU holds the whole model."""
         return self.tp is None and self.model.nccl is None and type(self).prefill is Engine.prefill
+
+    def _require_whole(self, what: str):
+        if not self.can_score:
+            raise ValueError(f"log probabilities of {what} are not available for a model spread over several GPUs")
 
     def prompt_scores(self, ids: Sequence[int], top: int = 0) -> PromptScores:
         """What ``prefill`` fills with the log probabilities of a prompt's tokens as it goes (the ``scores`` of every portion)."""
+        self._require_whole("a prompt")
         return PromptScores(ids, top, self.device)
 
     def prefill(self, slot: int, ids: Sequence[int], chunk: Optional[int] = None, scores: Optional[PromptScores] = None) -> int:
@@ -383,8 +388,7 @@ class Engine:
         self.require_ok()
         ids = list(ids)
         if scores is not None:
-            if not self.can_score:
-                raise ValueError("log probabilities of a prompt are not available for a model spread over several GPUs")
+            self._require_whole("a prompt")
             scores.expect(ids)
         if self.mixed_batches and len(ids) > self.max_rows:
             self.last_prefill_row = 0
@@ -447,7 +451,10 @@ class Engine:
 
     def logprobs(self, tokens: Sequence[int], top: int = 0, logits: Optional[torch.Tensor] = None) -> List[TokenScore]:
         """Log probability of one token per row, entropy and top alternatives, of ``logits`` or of the last step's rows (-1: a row without a
-        token)."""
+        token).  A model spread over several GPUs has part of its rows here at most: there ``logits`` are rows of the whole vocabulary that the
+        caller has put together."""
+        if logits is None or logits.shape[-1] != self.cfg.vocab:
+            self._require_whole("a step")
         lg = self.logits(len(tokens)) if logits is None else logits
         buf = ScoreBuffer(len(tokens), top, self.device)
         LP.token_logprobs(lg, torch.tensor(tokens, dtype=torch.int32).to(self.device), out=buf.out)

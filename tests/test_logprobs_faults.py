@@ -77,3 +77,29 @@ def test_scores_that_fail_in_a_step_fail_the_request_that_asked(serve, engine, g
     for i, (_, b) in plain.items():
         again = post(srv.port, "/v1/completions", {"prompt": f"request {i} goes on", "max_tokens": 200, "ignore_eos": True})[1]
         assert again["choices"][0]["text"] == b["choices"][0]["text"]
+
+
+def spread(kind):
+    """Engines of which this GPU holds a part, as far as the checks of a call look."""
+    from types import SimpleNamespace as N
+    import torch
+    from b200serve.parallel.pp import PipelineEngine
+    from b200serve.runtime.engine import Engine
+    e = object.__new__(PipelineEngine if kind == "pp" else Engine)
+    e.tp, e.model, e.device = (N(world=2) if kind == "tp" else None), N(nccl=(0, 2, None) if kind == "nccl" else None), torch.device("cpu")
+    e.cfg, e.broken, e.max_seqs = N(vocab=64, layer_specs=()), None, 1
+    e.logits = lambda m: torch.zeros(m, 32 if kind != "pp" else 64)
+    e.reset = lambda slot=None: pytest.fail("a slot was emptied for a call that is refused")
+    return e
+
+
+@pytest.mark.parametrize("kind", ["tp", "nccl", "pp"])
+def test_part_of_a_vocabulary_is_not_scored(kind):
+    """Sums over a slice of the vocabulary, or over rows that another stage holds, are no probabilities: refused, before anything is changed."""
+    import torch
+    e = spread(kind)
+    for call in (lambda: e.logprobs([1, 2]), lambda: e.logprobs([1], 3, torch.zeros(1, 32)), lambda: e.score([1, 2, 3]), lambda: e.prompt_scores([1, 2])):
+        with pytest.raises(ValueError, match="several GPUs"):
+            call()
+    with pytest.raises(ValueError, match="CUDA"):      # whole rows that the caller put together go to the kernel (no GPU here)
+        e.logprobs([1], 0, torch.zeros(1, 64))
