@@ -103,3 +103,30 @@ def test_part_of_a_vocabulary_is_not_scored(kind):
             call()
     with pytest.raises(ValueError, match="CUDA"):      # whole rows that the caller put together go to the kernel (no GPU here)
         e.logprobs([1], 0, torch.zeros(1, 64))
+
+
+# ------------------------------------------------------------------ a prompt's results
+def test_prompts_that_wait_hold_no_memory_of_the_device(monkeypatch):
+    import torch
+    from b200serve.runtime import scoring
+    made = []
+    buffer = scoring.ScoreBuffer
+    monkeypatch.setattr(scoring, "ScoreBuffer", lambda rows, top, device: made.append((rows, top)) or buffer(rows, top, device))
+    waiting = [scoring.PromptScores([5, 6, 7, 8], 3, torch.device("cpu")) for _ in range(4)]
+    assert not made and all(w.buf is None and w.next is None for w in waiting)
+    w = waiting[1]
+    with pytest.raises(ValueError, match="not the prompt's"):
+        w.expect([6])
+    assert not made
+    w.expect([5, 6])
+    tokens, out = w.take(2)
+    assert tokens.tolist() == [6, 7] and out.top_ids.shape == (2, 3)
+    w.expect([7, 8])
+    tokens, _ = w.take(2)
+    assert tokens.tolist() == [8, -1] and made == [(4, 3)]
+    assert len(w.read()) == 4
+    with pytest.raises(ValueError, match="at most"):      # what can be said at once is said at once
+        scoring.PromptScores([5], 33, torch.device("cpu"))
+    with pytest.raises((ValueError, RuntimeError, OverflowError)):
+        scoring.PromptScores([5, 1 << 32], 0, torch.device("cpu"))
+    assert scoring.PromptScores([], 2, torch.device("cpu")).read() == []
