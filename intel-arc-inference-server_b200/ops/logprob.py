@@ -115,6 +115,20 @@ def _stream(device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def slab_rows(m: int, n: int, top: int) -> int:
+    """Rows of ``m`` that ``score`` takes at a time, where there is room."""
+    return min(m, SLAB_ROWS if not top else max(256, SLAB_ELEMS // n // 256 * 256))
+
+
+def work_bytes(m: int, n: int, k: int, top: int, i8: bool, sms: int = 148) -> int:
+    """Workspace of ``score`` (``score_i8``) for ``m`` rows of ``k`` against ``n`` columns, for the memory plan: ``b2_score_work`` of a slab, or
+    a little more.  16 bytes for every part of a row (tiles of 256 columns, up to 512 rows ranges of them instead), the token's logit, with
+    alternatives the logits and a maximum of every 32, int8 rows and their scales."""
+    rows, chunks = slab_rows(m, n, top), (n + 31) // 32
+    parts = max(min(rows, 512) * min(sms, chunks), rows * ((n + 255) // 256) if rows > 512 else 0)
+    return 16 * parts + 4 * rows + (4 * 33 * chunks * rows if top else 0) + ((k + 15) // 16 * 16 + 4) * rows * i8 + 512
+
+
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
     """Rows of fp32 ``logits`` ``[m][vocabulary]`` (any row stride), one int32 token each.  ``out``: results to write, whose width is
     then ``top``."""
@@ -149,7 +163,7 @@ def _score(x, w, w_scale, tokens, top: Optional[int], out: Optional[Logprobs]) -
         return out
     top = out.top_ids.shape[1]
     room, run = _entry("b2_score_work", "iiiii", ctypes.c_longlong), _entry("b2_score", "plplpiiipipppppp")
-    step = min(m, SLAB_ROWS if not top else max(256, SLAB_ELEMS // n // 256 * 256))
+    step = slab_rows(m, n, top)
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return _score(x, w, w_scale, tokens, None, out)

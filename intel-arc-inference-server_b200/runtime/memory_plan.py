@@ -39,12 +39,13 @@ class MemoryPlan:
     max_len: int
     max_seqs: int
     num_pages: int
+    scores: int = 0
 
     def line(self) -> str:
         g = 2 ** 30
         return (f"memory: model {self.weights / g:.2f} GiB, kv {self.kv_pool / g:.2f} GiB ({self.num_pages} pages, "
                 f"{self.max_seqs} x {self.max_len}), decode state {self.step_scratch / g:.2f} GiB, prompt scratch "
-                f"{self.prefill_scratch / g:.2f} GiB, total {self.total / g:.2f} of {self.budget / g:.2f} GiB")
+                f"{self.prefill_scratch / g:.2f} GiB (scored prompts up to {self.scores / g:.2f}), total {self.total / g:.2f} of {self.budget / g:.2f} GiB")
 
 
 def weight_bytes(cfg: ModelConfig, int8_head: bool = False, tp: int = 1, ep: int = 1) -> int:
@@ -127,6 +128,13 @@ def prefill_scratch_bytes(cfg: ModelConfig, chunk: int, backend: str) -> int:
     return int(b)
 
 
+def score_scratch_bytes(cfg: ModelConfig, chunk: int, max_len: int, int8: bool = False) -> int:
+    """What log probabilities of a prompt hold while it is ingested (one prompt at a time): a portion's workspace, and the results."""
+    from ..ops.logprob import MAX_TOP, work_bytes
+    work = max(work_bytes(chunk, cfg.vocab, cfg.hidden, top, int8) for top in (0, MAX_TOP))
+    return work + max_len * 4 * (3 + 2 * MAX_TOP)
+
+
 def plan(cfg: ModelConfig, max_seqs: int, max_len, kv_dtype: str = "bf16", int8_head: bool = False,
          prefill_backend: str = "auto", prefill_chunk: int = 4096, tp: int = 1, ep: int = 1,
          budget: int = 0) -> MemoryPlan:
@@ -152,8 +160,12 @@ def plan(cfg: ModelConfig, max_seqs: int, max_len, kv_dtype: str = "bf16", int8_
     if fixed >= budget:
         raise ValueError(f"{cfg.name}: weights and scratch need {fixed / 2**30:.1f} GiB of {budget / 2**30:.1f} GiB "
                          "before any KV cache")
+    scores = score_scratch_bytes(cfg, prefill_chunk, 262144 if max_len == "auto" else int(max_len), int8_head) if tp * ep == 1 else 0
     if max_len == "auto":
-        pages = (budget - fixed) // page
+        # room for scored prompts too, unless that were half of what there is (they make do with fewer rows at a time, or fail alone); a
+        # given length is not refused for them either
+        free = budget - fixed
+        pages = (free - scores if free > 2 * scores else free) // page
         max_len = int(min(262144, (pages - 1) // max_seqs * cfg.page_size))
         if max_len < 2 * cfg.page_size:
             raise ValueError(f"{cfg.name}: no room for a KV cache of {max_seqs} sequences")
@@ -165,4 +177,4 @@ def plan(cfg: ModelConfig, max_seqs: int, max_len, kv_dtype: str = "bf16", int8_
         fit = ((budget - fixed) // page - 1) // max_seqs * cfg.page_size
         raise ValueError(f"{cfg.name}: {max_seqs} x {max_len} positions of {kv_dtype} KV need {kv / 2**30:.1f} GiB; "
                          f"{(budget - fixed) / 2**30:.1f} GiB are free after the model: at most {fit} positions fit")
-    return MemoryPlan(w, kv, st, pf, resident, total, budget, max_len, max_seqs, num_pages)
+    return MemoryPlan(w, kv, st, pf, resident, total, budget, max_len, max_seqs, num_pages, scores)

@@ -130,3 +130,39 @@ def test_prompts_that_wait_hold_no_memory_of_the_device(monkeypatch):
     with pytest.raises((ValueError, RuntimeError, OverflowError)):
         scoring.PromptScores([5, 1 << 32], 0, torch.device("cpu"))
     assert scoring.PromptScores([], 2, torch.device("cpu")).read() == []
+
+
+def test_the_memory_plan_leaves_room_for_scored_prompts():
+    from b200serve.models.config import preset
+    from b200serve.ops import logprob as LP
+    from b200serve.runtime import memory_plan as MP
+    cfg = preset("dense-27b")
+    auto = MP.plan(cfg, 64, "auto")
+    slab = LP.slab_rows(4096, cfg.vocab, 5) * cfg.vocab * 4
+    assert slab == 1024 * 151936 * 4 and auto.scores > slab
+    assert auto.max_len < 262144 and auto.total + auto.scores <= auto.budget      # (the reserve is in the total)
+    # a given length that fits beside the model is not refused; sharded models score no prompts
+    most = MP.plan(cfg, 64, "auto", tp=2, budget=auto.budget)
+    assert most.scores == 0
+    page = MP.kv_bytes_per_page(cfg, "bf16")
+    longer = auto.max_len + auto.scores // page // 64 * cfg.page_size
+    assert longer > auto.max_len and MP.plan(cfg, 64, longer).total <= auto.budget
+    # where they would take half of what is left, they do not
+    kw = {"prefill_backend": "bf16"}
+    given = MP.plan(cfg, 1, 1024, **kw)
+    few = MP.plan(cfg, 1, "auto", budget=given.total, **kw)
+    assert few.scores > given.kv_pool and few.max_len == 1024
+
+
+@pytest.mark.gpu
+def test_workspaces_are_what_the_plan_counts():
+    from b200serve.ops import logprob as LP
+    import ctypes
+    room = LP._entry("b2_score_work", "iiiii", ctypes.c_longlong)
+    for m, n, k, top, i8 in [(1, 700, 64, 0, 0), (128, 2048, 512, 3, 1), (129, 151936, 5120, 0, 0), (384, 102397, 200, 20, 1), (512, 151936, 2048, 5, 0),
+                             (513, 151936, 2048, 5, 0), (1024, 151933, 5120, 32, 1), (4096, 151936, 5120, 0, 1), (32768, 2051, 128, 0, 1), (4096, 2048, 512, 5, 0)]:
+        rows = LP.slab_rows(m, n, top)
+        need = 4 * max(room(r, n, k, top, i8) for r in (rows, max(1, m % rows), min(rows, 512), min(rows, 256), 1))
+        assert 0 < need <= LP.work_bytes(m, n, k, top, bool(i8))
+        if rows > 512:
+            assert LP.work_bytes(m, n, k, top, bool(i8)) <= 1.3 * need + (1 << 20)
