@@ -79,6 +79,10 @@ class Session:
     told: int = 0                      # of them, those that frames have carried
     place: Place = field(default_factory=Place)            # the end of the response's text, token by token
 
+    def known_ids(self) -> List[int]:
+        """What the prefix cache may know of the prompt: one whose tokens are scored goes through the model from its first token on."""
+        return self.prompt_ids if self.scores is None else []
+
 
 class Server:
     def __init__(self, engine: EngineIface, tok: TokIface, template: ChatTemplate, options: ServerOptions = None,
@@ -185,7 +189,7 @@ class Server:
                 return self._error(hid, 400, f"cannot score the prompt: {e}")
             if s.scores is None:
                 return self._error(hid, 400, "log probabilities of the prompt are not available on this server")
-        preferred = self.prefix.preferred_slot(ids) if self.prefix else -1
+        preferred = self.prefix.preferred_slot(s.known_ids()) if self.prefix else -1
         want_rows = 1 + (self.o.spec_max if self.o.spec != "off" else 0)
         if not self.sched.submit(hid, len(ids), max_new, preferred, want_rows):
             return self._error(hid, 503, "server is busy: too many requests waiting", "server_error")
@@ -231,9 +235,7 @@ class Server:
                 s = self.sessions[a["req"]]
                 s.slot = a["slot"]
                 self.by_slot[s.slot] = s
-                # a prompt whose tokens are scored goes through the model from its first token on
-                known = s.prompt_ids if s.scores is None else []
-                cached = self.prefix.begin(s.slot, known, self.o.prefix_split_last) if self.prefix else 0
+                cached = self.prefix.begin(s.slot, s.known_ids(), self.o.prefix_split_last) if self.prefix else 0
                 if not self.prefix:
                     self.engine.reset(s.slot)
                 s.cached_tokens = cached

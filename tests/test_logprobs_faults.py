@@ -166,3 +166,33 @@ def test_workspaces_are_what_the_plan_counts():
         assert 0 < need <= LP.work_bytes(m, n, k, top, bool(i8))
         if rows > 512:
             assert LP.work_bytes(m, n, k, top, bool(i8)) <= 1.3 * need + (1 << 20)
+
+
+# ------------------------------------------------------------------ what others had
+def test_a_scored_prompt_leaves_the_session_it_resembles_alone(serve):
+    """Nothing of a scored prompt comes from the cache: the slot that holds its beginning is not asked for, and the session there keeps it."""
+    from test_logprobs_server import Prefix
+    from test_prefix_store import FakeKV, run
+    from b200serve.server.prefix import PrefixStore
+    kv = FakeKV()
+    store = PrefixStore(kv, host_gb=0, block_tokens=32)
+    ids = list(range(3, 103))
+    run(store, kv, 1, ids)
+
+    class Slots(Prefix):
+        granted = ()
+
+        def preferred_slot(self, ids):
+            return store.preferred_slot(ids)
+
+        def begin(self, slot, ids, split_last=False):
+            self.granted += (slot,)
+            self.eng.reset(slot)
+            return 0
+    pre = Slots()
+    eng = pre.eng = MockEngine(vocab_size=V, max_len=2048, max_seqs=2)
+    srv = serve(eng, prefix=pre)
+    assert store.preferred_slot(ids + [7]) == 1
+    for extra, slot in (({}, 1), ({"echo": True, "logprobs": 0}, 0), ({"logprobs": 0}, 1), ({"echo": True}, 1)):
+        assert post(srv.port, "/v1/completions", {"prompt": ids + [7], "max_tokens": 1, **extra})[0] == 200
+        assert pre.granted[-1] == slot, extra
