@@ -166,9 +166,9 @@ class Server:
         if not ids:
             return self._error(hid, 400, "the prompt is empty")
         max_new = req.max_tokens or self.o.default_max_tokens
-        if len(ids) + 1 > self.engine.max_len:
+        if len(ids) + (not req.score_only) > self.engine.max_len:      # (a prompt that is only scored needs no place behind it)
             return self._error(hid, 400, f"the prompt has {len(ids)} tokens; the context holds {self.engine.max_len}")
-        max_new = min(max_new, self.engine.max_len - len(ids))
+        max_new = max(1, min(max_new, self.engine.max_len - len(ids)))
         s = Session(hid, req, ids, thinking=thinking, rid=("chatcmpl-" if chat else "cmpl-") + uuid.uuid4().hex[:24],
                     created=int(time.time()), t0=time.time())
         s.rng_seed = req.seed if req.has_seed else int.from_bytes(os.urandom(6), "little")

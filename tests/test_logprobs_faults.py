@@ -196,3 +196,30 @@ def test_a_scored_prompt_leaves_the_session_it_resembles_alone(serve):
     for extra, slot in (({}, 1), ({"echo": True, "logprobs": 0}, 0), ({"logprobs": 0}, 1), ({"echo": True}, 1)):
         assert post(srv.port, "/v1/completions", {"prompt": ids + [7], "max_tokens": 1, **extra})[0] == 200
         assert pre.granted[-1] == slot, extra
+
+
+@pytest.mark.parametrize("chunk", [4096, 24])
+def test_a_prompt_that_fills_the_context_can_be_scored(serve, chunk):
+    srv = serve(MockEngine(vocab_size=V, max_len=64, max_seqs=1), prefill_chunk=chunk)
+    body = {"max_tokens": 0, "echo": True, "logprobs": 1}
+    st, got = post(srv.port, "/v1/completions", {"prompt": "x" * 64, **body})
+    assert st == 200 and len(got["choices"][0]["logprobs"]["tokens"]) == 64 and got["usage"]["completion_tokens"] == 0
+    for text, more in (("x" * 65, body), ("x" * 64, {"max_tokens": 1}), ("x" * 64, {"max_tokens": 1, "echo": True, "logprobs": 1})):
+        st, got = post(srv.port, "/v1/completions", {"prompt": text, **more})
+        assert st == 400 and "context holds 64" in got["error"]["message"]
+    st, got = post(srv.port, "/v1/completions", {"prompt": "x" * 63, "max_tokens": 5, "ignore_eos": True})
+    assert st == 200 and got["usage"]["completion_tokens"] == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["small-dense", "small-hybrid", "napadra-mini"])
+def test_a_prompt_that_fills_the_engine(name):
+    import math
+    from test_logprobs_engine import engine, prompt
+    eng = engine(name)
+    ids = prompt(eng.cfg, eng.max_len, 9)
+    got = eng.score(ids, 1)
+    assert len(got) == eng.max_len == eng.seq_len[0] and all(math.isfinite(s.logprob) for s in got[1:])
+    with pytest.raises(ValueError, match="max_len"):
+        eng.score(ids + [1])
+    assert eng.score(ids, 1)[1:] == got[1:]
