@@ -223,3 +223,52 @@ def test_a_prompt_that_fills_the_engine(name):
     with pytest.raises(ValueError, match="max_len"):
         eng.score(ids + [1])
     assert eng.score(ids, 1)[1:] == got[1:]
+
+
+# ------------------------------------------------------------------ the host's sums
+def test_the_host_puts_no_vocabulary_in_order(monkeypatch):
+    """A row's alternatives on the serving thread: of 100,000 logits only those that can be among them are sorted, and none for a token alone."""
+    import numpy as np
+    from b200serve.server.logprobs import host_logprob
+    sizes = []
+    for name in ("argsort", "lexsort", "sort"):
+        real = getattr(np, name)
+
+        def noted(a, *args, real=real, **kw):
+            sizes.append(np.asarray(a).shape[-1])
+            return real(a, *args, **kw)
+        monkeypatch.setattr(np, name, noted)
+    z = np.random.default_rng(1).permutation(100000).astype(np.float32)
+    assert host_logprob(z, 7, 20).top[0][0] == int(z.argmax()) and max(sizes, default=0) <= 64
+    sizes.clear()
+    host_logprob(z, 7, 0)
+    assert not sizes
+
+
+def test_host_alternatives_by_the_definition():
+    """Larger first, ties to the lower id, banned ids behind numbers, NaN behind those: against a sort of the whole row."""
+    import math
+    import numpy as np
+    from b200serve.server.logprobs import host_logprob
+    rng = np.random.default_rng(2)
+    for n in (1, 2, 7, 400):
+        for bad in (0, 0.5, 1.0):
+            for nan in (False, True):
+                z = rng.integers(-3, 4, n).astype(np.float32)
+                z[rng.random(n) < bad] = -np.inf
+                if nan:
+                    z[rng.random(n) < 0.3] = np.nan
+                want = sorted(range(n), key=lambda i: (math.isnan(z[i]), -z[i] if not math.isnan(z[i]) else 0, i))
+                finite = [float(v) for v in z if math.isfinite(v)]
+                lse = math.log(sum(math.exp(v) for v in finite)) if finite else math.nan
+                for top in (0, 1, 5, 20):
+                    for t in (0, n - 1, -1, n):
+                        s = host_logprob(z, t, top)
+                        assert [i for i, _ in s.top] == want[:top]
+                        for i, lp in [*s.top, (t, s.logprob)]:
+                            if not 0 <= i < n or np.isnan(z).any():
+                                assert math.isnan(lp)
+                            elif not math.isfinite(z[i]):
+                                assert lp == -math.inf
+                            else:      # 64 bits: sums of 400 terms
+                                assert abs(lp - (float(z[i]) - lse)) <= 1e-12
