@@ -187,6 +187,34 @@ class ReplicaRouter(EngineIface):
         r, s = self._where(slot)
         return np.asarray(self._call(r, "logits", s, row))
 
+    def logprobs(self, items, top=0):
+        """Every rank scores its own slots' rows on its device: a few numbers a token come back instead of the rows."""
+        by_rank: Dict[int, List[int]] = {}
+        for i, (g, _, _) in enumerate(items):
+            by_rank.setdefault(self._where(int(g))[0], []).append(i)
+        part = lambda r: [(self._where(int(items[i][0]))[1],) + tuple(items[i][1:]) for i in by_rank[r]]        # noqa: E731
+        for r in by_rank:
+            if r != 0:
+                self.calls[r] += 1
+                self.plane.send(r, ("logprobs", (part(r), top)))
+        got = {}
+        if 0 in by_rank:
+            self.calls[0] += 1
+            try:
+                got[0] = self.local.logprobs(part(0), top)
+            except Exception as e:  # noqa: BLE001
+                got[0] = e
+        for r in by_rank:
+            if r != 0:
+                got[r] = self.plane.recv(r)      # (all of them, before anything is raised: an answer left behind would be the next call's)
+        for res in got.values():
+            if isinstance(res, Exception):
+                raise res
+        if any(res is None for res in got.values()):
+            return None
+        where = {i: res for r, idx in by_rank.items() for i, res in zip(idx, got[r])}
+        return [where[i] for i in range(len(items))]
+
     def step(self, rows: Dict[int, List[int]]):
         by_rank: Dict[int, Dict[int, List[int]]] = {}
         for g, toks in rows.items():

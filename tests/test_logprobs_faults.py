@@ -272,3 +272,71 @@ def test_host_alternatives_by_the_definition():
                                 assert lp == -math.inf
                             else:      # 64 bits: sums of 400 terms
                                 assert abs(lp - (float(z[i]) - lse)) <= 1e-12
+
+
+# ------------------------------------------------------------------ replicas
+def _replicas(rank, world, port, q):
+    import os
+    import sys
+    import torch.distributed as dist
+    sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    from b200serve.parallel import launch as L
+    from b200serve.server.iface import MockEngine
+    from b200serve.server.logprobs import host_logprob
+    os.environ["MASTER_ADDR"], os.environ["MASTER_PORT"] = "127.0.0.1", str(port)
+    dist.init_process_group("gloo", rank=rank, world_size=world)
+    plane = L.ControlPlane()
+
+    class Own(MockEngine):
+        asked, mood = [], "score"
+
+        def logprobs(self, items, top=0):
+            self.asked.append((list(items), top))
+            if self.mood == "fail":
+                raise RuntimeError("no scores")
+            return None if self.mood == "none" else [host_logprob(self._logits[s][r], t, top) for s, r, t in items]
+
+        def set_mood(self, mood):
+            self.mood = mood
+
+        def logits(self, slot, row=0):
+            assert False, "a whole row was asked for"
+    eng = Own(vocab_size=259, max_seqs=2)
+    if rank:
+        q.put((rank, L.serve_replica_worker(eng, plane), eng.asked))
+        return
+    r = L.ReplicaRouter(eng, plane)
+    for slot in (0, 1, 3, 4):
+        r.prefill(slot, [10 + slot, 11])
+    r.step({1: [7, 8], 4: [9]})
+    items = [(4, 0, 5), (0, 0, 6), (1, 1, 7), (3, 0, 8), (1, 0, 9)]
+    got = [r.logprobs(items, 2)]
+    for mood, who in (("none", 2), ("fail", 1), ("fail", 0), ("score", 0)):
+        r._call(who, "set_mood", mood)
+        try:
+            got.append(r.logprobs(items, 2))
+        except RuntimeError as e:
+            got.append(str(e))
+        r._call(who, "set_mood", "score")
+        assert r.length(4) == 3      # the answers are still those of their calls
+    r.shutdown()
+    # the same engine alone, with all slots
+    one = MockEngine(vocab_size=259, max_seqs=6)
+    for slot in (0, 1, 3, 4):
+        one.prefill(slot, [10 + slot, 11])
+    one.step({1: [7, 8], 4: [9]})
+    q.put((0, got, [host_logprob(one.logits(s, row), t, 2) for s, row, t in items]))
+
+
+def test_replicas_score_their_own_rows():
+    import torch.multiprocessing as mp
+    ctx = mp.get_context("spawn")
+    q = ctx.Queue()
+    ps = [ctx.Process(target=_replicas, args=(r, 3, 29709, q)) for r in range(3)]
+    [p.start() for p in ps]
+    res = {r[0]: r[1:] for r in (q.get(timeout=120) for _ in ps)}
+    [p.join(timeout=60) for p in ps]
+    assert all(p.exitcode == 0 for p in ps)
+    got, want = res[0]
+    assert got[0] == want == got[4] and got[1] is None and "no scores" in got[2] and "no scores" in got[3]
+    assert res[1][1][0] == ([(1, 0, 8)], 2) and res[2][1][0] == ([(0, 0, 5)], 2)
