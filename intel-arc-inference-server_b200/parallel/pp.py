@@ -132,6 +132,7 @@ class PipelineEngine(Engine):
         import torch.distributed as dist
         from ..runtime.prefill import PrefillRunner
         self.require_ok()
+        self.check_ids(ids)
         cfg, mdl = self.cfg, self.model
         if self._pp_runner is None:
             saved, self.prefill_backend = self.prefill_backend, "auto"

@@ -373,6 +373,13 @@ class Engine:
         """``prefill`` takes ``scores``, and the last step's logits are whole rows: one GPU holds the whole model."""
         return self.tp is None and self.model.nccl is None and type(self).prefill is Engine.prefill
 
+    def check_ids(self, ids: Sequence[int]):
+        """Tokens outside the vocabulary are refused before anything runs: the prompt pass gathers embeddings by them, and the device would not
+        survive it.  (A step's rows flag them and go on.)"""
+        if len(ids) and not (0 <= min(ids) and max(ids) < self.cfg.vocab):
+            bad = next(t for t in ids if not 0 <= t < self.cfg.vocab)
+            raise ValueError(f"token {int(bad)} is outside the vocabulary of {self.cfg.vocab}")
+
     def _require_whole(self, what: str):
         if not self.can_score:
             raise ValueError(f"log probabilities of {what} are not available for a model spread over several GPUs")
@@ -380,6 +387,7 @@ class Engine:
     def prompt_scores(self, ids: Sequence[int], top: int = 0) -> PromptScores:
         """What ``prefill`` fills with the log probabilities of a prompt's tokens as it goes (the ``scores`` of every portion)."""
         self._require_whole("a prompt")
+        self.check_ids(ids)
         return PromptScores(ids, top, self.device)
 
     def prefill(self, slot: int, ids: Sequence[int], chunk: Optional[int] = None, scores: Optional[PromptScores] = None) -> int:
@@ -395,6 +403,7 @@ class Engine:
             self._snap = None
             return self._batch_runner().prefill(slot, ids, chunk, scores)
         if self._use_tc_prefill(len(ids)):
+            self.check_ids(ids)
             if self._prefill is None:
                 if self.tp is not None:
                     from ..parallel.tp_prefill import TpPrefillRunner

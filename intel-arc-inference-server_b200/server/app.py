@@ -161,6 +161,8 @@ class Server:
                 ids = self.tok.encode(prompt)
             else:
                 ids = list(req.prompt_ids) or self.tok.encode(req.prompt)
+                if req.prompt_ids and max(req.prompt_ids) >= self.engine.vocab_size:
+                    raise ValueError(f"token {max(req.prompt_ids)} is outside the vocabulary of {self.engine.vocab_size}")
         except Exception as e:  # noqa: BLE001  (template errors are the client's)
             return self._error(hid, 400, f"cannot render the prompt: {e}")
         if not ids:

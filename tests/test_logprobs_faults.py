@@ -340,3 +340,34 @@ def test_replicas_score_their_own_rows():
     got, want = res[0]
     assert got[0] == want == got[4] and got[1] is None and "no scores" in got[2] and "no scores" in got[3]
     assert res[1][1][0] == ([(1, 0, 8)], 2) and res[2][1][0] == ([(0, 0, 5)], 2)
+
+
+# ------------------------------------------------------------------ tokens that are none
+@pytest.mark.parametrize("bad", [64, 1 << 20, -1])
+def test_tokens_outside_the_vocabulary_are_refused_on_the_host(bad):
+    """The prompt pass gathers embeddings by token: no such id may reach the device."""
+    from types import SimpleNamespace as N
+    from b200serve.parallel.pp import PipelineEngine
+    from b200serve.runtime.engine import Engine
+    ids = [3] * 100
+    ids[41] = bad
+
+    def fake(cls):
+        e = object.__new__(cls)
+        e.tp, e.model, e.broken, e.max_rows, e.prefill_backend, e._prefill = None, N(nccl=None), None, 8, "bf16", None
+        e.cfg, e.kv = N(vocab=64, layer_specs=(), head_dim=128, n_gdn_layers=0), N(kv_int8=False)
+        e.reset = lambda slot=None: pytest.fail("a slot was emptied for a call that is refused")
+        return e
+    e, p = fake(Engine), fake(PipelineEngine)
+    for call in (lambda: e.prefill(0, ids), lambda: e.score(ids), lambda: e.score([bad, 1]), lambda: e.prompt_scores(ids), lambda: p.prefill(0, ids)):
+        with pytest.raises(ValueError, match=f"token {bad} is outside"):
+            call()
+
+
+@pytest.mark.parametrize("more", [{}, {"echo": True, "logprobs": 0}, {"echo": True, "max_tokens": 0}])
+def test_prompt_ids_outside_the_vocabulary_are_a_bad_request(serve, more):
+    srv = serve(MockEngine(vocab_size=V, max_len=512, max_seqs=1))
+    for ids in ([V] * 2, [5, 6, 4000000000], [5] * 100 + [V]):
+        st, body = post(srv.port, "/v1/completions", {"prompt": ids, "max_tokens": 2, **more})
+        assert st == 400 and "outside the vocabulary" in body["error"]["message"]
+    assert post(srv.port, "/v1/completions", {"prompt": [V - 1, 3], "max_tokens": 2, **more})[0] == 200
