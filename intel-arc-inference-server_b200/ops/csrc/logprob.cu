@@ -243,6 +243,8 @@ extern "C" int b2_logprob_rows(const float* z, long long ld, int m, int n, const
   // CTAs of a row: as many as it has tiles, and as leave four to an SM; sixteen, whose joining costs most, where there are two to an SM.
   // Rows of 151936, 10 alternatives, us with 1 / 2 / 4 / 8 / 16 CTAs a row (an earlier form): 8 rows 27.4 / 16.5 / 11.2 / 8.1 / 7.9, 32 rows 27.6 / 16.6 /
   // 11.5 / 9.7 / 14.3, 100 rows 41.8 / 26.8 / 19.0 / 23.0 / 34.2, 200 rows 49.7 / 32.6 / 37.9 / 39.2 / 63.6, 500 rows 65.8 / 67.5 / 78.4 / 94.8 / 153.4.
+  // What the rule does not see is how many SMs get one CTA more than the others: 297 to 400 rows have a CTA each, some SMs three of them, and take 39
+  // to 42 us whatever their number (27.5 to 37 of bytes).
   const int tiles = ((n + 6) / 4 + kTile - 1) / kTile, sms = sm_count();
   int parts = 1;
   while (parts < kParts && 2 * parts <= tiles && 2ll * parts * m <= (2 * parts == kParts ? 2 : 4) * sms) parts *= 2;

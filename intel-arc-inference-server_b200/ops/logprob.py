@@ -5,7 +5,7 @@ A row's logits z, its token t, S = sum exp(z - max z):
     log p(t) = z_t - max z - ln S        H = - sum p ln p        the ``top`` largest z, of equal ones the lower id first
 
 ``token_logprobs`` takes logits that are there (a decode or verify step's, ``Engine.logits``); ``score`` and ``score_i8`` take rows
-behind the final norm and the lm_head, and keep no logits.  All sums are fp32.
+behind the final norm and the lm_head, and store no logits, or with alternatives those of a slab of rows at a time.  All sums are fp32.
 
 A token outside the vocabulary (-1: no token) has log probability NaN; its row's other results are as ever.  A row without a finite
 logit (every id banned) has log probabilities of -inf and entropy 0.  A NaN or +inf among a row's logits makes its numbers NaN.
@@ -196,7 +196,8 @@ def score(x: torch.Tensor, head: torch.Tensor, tokens: torch.Tensor, top: Option
 
 def score_i8(x: torch.Tensor, head: tuple, tokens: torch.Tensor, top: Optional[int] = None, out: Optional[Logprobs] = None) -> Logprobs:
     """Rows ``x`` ``[m][k]`` bf16 against an int8 lm_head (``[vocabulary][k]``, fp32 scale per row), rows of both at multiples of 16
-    bytes: rows are quantised per token (s = max|x| / 127, q = rint(x / s), as the int8 prompt pass does) and logits are (q . w) s s_w."""
+    bytes: rows are quantised per token (s = max|x| / 127, q = rint(x (1 / s)) with the inverse rounded to fp32, as the int8 prompt pass does)
+    and logits are (q . w) s s_w."""
     w8, scale = head
     if scale.dtype is not torch.float32 or scale.shape != (w8.shape[0],) or scale.device != x.device or not scale.is_contiguous():
         raise ValueError(f"scales of the head: {w8.shape[0]} contiguous fp32 numbers on {x.device}")
