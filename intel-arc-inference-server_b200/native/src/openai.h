@@ -96,7 +96,7 @@ inline ChatRequest parse_request(const std::string& body, bool chat) {
     if (p->is_string()) r.prompt = p->as_string();
     else if (p->is_array() && p->size() > 0 && (*p)[0].is_int()) {
       for (const Json& t : p->items()) {
-        if (!t.is_int() || t.as_int() < 0) throw BadRequest("prompt token ids must be non-negative integers");
+        if (!t.is_int() || t.as_int() < 0 || t.as_int() > 0xffffffffll) throw BadRequest("prompt token ids must be non-negative integers of 32 bits");
         r.prompt_ids.push_back((uint32_t)t.as_int());
       }
     } else if (p->is_array() && p->size() == 1 && (*p)[0].is_string()) r.prompt = (*p)[0].as_string();

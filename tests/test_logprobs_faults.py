@@ -371,3 +371,12 @@ def test_prompt_ids_outside_the_vocabulary_are_a_bad_request(serve, more):
         st, body = post(srv.port, "/v1/completions", {"prompt": ids, "max_tokens": 2, **more})
         assert st == 400 and "outside the vocabulary" in body["error"]["message"]
     assert post(srv.port, "/v1/completions", {"prompt": [V - 1, 3], "max_tokens": 2, **more})[0] == 200
+
+
+@pytest.mark.parametrize("bad", [(1 << 32) + 5, 1 << 32, (1 << 62) + 3])
+def test_prompt_ids_of_more_than_32_bits_are_a_bad_request(serve, bad):
+    """Cut to 32 bits they would be other tokens."""
+    srv = serve(MockEngine(vocab_size=V, max_len=512, max_seqs=1))
+    for ids in ([bad], [5, bad, 6]):
+        st, body = post(srv.port, "/v1/completions", {"prompt": ids, "max_tokens": 2})
+        assert st == 400 and "prompt token ids" in body["error"]["message"]
