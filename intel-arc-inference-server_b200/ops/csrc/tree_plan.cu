@@ -1,0 +1,300 @@
+// Steps over token trees: what a step's rows are and where they stand (plan), and what stays of them (commit).
+//
+//   plan    lengths, rows and pages of every request -> first rows, and of every row its request, position, cache slot, parent and
+//           ancestors; new pages come off the end of a free list into the block table
+//   commit  the accepted path of every tree (node 0, then the child whose token is its parent's target, as long as there is one); the
+//           path's keys and values move from the tree's pages to the request's positions, in all layers
+//
+// Plan is one CTA of 1024 threads: everything hangs on three prefix sums over the requests, and a launch is all that a call costs.
+#include "common.cuh"
+
+using namespace b2;
+
+namespace {
+
+constexpr int kPage = 16, kMaxNodes = 64, kMaxReq = 1024;
+
+enum : int { PLAN_POOL = 1, PLAN_TABLE = 2, PLAN_ROWS = 4, PLAN_COUNT = 8, PLAN_PARENT = 16, PLAN_LENGTH = 32, PLAN_PAGE = 64 };
+
+struct TreePlanParams {
+  const int *lengths, *counts, *parents;   // parents null: rows at consecutive positions
+  int* block_table;
+  const int* tree_table;
+  int* free;
+  const int *n_free, *held;
+  int *n_free_out, *held_out;
+  int B, max_blocks, tree_blocks, free_cap, max_rows, max_nodes, num_pages;
+  int rows;                                // parents there are (max_rows without)
+  int *out_lengths, *row_start, *row_req, *row_pos, *slots, *out_parents, *status;
+  unsigned long long* masks;
+};
+
+// Exclusive prefix sums of one number per thread over the CTA; the total in `total`.
+__device__ __forceinline__ long long scan_1024(long long v, long long* warp_sums, long long& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    long long w = warp_sums[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    warp_sums[lane] = w;
+  }
+  __syncthreads();
+  total = warp_sums[31];
+  return x - v + (warp ? warp_sums[warp - 1] : 0);
+}
+
+__global__ void __launch_bounds__(1024) tree_plan_kernel(const TreePlanParams p) {
+  __shared__ long long sums[32];
+  __shared__ int s_start[kMaxReq + 1], s_need[kMaxReq], s_held[kMaxReq], s_first[kMaxReq], s_len[kMaxReq];
+  __shared__ int s_status;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  pdl_launch_dependents();
+  const bool tree = p.parents != nullptr, mine = tid < p.B;
+  if (tid == 0) s_status = 0;
+  const int count = mine ? p.counts[tid] : 0, held = mine ? p.held[tid] : 0, n_free = *p.n_free;
+  const int length = mine && count >= 0 ? p.lengths[tid] : 0;
+  __syncthreads();
+  if (mine) {
+    int bad = 0;
+    if (length < 0) bad |= PLAN_LENGTH;
+    if (held < 0 || held > p.max_blocks) bad |= PLAN_TABLE;
+    if (tree && count > p.max_nodes) bad |= PLAN_COUNT;
+    if (n_free < 0 || n_free > p.free_cap) bad |= PLAN_POOL;
+    if (bad) atomicOr(&s_status, bad);
+  }
+  long long total;
+  const long long start = scan_1024(max(count, 0), sums, total);
+  if (total > p.rows && tid == 0) atomicOr(&s_status, PLAN_ROWS);
+  if (mine) {
+    s_start[tid] = (int)min(start, (long long)p.rows);
+    s_need[tid] = tree ? 0 : max(count, 0);
+    s_held[tid] = held;
+    s_len[tid] = length;
+  }
+  if (tid == 0) s_start[p.B] = (int)min(total, (long long)p.rows);
+  __syncthreads();
+  if (s_status == 0 && tree) {
+    // ---- a warp per tree: ancestors by walking up (a node's parent stands before it, so every walk ends)
+    for (int b = warp; b < p.B; b += 32) {
+      const int r0 = s_start[b], n = s_start[b + 1] - r0;
+      int deepest = 0;
+      bool bad = false;
+      for (int i = lane; i < n; i += 32) {
+        const int up = p.parents[r0 + i];
+        bad |= up < -1 || up >= i;
+      }
+      bad = __any_sync(0xffffffffu, bad);
+      if (bad) {
+        if (lane == 0) atomicOr(&s_status, PLAN_PARENT);
+        continue;
+      }
+      for (int i = lane; i < n; i += 32) {
+        unsigned long long mask = 0;
+        for (int at = i; at >= 0; at = p.parents[r0 + at]) mask |= 1ull << at;
+        const int depth = __popcll(mask);
+        deepest = max(deepest, depth);
+      }
+      for (int o = 16; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor_sync(0xffffffffu, deepest, o));
+      if (lane == 0) s_need[b] = deepest;
+    }
+    __syncthreads();
+  }
+  // ---- pages: those of requests that left go back, then what is missing comes off the end of the list
+  const int need = mine && s_status == 0 ? s_need[tid] : 0;
+  const long long want = need > 0 ? max((long long)held, ((long long)length + need + kPage - 1) / kPage) : held;
+  const bool left = mine && count < 0;
+  if (mine && !left && want > p.max_blocks) atomicOr(&s_status, PLAN_TABLE);
+  long long back, take;
+  const long long back0 = scan_1024(left ? held : 0, sums, back);
+  const long long take0 = scan_1024(mine && !left ? want - held : 0, sums, take);
+  if (mine) s_first[tid] = (int)take0;
+  if (tid == 0 && ((long long)n_free + back > p.free_cap || take > (long long)n_free + back)) atomicOr(&s_status, PLAN_POOL);
+  __syncthreads();
+  const int status = s_status;
+  if (status == 0 && left)
+    for (int i = 0; i < held; ++i) {
+      int* at = p.block_table + (size_t)tid * p.max_blocks + i;
+      p.free[n_free + back0 + i] = *at;
+      *at = 0;
+    }
+  __syncthreads();
+  const long long top = (long long)n_free + back - 1;     // the page that is taken first
+  if (status == 0 && mine && !left)
+    for (int i = 0; i < (int)(want - held); ++i) p.block_table[(size_t)tid * p.max_blocks + held + i] = p.free[top - take0 - i];
+  if (mine) {
+    p.held_out[tid] = status ? held : left ? 0 : (int)want;
+    p.out_lengths[tid] = status ? 0 : length;
+  }
+  if (tid == 0) p.n_free_out[0] = status ? n_free : (int)(n_free + back - take);
+  for (int b = tid; b <= p.B; b += 1024) p.row_start[b] = status ? 0 : s_start[b];
+  // ---- rows
+  const int rows = status ? 0 : s_start[p.B];
+  bool bad_page = false;
+  for (int r = tid; r < p.max_rows; r += 1024) {
+    int req = -1, pos = -1, slot = -1, up = -1;
+    unsigned long long mask = 0;
+    if (r < rows) {
+      int lo = 0, hi = p.B - 1;       // the last request that starts at or before r
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (s_start[mid] <= r) lo = mid; else hi = mid - 1;
+      }
+      req = lo;
+      const int i = r - s_start[req];
+      int page;
+      if (tree) {
+        up = p.parents[r];
+        for (int at = i; at >= 0; at = p.parents[s_start[req] + at]) mask |= 1ull << at;
+        pos = s_len[req] + __popcll(mask) - 1;
+        page = p.tree_table[(size_t)req * p.tree_blocks + i / kPage];
+        slot = i % kPage;
+      } else {
+        pos = s_len[req] + i;
+        const int block = pos / kPage;
+        page = block < s_held[req] ? p.block_table[(size_t)req * p.max_blocks + block] : p.free[top - s_first[req] - (block - s_held[req])];
+        slot = pos % kPage;
+      }
+      if (page < 0 || page >= p.num_pages) {
+        bad_page = true;
+        slot = -1;
+      } else {
+        slot += page * kPage;
+      }
+    }
+    p.row_req[r] = req;
+    p.row_pos[r] = pos;
+    p.slots[r] = slot;
+    if (tree) {
+      p.masks[r] = mask;
+      p.out_parents[r] = up;
+    }
+  }
+  const int any_bad = __syncthreads_or(bad_page);
+  if (tid == 0) p.status[0] = status | (any_bad ? PLAN_PAGE : 0);
+}
+
+struct TreeCommitParams {
+  const int *lengths, *row_start, *parents, *tokens, *targets, *block_table, *tree_table;
+  int B, max_blocks, tree_blocks, planes, num_pages, n_kv, rows;
+  uint8_t *k, *v;
+  long long plane_bytes;          // from plane to plane of k and v
+  float *k_scale, *v_scale;
+  long long plane_scales;
+  int row_bytes;
+  int *path, *count, *next_token, *out_lengths;
+};
+
+__global__ void __launch_bounds__(256) tree_commit_kernel(const TreeCommitParams p) {
+  __shared__ int s_n, s_src[kMaxNodes], s_dst[kMaxNodes], s_path[kMaxNodes];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (tid < 32) {
+    const int r0 = p.row_start[b], end = p.row_start[b + 1], length = p.lengths[b];
+    const int n = min(end, p.rows) - r0;       // (fewer tokens than rows: an error below)
+    if (end > p.rows && lane == 0 && blockIdx.y == 0) record_error(ERR_BAD_ARG, b);
+    int at = 0, len = 0, next = -1;
+    if (n > 0) {
+      const int i0 = lane, i1 = lane + 32;
+      const int up0 = i0 < n ? p.parents[r0 + i0] : -2, up1 = i1 < n ? p.parents[r0 + i1] : -2;
+      const int tok0 = i0 < n ? p.tokens[r0 + i0] : 0, tok1 = i1 < n ? p.tokens[r0 + i1] : 0;
+      const int tgt0 = i0 < n ? p.targets[r0 + i0] : 0, tgt1 = i1 < n ? p.targets[r0 + i1] : 0;
+      for (;;) {
+        if (lane == 0) s_path[len] = at;
+        ++len;
+        const int want0 = __shfl_sync(0xffffffffu, tgt0, at & 31), want1 = __shfl_sync(0xffffffffu, tgt1, at & 31);
+        next = at < 32 ? want0 : want1;
+        const unsigned f0 = __ballot_sync(0xffffffffu, up0 == at && tok0 == next && i0 > at);
+        const unsigned f1 = __ballot_sync(0xffffffffu, up1 == at && tok1 == next && i1 > at);
+        if (!(f0 | f1)) break;
+        at = f0 ? __ffs(f0) - 1 : 31 + __ffs(f1);      // a child stands behind its parent: the walk ends
+      }
+    }
+    __syncwarp();
+    for (int i = lane; i < kMaxNodes; i += 32) {
+      const int node = i < len ? s_path[i] : -1;
+      if (i < len) {
+        const int block = (length + i) / kPage;
+        int src = p.tree_table[(size_t)b * p.tree_blocks + node / kPage], dst = block < p.max_blocks ? p.block_table[(size_t)b * p.max_blocks + block] : -1;
+        if (src < 0 || src >= p.num_pages || dst < 0 || dst >= p.num_pages) {
+          if (blockIdx.y == 0) record_error(ERR_BAD_ARG, b);
+          src = dst = -1;
+        }
+        s_src[i] = src < 0 ? -1 : src * kPage * p.n_kv + node % kPage;
+        s_dst[i] = src < 0 ? -1 : dst * kPage * p.n_kv + (length + i) % kPage;
+      }
+      if (blockIdx.y == 0) p.path[b * kMaxNodes + i] = node;
+    }
+    if (lane == 0) {
+      s_n = len;
+      if (blockIdx.y == 0) {
+        p.count[b] = len;
+        p.next_token[b] = next;
+        p.out_lengths[b] = length + len;
+      }
+    }
+  }
+  __syncthreads();
+  const int n = s_n, per = p.row_bytes >> 4, each = n * p.n_kv * per;
+  for (int plane = blockIdx.y; plane < p.planes; plane += gridDim.y) {
+    for (int j = tid; j < 2 * each; j += 256) {
+      const int w = j >= each, e = w ? j - each : j;
+      const int i = e / (p.n_kv * per), rest = e - i * p.n_kv * per, h = rest / per, piece = rest - h * per;
+      if (s_src[i] < 0) continue;
+      uint8_t* base = (w ? p.v : p.k) + plane * p.plane_bytes + 16 * piece;
+      *reinterpret_cast<uint4*>(base + ((long long)s_dst[i] + h * kPage) * p.row_bytes) =
+          *reinterpret_cast<const uint4*>(base + ((long long)s_src[i] + h * kPage) * p.row_bytes);
+    }
+    if (p.k_scale)
+      for (int j = tid; j < 2 * n * p.n_kv; j += 256) {
+        const int w = j >= n * p.n_kv, e = w ? j - n * p.n_kv : j, i = e / p.n_kv, h = e - i * p.n_kv;
+        if (s_src[i] < 0) continue;
+        float* base = (w ? p.v_scale : p.k_scale) + plane * p.plane_scales;
+        base[(long long)s_dst[i] + h * kPage] = base[(long long)s_src[i] + h * kPage];
+      }
+  }
+}
+
+}  // namespace
+
+extern "C" int b2_tree_plan(const int* lengths, const int* counts, const int* parents, int* block_table, const int* tree_table, int* free,
+                            const int* n_free, const int* held, int* n_free_out, int* held_out, int* out_lengths, int* row_start, int* row_req,
+                            int* row_pos, int* slots, int* out_parents, void* masks, int* status, int B, int max_blocks, int tree_blocks, int free_cap,
+                            int max_rows, int max_nodes, int num_pages, int rows, void* stream) {
+  if (B < 1 || B > kMaxReq || rows < 0 || rows > max_rows || max_nodes < 1 || max_nodes > kMaxNodes || max_nodes > tree_blocks * kPage) return -1;
+  TreePlanParams p;
+  p.lengths = lengths; p.counts = counts; p.parents = parents; p.block_table = block_table; p.tree_table = tree_table; p.free = free;
+  p.n_free = n_free; p.held = held; p.n_free_out = n_free_out; p.held_out = held_out; p.out_lengths = out_lengths; p.row_start = row_start;
+  p.row_req = row_req; p.row_pos = row_pos; p.slots = slots; p.out_parents = out_parents; p.masks = (unsigned long long*)masks; p.status = status;
+  p.B = B; p.max_blocks = max_blocks; p.tree_blocks = tree_blocks; p.free_cap = free_cap; p.max_rows = max_rows; p.max_nodes = max_nodes;
+  p.num_pages = num_pages; p.rows = rows;
+  return b2_launch(tree_plan_kernel, dim3(1), dim3(1024), 0, (cudaStream_t)stream, true, p);
+}
+
+extern "C" int b2_tree_commit(const int* lengths, const int* row_start, const int* parents, const int* tokens, const int* targets,
+                              const int* block_table, const int* tree_table, void* k, void* v, long long plane_bytes, float* k_scale,
+                              float* v_scale, long long plane_scales, int* path, int* count, int* next_token, int* out_lengths, int B, int max_blocks,
+                              int tree_blocks, int planes, int num_pages, int n_kv, int row_bytes, int rows, void* stream) {
+  if (B < 1 || B > kMaxReq || planes < 1 || row_bytes % 16 || ((uintptr_t)k | (uintptr_t)v | (uintptr_t)plane_bytes) % 16) return -1;
+  TreeCommitParams p;
+  p.lengths = lengths; p.row_start = row_start; p.parents = parents; p.tokens = tokens; p.targets = targets; p.block_table = block_table;
+  p.tree_table = tree_table; p.B = B; p.max_blocks = max_blocks; p.tree_blocks = tree_blocks; p.planes = planes; p.num_pages = num_pages;
+  p.n_kv = n_kv; p.rows = rows; p.k = (uint8_t*)k; p.v = (uint8_t*)v; p.plane_bytes = plane_bytes; p.k_scale = k_scale; p.v_scale = v_scale;
+  p.plane_scales = plane_scales; p.row_bytes = row_bytes; p.path = path; p.count = count; p.next_token = next_token; p.out_lengths = out_lengths;
+  return b2_launch(tree_commit_kernel, dim3(B, min(planes, 65535)), dim3(256), 0, (cudaStream_t)stream, true, p);
+}
+
+B2_DEFINE_STATUS(tree)

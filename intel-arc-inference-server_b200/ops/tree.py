@@ -1,0 +1,276 @@
+"""Steps over token trees: several drafted continuations of a request, verified at once over its paged cache (``csrc/tree_plan.cu``,
+``csrc/tree_rope.cu``, ``csrc/tree_attn.cu``).
+
+A step's rows are the nodes of its requests' trees, a request's one after another, a parent before its children; node 0 is the request's next
+token, which is not in the cache yet.  Nodes stand in pages of their own (``tree_table``), node i at place i, until the step is settled:
+
+    plan         lengths and trees -> rows' requests, positions, cache slots and ancestors; pages for what the longest path can add
+    rope_append  a layer's qkv rows turned by their positions; queries out, keys and values to the rows' slots
+    attention    every row over its request's cached positions and its own ancestors
+    commit       the accepted path of every tree; its keys and values move to the request's positions, in all layers
+
+``plan`` without parents lays out rows at consecutive positions (prompt portions, decode rows) for ``rope_append``: their slots are the
+request's own.  Everything happens on the current stream, nothing waits for the host: lengths, tables and the list of free pages stay on the
+device, and a step can be captured into a CUDA graph.  What only the device knows is checked there; a plan that cannot be made leaves pages
+and tables as they are and no rows (``TreeStep.check``).
+
+Caches are ``KVCache`` planes: ``[page][kv head][16][D]`` with D 64 or 128, bf16, or int8 with fp32 scales ``[page][kv head][16]``.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from . import lib as K
+from .logprob import _elsewhere, _entry, _rows_of, _stream
+
+PAGE = 16
+MAX_NODES = 64          # nodes of a tree: an ancestor mask is one 64-bit word
+MAX_REQUESTS = 1024
+MAX_ROWS = 1 << 20
+
+_FAULTS = {1: "the pool has not enough pages, or no room for those that come back", 2: "a block table is too short, or a request holds more pages than its table has",
+           4: "more rows than the step has room for", 8: "a tree of too many nodes", 16: "a parent that does not stand before its child",
+           32: "a negative length", 64: "a table names a page that is not there"}
+
+
+def _flat(t: torch.Tensor, dtype, shape, what: str, device=None) -> torch.Tensor:
+    if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous() or device is not None and t.device != device:
+        raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on {device or 'a CUDA device'}, not {t.dtype} {list(t.shape)} on {t.device}")
+    return t
+
+
+class PagePool:
+    """Free pages, the last of the first ``n_free`` taken first (int32 ``[capacity]`` and ``[1]``), and the pages that every request holds
+    (int32 ``[requests]``)."""
+
+    def __init__(self, free: torch.Tensor, n_free: torch.Tensor, held: torch.Tensor):
+        _flat(free, torch.int32, (free.numel(),), "free pages")
+        self.free, self.n_free = free, _flat(n_free, torch.int32, (1,), "number of free pages", free.device)
+        self.held = _flat(held, torch.int32, (held.numel(),), "pages of the requests", free.device)
+
+
+class TreeCache:
+    """Keys and values of one layer, ``[pages][kv heads][16][D]``, or of several ``[layers]...``; int8 with scales."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None):
+        i8 = k_scale is not None
+        if k.dtype is not (torch.int8 if i8 else torch.bfloat16) or (v_scale is not None) != i8:
+            raise ValueError("a cache in bf16, or in int8 with scales of keys and values")
+        if k.dim() not in (4, 5) or k.shape[-2] != PAGE or k.shape[-1] not in (64, 128) or min(k.shape) < 1:
+            raise ValueError(f"a cache is [layers][pages][kv heads][{PAGE}][64 or 128], not {list(k.shape)}")
+        for t, dtype, shape in ((k, k.dtype, k.shape), (v, k.dtype, k.shape)) + (((k_scale, torch.float32, k.shape[:-1]), (v_scale, torch.float32, k.shape[:-1])) if i8 else ()):
+            if t.shape != shape or t.dtype is not dtype or t.device != k.device or not t.is_cuda or not (t[0] if k.dim() == 5 else t).is_contiguous():
+                raise ValueError("keys, values and scales of one shape, contiguous inside a layer, on one CUDA device")
+        if k.dim() == 5:
+            layer = k[0].numel()
+            if k.shape[0] > 1 and (k.stride(0) < layer or k.stride(0) != v.stride(0) or i8 and (k_scale.stride(0) != v_scale.stride(0) or k_scale.stride(0) < layer // k.shape[-1])):
+                raise ValueError("layers that do not overlap, as far apart in the values as in the keys")
+        if (k.data_ptr() | v.data_ptr()) % 16 or k.dim() == 5 and k.stride(0) * k.element_size() % 16:
+            raise ValueError("a layer's keys and values begin at multiples of 16 bytes")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.layers = k.shape[0] if k.dim() == 5 else 1
+        self.pages, self.heads, _, self.d = k.shape[-4:]
+        if self.pages * self.heads * PAGE >= 1 << 31:
+            raise ValueError("a layer of fewer than 2^31 rows")
+        self.device, self.i8 = k.device, i8
+        self._kv = (k.data_ptr(), v.data_ptr())
+        self._scales = (k_scale.data_ptr(), v_scale.data_ptr()) if i8 else (None, None)
+
+
+class TreeStep:
+    """What ``plan`` leaves of a step, for up to ``max_rows`` rows: ``lengths`` ``[requests]`` and ``row_start`` ``[requests + 1]``; of every row
+    its request ``row_req``, position ``row_pos``, cache slot ``slots`` (page x 16 + place), parent ``parents`` and, 64 bits, ancestors ``masks``
+    (bit j: node j of its tree, itself among them; a program may clear or set bits before ``attention``).  Rows behind the last request's
+    are -1 (masks 0).
+
+    ``block_table`` int32 ``[requests][blocks]``: pages of the requests' positions, filled up by ``plan``.  ``tree_table`` int32
+    ``[requests][blocks]``: pages of their trees.  ``num_pages``: pages that tables may name.  ``max_nodes``: of a tree, at most."""
+
+    def __init__(self, block_table: torch.Tensor, tree_table: torch.Tensor, max_rows: int, num_pages: int, max_nodes: int = MAX_NODES):
+        b, dev = block_table.shape[0], block_table.device
+        _flat(block_table, torch.int32, (b, block_table.shape[-1]), "block table")
+        _flat(tree_table, torch.int32, (b, tree_table.shape[-1]), "tree table", dev)
+        if not 1 <= b <= MAX_REQUESTS or block_table.shape[1] < 1:
+            raise ValueError(f"a step of 1 to {MAX_REQUESTS} requests, whose tables hold a page at least")
+        if not 1 <= max_rows <= MAX_ROWS:
+            raise ValueError(f"a step of 1 to {MAX_ROWS} rows")
+        if not 1 <= max_nodes <= min(MAX_NODES, PAGE * tree_table.shape[1]):
+            raise ValueError(f"trees of 1 to {min(MAX_NODES, PAGE * tree_table.shape[1])} nodes, not {max_nodes}")
+        if not 1 <= num_pages < 1 << 27:
+            raise ValueError("tables of 1 to 2^27 pages")
+        self.block_table, self.tree_table, self.device = block_table, tree_table, dev
+        self.requests, self.max_rows, self.num_pages, self.max_nodes = b, max_rows, num_pages, max_nodes
+        one = lambda n, t=torch.int32: torch.full((n,), -1, dtype=t, device=dev)          # noqa: E731
+        self.lengths = torch.zeros(b, dtype=torch.int32, device=dev)
+        self.row_start = torch.zeros(b + 1, dtype=torch.int32, device=dev)
+        self.row_req, self.row_pos, self.slots, self.parents = one(max_rows), one(max_rows), one(max_rows), one(max_rows)
+        self.masks = torch.zeros(max_rows, dtype=torch.int64, device=dev)
+        self.status = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.tree: Optional[bool] = None       # the last plan's rows are trees'
+        self._tables = (block_table.data_ptr(), tree_table.data_ptr())
+        self._rows = (self.row_start.data_ptr(), self.row_req.data_ptr(), self.row_pos.data_ptr())
+        self._plan = (self.lengths.data_ptr(), *self._rows, self.slots.data_ptr(), self.parents.data_ptr(), self.masks.data_ptr(), self.status.data_ptr())
+
+    def check(self):
+        """Waits for the last plan and raises where it could not be made."""
+        word = int(self.status[0])
+        if word:
+            raise K.KernelError("plan: " + "; ".join(text for bit, text in _FAULTS.items() if word & bit))
+
+
+class Accepted:
+    """What ``commit`` says of every request: ``path`` ``[requests][64]`` nodes of the accepted path, -1 behind it; their number ``count``;
+    ``next_token``, the target of the last one (-1: no rows); ``lengths`` with the path's."""
+
+    def __init__(self, path: torch.Tensor, count: torch.Tensor, next_token: torch.Tensor, lengths: torch.Tensor):
+        b, dev = count.numel(), count.device
+        self.path, self.count = _flat(path, torch.int32, (b, MAX_NODES), "accepted path", dev), _flat(count, torch.int32, (b,), "accepted nodes")
+        self.next_token, self.lengths = _flat(next_token, torch.int32, (b,), "next tokens", dev), _flat(lengths, torch.int32, (b,), "lengths", dev)
+        self._out = (path.data_ptr(), count.data_ptr(), next_token.data_ptr(), lengths.data_ptr())
+
+    @staticmethod
+    def empty(requests: int, device) -> "Accepted":
+        f = lambda *s: torch.empty(s, dtype=torch.int32, device=device)         # noqa: E731
+        return Accepted(f(requests, MAX_NODES), f(requests), f(requests), f(requests))
+
+
+def plan(step: TreeStep, lengths: torch.Tensor, counts: torch.Tensor, parents: Optional[torch.Tensor], pool: PagePool, after: Optional[PagePool] = None) -> TreeStep:
+    """Lays out a step.  ``lengths``: cached positions of every request; ``counts``: its rows (0: none; -1: the request leaves and its pages go
+    back).  ``parents``: of all rows, one request's after another, each the number of a node before it in its tree, or -1; None: the rows of a
+    request are consecutive positions from its length on.  Block tables get the pages that are missing up to a request's length and longest path
+    (``parents`` None: all its rows), in the order of the requests.  ``after``: where the pool's numbers are written (over the same free
+    pages; None: in place)."""
+    b, dev = step.requests, step.device
+    after = pool if after is None else after
+    _flat(lengths, torch.int32, (b,), "lengths", dev)
+    _flat(counts, torch.int32, (b,), "rows of the requests", dev)
+    if parents is not None and (parents.dtype is not torch.int32 or parents.dim() != 1 or parents.device != dev or not parents.is_contiguous() or parents.numel() > step.max_rows):
+        raise ValueError(f"parents: up to {step.max_rows} contiguous int32 numbers on {dev}")
+    if pool.held.numel() != b or pool.free.device != dev or after.held.numel() != b or after.free.data_ptr() != pool.free.data_ptr():
+        raise ValueError(f"pools of {b} requests on {dev}, over the same free pages")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return plan(step, lengths, counts, parents, pool, after)
+    rows = step.max_rows if parents is None else parents.numel()
+    K._check(_entry("b2_tree_plan", "p" * 18 + "i" * 8 + "p")(
+        lengths.data_ptr(), counts.data_ptr(), None if parents is None else parents.data_ptr(), *step._tables, pool.free.data_ptr(), pool.n_free.data_ptr(),
+        pool.held.data_ptr(), after.n_free.data_ptr(), after.held.data_ptr(), *step._plan, b, step.block_table.shape[1], step.tree_table.shape[1],
+        pool.free.numel(), step.max_rows, step.max_nodes, step.num_pages, rows, _stream(dev)), "tree_plan")
+    step.tree = parents is not None
+    return step
+
+
+def _check_cache(step: TreeStep, cache: TreeCache, layers: bool):
+    if step.tree is None:
+        raise ValueError("the step has no plan yet")
+    if cache.device != step.device or cache.pages < step.num_pages or cache.layers > 1 and not layers:
+        raise ValueError(f"{'a' if layers else 'one layer of a'} cache of at least {step.num_pages} pages on {step.device}")
+
+
+def rope_append(step: TreeStep, qkv: torch.Tensor, rope: tuple, q: torch.Tensor, cache: TreeCache, interleaved: bool = False) -> torch.Tensor:
+    """Rows of a qkv projection, ``[rows][(n_q + 2 n_kv) D]`` bf16 or fp32, or fp32 partial sums ``[slices][rows][...]``: queries turned into ``q``
+    (bf16 ``[rows][n_q D]``), keys turned and values as they are into the cache at the step's slots.  ``rope``: (cos, sin) tables fp32
+    ``[positions][pairs]``, for the first 2 x pairs dimensions of a head (pairs a multiple of 4): pair i is dimensions i and i + pairs, or with
+    ``interleaved`` 2 i and 2 i + 1.  Scaled positions and factors are the tables' (``models.config.Rotary``).  Rows behind the step's are left."""
+    _check_cache(step, cache, False)
+    dev, d, n_kv = step.device, cache.d, cache.heads
+    slices, slice_elems, x = 0, 0, qkv
+    if qkv.dtype is torch.float32:
+        slices = 1
+        if qkv.dim() == 3:
+            slices, slice_elems, x = qkv.shape[0], qkv.stride(0), qkv[0] if qkv.shape[0] else qkv
+    rows, n, ld, at = _rows_of(x, qkv.dtype, "rows", 16 if slices else 8)
+    if qkv.dtype not in (torch.bfloat16, torch.float32) or x.device != dev or not 1 <= rows <= step.max_rows or at % 16 or slice_elems % 4:
+        raise ValueError(f"rows: 1 to {step.max_rows} of bf16 or fp32 on {dev}, slices and the first row at multiples of 16 bytes")
+    n_q, rest = divmod(n, d)
+    n_q -= 2 * n_kv
+    if rest or n_q < 1 or n_q % n_kv:
+        raise ValueError(f"rows of {n} columns: heads of {d}, {n_kv} of keys and of values")
+    mq, cols, ldq, pq = _rows_of(q, torch.bfloat16, "queries", 8)
+    if mq != rows or cols != n_q * d or q.device != dev or pq % 16:
+        raise ValueError(f"queries: {rows} rows of {n_q * d} on {dev}")
+    cos, sin = rope
+    if cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] % 4 or 2 * cos.shape[1] > d or (cos.data_ptr() | sin.data_ptr()) % 16:
+        raise ValueError(f"rotation: tables of positions x pairs, a multiple of 4 up to {d // 2}")
+    _flat(cos, torch.float32, cos.shape, "cosines", dev)
+    _flat(sin, torch.float32, cos.shape, "sines", dev)
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return rope_append(step, qkv, rope, q, cache, interleaved)
+    K._check(_entry("b2_tree_rope", "pllippippiiiiiiplppppl" + "p")(
+        at, ld, slice_elems, slices, step._rows[2], step.slots.data_ptr(), rows, cos.data_ptr(), sin.data_ptr(), 2 * cos.shape[1], cos.shape[0], int(interleaved), n_q, n_kv, d,
+        pq, ldq, *cache._kv, *cache._scales, cache.pages * PAGE, _stream(dev)), "tree_rope")
+    return q
+
+
+def attention(step: TreeStep, q: torch.Tensor, cache: TreeCache, out: torch.Tensor, scale: float, window: int = 0) -> torch.Tensor:
+    """Rows ``q`` ``[rows][n_q D]`` bf16 over one layer's cache into ``out`` (the same shape, bf16): softmax in fp32 over the request's cached
+    positions and the nodes of the row's mask, ``window`` > 0: those less than ``window`` positions before the row.  A row that sees nothing is
+    0, whatever the places hold that it does not see; rows behind the step's are left."""
+    _check_cache(step, cache, False)
+    dev, d, n_kv = step.device, cache.d, cache.heads
+    if not step.tree:
+        raise ValueError("the step's rows are no trees'")
+    rows, n, ldq, pq = _rows_of(q, torch.bfloat16, "queries", 16)
+    mo, no, ldo, po = _rows_of(out, torch.bfloat16, "outputs", 16)
+    n_q = n // d
+    if n != n_q * d or n_q < 1 or n_q % n_kv or n_q // n_kv > MAX_GROUP or not 1 <= rows <= step.max_rows or q.device != dev:
+        raise ValueError(f"queries: 1 to {step.max_rows} rows of heads of {d}, 1 to {MAX_GROUP} to each of {n_kv} key heads, on {dev}")
+    if mo != rows or no != n or out.device != dev:
+        raise ValueError(f"outputs: {rows} rows of {n} on {dev}")
+    if window < 0 or not abs(scale) < float("inf"):
+        raise ValueError("a window of 0 (none) or more positions, a finite scale")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return attention(step, q, cache, out, scale, window)
+    fn = _attention_entry()
+    K._check(fn(pq, ldq, *cache._kv, *cache._scales, step._plan[0], *step._rows, *step._tables, step._plan[6], po, ldo, rows, step.requests, step.block_table.shape[1],
+                step.tree_table.shape[1], cache.pages, n_q, n_kv, d, window, scale, _stream(dev)), "tree_attention")
+    return out
+
+
+MAX_GROUP = 64          # query heads to a key head
+_attention_fn = None
+
+
+def _attention_entry():
+    global _attention_fn
+    if _attention_fn is None:
+        fn = K.lib().b2_tree_attention
+        p, q, i = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+        fn.restype, fn.argtypes = ctypes.c_int, [p, q] + [p] * 12 + [q] + [i] * 9 + [ctypes.c_float, p]
+        _attention_fn = fn
+    return _attention_fn
+
+
+def commit(step: TreeStep, tokens: torch.Tensor, targets: torch.Tensor, cache: TreeCache, accepted: Optional[Accepted] = None) -> Accepted:
+    """Settles a step.  ``tokens``: the rows' tokens; ``targets``: the token that the model gives behind each row (its arg-max, or a draw), int32
+    ``[rows]``.  The path begins at a tree's node 0 and goes on with the child whose token is its parent's target, of equal ones the first.
+    Its keys and values move from the tree's pages to the request's positions in every layer of ``cache``; nothing else is touched.
+    ``accepted.lengths`` may be the tensor that the next ``plan`` reads."""
+    _check_cache(step, cache, True)
+    dev, b = step.device, step.requests
+    if not step.tree:
+        raise ValueError("the step's rows are no trees'")
+    if tokens.dim() != 1 or not 1 <= tokens.numel() <= step.max_rows:
+        raise ValueError(f"tokens: of 1 to {step.max_rows} rows")
+    _flat(tokens, torch.int32, tokens.shape, "tokens", dev)
+    _flat(targets, torch.int32, tokens.shape, "targets", dev)
+    if accepted is None:
+        accepted = Accepted.empty(b, dev)
+    elif accepted.count.numel() != b or accepted.count.device != dev or accepted._out[3] == step._plan[0]:
+        raise ValueError(f"results of {b} requests on {dev}, apart from the step's own")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return commit(step, tokens, targets, cache, accepted)
+    k, ks = cache.k, cache.k_scale
+    five = k.dim() == 5
+    K._check(_entry("b2_tree_commit", "p" * 9 + "lppl" + "pppp" + "i" * 8 + "p")(
+        step._plan[0], step._rows[0], step._plan[5], tokens.data_ptr(), targets.data_ptr(), *step._tables, *cache._kv, k.stride(0) * k.element_size() if five else 0,
+        *cache._scales, ks.stride(0) if five and ks is not None else 0, *accepted._out, b, step.block_table.shape[1], step.tree_table.shape[1], cache.layers, cache.pages,
+        cache.heads, cache.d * k.element_size(), tokens.numel(), _stream(dev)), "tree_commit")
+    return accepted
