@@ -19,7 +19,7 @@ Caches are ``KVCache`` planes: ``[page][kv head][16][D]`` with D 64 or 128, bf16
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
+import functools
 from typing import Optional
 
 import torch
@@ -222,29 +222,33 @@ def attention(step: TreeStep, q: torch.Tensor, cache: TreeCache, out: torch.Tens
         raise ValueError(f"queries: 1 to {step.max_rows} rows of heads of {d}, 1 to {MAX_GROUP} to each of {n_kv} key heads, on {dev}")
     if mo != rows or no != n or out.device != dev:
         raise ValueError(f"outputs: {rows} rows of {n} on {dev}")
-    if window < 0 or not abs(scale) < float("inf"):
-        raise ValueError("a window of 0 (none) or more positions, a finite scale")
+    if window < 0 or not 0 < scale < float("inf"):
+        raise ValueError("a window of 0 (none) or more positions, a scale above 0")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return attention(step, q, cache, out, scale, window)
-    fn = _attention_entry()
-    K._check(fn(pq, ldq, *cache._kv, *cache._scales, step._plan[0], *step._rows, *step._tables, step._plan[6], po, ldo, rows, step.requests, step.block_table.shape[1],
-                step.tree_table.shape[1], cache.pages, n_q, n_kv, d, window, scale, _stream(dev)), "tree_attention")
+    fn, work = _attention_entry(), torch.empty(_attention_work(step.requests, step.block_table.shape[1], n_q, n_kv, d, step.max_nodes, dev.index), dtype=torch.float32, device=dev)
+    K._check(fn(pq, ldq, *cache._kv, *cache._scales, step._plan[0], *step._rows, *step._tables, step._plan[6], po, work.data_ptr(), ldo, rows, step.requests,
+                step.block_table.shape[1], step.tree_table.shape[1], cache.pages, n_q, n_kv, d, step.max_nodes, window, scale, _stream(dev)), "tree_attention")
+    K.launch_count += 1      # segments added up
     return out
 
 
 MAX_GROUP = 64          # query heads to a key head
-_attention_fn = None
 
 
+@functools.lru_cache(maxsize=None)
+def _attention_work(requests: int, blocks: int, n_q: int, n_kv: int, d: int, max_nodes: int, device: int) -> int:
+    """fp32 words of workspace on the device, which is the current one."""
+    return _entry("b2_tree_attention_work", "iiiiii", ctypes.c_longlong)(requests, blocks, n_q, n_kv, d, max_nodes)
+
+
+@functools.lru_cache(maxsize=None)
 def _attention_entry():
-    global _attention_fn
-    if _attention_fn is None:
-        fn = K.lib().b2_tree_attention
-        p, q, i = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
-        fn.restype, fn.argtypes = ctypes.c_int, [p, q] + [p] * 12 + [q] + [i] * 9 + [ctypes.c_float, p]
-        _attention_fn = fn
-    return _attention_fn
+    fn = K.lib().b2_tree_attention
+    p, q, i = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+    fn.restype, fn.argtypes = ctypes.c_int, [p, q] + [p] * 13 + [q] + [i] * 10 + [ctypes.c_float, p]
+    return fn
 
 
 def commit(step: TreeStep, tokens: torch.Tensor, targets: torch.Tensor, cache: TreeCache, accepted: Optional[Accepted] = None) -> Accepted:

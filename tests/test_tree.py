@@ -583,7 +583,7 @@ def test_refusals():
     small = make_cache(s.pages - 1, 2, 128, False)
     # attention
     for bad in ((step, q.float(), cache, out, 0.1), (step, q, cache, out[:7], 0.1), (step, bf(9, 512), cache, bf(9, 512), 0.1), (step, q[:, :500], cache, out[:, :500], 0.1),
-                (step, bf(8, 384), cache, bf(8, 384), 0.1), (step, q, many, out, 0.1), (step, q, small, out, 0.1), (step, q, cache, out, 0.1, -1), (step, q, cache, out, INF),
+                (step, bf(8, 384), cache, bf(8, 384), 0.1), (step, q, many, out, 0.1), (step, q, small, out, 0.1), (step, q, cache, out, 0.1, -1), (step, q, cache, out, INF), (step, q, cache, out, 0.0), (step, q, cache, out, -0.1),
                 (step, q, cache, out, NAN), (step, bf(8, 513)[:, 1:], cache, out, 0.1), (step, q.cpu(), cache, out, 0.1), (step, q[:0], cache, out[:0], 0.1),
                 (step, bf(8, 2 * 65 * 128), cache, bf(8, 2 * 65 * 128), 0.1), (step, q, cache, out.t().contiguous().t(), 0.1)):
         no(T.attention, *bad)
