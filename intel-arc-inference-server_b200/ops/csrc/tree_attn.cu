@@ -13,13 +13,17 @@
 // begins and ends inside a request as a rule: what it has of one is a segment.  A segment that is all of a request's key head writes results;
 // the others leave unnormalised sums against their running maximum, and a second kernel adds them up in the order of the keys.
 //
-// A CTA: one warp copies (tiled TMA, 16 keys x 64 dims a box, 128-byte swizzle; pages behind the end are asked for outside the tensor and
-// come as zeros), one thread per query tile issues the products, a thread per query row does the softmax: scores come from tensor memory, P goes
-// back there as the A operand of P V; the accumulator is rescaled only where a row's maximum grew by more than 2^6.  Score buffers are
-// double, so that the next scores are under way while a tile's softmax runs.  Up to 128 query rows (NW 1) two CTAs share an SM; beyond (NW 2)
-// a CTA has two query tiles that share every K / V tile.  More than 256 rows take further CTAs (blockIdx.y) over the same keys.
-// An 8-bit cache comes in as bytes (bulk copies, scales with them), four warps make integers in bf16 of them, which are exact; K's scale goes on
-// the scores and V's on the weights, both in fp32.
+// A CTA: two threads copy (tiled TMA, 16 keys x 64 dims a box, 128-byte swizzle; pages behind the end are asked for outside the tensor and
+// come as zeros); two threads issue products and two groups of 256 threads do softmax, two threads to a query row of which each has 32 of a
+// tile's 64 keys.  Scores come from tensor memory into registers once, and their place is free for the next ones; P goes back to tensor memory
+// as the A operand of P V; the accumulator is rescaled only where a row's maximum grew by more than 2^6.
+//   up to 128 query rows (NW 1): both groups have the same rows and take every other tile, each with its own maxima, sums and accumulator, which
+//     meet at the segment's end; the queries are in tensor memory.  One softmax takes longer than its tile's bytes, two at a time do not.
+//   up to 256 (NW 2): a group has a query tile of its own and both share every K / V tile; the queries are in shared memory.
+// More rows take further CTAs (blockIdx.y) over the same keys.
+// An 8-bit cache comes in as bytes (bulk copies, scales with them), eight warps make integers in bf16 of them, which are exact; K's scale goes on
+// the scores and V's on the weights, both in fp32.  Of four dimensions the second and the third change places on the way (pairs come apart that
+// way), which the queries follow and the results undo.
 #include "common.cuh"
 
 using namespace b2;
@@ -50,15 +54,15 @@ struct Form {
   static constexpr int NDK = NDK_, NW = NW_, D = NDK_ * 64;
   static constexpr bool I8 = I8_;
   static constexpr int T_BYTES = BK * NDK * 128;                 // a K or V tile: [64-dim blocks][64 keys][128 bytes]
-  static constexpr int KVS = I8_ ? NW_ : (NW_ == 1 ? (NDK_ == 1 ? 4 : 2) : 4);      // operand tiles
-  static constexpr int RS = I8_ ? (NW_ == 1 ? (NDK_ == 1 ? 4 : 2) : 4) : 0;         // stages of bytes
+  static constexpr int KS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 6 : 4) * (3 - NDK_), VS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 7 : 5) * (3 - NDK_);     // operand tiles
+  static constexpr int RS = I8_ ? 5 * (3 - NDK_) : 0;                                                     // stages of bytes
   static constexpr int S_BYTES = 2 * BK * D + 2 * BK * 4;        // keys, values, their scales
-  static constexpr int Q_BYTES = NW * BQ * NDK * 128;
-  static constexpr int kMma = 1, kSoft = 1 + NW, kConv = kSoft + 4 * NW, kWarps = kConv + (I8_ ? 4 : 0), kThreads = kWarps * 32;
-  static constexpr int TMEM = NW == 1 ? 256 : 512;
-  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + KVS * T_BYTES, OFF_ST = OFF_V + KVS * T_BYTES, OFF_SC = OFF_ST + RS * S_BYTES,
-                       OFF_CUM = OFF_SC + (I8_ ? 4 * 2 * BK * 4 : 0), OFF_BAR = OFF_CUM + (kMaxReq + 8) * 4, SMEM = OFF_BAR + 512 + 1024;
-  static_assert(SMEM <= (NW == 1 ? 115712 : 227 * 1024), "shared memory");
+  static constexpr int Q_BYTES = NW == 1 ? 0 : NW * BQ * NDK * 128;
+  static constexpr int kMma = 2, kSoft = 4, kConv = kSoft + 16, kConvThreads = 256, kWarps = kConv + (I8_ ? kConvThreads / 32 : 0), kThreads = kWarps * 32;
+  static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + KS * T_BYTES, OFF_ST = OFF_V + VS * T_BYTES, OFF_SC = OFF_ST + RS * S_BYTES,
+                       OFF_X = OFF_SC + (I8_ ? 4 * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * 2 * BQ * 4, OFF_BAR = OFF_CUM + (kMaxReq + 8) * 4,
+                       SMEM = OFF_BAR + 1024 + 1024;
+  static_assert(SMEM <= 227 * 1024 && KS <= 14 && VS <= 14 && RS <= 14, "shared memory");
 };
 
 // V as an MN-major operand: rows are keys of 128 bytes (64 dims), 8-key groups 1024 bytes apart, the next 64 dims a block further.
@@ -72,7 +76,30 @@ __device__ __forceinline__ uint64_t make_desc_v(uint32_t smem_addr) {
   return d;
 }
 
-__device__ __forceinline__ void st_32(uint32_t taddr, const uint32_t (&r)[32]) { B2_TMEM_ST_32(taddr, r); }
+// columns of the thread's row between registers and tensor memory
+__device__ __forceinline__ void st_16(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void st_8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]),
+               "r"(r[7]), "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void ld_16(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                 "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {      // a look that never waits
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 __device__ __forceinline__ uint32_t bytes_bf16(uint32_t w) {      // even bytes as integers in bf16: 128 + (b & 127) less 128, or 256 where the sign is set
   uint32_t lo = (w & 0x007f007fu) | 0x43004300u, hi = (w & 0x00800080u) | 0x43004300u, d;
@@ -121,46 +148,49 @@ __device__ __forceinline__ bool next_segment(const TreeAttnParams& p, const int*
 }
 
 template <class F>
-__global__ void __launch_bounds__(F::kThreads, F::NW == 1 ? 2 : 1)
+__global__ void __launch_bounds__(F::kThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeAttnParams p) {
-  constexpr int NDK = F::NDK, NW = F::NW, KVS = F::KVS, D = F::D, RS = F::I8 ? F::RS : 1;
+  constexpr int NDK = F::NDK, NW = F::NW, KS = F::KS, VS = F::VS, D = F::D, RS = F::I8 ? F::RS : 1;
+  constexpr int kStep = NW == 1 ? 2 : 1;      // a group's next tile
   extern __shared__ uint8_t smem_raw[];
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t q_s = base, k_s0 = base + F::OFF_K, v_s0 = base + F::OFF_V, st_s0 = base + F::OFF_ST, bars = base + F::OFF_BAR;
   int* const s_cum = reinterpret_cast<int*>(gen + F::OFF_CUM);
   float* const s_scale = reinterpret_cast<float*>(gen + F::OFF_SC);       // [4][K, V][64]
-  const uint32_t b_kfull = bars, b_kempty = bars + 32, b_vfull = bars + 64, b_vempty = bars + 96, b_rfull = bars + 128, b_rempty = bars + 160;
-  auto b_q = [&](int w) { return bars + 192 + w * 8; };
-  auto b_sfull = [&](int w, int s) { return bars + 208 + (w * 2 + s) * 8; };
-  auto b_pfull = [&](int w, int s) { return bars + 240 + (w * 2 + s) * 8; };
-  auto b_odone = [&](int w, int s) { return bars + 272 + (w * 2 + s) * 8; };
-  auto b_scale = [&](int g) { return bars + 304 + (g & 3) * 8; };
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gen + F::OFF_BAR + 344);
-  int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 384);      // [16]
+  float* const s_x = reinterpret_cast<float*>(gen + F::OFF_X);            // [group][parity][half][128]
+  const uint32_t b_kfull = bars, b_kempty = bars + 112, b_vfull = bars + 224, b_vempty = bars + 336, b_rfull = bars + 448, b_rempty = bars + 560, b_q = bars + 672;
+  auto b_sfull = [&](int w) { return bars + 680 + w * 8; };
+  auto b_sfree = [&](int w) { return bars + 696 + w * 8; };
+  auto b_pfull = [&](int w) { return bars + 712 + w * 8; };
+  auto b_odone = [&](int w) { return bars + 728 + w * 8; };
+  auto b_scale = [&](int g) { return bars + 744 + (g & 3) * 8; };
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gen + F::OFF_BAR + 776);
+  int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 784);      // [warps]
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
-    for (int i = 0; i < KVS; ++i) {
-      mbar_init(b_kfull + 8 * i, F::I8 ? 128 : 1);
+    for (int i = 0; i < KS; ++i) {
+      mbar_init(b_kfull + 8 * i, F::I8 ? F::kConvThreads : 1);
       mbar_init(b_kempty + 8 * i, NW);
-      mbar_init(b_vfull + 8 * i, F::I8 ? 128 : 1);
+    }
+    for (int i = 0; i < VS; ++i) {
+      mbar_init(b_vfull + 8 * i, F::I8 ? F::kConvThreads : 1);
       mbar_init(b_vempty + 8 * i, NW);
     }
     if (F::I8) {
       for (int i = 0; i < RS; ++i) {
-        mbar_init(b_rfull + 8 * i, 1);
-        mbar_init(b_rempty + 8 * i, 128);
+        mbar_init(b_rfull + 8 * i, 2);
+        mbar_init(b_rempty + 8 * i, F::kConvThreads);
       }
       for (int i = 0; i < 4; ++i) mbar_init(b_scale(i), 128);
     }
-    for (int w = 0; w < NW; ++w) {
-      mbar_init(b_q(w), 128);
-      for (int s = 0; s < 2; ++s) {
-        mbar_init(b_sfull(w, s), 1);
-        mbar_init(b_pfull(w, s), 128);
-        mbar_init(b_odone(w, s), 1);
-      }
+    mbar_init(b_q, 512);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(b_sfull(w), 1);
+      mbar_init(b_sfree(w), 256);
+      mbar_init(b_pfull(w), 256);
+      mbar_init(b_odone(w), 1);
     }
     mbar_fence_init();
     if (!F::I8) {
@@ -169,7 +199,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
   }
   if (warp == F::kMma) {
-    tmem_alloc(smem_u32(tmem_slot), F::TMEM);
+    tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
   pdl_wait();
@@ -193,7 +223,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     if (lane == 31) s_sums[warp] = x;
     __syncthreads();
     int before = x - mine;
-    for (int w = 0; w < warp; ++w) before += s_sums[w];
+    if (b0 < p.B)
+      for (int w = 0; w < warp; ++w) before += s_sums[w];
     for (int b = b0; b < min(b0 + per, p.B); ++b) s_cum[b + 1] += before;
     if (tid == 0) s_cum[0] = 0;
   }
@@ -201,8 +232,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  auto t_s = [&](int w, int s) { return tmem_base + (uint32_t)(w * 2 + s) * BK; };
-  auto t_o = [&](int w) { return tmem_base + (uint32_t)(NW * 2 * BK + w * D); };
+  // tensor memory: queries 64 columns (NW 1), scores 2 x 64, weights 2 x 32, accumulators 2 x D
+  const uint32_t t_q = tmem_base;
+  auto t_s = [&](int w) { return tmem_base + 64 + (uint32_t)w * 64; };
+  auto t_p = [&](int w) { return tmem_base + 192 + (uint32_t)w * 32; };
+  auto t_o = [&](int w) { return tmem_base + 256 + (uint32_t)w * D; };
 
   const long long total = (long long)s_cum[p.B] * p.n_kv, each = (total + gridDim.x - 1) / gridDim.x;
   if (blockIdx.x == 0 && blockIdx.y == 0) {
@@ -220,11 +254,18 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     k.b = lo;
   }
+  // keys of tile t of the walk's request
+  auto keys_of = [&](int t) { return t == k.r.nt - 1 ? k.r.n : min(BK, k.r.length - (k.r.first + t) * BK); };
 
-  if (warp == 0) {
-    // ---------------------------------------------------------- copies: lanes issue one box (bf16) or one run of bytes (8-bit) each
+  if (warp < F::kMma) {
+    // ---------------------------------------------------------- copies of keys (warp 0) and of values (warp 1): page numbers in the lanes, one
+    // thread issues (eight lanes that issue a box each are served one after another: 1850 cycles for a tile's 16 boxes)
     bool ok = true;
     int g = 0;
+    const bool is_v = warp == 1;
+    const int kd = F::I8 ? RS : is_v ? VS : KS;      // depth of this warp's ring
+    const uint32_t full0 = F::I8 ? b_rfull : is_v ? b_vfull : b_kfull, empty0 = F::I8 ? b_rempty : is_v ? b_vempty : b_kempty;
+    int s = 0, par = 0;
     while (ok && next_segment<F>(p, s_cum, k)) {
       const int limit = min((k.r.length + kPage - 1) / kPage, p.max_blocks), tree_pages = (k.r.n + kPage - 1) / kPage;
       const int* bt = p.block_table + (size_t)k.r.b * p.max_blocks;
@@ -245,219 +286,253 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           ids = ahead;
           ahead = entry(at + 32 + lane);
         }
-        const int pg = F::I8 ? (lane >> 2) & 3 : (lane / NDK) & 3;
-        int page = __shfl_sync(0xffffffffu, tree ? tree_ids : ids, tree ? pg : pi - at + pg);
-        const bool there = page >= 0;
-        if constexpr (F::I8) {
-          const int s = g % RS;
-          const uint32_t full = b_rfull + 8 * s, st = st_s0 + s * F::S_BYTES;
-          if (g >= RS) ok = mbar_wait(b_rempty + 8 * s, ((g / RS) & 1) ^ 1, ERR_ATTN_WAIT);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          const int pages = __popc(__ballot_sync(0xffffffffu, lane < 16 && there)) >> 2;
-          if (lane == 0) mbar_expect_tx(full, pages * (2 * kPage * D + 2 * kPage * 4));
-          __syncwarp();
-          if (lane < 16 && there) {
-            const long long row = ((long long)page * p.n_kv + k.h) * kPage;
-            const int which = lane & 3;
-            if (which < 2) bulk_g2s(st + which * (BK * D) + pg * (kPage * D), (which ? p.v8 : p.k8) + row * D, kPage * D, full);
-            else bulk_g2s(st + 2 * BK * D + (which - 2) * (BK * 4) + pg * (kPage * 4), (which == 3 ? p.v_scale : p.k_scale) + row, kPage * 4, full);
+        int page[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) page[x] = __shfl_sync(0xffffffffu, tree ? tree_ids : ids, tree ? x : pi - at + x);
+        if (lane == 0) {
+          if (g >= kd) ok = mbar_wait(empty0 + 8 * s, par ^ 1, ERR_ATTN_WAIT);
+          if (ok) {
+            const uint32_t full = full0 + 8 * s;
+            if constexpr (F::I8) {
+              int pages = 0;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) pages += page[x] >= 0;
+              mbar_expect_tx(full, pages * (kPage * D + kPage * 4));
+              const uint32_t st = st_s0 + s * F::S_BYTES + (is_v ? BK * D : 0), sc = st_s0 + s * F::S_BYTES + 2 * BK * D + (is_v ? BK * 4 : 0);
+              const int8_t* data = is_v ? p.v8 : p.k8;
+              const float* scale = is_v ? p.v_scale : p.k_scale;
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                if (page[x] >= 0) {
+                  const long long row = ((long long)page[x] * p.n_kv + k.h) * kPage;
+                  bulk_g2s(st + x * (kPage * D), data + row * D, kPage * D, full);
+                  bulk_g2s(sc + x * (kPage * 4), scale + row, kPage * 4, full);
+                }
+            } else {
+              mbar_expect_tx(full, F::T_BYTES);
+              const uint32_t dst = (is_v ? v_s0 : k_s0) + s * F::T_BYTES;
+              const CUtensorMap* map = is_v ? &map_v : &map_k;
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const int row = (page[x] >= 0 ? page[x] * p.n_kv + k.h : p.num_pages * p.n_kv) * kPage;
+#pragma unroll
+                for (int c = 0; c < NDK; ++c) tma_load_2d(dst + c * (BK * 128) + x * (kPage * 128), map, c * 64, row, full);
+              }
+            }
           }
-        } else {
-          const int s = g % KVS, ph = (g / KVS) & 1;
-          const int row = there ? (page * p.n_kv + k.h) * kPage : p.num_pages * p.n_kv * kPage, c = lane % NDK;
-          const uint32_t dst = s * F::T_BYTES + c * (BK * 128) + pg * (kPage * 128);
-          if (g >= KVS) ok = mbar_wait(b_kempty + 8 * s, ph ^ 1, ERR_ATTN_WAIT);
-          if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-          if (lane == 0) mbar_expect_tx(b_kfull + 8 * s, F::T_BYTES);
-          __syncwarp();
-          if (lane < 4 * NDK) tma_load_2d(k_s0 + dst, &map_k, c * 64, row, b_kfull + 8 * s);
-          if (g >= KVS) ok = mbar_wait(b_vempty + 8 * s, ph ^ 1, ERR_ATTN_WAIT);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            mbar_wait(b_kfull + 8 * s, ph, ERR_ATTN_WAIT);      // the K copies just issued
-            break;
-          }
-          if (lane == 0) mbar_expect_tx(b_vfull + 8 * s, F::T_BYTES);
-          __syncwarp();
-          if (lane < 4 * NDK) tma_load_2d(v_s0 + dst, &map_v, c * 64, row, b_vfull + 8 * s);
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (++s == kd) { s = 0; par ^= 1; }
       }
     }
-    if (!ok) {      // copies in flight end before the CTA does
-      if constexpr (F::I8)
-        for (int i = max(0, g - RS); i < g; ++i) mbar_wait(b_rfull + 8 * (i % RS), (i / RS) & 1, ERR_ATTN_WAIT);
-      else
-        for (int i = max(0, g - KVS); i < g; ++i) {
-          mbar_wait(b_kfull + 8 * (i % KVS), (i / KVS) & 1, ERR_ATTN_WAIT);
-          mbar_wait(b_vfull + 8 * (i % KVS), (i / KVS) & 1, ERR_ATTN_WAIT);
-        }
-    }
+    if (!ok && lane == 0)      // copies in flight end before the CTA does
+      for (int i = max(0, g - kd); i < g; ++i) mbar_wait(full0 + 8 * (i % kd), (i / kd) & 1, ERR_ATTN_WAIT);
   } else if (warp < F::kSoft) {
-    // ---------------------------------------------------------- products of query tile w
+    // ---------------------------------------------------------- products of group w
     const int w = warp - F::kMma;
     constexpr uint32_t idesc_qk = make_idesc(1, 1, BQ, BK);
     constexpr uint32_t idesc_pv = make_idesc(1, 1, BQ, D) | (1u << 16);      // V is MN-major
     const uint32_t hi_k = (uint32_t)(make_desc_sw128(0) >> 32), hi_v = (uint32_t)(make_desc_v(0) >> 32);
     const uint32_t ql = (uint32_t)make_desc_sw128(q_s + w * (BQ * NDK * 128)), k_lo = (uint32_t)make_desc_sw128(k_s0), v_lo = (uint32_t)make_desc_v(v_s0);
-    auto issue_qk = [&](int j) -> bool {
-      const int s = j & 1, ks = j % KVS;
-      if (!mbar_wait(b_kfull + 8 * ks, (j / KVS) & 1, ERR_ATTN_WAIT)) return false;
-      if (j >= 2 && !mbar_wait(b_odone(w, s), ((j >> 1) - 1) & 1, ERR_ATTN_WAIT)) return false;      // the buffer holds P(j - 2) until its product has read it
+    bool ok = true, live = true;
+    int g0 = 0, j = 0, seg = 0;      // tiles of all segments before, this group's tiles so far
+    auto issue_qk = [&](int g, int jj) -> bool {
+      const int ks = g % KS;
+      if (!mbar_wait(b_kfull + 8 * ks, (g / KS) & 1, ERR_ATTN_WAIT)) return false;
+      if (jj >= 1 && !mbar_wait(b_sfree(w), (jj - 1) & 1, ERR_ATTN_WAIT)) return false;      // the scores before are in registers
       tc_fence_after();
-      const uint32_t kl = k_lo + ks * (F::T_BYTES >> 4), ts = t_s(w, s);
+      const uint32_t kl = k_lo + ks * (F::T_BYTES >> 4);
+      if (live) {
 #pragma unroll
-      for (int x = 0; x < 4 * NDK; ++x)
-        umma_f16_w(ts, ql + (((x >> 2) * (BQ * 128) + (x & 3) * 32) >> 4), hi_k, kl + (((x >> 2) * (BK * 128) + (x & 3) * 32) >> 4), hi_k, idesc_qk, x != 0);
-      tc_commit(b_sfull(w, s));
+        for (int x = 0; x < 4 * NDK; ++x) {
+          const uint32_t kx = kl + (((x >> 2) * (BK * 128) + (x & 3) * 32) >> 4);
+          if constexpr (NW == 1) umma_f16_ts_w(t_s(w), t_q + 8 * x, kx, hi_k, idesc_qk, x != 0);
+          else umma_f16_w(t_s(w), ql + (((x >> 2) * (BQ * 128) + (x & 3) * 32) >> 4), hi_k, kx, hi_k, idesc_qk, x != 0);
+        }
+      }
+      tc_commit(b_sfull(w));
       tc_commit(b_kempty + 8 * ks);
       return true;
     };
-    bool ok = true;
-    int g = 0, seg = 0;
     while (ok && next_segment<F>(p, s_cum, k)) {
+      live = NW == 1 || w * BQ < k.tok * p.gqa;      // (a second query tile without rows only hands tiles back)
+      const int i0 = NW == 1 ? (w - g0) & 1 : 0;
       if (lane == 0) {
-        ok = mbar_wait(b_q(w), seg & 1, ERR_ATTN_WAIT);
-        if (ok) ok = issue_qk(g);
+        ok = mbar_wait(b_q, seg & 1, ERR_ATTN_WAIT);
+        if (ok && i0 < k.count) ok = issue_qk(g0 + i0, j);
       }
-      for (int i = 0; i < k.count; ++i, ++g) {
-        const int s = g & 1, ks = g % KVS, t = k.ts + i;
-        const int valid = t == k.r.nt - 1 ? k.r.n : min(BK, k.r.length - (k.r.first + t) * BK);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      for (int i = i0; i < k.count && ok; i += kStep, ++j) {
+        const int g = g0 + i, vs = g % VS, valid = keys_of(k.ts + i);
         const bool tail = !F::I8 && (valid & 15) != 0;
+        bool ahead = false;      // the next scores' product is issued
         if (lane == 0) {
-          if (ok && i + 1 < k.count) ok = issue_qk(g + 1);
-          if (ok) ok = mbar_wait(b_pfull(w, s), (g >> 1) & 1, ERR_ATTN_WAIT);
-          if (ok) ok = mbar_wait(b_vfull + 8 * ks, (g / KVS) & 1, ERR_ATTN_WAIT);
+          // the next scores first, if their keys are here; else not before this tile's product, which their place may be waiting for
+          if (i + kStep < k.count && mbar_test(b_kfull + 8 * ((g + kStep) % KS), ((g + kStep) / KS) & 1)) {
+            ok = issue_qk(g + kStep, j + 1);
+            ahead = true;
+          }
+          if (ok) ok = mbar_wait(b_pfull(w), j & 1, ERR_ATTN_WAIT);
+          if (ok) ok = mbar_wait(b_vfull + 8 * vs, (g / VS) & 1, ERR_ATTN_WAIT);
         }
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         if (tail) {
           // values behind the last key's are anything: their weights are 0, but 0 x infinity is not
-          if (!mbar_wait(b_vfull + 8 * ks, (g / KVS) & 1, ERR_ATTN_WAIT)) ok = false;      // (over: every lane sees the copies)
+          mbar_wait(b_vfull + 8 * vs, (g / VS) & 1, ERR_ATTN_WAIT);      // (over: every lane sees the copies)
           const int end = (valid + 15) & ~15;
           for (int x = lane; x < (end - valid) * NDK * 8; x += 32) {
             const int row = valid + x / (NDK * 8), c = x % (NDK * 8);
-            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v_s0 + ks * F::T_BYTES + (c >> 3) * (BK * 128) + row * 128 + (c & 7) * 16), "r"(0) : "memory");
+            asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v_s0 + vs * F::T_BYTES + (c >> 3) * (BK * 128) + row * 128 + (c & 7) * 16), "r"(0) : "memory");
           }
           fence_proxy_async_smem();
           __syncwarp();
         }
         if (lane == 0) {
           tc_fence_after();
-          const uint32_t vl = v_lo + ks * (F::T_BYTES >> 4), tp = t_s(w, s);
+          const uint32_t vl = v_lo + vs * (F::T_BYTES >> 4);
+          if (live) {
 #pragma unroll
-          for (int x = 0; x < 4; ++x)      // 16 keys a step; P in tensor memory, 8 columns of pairs
-            umma_f16_ts_w(t_o(w), tp + 8 * x, vl + ((x * 16 * 128) >> 4), hi_v, idesc_pv, (i | x) != 0);
-          tc_commit(b_odone(w, s));
-          tc_commit(b_vempty + 8 * ks);
+            for (int x = 0; x < 4; ++x)      // 16 keys a step; P in tensor memory, 8 columns of pairs
+              umma_f16_ts_w(t_o(w), t_p(w) + 8 * x, vl + ((x * 16 * 128) >> 4), hi_v, idesc_pv, i != i0 || x != 0);
+          }
+          tc_commit(b_odone(w));
+          tc_commit(b_vempty + 8 * vs);
+          if (!ahead && i + kStep < k.count) ok = issue_qk(g + kStep, j + 1);
         }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
       }
+      g0 += k.count;
       ++seg;
     }
   } else if (warp < F::kConv) {
-    // ---------------------------------------------------------- softmax: a thread per query row of tile w
+    // ---------------------------------------------------------- softmax: two threads per query row of group w
     constexpr float kLazy = 6.f;
-    const int w = (warp - F::kSoft) >> 2, quarter = warp & 3, r = quarter * 32 + lane;
+    const int sw = warp - F::kSoft, w = sw >> 3, half = (sw >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+    const int pair = 1 + w * 4 + quarter;      // named barrier of the row's two warps
+    float* const x_mine = s_x + (w * 4 + half) * BQ + r;       // [parity 0]; parity 1 is 2 BQ further
+    float* const x_other = s_x + (w * 4 + (half ^ 1)) * BQ + r;
+    // once a wait has run out no other is made, but every barrier is still come to
     bool ok = true;
-    int g = 0;
-    while (ok && next_segment<F>(p, s_cum, k)) {
-      const int rr = w * BQ + r, live_rows = k.tok * p.gqa;
-      const bool row_ok = rr < live_rows, warp_ok = w * BQ + quarter * 32 < live_rows;
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ERR_ATTN_WAIT));
+    };
+    int g0 = 0, j = 0, seg = 0;
+    while (next_segment<F>(p, s_cum, k)) {
+      const int rr = (NW == 1 ? 0 : w * BQ) + r, live_rows = k.tok * p.gqa;
+      const bool row_ok = rr < live_rows, warp_ok = rr - lane < live_rows;
       const int node = blockIdx.y * p.group_tokens + rr / p.gqa, head = k.h * p.gqa + rr % p.gqa, row = k.r.r0 + node;
-      // ---- the row's query (the products of the segment before have read theirs: their scores were here)
-      if (row_ok) {
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + row * p.ldq + head * D);
-        uint4 x[8 * NDK];
+      // ---- the queries: the products of the segment before are done, all threads came by its end
+      {
+        constexpr int NV = NW == 1 ? D / 32 : D / 16;      // pieces of 8 dims that this thread brings: a quarter of its row, or half
+        const int c0 = NW == 1 ? (w * 2 + half) * NV : half * NV;
+        uint4 x[NV] = {};
+        if (row_ok) {
+          const uint4* src = reinterpret_cast<const uint4*>(p.q + row * p.ldq + head * D) + c0;
 #pragma unroll
-        for (int c = 0; c < 8 * NDK; ++c) x[c] = src[c];
+          for (int c = 0; c < NV; ++c) x[c] = src[c];
+        }
+        if constexpr (F::I8) {
 #pragma unroll
-        for (int c = 0; c < 8 * NDK; ++c)
-          *reinterpret_cast<uint4*>(gen + w * (BQ * NDK * 128) + (c >> 3) * (BQ * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x[c];
+          for (int c = 0; c < NV; ++c)
+            x[c] = make_uint4(__byte_perm(x[c].x, x[c].y, 0x5410), __byte_perm(x[c].x, x[c].y, 0x7632), __byte_perm(x[c].z, x[c].w, 0x5410), __byte_perm(x[c].z, x[c].w, 0x7632));
+        }
+        if constexpr (NW == 1) {
+          if constexpr (NV == 4) st_16(t_q + lane_addr + c0 * 4, reinterpret_cast<const uint32_t*>(x));
+          else st_8(t_q + lane_addr + c0 * 4, reinterpret_cast<const uint32_t*>(x));
+          tmem_st_wait();
+          tc_fence_before();
+        } else {
+#pragma unroll
+          for (int c = 0; c < NV; ++c)
+            *reinterpret_cast<uint4*>(gen + w * (BQ * NDK * 128) + ((c0 + c) >> 3) * (BQ * 128) + r * 128 + ((((c0 + c) & 7) ^ (r & 7)) << 4)) = x[c];
+          fence_proxy_async_smem();
+        }
+        mbar_arrive(b_q);
       }
-      fence_proxy_async_smem();
-      mbar_arrive(b_q(w));
-      const int pos = row_ok && p.window > 0 ? p.row_pos[row] : 0, lo = p.window > 0 ? pos - p.window + 1 : 0;      // the first position that is seen
+      wait(b_q, seg & 1);      // (all threads are done with the segment before)
+      ++seg;
+      const int lo = row_ok && p.window > 0 ? p.row_pos[row] - p.window + 1 : 0;      // the first position that is seen
       unsigned long long mask = 0;
       if (row_ok && k.ts + k.count == k.r.nt) {
         mask = p.masks[row];
         if (k.r.n < 64) mask &= (1ull << k.r.n) - 1;
         if (lo > k.r.length)
-          for (int j = 0; j < k.r.n; ++j)
-            if (p.row_pos[k.r.r0 + j] < lo) mask &= ~(1ull << j);
+          for (int i = 0; i < k.r.n; ++i)
+            if (p.row_pos[k.r.r0 + i] < lo) mask &= ~(1ull << i);
       }
       float mref = -INFINITY, l = 0.f;
-      for (int i = 0; i < k.count; ++i, ++g) {
-        const int s = g & 1, t = k.ts + i;
-        if (ok) ok = mbar_wait(b_sfull(w, s), (g >> 1) & 1, ERR_ATTN_WAIT);
-        if (!ok) break;
+      const int i0 = NW == 1 ? (w - g0) & 1 : 0;
+      for (int i = i0; i < k.count; i += kStep, ++j) {
+        const int g = g0 + i, t = k.ts + i;
+        wait(b_sfull(w), j & 1);
+        if (F::I8) wait(b_scale(g), (g >> 2) & 1);
         if (!warp_ok) {      // rows of nobody: the products take what is there
-          mbar_arrive(b_pfull(w, s));
+          mbar_arrive(b_sfree(w));
+          if (i != i0) wait(b_odone(w), (j - 1) & 1);
+          mbar_arrive(b_pfull(w));
           continue;
         }
-        if (F::I8) ok = mbar_wait(b_scale(g), (g >> 2) & 1, ERR_ATTN_WAIT);
         tc_fence_after();
-        unsigned long long vis = mask;
+        uint32_t v[32];
+        B2_TMEM_LD_32(t_s(w) + lane_addr + half * 32, v);
+        uint32_t vis = half ? (uint32_t)(mask >> 32) : (uint32_t)mask;
         if (t != k.r.nt - 1) {
-          const int key0 = (k.r.first + t) * BK, end = min(BK, k.r.length - key0), begin = max(0, lo - key0);
-          vis = end >= BK ? ~0ull : (1ull << end) - 1;
-          if (begin > 0) vis = begin >= BK ? 0ull : vis & (~0ull << begin);
+          const int key0 = (k.r.first + t) * BK + half * 32, end = min(32, k.r.length - key0), begin = max(0, lo - key0);
+          vis = end >= 32 ? 0xffffffffu : end > 0 ? (1u << end) - 1 : 0u;
+          if (begin > 0) vis = begin >= 32 ? 0u : vis & (0xffffffffu << begin);
         }
-        uint32_t v[2][32];
-        B2_TMEM_LD_32(t_s(w, s) + lane_addr, v[0]);
-        B2_TMEM_LD_32(t_s(w, s) + lane_addr + 32, v[1]);
+        const bool whole_tile = __all_sync(0xffffffffu, vis == 0xffffffffu);
         tmem_ld_wait();
-        const float* sc = s_scale + (g & 3) * (2 * BK);
+        tc_fence_before();
+        mbar_arrive(b_sfree(w));
+        const float* sc = s_scale + (g & 3) * (2 * BK) + half * 32;
         if constexpr (F::I8) {
 #pragma unroll
-          for (int j = 0; j < 64; j += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(sc + j);
-            const float ff[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[j >> 5][(j & 31) + e] = __float_as_uint(__uint_as_float(v[j >> 5][(j & 31) + e]) * ff[e]);
+          for (int c = 0; c < 32; c += 4) {
+            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + c);
+            unsigned long long a, b;
+            asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "r"(v[c]), "r"(v[c + 1]));
+            asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(v[c + 2]), "r"(v[c + 3]));
+            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(f.x));
+            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(b) : "l"(f.y));
+            asm("mov.b64 {%0, %1}, %2;" : "=r"(v[c]), "=r"(v[c + 1]) : "l"(a));
+            asm("mov.b64 {%0, %1}, %2;" : "=r"(v[c + 2]), "=r"(v[c + 3]) : "l"(b));
           }
         }
-        if (__any_sync(0xffffffffu, vis != ~0ull)) {
-          const uint32_t half[2] = {(uint32_t)vis, (uint32_t)(vis >> 32)};
+        if (!whole_tile) {
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (!(half[j >> 5] >> (j & 31) & 1)) v[j >> 5][j & 31] = 0xff800000u;
+          for (int c = 0; c < 32; ++c)
+            if (!(vis >> c & 1)) v[c] = 0xff800000u;
         }
-        float ma = -INFINITY, mb = -INFINITY;
+        float ma = __uint_as_float(v[0]), mb = __uint_as_float(v[1]);
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          asm("max.f32 %0, %0, %1, %2;" : "+f"(ma) : "f"(__uint_as_float(v[0][j])), "f"(__uint_as_float(v[0][j + 1])));
-          asm("max.f32 %0, %0, %1, %2;" : "+f"(mb) : "f"(__uint_as_float(v[1][j])), "f"(__uint_as_float(v[1][j + 1])));
+        for (int c = 2; c < 32; c += 4) {
+          asm("max.f32 %0, %0, %1, %2;" : "+f"(ma) : "f"(__uint_as_float(v[c])), "f"(__uint_as_float(v[c + 1])));
+          if (c + 3 < 32) asm("max.f32 %0, %0, %1, %2;" : "+f"(mb) : "f"(__uint_as_float(v[c + 2])), "f"(__uint_as_float(v[c + 3])));
         }
+        float tmax = fmaxf(ma, mb);
+        x_mine[(j & 1) * (2 * BQ)] = tmax;
+        pair_sync(pair);
+        tmax = fmaxf(tmax, x_other[(j & 1) * (2 * BQ)]);
         const float factor = F::I8 ? 1.f : p.scale_log2;
-        const float tmax = fmaxf(ma, mb) * factor;
+        tmax *= factor;
         float alpha = 1.f;
         if (tmax > mref + kLazy || (mref == -INFINITY && tmax > -INFINITY)) {
           alpha = exp2f(mref - tmax);      // 0 at the row's first key
           mref = tmax;
         }
         const float nm = mref == -INFINITY ? 0.f : -mref;
-        if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-          ok = mbar_wait(b_odone(w, s ^ 1), ((g - 1) >> 1) & 1, ERR_ATTN_WAIT);
-          tc_fence_after();
-#pragma unroll 1
-          for (int c = 0; c < 2 * NDK; ++c) {
-            uint32_t o[32];
-            B2_TMEM_LD_32(t_o(w) + lane_addr + c * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            B2_TMEM_ST_32(t_o(w) + lane_addr + c * 32, o);
-          }
-          tmem_st_wait();
-        }
         unsigned long long sc2, nm2, acc0 = 0ull, acc1 = 0ull;
         asm("mov.b64 %0, {%1, %1};" : "=l"(sc2) : "f"(factor));
         asm("mov.b64 %0, {%1, %1};" : "=l"(nm2) : "f"(nm));
-        uint32_t pk[32];
+        uint32_t pk[16];
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
+        for (int c = 0; c < 16; ++c) {
           unsigned long long xy;
-          asm("mov.b64 %0, {%1, %2};" : "=l"(xy) : "r"(v[j >> 4][(2 * j) & 31]), "r"(v[j >> 4][(2 * j + 1) & 31]));
+          asm("mov.b64 %0, {%1, %2};" : "=l"(xy) : "r"(v[2 * c]), "r"(v[2 * c + 1]));
           if (F::I8) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(xy) : "l"(nm2));
           else asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(xy) : "l"(sc2), "l"(nm2));
           float x0, x1, e0, e1;
@@ -466,55 +541,113 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(x1));
           unsigned long long ee;
           asm("mov.b64 %0, {%1, %2};" : "=l"(ee) : "f"(e0), "f"(e1));
-          if (j & 1) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc1) : "l"(ee));
+          if (c & 1) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc1) : "l"(ee));
           else asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc0) : "l"(ee));
           if constexpr (F::I8) {
-            const float2 f = *reinterpret_cast<const float2*>(sc + BK + 2 * j);
-            // (a weight of nothing stays nothing, whatever the scale behind the last key is)
-            pk[j] = pack_bf16(e0 > 0.f ? e0 * f.x : 0.f, e1 > 0.f ? e1 * f.y : 0.f);
-          } else {
-            pk[j] = pack_bf16(e0, e1);
+            const unsigned long long f = *reinterpret_cast<const unsigned long long*>(sc + BK + 2 * c);
+            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(ee) : "l"(f));
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(ee));
           }
+          pk[c] = pack_bf16(e0, e1);
         }
-        st_32(t_s(w, s) + lane_addr, pk);
-        tmem_st_wait();
         float a0, a1, a2, a3;
         asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(acc0));
         asm("mov.b64 {%0, %1}, %2;" : "=f"(a2), "=f"(a3) : "l"(acc1));
-        l = l * alpha + (a0 + a1) + (a2 + a3);
-        tc_fence_before();
-        mbar_arrive(b_pfull(w, s));
-      }
-      if (!ok) break;
-      // ---- the segment's sums, once its last product is done
-      ok = mbar_wait(b_odone(w, (g - 1) & 1), ((g - 1) >> 1) & 1, ERR_ATTN_WAIT);
-      if (!ok) break;
-      tc_fence_after();
-      if (warp_ok) {
-        const bool whole = k.count == k.r.nt;
-        const float inv = l > 0.f ? 1.f / l : 0.f;
-        const size_t slot = (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (k.u - k.count != k.u0)) * (NW * BQ) + rr;
-        __nv_bfloat16* dst = p.out + row * p.ldo + head * D;
+        l = l * alpha + ((a0 + a1) + (a2 + a3));
+        if (i != i0) {      // the product before has read its weights, and the accumulator is whole
+          wait(b_odone(w), (j - 1) & 1);
+          tc_fence_after();
+          if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll 1
-        for (int c = 0; c < 2 * NDK; ++c) {
-          uint32_t o[32];
-          B2_TMEM_LD_32(t_o(w) + lane_addr + c * 32, o);
-          tmem_ld_wait();
-          if (!row_ok) continue;
-          if (whole) {
+            for (int c = 0; c < 2 * NDK; ++c) {      // this thread's half of the row
+              uint32_t o[16];
+              ld_16(t_o(w) + lane_addr + half * (D / 2) + c * 16, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-              *reinterpret_cast<uint4*>(dst + c * 32 + 8 * j) = make_uint4(
-                  pack_bf16(__uint_as_float(o[8 * j]) * inv, __uint_as_float(o[8 * j + 1]) * inv), pack_bf16(__uint_as_float(o[8 * j + 2]) * inv, __uint_as_float(o[8 * j + 3]) * inv),
-                  pack_bf16(__uint_as_float(o[8 * j + 4]) * inv, __uint_as_float(o[8 * j + 5]) * inv), pack_bf16(__uint_as_float(o[8 * j + 6]) * inv, __uint_as_float(o[8 * j + 7]) * inv));
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) *reinterpret_cast<uint4*>(p.part_o + slot * D + c * 32 + 4 * j) = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              st_16(t_o(w) + lane_addr + half * (D / 2) + c * 16, o);
+            }
           }
         }
-        if (!whole && row_ok) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(mref, l);
+        st_16(t_p(w) + lane_addr + half * 16, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(b_pfull(w));
+      }
+      // ---- the segment's sums, once its last product is done
+      if (i0 < k.count) wait(b_odone(w), (j - 1) & 1);
+      // sums of the halves meet in the slots of the parity that the group's last tile did not use; maxima (one group's, for the other) in
+      // those that it used, behind the barrier that all threads come to
+      x_mine[(j & 1) * (2 * BQ)] = l;
+      pair_sync(pair);
+      l += x_other[(j & 1) * (2 * BQ)];
+      tc_fence_before();
+      if (NW == 1) {
+        if (half == 0) x_mine[((j & 1) ^ 1) * (2 * BQ)] = mref;      // read by the other group, at this group's parity
+        else x_mine[((j & 1) ^ 1) * (2 * BQ)] = l;
+      }
+      asm volatile("bar.sync 9, 512;" ::: "memory");
+      tc_fence_after();
+      const bool whole = k.count == k.r.nt;
+      const size_t slot = (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (k.u - k.count != k.u0)) * (NW * BQ) + rr;
+      if (warp_ok) {
+        float f[2] = {1.f, 0.f}, best = mref, sum = l;
+        if constexpr (NW == 1) {
+          // tiles of the other group so far: its parity
+          const int other_j = (w == 0) ? (g0 + k.count) / 2 : (g0 + k.count + 1) / 2;
+          const float* xo = s_x + (w ^ 1) * 4 * BQ + ((other_j & 1) ^ 1) * (2 * BQ) + r;
+          const float mo = xo[0], lo2 = xo[BQ];
+          best = fmaxf(mref, mo);
+          const float fm = mref == -INFINITY ? 0.f : exp2f(mref - best), fo = mo == -INFINITY ? 0.f : exp2f(mo - best);
+          sum = l * fm + lo2 * fo;
+          f[w] = fm;
+          f[w ^ 1] = fo;
+        }
+        const float inv = whole ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
+        constexpr int NC = NW == 1 ? NDK : 2 * NDK;      // pieces of 16 columns that this thread writes: a quarter of the row, or half
+        const int c0 = NW == 1 ? (w * 2 + half) * NC * 16 : half * NC * 16;
+        __nv_bfloat16* dst = p.out + row * p.ldo + head * D + c0;
+        float* part = p.part_o + slot * D + c0;
+#pragma unroll 1
+        for (int c = 0; c < NC; ++c) {
+          uint32_t o[16], o1[16];
+          if constexpr (NW == 1) {
+            ld_16(t_o(0) + lane_addr + c0 + c * 16, o);
+            ld_16(t_o(1) + lane_addr + c0 + c * 16, o1);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              o[e] = __float_as_uint(((f[0] > 0.f ? f[0] * __uint_as_float(o[e]) : 0.f) + (f[1] > 0.f ? f[1] * __uint_as_float(o1[e]) : 0.f)) * inv);
+          } else {
+            ld_16(t_o(w) + lane_addr + c0 + c * 16, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
+          }
+          if (!row_ok) continue;
+          if constexpr (F::I8) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+              const uint32_t t2 = o[e + 1];
+              o[e + 1] = o[e + 2];
+              o[e + 2] = t2;
+            }
+          }
+          if (whole) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<uint4*>(dst + c * 16 + 8 * e) = make_uint4(
+                  pack_bf16(__uint_as_float(o[8 * e]), __uint_as_float(o[8 * e + 1])), pack_bf16(__uint_as_float(o[8 * e + 2]), __uint_as_float(o[8 * e + 3])),
+                  pack_bf16(__uint_as_float(o[8 * e + 4]), __uint_as_float(o[8 * e + 5])), pack_bf16(__uint_as_float(o[8 * e + 6]), __uint_as_float(o[8 * e + 7])));
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(part + c * 16 + 4 * e) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
+        }
+        if (!whole && row_ok && half == 0 && (NW == 2 || w == 0)) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(best, sum);
       }
       tc_fence_before();
+      g0 += k.count;
     }
   } else if constexpr (F::I8) {
     // ---------------------------------------------------------- bytes to integers in bf16: a thread's piece is 16 bytes of a key
@@ -523,15 +656,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     int g = 0;
     auto expand = [&](uint32_t src, uint32_t dst) {
 #pragma unroll
-      for (int x = ct; x < BK * D / 16; x += 128) {
-        const int row = x / (D / 16), c = x % (D / 16);
+      for (int u = 0; u < BK * D / 16 / F::kConvThreads; ++u) {
+        const int x = ct + F::kConvThreads * u, row = x / (D / 16), c = x % (D / 16);
         uint32_t ww[4], o[8];
         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ww[0]), "=r"(ww[1]), "=r"(ww[2]), "=r"(ww[3]) : "r"(src + x * 16));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t ev = bytes_bf16(ww[j]), od = bytes_bf16(ww[j] >> 8);
-          o[2 * j] = __byte_perm(ev, od, 0x5410);
-          o[2 * j + 1] = __byte_perm(ev, od, 0x7632);
+        for (int y = 0; y < 4; ++y) {
+          o[2 * y] = bytes_bf16(ww[y]);
+          o[2 * y + 1] = bytes_bf16(ww[y] >> 8);
         }
         // (the second 64 dims' pieces go the other way round, so that eight threads' stores meet eight banks of 16 bytes)
         const uint32_t to = dst + (c >> 2) * (BK * 128) + row * 128;
@@ -548,22 +680,24 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     };
     while (ok && next_segment<F>(p, s_cum, k))
       for (int i = 0; i < k.count; ++i, ++g) {
-        const int rs = g % RS, ks = g % KVS, ph = ((g / KVS) & 1) ^ 1;
+        const int rs = g % RS, ks = g % KS, vs = g % VS;
         const uint32_t st = st_s0 + rs * F::S_BYTES;
         ok = mbar_wait(b_rfull + 8 * rs, (g / RS) & 1, ERR_ATTN_WAIT);
-        if (ok && g >= KVS) ok = mbar_wait(b_kempty + 8 * ks, ph, ERR_ATTN_WAIT);
+        if (ok && g >= KS) ok = mbar_wait(b_kempty + 8 * ks, ((g / KS) & 1) ^ 1, ERR_ATTN_WAIT);
         if (!ok) break;
-        // the scales of tile g - 4 are read: the place of its keys came free with the scores of tile g - KVS, which waited for the product of
-        // tile g - KVS - 2 at least
-        const float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + ct * 4);
-        s_scale[(g & 3) * (2 * BK) + ct] = ct < BK ? f * p.scale_log2 : f;
-        mbar_arrive(b_scale(g));
+        // the scales of tile g - 4 are read: the places of the values of tiles g - 2 and g - 1 came free with the products of tiles g - 2 - VS and
+        // g - 1 - VS, the same group's or a later one's.  Behind the last key they are anything, and made 0: what a place holds that nobody sees must not reach a sum.
+        if (ct < 2 * BK) {
+          const float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + ct * 4);
+          s_scale[(g & 3) * (2 * BK) + ct] = (ct & (BK - 1)) >= keys_of(k.ts + i) ? 0.f : ct < BK ? f * p.scale_log2 : f;
+          mbar_arrive(b_scale(g));
+        }
         expand(st, k_s0 + ks * F::T_BYTES);
         mbar_arrive(b_kfull + 8 * ks);
-        if (g >= KVS) ok = mbar_wait(b_vempty + 8 * ks, ph, ERR_ATTN_WAIT);
+        if (g >= VS) ok = mbar_wait(b_vempty + 8 * vs, ((g / VS) & 1) ^ 1, ERR_ATTN_WAIT);
         if (!ok) break;
-        expand(st + BK * D, v_s0 + ks * F::T_BYTES);
-        mbar_arrive(b_vfull + 8 * ks);
+        expand(st + BK * D, v_s0 + vs * F::T_BYTES);
+        mbar_arrive(b_vfull + 8 * vs);
         mbar_arrive(b_rempty + 8 * rs);
       }
   }
@@ -571,7 +705,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   __syncthreads();
   if (warp == F::kMma) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, F::TMEM);
+    tmem_dealloc(tmem_base, 512);
   }
 }
 
@@ -673,7 +807,7 @@ Shape shape_of(int B, int max_blocks, int n_kv, int gqa, int max_nodes) {
   s.groups = (max_nodes + most - 1) / most;
   s.tokens = (max_nodes + s.groups - 1) / s.groups;
   const long long units = (long long)B * n_kv * (max_blocks / 4 + 2);      // tiles there can be
-  const long long c = (long long)sm_count() * (s.nw == 1 ? 2 : 1) / s.groups;
+  const long long c = (long long)sm_count() / s.groups;
   s.columns = (int)(c < 1 ? 1 : c < units ? c : units);
   return s;
 }
