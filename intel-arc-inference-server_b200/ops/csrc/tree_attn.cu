@@ -24,13 +24,13 @@
 // An 8-bit cache comes in as bytes (bulk copies, scales with them), eight warps make integers in bf16 of them, which are exact; K's scale goes on
 // the scores and V's on the weights, both in fp32.  Of four dimensions the second and the third change places on the way (pairs come apart that
 // way), which the queries follow and the results undo.
-#include "common.cuh"
+#include "tree.cuh"
 
 using namespace b2;
 
 namespace {
 
-constexpr int kPage = 16, kMaxNodes = 64, kMaxReq = 1024;
+constexpr int kPage = kTreePage, kMaxNodes = kTreeNodes, kMaxReq = kTreeRequests;
 constexpr int BQ = 128, BK = 64;
 
 struct TreeAttnParams {
@@ -830,36 +830,40 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const TreeAttnParams& p
 
 }  // namespace
 
-// fp32 words of workspace for b2_tree_attention
-extern "C" long long b2_tree_attention_work(int B, int max_blocks, int n_q, int n_kv, int D, int max_nodes) {
-  const Shape s = shape_of(B, max_blocks, n_kv, n_q / n_kv, max_nodes);
-  return 2ll * s.groups * s.columns * s.nw * BQ * (D + 2) + (B + 2 + 3) / 4 * 4;
+// Tensor maps of a bf16 cache's first layer into the structure.
+extern "C" int b2_tree_cache(B2TreeCache* c) {
+  if (c->k_scale || (c->d != 64 && c->d != 128)) return c->k_scale ? 0 : -1;
+  const uint64_t rows = (uint64_t)c->pages * c->heads * kPage;
+  const int rc = cache_map(&c->map_k, c->k, rows, c->d);
+  return rc ? rc : cache_map(&c->map_v, c->v, rows, c->d);
 }
 
-extern "C" int b2_tree_attention(const void* q, long long ldq, const void* k, const void* v, const float* k_scale, const float* v_scale, const int* lengths,
-                                 const int* row_start, const int* row_req, const int* row_pos, const int* block_table, const int* tree_table,
-                                 const void* masks, void* out, float* work, long long ldo, int rows, int B, int max_blocks, int tree_blocks, int num_pages,
-                                 int n_q, int n_kv, int D, int max_nodes, int window, float scale, void* stream) {
-  if (rows < 1 || B < 1 || B > kMaxReq || n_q < 1 || n_kv < 1 || n_q % n_kv || n_q / n_kv > 64 || (D != 64 && D != 128) || max_nodes < 1 || max_nodes > kMaxNodes || num_pages < 1)
+// fp32 words of workspace for b2_tree_attention on the current device
+extern "C" long long b2_tree_attention_work(const B2TreeStep* t, int n_q, int n_kv, int D) {
+  const Shape s = shape_of(t->requests, t->max_blocks, n_kv, n_q / n_kv, t->max_nodes);
+  return 2ll * s.groups * s.columns * s.nw * BQ * (D + 2) + (t->requests + 2 + 3) / 4 * 4;
+}
+
+extern "C" int b2_tree_attention(const B2TreeStep* step, const B2TreeCache* cache, const void* q, long long ldq, void* out, long long ldo, float* work, int rows,
+                                 int n_q, int window, float scale, void* stream) {
+  const B2TreeStep& t = *step;
+  const B2TreeCache& c = *cache;
+  if (rows < 1 || t.requests < 1 || t.requests > kMaxReq || n_q < 1 || c.heads < 1 || n_q % c.heads || n_q / c.heads > 64 || (c.d != 64 && c.d != 128) || t.max_nodes < 1 ||
+      t.max_nodes > kMaxNodes || c.pages < 1)
     return -1;
-  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)work | (uintptr_t)k_scale | (uintptr_t)v_scale) % 16 || ldq % 8 || ldo % 8) return -2;
-  const Shape s = shape_of(B, max_blocks, n_kv, n_q / n_kv, max_nodes);
+  if (((uintptr_t)q | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)out | (uintptr_t)work | (uintptr_t)c.k_scale | (uintptr_t)c.v_scale) % 16 || ldq % 8 || ldo % 8) return -2;
+  const Shape s = shape_of(t.requests, t.max_blocks, c.heads, n_q / c.heads, t.max_nodes);
   TreeAttnParams p;
-  p.q = (const __nv_bfloat16*)q; p.ldq = ldq; p.k8 = (const int8_t*)k; p.v8 = (const int8_t*)v; p.k_scale = k_scale; p.v_scale = v_scale;
-  p.lengths = lengths; p.row_start = row_start; p.row_req = row_req; p.row_pos = row_pos; p.block_table = block_table; p.tree_table = tree_table;
-  p.masks = (const unsigned long long*)masks; p.B = B; p.max_blocks = max_blocks; p.tree_blocks = tree_blocks; p.num_pages = num_pages; p.rows = rows;
-  p.n_q = n_q; p.n_kv = n_kv; p.gqa = n_q / n_kv; p.window = window; p.group_tokens = s.tokens; p.scale_log2 = scale * 1.4426950408889634f;
+  p.q = (const __nv_bfloat16*)q; p.ldq = ldq; p.k8 = (const int8_t*)c.k; p.v8 = (const int8_t*)c.v; p.k_scale = c.k_scale; p.v_scale = c.v_scale;
+  p.lengths = t.lengths; p.row_start = t.row_start; p.row_req = t.row_req; p.row_pos = t.row_pos; p.block_table = t.block_table; p.tree_table = t.tree_table;
+  p.masks = t.masks; p.B = t.requests; p.max_blocks = t.max_blocks; p.tree_blocks = t.tree_blocks; p.num_pages = c.pages; p.rows = rows;
+  p.n_q = n_q; p.n_kv = c.heads; p.gqa = n_q / c.heads; p.window = window; p.group_tokens = s.tokens; p.scale_log2 = scale * 1.4426950408889634f;
   p.out = (__nv_bfloat16*)out; p.ldo = ldo;
   const size_t slots = 2ull * s.groups * s.columns * s.nw * BQ;
-  p.part_o = work; p.part_ml = work + slots * D; p.sched = reinterpret_cast<int*>(work + slots * (D + 2));
-  CUtensorMap mk = {}, mv = {};
-  if (!k_scale) {
-    int rc = cache_map(&mk, k, (uint64_t)num_pages * n_kv * kPage, D);
-    if (!rc) rc = cache_map(&mv, v, (uint64_t)num_pages * n_kv * kPage, D);
-    if (rc) return rc;
-  }
+  p.part_o = work; p.part_ml = work + slots * c.d; p.sched = reinterpret_cast<int*>(work + slots * (c.d + 2));
+  const CUtensorMap &mk = c.map_k, &mv = c.map_v;
   const cudaStream_t st = (cudaStream_t)stream;
-  switch ((D == 128 ? 4 : 0) + (k_scale ? 2 : 0) + s.nw - 1) {
+  switch ((c.d == 128 ? 4 : 0) + (c.k_scale ? 2 : 0) + s.nw - 1) {
     case 0: return launch<Form<1, false, 1>>(mk, mv, p, s, st);
     case 1: return launch<Form<1, false, 2>>(mk, mv, p, s, st);
     case 2: return launch<Form<1, true, 1>>(mk, mv, p, s, st);

@@ -6,13 +6,13 @@
 //           path's keys and values move from the tree's pages to the request's positions, in all layers
 //
 // Plan is one CTA of 1024 threads: everything hangs on three prefix sums over the requests, and a launch is all that a call costs.
-#include "common.cuh"
+#include "tree.cuh"
 
 using namespace b2;
 
 namespace {
 
-constexpr int kPage = 16, kMaxNodes = 64, kMaxReq = 1024;
+constexpr int kPage = kTreePage, kMaxNodes = kTreeNodes, kMaxReq = kTreeRequests;
 
 enum : int { PLAN_POOL = 1, PLAN_TABLE = 2, PLAN_ROWS = 4, PLAN_COUNT = 8, PLAN_PARENT = 16, PLAN_LENGTH = 32, PLAN_PAGE = 64 };
 
@@ -270,31 +270,33 @@ __global__ void __launch_bounds__(256) tree_commit_kernel(const TreeCommitParams
 
 }  // namespace
 
-extern "C" int b2_tree_plan(const int* lengths, const int* counts, const int* parents, int* block_table, const int* tree_table, int* free,
-                            const int* n_free, const int* held, int* n_free_out, int* held_out, int* out_lengths, int* row_start, int* row_req,
-                            int* row_pos, int* slots, int* out_parents, void* masks, int* status, int B, int max_blocks, int tree_blocks, int free_cap,
-                            int max_rows, int max_nodes, int num_pages, int rows, void* stream) {
-  if (B < 1 || B > kMaxReq || rows < 0 || rows > max_rows || max_nodes < 1 || max_nodes > kMaxNodes || max_nodes > tree_blocks * kPage) return -1;
+// parents: of `rows` rows, or null (rows: the step's room)
+extern "C" int b2_tree_plan(const B2TreeStep* step, const B2TreePool* pool, const B2TreePool* after, const int* lengths, const int* counts, const int* parents,
+                            int rows, void* stream) {
+  const B2TreeStep& t = *step;
+  if (t.requests < 1 || t.requests > kMaxReq || rows < 0 || rows > t.max_rows || t.max_nodes < 1 || t.max_nodes > kMaxNodes || t.max_nodes > t.tree_blocks * kPage) return -1;
   TreePlanParams p;
-  p.lengths = lengths; p.counts = counts; p.parents = parents; p.block_table = block_table; p.tree_table = tree_table; p.free = free;
-  p.n_free = n_free; p.held = held; p.n_free_out = n_free_out; p.held_out = held_out; p.out_lengths = out_lengths; p.row_start = row_start;
-  p.row_req = row_req; p.row_pos = row_pos; p.slots = slots; p.out_parents = out_parents; p.masks = (unsigned long long*)masks; p.status = status;
-  p.B = B; p.max_blocks = max_blocks; p.tree_blocks = tree_blocks; p.free_cap = free_cap; p.max_rows = max_rows; p.max_nodes = max_nodes;
-  p.num_pages = num_pages; p.rows = rows;
+  p.lengths = lengths; p.counts = counts; p.parents = parents; p.block_table = t.block_table; p.tree_table = t.tree_table; p.free = pool->free;
+  p.n_free = pool->n_free; p.held = pool->held; p.n_free_out = after->n_free; p.held_out = after->held; p.out_lengths = t.lengths; p.row_start = t.row_start;
+  p.row_req = t.row_req; p.row_pos = t.row_pos; p.slots = t.slots; p.out_parents = t.parents; p.masks = t.masks; p.status = t.status;
+  p.B = t.requests; p.max_blocks = t.max_blocks; p.tree_blocks = t.tree_blocks; p.free_cap = pool->capacity; p.max_rows = t.max_rows; p.max_nodes = t.max_nodes;
+  p.num_pages = t.num_pages; p.rows = rows;
   return b2_launch(tree_plan_kernel, dim3(1), dim3(1024), 0, (cudaStream_t)stream, true, p);
 }
 
-extern "C" int b2_tree_commit(const int* lengths, const int* row_start, const int* parents, const int* tokens, const int* targets,
-                              const int* block_table, const int* tree_table, void* k, void* v, long long plane_bytes, float* k_scale,
-                              float* v_scale, long long plane_scales, int* path, int* count, int* next_token, int* out_lengths, int B, int max_blocks,
-                              int tree_blocks, int planes, int num_pages, int n_kv, int row_bytes, int rows, void* stream) {
-  if (B < 1 || B > kMaxReq || planes < 1 || row_bytes % 16 || ((uintptr_t)k | (uintptr_t)v | (uintptr_t)plane_bytes) % 16) return -1;
+extern "C" int b2_tree_commit(const B2TreeStep* step, const B2TreeCache* cache, const B2TreeAccepted* accepted, const int* tokens, const int* targets, int rows,
+                              void* stream) {
+  const B2TreeStep& t = *step;
+  const B2TreeCache& c = *cache;
+  const int row_bytes = c.d * (c.k_scale ? 1 : 2);
+  if (t.requests < 1 || t.requests > kMaxReq || c.layers < 1 || row_bytes % 16 || ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.layer_bytes) % 16) return -1;
   TreeCommitParams p;
-  p.lengths = lengths; p.row_start = row_start; p.parents = parents; p.tokens = tokens; p.targets = targets; p.block_table = block_table;
-  p.tree_table = tree_table; p.B = B; p.max_blocks = max_blocks; p.tree_blocks = tree_blocks; p.planes = planes; p.num_pages = num_pages;
-  p.n_kv = n_kv; p.rows = rows; p.k = (uint8_t*)k; p.v = (uint8_t*)v; p.plane_bytes = plane_bytes; p.k_scale = k_scale; p.v_scale = v_scale;
-  p.plane_scales = plane_scales; p.row_bytes = row_bytes; p.path = path; p.count = count; p.next_token = next_token; p.out_lengths = out_lengths;
-  return b2_launch(tree_commit_kernel, dim3(B, min(planes, 65535)), dim3(256), 0, (cudaStream_t)stream, true, p);
+  p.lengths = t.lengths; p.row_start = t.row_start; p.parents = t.parents; p.tokens = tokens; p.targets = targets; p.block_table = t.block_table;
+  p.tree_table = t.tree_table; p.B = t.requests; p.max_blocks = t.max_blocks; p.tree_blocks = t.tree_blocks; p.planes = c.layers; p.num_pages = c.pages;
+  p.n_kv = c.heads; p.rows = rows; p.k = (uint8_t*)c.k; p.v = (uint8_t*)c.v; p.plane_bytes = c.layer_bytes; p.k_scale = c.k_scale; p.v_scale = c.v_scale;
+  p.plane_scales = c.layer_scales; p.row_bytes = row_bytes; p.path = accepted->path; p.count = accepted->count; p.next_token = accepted->next_token;
+  p.out_lengths = accepted->lengths;
+  return b2_launch(tree_commit_kernel, dim3(t.requests, min(c.layers, 65535)), dim3(256), 0, (cudaStream_t)stream, true, p);
 }
 
 B2_DEFINE_STATUS(tree)

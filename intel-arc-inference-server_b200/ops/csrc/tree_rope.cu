@@ -6,13 +6,16 @@
 //
 // Rows without a slot (-1) are left as they are.  Products and sums are rounded one by one, as the definition says them: an 8-bit value
 // next to a border then is the same number whoever computes it.
-#include "common.cuh"
+//
+// The bytes are the bound.  A thread takes four pairs of a head -- eight dimensions, in two pieces of four -- of HC heads of a row: a pair needs no
+// other thread, and cosines and sines are read once for the row's heads.  All of a thread's loads are in flight together.
+#include "tree.cuh"
 
 using namespace b2;
 
 namespace {
 
-constexpr int kPage = 16;
+constexpr int kPage = kTreePage;
 
 struct TreeRopeParams {
   const void* qkv;          // bf16 [rows][ld], or fp32 [slices][rows][ld], slices added in order
@@ -20,116 +23,145 @@ struct TreeRopeParams {
   int slices;               // 0: bf16
   const int *pos, *slots;
   int rows;
-  const float *cos_t, *sin_t;      // [positions][rot / 2]
-  int rot, positions, interleaved;
-  int n_q, n_kv, D;
+  const float *cos_t, *sin_t;      // [positions][pairs]
+  int pairs, positions, interleaved;
+  int n_q, n_kv;
   __nv_bfloat16* q;
   long long ldq;
   void *k, *v;
   float *k_scale, *v_scale;        // null: bf16 cache
   long long num_slots;
+  int chunks;                      // groups of HC heads in a row
 };
 
-// D / 4 lanes take a row's head, four dimensions each.
-template <int D>
+template <int D, int HC, bool F32>
 __global__ void __launch_bounds__(256) tree_rope_kernel(const TreeRopeParams p) {
-  constexpr int G = D / 4;
+  constexpr int G = D / 8;             // threads to a head
   pdl_wait();
   pdl_launch_dependents();
-  const int heads = p.n_q + 2 * p.n_kv;
+  const int heads = p.n_q + 2 * p.n_kv, n_turn = p.n_q + p.n_kv;
   const int l = threadIdx.x % G, item = blockIdx.x * (256 / G) + threadIdx.x / G;
-  const int row = min(item / heads, p.rows - 1), head = item - (item / heads) * heads;      // (groups past the end go along for the shuffles)
+  const int row = min(item / p.chunks, p.rows - 1), h0 = (item - (item / p.chunks) * p.chunks) * HC;      // (groups past the end go along for the shuffles)
   const int pos = p.pos[row], slot = p.slots[row];
-  bool live = item < p.rows * heads && slot >= 0;
+  bool live = item < p.rows * p.chunks && slot >= 0;
   if (live && (pos < 0 || pos >= p.positions || slot >= p.num_slots)) {
     if (l == 0) record_error(ERR_BAD_ARG, row);
     live = false;
   }
-  const int e = head * D + 4 * l;
-  float x[4] = {0.f, 0.f, 0.f, 0.f};
-  if (live) {
-    if (p.slices) {
-      const float* src = reinterpret_cast<const float*>(p.qkv) + row * p.ld + e;
-      float4 a = *reinterpret_cast<const float4*>(src);
-#pragma unroll 4
-      for (int s = 1; s < p.slices; ++s) {
-        const float4 t = *reinterpret_cast<const float4*>(src + s * p.slice);
-        a.x += t.x; a.y += t.y; a.z += t.z; a.w += t.w;
-      }
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+  // ---- the thread's dimensions: two pieces of four, off_a and off_b
+  const bool turn = 4 * l < p.pairs;
+  const int off_a = turn && !p.interleaved ? 4 * l : 8 * l, off_b = turn && !p.interleaved ? p.pairs + 4 * l : 8 * l + 4;
+  float x[HC][8];
+#pragma unroll
+  for (int c = 0; c < HC; ++c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[c][e] = 0.f;
+    if (!live || h0 + c >= heads) continue;
+    if constexpr (F32) {
+      const float* src = reinterpret_cast<const float*>(p.qkv) + row * p.ld + (h0 + c) * D;
+      const float4 a = *reinterpret_cast<const float4*>(src + off_a), b = *reinterpret_cast<const float4*>(src + off_b);
+      x[c][0] = a.x; x[c][1] = a.y; x[c][2] = a.z; x[c][3] = a.w; x[c][4] = b.x; x[c][5] = b.y; x[c][6] = b.z; x[c][7] = b.w;
     } else {
-      const uint2 t = *reinterpret_cast<const uint2*>(reinterpret_cast<const __nv_bfloat16*>(p.qkv) + row * p.ld + e);
-      x[0] = bf16_lo(t.x); x[1] = bf16_hi(t.x); x[2] = bf16_lo(t.y); x[3] = bf16_hi(t.y);
+      const __nv_bfloat16* src = reinterpret_cast<const __nv_bfloat16*>(p.qkv) + row * p.ld + (h0 + c) * D;
+      const uint2 a = *reinterpret_cast<const uint2*>(src + off_a), b = *reinterpret_cast<const uint2*>(src + off_b);
+      x[c][0] = bf16_lo(a.x); x[c][1] = bf16_hi(a.x); x[c][2] = bf16_lo(a.y); x[c][3] = bf16_hi(a.y);
+      x[c][4] = bf16_lo(b.x); x[c][5] = bf16_hi(b.x); x[c][6] = bf16_lo(b.y); x[c][7] = bf16_hi(b.y);
     }
   }
-  if (head < p.n_q + p.n_kv || !live) {      // (lanes of one head go the same way; dead ones come along)
-    const int half = p.rot >> 1;
-    if (p.interleaved) {
-      if (live && 4 * l < p.rot) {
-        const float2 c = *reinterpret_cast<const float2*>(p.cos_t + (size_t)pos * half + 2 * l), s = *reinterpret_cast<const float2*>(p.sin_t + (size_t)pos * half + 2 * l);
-        const float a0 = x[0], b0 = x[1], a1 = x[2], b1 = x[3];
-        x[0] = __fsub_rn(__fmul_rn(a0, c.x), __fmul_rn(b0, s.x));
-        x[1] = __fadd_rn(__fmul_rn(b0, c.x), __fmul_rn(a0, s.x));
-        x[2] = __fsub_rn(__fmul_rn(a1, c.y), __fmul_rn(b1, s.y));
-        x[3] = __fadd_rn(__fmul_rn(b1, c.y), __fmul_rn(a1, s.y));
+  float4 cs = make_float4(1.f, 1.f, 1.f, 1.f), sn = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (live && turn && h0 < n_turn) {
+    cs = __ldg(reinterpret_cast<const float4*>(p.cos_t + (size_t)pos * p.pairs) + l);
+    sn = __ldg(reinterpret_cast<const float4*>(p.sin_t + (size_t)pos * p.pairs) + l);
+  }
+  if constexpr (F32) {
+#pragma unroll 1
+    for (int s = 1; s < p.slices; ++s) {
+#pragma unroll
+      for (int c = 0; c < HC; ++c) {
+        if (!live || h0 + c >= heads) continue;
+        const float* src = reinterpret_cast<const float*>(p.qkv) + s * p.slice + row * p.ld + (h0 + c) * D;
+        const float4 a = *reinterpret_cast<const float4*>(src + off_a), b = *reinterpret_cast<const float4*>(src + off_b);
+        x[c][0] += a.x; x[c][1] += a.y; x[c][2] += a.z; x[c][3] += a.w; x[c][4] += b.x; x[c][5] += b.y; x[c][6] += b.z; x[c][7] += b.w;
       }
     }
   }
-  {
-    const int half = p.rot >> 1, hl = half >> 2;       // lanes of half the rotated part
-    const bool low = l < hl;
-    const int other = low ? l + hl : l - hl;
-    float y[4];
+  const float cc[4] = {cs.x, cs.y, cs.z, cs.w}, ss[4] = {sn.x, sn.y, sn.z, sn.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], other & (G - 1), G);
-    if (!p.interleaved && live && head < p.n_q + p.n_kv && l < 2 * hl) {
-      const int j = 4 * (low ? l : l - hl);
-      const float4 c = *reinterpret_cast<const float4*>(p.cos_t + (size_t)pos * half + j), s = *reinterpret_cast<const float4*>(p.sin_t + (size_t)pos * half + j);
-      const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+  for (int c = 0; c < HC; ++c) {
+    const int head = h0 + c;
+    if (turn && head < n_turn) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        x[i] = low ? __fsub_rn(__fmul_rn(x[i], cc[i]), __fmul_rn(y[i], ss[i])) : __fadd_rn(__fmul_rn(x[i], cc[i]), __fmul_rn(y[i], ss[i]));
+      for (int e = 0; e < 4; ++e) {
+        const float a = p.interleaved ? x[c][2 * e] : x[c][e], b = p.interleaved ? x[c][2 * e + 1] : x[c][4 + e];
+        const float ya = __fsub_rn(__fmul_rn(a, cc[e]), __fmul_rn(b, ss[e])), yb = __fadd_rn(__fmul_rn(b, cc[e]), __fmul_rn(a, ss[e]));
+        if (p.interleaved) { x[c][2 * e] = ya; x[c][2 * e + 1] = yb; } else { x[c][e] = ya; x[c][4 + e] = yb; }
+      }
+    }
+    const bool is_q = head < p.n_q, is_v = head >= n_turn;
+    const bool write = live && head < heads;
+    __nv_bfloat16* dst = nullptr;
+    long long at = 0;
+    if (is_q) {
+      dst = p.q + row * p.ldq + head * D;
+    } else {
+      at = ((long long)(max(slot, 0) / kPage) * p.n_kv + (head - (is_v ? n_turn : p.n_q))) * kPage + max(slot, 0) % kPage;
+      dst = reinterpret_cast<__nv_bfloat16*>(is_v ? p.v : p.k) + at * D;
+    }
+    if (is_q || !p.k_scale) {
+      if (write) {
+        *reinterpret_cast<uint2*>(dst + off_a) = make_uint2(pack_bf16(x[c][0], x[c][1]), pack_bf16(x[c][2], x[c][3]));
+        *reinterpret_cast<uint2*>(dst + off_b) = make_uint2(pack_bf16(x[c][4], x[c][5]), pack_bf16(x[c][6], x[c][7]));
+      }
+    }
+    if (p.k_scale) {
+      float largest = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(x[c][e]));
+#pragma unroll
+      for (int o = G / 2; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o, G));
+      if (write && !is_q) {
+        const float scale = largest > 0.f ? largest / 127.f : 1.f, inv = 1.f / scale;
+        uint32_t w[2] = {0, 0};
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e >> 2] |= (uint32_t)(__float2int_rn(__fmul_rn(x[c][e], inv)) & 0xff) << (8 * (e & 3));
+        int8_t* d8 = reinterpret_cast<int8_t*>(is_v ? p.v : p.k) + at * D;
+        *reinterpret_cast<uint32_t*>(d8 + off_a) = w[0];
+        *reinterpret_cast<uint32_t*>(d8 + off_b) = w[1];
+        if (l == 0) (is_v ? p.v_scale : p.k_scale)[at] = scale;
+      }
     }
   }
-  if (head < p.n_q) {
-    if (live) *reinterpret_cast<uint2*>(p.q + row * p.ldq + e) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-    if (!p.k_scale) return;
-  }
-  const bool is_v = head >= p.n_q + p.n_kv;
-  const int kh = is_v ? head - p.n_q - p.n_kv : head - p.n_q;
-  const long long at = live && head >= p.n_q ? ((long long)(slot / kPage) * p.n_kv + kh) * kPage + slot % kPage : 0;
-  if (!p.k_scale) {
-    if (live) *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(is_v ? p.v : p.k) + at * D + 4 * l) = make_uint2(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]));
-    return;
-  }
-  float largest = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-#pragma unroll
-  for (int o = G / 2; o > 0; o >>= 1) largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o, G));
-  if (!live || head < p.n_q) return;
-  const float scale = largest > 0.f ? largest / 127.f : 1.f, inv = 1.f / scale;
-  uint32_t w = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w |= (uint32_t)(__float2int_rn(__fmul_rn(x[i], inv)) & 0xff) << (8 * i);
-  *reinterpret_cast<uint32_t*>(reinterpret_cast<int8_t*>(is_v ? p.v : p.k) + at * D + 4 * l) = w;
-  if (l == 0) (is_v ? p.v_scale : p.k_scale)[at] = scale;
+}
+
+template <int D, bool F32>
+int launch(const TreeRopeParams& q, cudaStream_t st) {
+  TreeRopeParams p = q;
+  const int heads = p.n_q + 2 * p.n_kv;
+  const long long items = (long long)p.rows * heads;
+  // four heads a thread where that still gives every SM 2048 threads
+  const bool four = items * (D / 8) >= 4ll * 148 * 2048;
+  p.chunks = four ? (heads + 3) / 4 : heads;
+  const long long groups = (long long)p.rows * p.chunks, per = 256 / (D / 8);
+  if (groups > 0x7fffffffll - 1024) return -3;
+  const dim3 grid((unsigned)((groups + per - 1) / per));
+  if (four) return b2_launch(tree_rope_kernel<D, 4, F32>, grid, dim3(256), 0, st, true, p);
+  return b2_launch(tree_rope_kernel<D, 1, F32>, grid, dim3(256), 0, st, true, p);
 }
 
 }  // namespace
 
-extern "C" int b2_tree_rope(const void* qkv, long long ld, long long slice, int slices, const int* pos, const int* slots, int rows, const float* cos_t,
-                            const float* sin_t, int rot, int positions, int interleaved, int n_q, int n_kv, int D, void* q, long long ldq, void* k,
-                            void* v, float* k_scale, float* v_scale, long long num_slots, void* stream) {
-  if (rows < 1 || (D != 64 && D != 128) || rot < 0 || rot % 8 || rot > D || n_q < 1 || n_kv < 1) return -1;
-  if (((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 || ld % 4 || ldq % 4 || slice % 4) return -2;
+extern "C" int b2_tree_rope(const B2TreeStep* step, const B2TreeCache* cache, const void* qkv, long long ld, long long slice, int slices, int rows, const float* cos_t,
+                            const float* sin_t, int pairs, int positions, int interleaved, int n_q, void* q, long long ldq, void* stream) {
+  const B2TreeCache& c = *cache;
+  if (rows < 1 || rows > step->max_rows || (c.d != 64 && c.d != 128) || pairs < 0 || pairs % 4 || 2 * pairs > c.d || n_q < 1 || c.heads < 1) return -1;
+  if (((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 || ld % 4 || ldq % 4 || slice % 4) return -2;
   TreeRopeParams p;
-  p.qkv = qkv; p.ld = ld; p.slice = slice; p.slices = slices; p.pos = pos; p.slots = slots; p.rows = rows; p.cos_t = cos_t; p.sin_t = sin_t;
-  p.rot = rot; p.positions = positions; p.interleaved = interleaved; p.n_q = n_q; p.n_kv = n_kv; p.D = D; p.q = (__nv_bfloat16*)q; p.ldq = ldq;
-  p.k = k; p.v = v; p.k_scale = k_scale; p.v_scale = v_scale; p.num_slots = num_slots;
-  const long long items = (long long)rows * (n_q + 2 * n_kv), per = 256 / (D / 4);
-  if (items > 0x7fffffffll - 1024) return -3;
-  const dim3 grid((unsigned)((items + per - 1) / per));
-  if (D == 64) return b2_launch(tree_rope_kernel<64>, grid, dim3(256), 0, (cudaStream_t)stream, true, p);
-  return b2_launch(tree_rope_kernel<128>, grid, dim3(256), 0, (cudaStream_t)stream, true, p);
+  p.qkv = qkv; p.ld = ld; p.slice = slice; p.slices = slices; p.pos = step->row_pos; p.slots = step->slots; p.rows = rows; p.cos_t = cos_t; p.sin_t = sin_t;
+  p.pairs = pairs; p.positions = positions; p.interleaved = interleaved; p.n_q = n_q; p.n_kv = c.heads; p.q = (__nv_bfloat16*)q; p.ldq = ldq;
+  p.k = c.k; p.v = c.v; p.k_scale = c.k_scale; p.v_scale = c.v_scale; p.num_slots = (long long)c.pages * kPage; p.chunks = 0;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (c.d == 64) return slices ? launch<64, true>(p, st) : launch<64, false>(p, st);
+  return slices ? launch<128, true>(p, st) : launch<128, false>(p, st);
 }
 
 B2_DEFINE_STATUS(treerope)

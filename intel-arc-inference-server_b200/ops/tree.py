@@ -25,7 +25,7 @@ from typing import Optional
 import torch
 
 from . import lib as K
-from .logprob import _elsewhere, _entry, _rows_of, _stream
+from .logprob import _elsewhere, _rows_of, _stream
 
 PAGE = 16
 MAX_NODES = 64          # nodes of a tree: an ancestor mask is one 64-bit word
@@ -37,10 +37,58 @@ _FAULTS = {1: "the pool has not enough pages, or no room for those that come bac
            32: "a negative length", 64: "a table names a page that is not there"}
 
 
+_P, _L, _I = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+
+
+class _Step(ctypes.Structure):          # csrc/tree.cuh
+    _fields_ = [(n, _P) for n in ("block_table", "tree_table", "lengths", "row_start", "row_req", "row_pos", "slots", "parents", "masks", "status")] + [
+        (n, _I) for n in ("requests", "max_blocks", "tree_blocks", "max_rows", "max_nodes", "num_pages")]
+
+
+class _Pool(ctypes.Structure):
+    _fields_ = [("free", _P), ("n_free", _P), ("held", _P), ("capacity", _I)]
+
+
+class _Cache(ctypes.Structure):
+    _fields_ = [("maps", ctypes.c_uint8 * 256), ("k", _P), ("v", _P), ("k_scale", _P), ("v_scale", _P), ("layer_bytes", _L), ("layer_scales", _L),
+                ("layers", _I), ("pages", _I), ("heads", _I), ("d", _I)]
+
+
+class _Accepted(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("path", "count", "next_token", "lengths")]
+
+
+@functools.lru_cache(maxsize=None)
+def _fn():
+    """The library's entry points with their argument types."""
+    out = {}
+    for name, result, args in (("plan", _I, [_P] * 6 + [_I, _P]), ("rope", _I, [_P] * 3 + [_L, _L, _I, _I, _P, _P, _I, _I, _I, _I, _P, _L, _P]), ("cache", _I, [_P]),
+                               ("attention", _I, [_P] * 3 + [_L, _P, _L, _P, _I, _I, _I, ctypes.c_float, _P]), ("attention_work", _L, [_P, _I, _I, _I]),
+                               ("commit", _I, [_P] * 5 + [_I, _P])):
+        fn = getattr(K.lib(), "b2_tree_" + name)
+        fn.restype, fn.argtypes = result, args
+        out[name] = fn
+    return out
+
+
+def _aligned(kind):
+    """A structure whose first field begins at a multiple of 64 bytes."""
+    room = (ctypes.c_uint8 * (ctypes.sizeof(kind) + 64))()
+    at = kind.from_buffer(room, -ctypes.addressof(room) % 64)
+    return at, ctypes.addressof(at)
+
+
 def _flat(t: torch.Tensor, dtype, shape, what: str, device=None) -> torch.Tensor:
     if t.dtype is not dtype or t.shape != shape or not t.is_cuda or not t.is_contiguous() or device is not None and t.device != device:
         raise ValueError(f"{what}: contiguous {dtype} {list(shape)} on {device or 'a CUDA device'}, not {t.dtype} {list(t.shape)} on {t.device}")
     return t
+
+
+def _words(t: torch.Tensor, n: int, what: str, device) -> int:
+    """Address of ``n`` int32 numbers."""
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or t.get_device() != device.index or not t.is_contiguous():
+        raise ValueError(f"{what}: {n} contiguous int32 numbers on {device}, not {t.dtype} {list(t.shape)} on {t.device}")
+    return t.data_ptr()
 
 
 class PagePool:
@@ -51,6 +99,8 @@ class PagePool:
         _flat(free, torch.int32, (free.numel(),), "free pages")
         self.free, self.n_free = free, _flat(n_free, torch.int32, (1,), "number of free pages", free.device)
         self.held = _flat(held, torch.int32, (held.numel(),), "pages of the requests", free.device)
+        self._c = _Pool(free.data_ptr(), n_free.data_ptr(), held.data_ptr(), free.numel())
+        self._at, self._requests, self._device = ctypes.addressof(self._c), held.numel(), free.device
 
 
 class TreeCache:
@@ -77,8 +127,16 @@ class TreeCache:
         if self.pages * self.heads * PAGE >= 1 << 31:
             raise ValueError("a layer of fewer than 2^31 rows")
         self.device, self.i8 = k.device, i8
-        self._kv = (k.data_ptr(), v.data_ptr())
-        self._scales = (k_scale.data_ptr(), v_scale.data_ptr()) if i8 else (None, None)
+        if i8 and (k_scale.data_ptr() | v_scale.data_ptr() | (k_scale.stride(0) * 4 if k.dim() == 5 else 0)) % 16:
+            raise ValueError("a layer's scales begin at multiples of 16 bytes")
+        self._c, self._at = _aligned(_Cache)
+        c, five = self._c, k.dim() == 5
+        c.k, c.v, c.layers, c.pages, c.heads, c.d = k.data_ptr(), v.data_ptr(), self.layers, self.pages, self.heads, self.d
+        c.k_scale, c.v_scale = (k_scale.data_ptr(), v_scale.data_ptr()) if i8 else (None, None)
+        c.layer_bytes, c.layer_scales = (k.stride(0) * k.element_size(), k_scale.stride(0) if i8 else 0) if five else (0, 0)
+        with torch.cuda.device(k.device):
+            K._check(_fn()["cache"](self._at), "tree_cache")
+        K.launch_count -= 1      # (nothing is launched)
 
 
 class TreeStep:
@@ -111,9 +169,10 @@ class TreeStep:
         self.masks = torch.zeros(max_rows, dtype=torch.int64, device=dev)
         self.status = torch.zeros(1, dtype=torch.int32, device=dev)
         self.tree: Optional[bool] = None       # the last plan's rows are trees'
-        self._tables = (block_table.data_ptr(), tree_table.data_ptr())
-        self._rows = (self.row_start.data_ptr(), self.row_req.data_ptr(), self.row_pos.data_ptr())
-        self._plan = (self.lengths.data_ptr(), *self._rows, self.slots.data_ptr(), self.parents.data_ptr(), self.masks.data_ptr(), self.status.data_ptr())
+        self._c = _Step(*(t.data_ptr() for t in (block_table, tree_table, self.lengths, self.row_start, self.row_req, self.row_pos, self.slots, self.parents, self.masks,
+                                                 self.status)), b, block_table.shape[1], tree_table.shape[1], max_rows, max_nodes, num_pages)
+        self._at, self._lengths, self._work = ctypes.addressof(self._c), self.lengths.data_ptr(), {}
+        self._floats = torch.empty(0, device=dev)
 
     def check(self):
         """Waits for the last plan and raises where it could not be made."""
@@ -130,7 +189,8 @@ class Accepted:
         b, dev = count.numel(), count.device
         self.path, self.count = _flat(path, torch.int32, (b, MAX_NODES), "accepted path", dev), _flat(count, torch.int32, (b,), "accepted nodes")
         self.next_token, self.lengths = _flat(next_token, torch.int32, (b,), "next tokens", dev), _flat(lengths, torch.int32, (b,), "lengths", dev)
-        self._out = (path.data_ptr(), count.data_ptr(), next_token.data_ptr(), lengths.data_ptr())
+        self._c = _Accepted(path.data_ptr(), count.data_ptr(), next_token.data_ptr(), lengths.data_ptr())
+        self._at, self._requests, self._device, self._lengths = ctypes.addressof(self._c), b, dev, lengths.data_ptr()
 
     @staticmethod
     def empty(requests: int, device) -> "Accepted":
@@ -145,21 +205,21 @@ def plan(step: TreeStep, lengths: torch.Tensor, counts: torch.Tensor, parents: O
     (``parents`` None: all its rows), in the order of the requests.  ``after``: where the pool's numbers are written (over the same free
     pages; None: in place)."""
     b, dev = step.requests, step.device
-    after = pool if after is None else after
-    _flat(lengths, torch.int32, (b,), "lengths", dev)
-    _flat(counts, torch.int32, (b,), "rows of the requests", dev)
-    if parents is not None and (parents.dtype is not torch.int32 or parents.dim() != 1 or parents.device != dev or not parents.is_contiguous() or parents.numel() > step.max_rows):
-        raise ValueError(f"parents: up to {step.max_rows} contiguous int32 numbers on {dev}")
-    if pool.held.numel() != b or pool.free.device != dev or after.held.numel() != b or after.free.data_ptr() != pool.free.data_ptr():
+    if after is None:
+        after = pool
+    at, counts_at = _words(lengths, b, "lengths", dev), _words(counts, b, "rows of the requests", dev)
+    rows, parents_at = step.max_rows, None
+    if parents is not None:
+        rows = parents.numel()
+        parents_at = _words(parents, rows, "parents", dev)
+        if rows > step.max_rows:
+            raise ValueError(f"parents: of up to {step.max_rows} rows, not {rows}")
+    if pool._requests != b or after._requests != b or pool._device != dev or after._c.free != pool._c.free:
         raise ValueError(f"pools of {b} requests on {dev}, over the same free pages")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return plan(step, lengths, counts, parents, pool, after)
-    rows = step.max_rows if parents is None else parents.numel()
-    K._check(_entry("b2_tree_plan", "p" * 18 + "i" * 8 + "p")(
-        lengths.data_ptr(), counts.data_ptr(), None if parents is None else parents.data_ptr(), *step._tables, pool.free.data_ptr(), pool.n_free.data_ptr(),
-        pool.held.data_ptr(), after.n_free.data_ptr(), after.held.data_ptr(), *step._plan, b, step.block_table.shape[1], step.tree_table.shape[1],
-        pool.free.numel(), step.max_rows, step.max_nodes, step.num_pages, rows, _stream(dev)), "tree_plan")
+    K._check(_fn()["plan"](step._at, pool._at, after._at, at, counts_at, parents_at, rows, _stream(dev)), "tree_plan")
     step.tree = parents is not None
     return step
 
@@ -201,9 +261,8 @@ def rope_append(step: TreeStep, qkv: torch.Tensor, rope: tuple, q: torch.Tensor,
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return rope_append(step, qkv, rope, q, cache, interleaved)
-    K._check(_entry("b2_tree_rope", "pllippippiiiiiiplppppl" + "p")(
-        at, ld, slice_elems, slices, step._rows[2], step.slots.data_ptr(), rows, cos.data_ptr(), sin.data_ptr(), 2 * cos.shape[1], cos.shape[0], int(interleaved), n_q, n_kv, d,
-        pq, ldq, *cache._kv, *cache._scales, cache.pages * PAGE, _stream(dev)), "tree_rope")
+    K._check(_fn()["rope"](step._at, cache._at, at, ld, slice_elems, slices, rows, cos.data_ptr(), sin.data_ptr(), cos.shape[1], cos.shape[0], int(interleaved), n_q, pq, ldq,
+                           _stream(dev)), "tree_rope")
     return q
 
 
@@ -227,28 +286,16 @@ def attention(step: TreeStep, q: torch.Tensor, cache: TreeCache, out: torch.Tens
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return attention(step, q, cache, out, scale, window)
-    fn, work = _attention_entry(), torch.empty(_attention_work(step.requests, step.block_table.shape[1], n_q, n_kv, d, step.max_nodes, dev.index), dtype=torch.float32, device=dev)
-    K._check(fn(pq, ldq, *cache._kv, *cache._scales, step._plan[0], *step._rows, *step._tables, step._plan[6], po, work.data_ptr(), ldo, rows, step.requests,
-                step.block_table.shape[1], step.tree_table.shape[1], cache.pages, n_q, n_kv, d, step.max_nodes, window, scale, _stream(dev)), "tree_attention")
+    room = step._work.get((n_q, n_kv, d))
+    if room is None:
+        room = step._work[n_q, n_kv, d] = _fn()["attention_work"](step._at, n_q, n_kv, d)
+    work = step._floats.new_empty(room)      # this call's own: calls of one step on several streams share nothing
+    K._check(_fn()["attention"](step._at, cache._at, pq, ldq, po, ldo, work.data_ptr(), rows, n_q, window, scale, _stream(dev)), "tree_attention")
     K.launch_count += 1      # segments added up
     return out
 
 
 MAX_GROUP = 64          # query heads to a key head
-
-
-@functools.lru_cache(maxsize=None)
-def _attention_work(requests: int, blocks: int, n_q: int, n_kv: int, d: int, max_nodes: int, device: int) -> int:
-    """fp32 words of workspace on the device, which is the current one."""
-    return _entry("b2_tree_attention_work", "iiiiii", ctypes.c_longlong)(requests, blocks, n_q, n_kv, d, max_nodes)
-
-
-@functools.lru_cache(maxsize=None)
-def _attention_entry():
-    fn = K.lib().b2_tree_attention
-    p, q, i = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
-    fn.restype, fn.argtypes = ctypes.c_int, [p, q] + [p] * 13 + [q] + [i] * 10 + [ctypes.c_float, p]
-    return fn
 
 
 def commit(step: TreeStep, tokens: torch.Tensor, targets: torch.Tensor, cache: TreeCache, accepted: Optional[Accepted] = None) -> Accepted:
@@ -260,21 +307,16 @@ def commit(step: TreeStep, tokens: torch.Tensor, targets: torch.Tensor, cache: T
     dev, b = step.device, step.requests
     if not step.tree:
         raise ValueError("the step's rows are no trees'")
-    if tokens.dim() != 1 or not 1 <= tokens.numel() <= step.max_rows:
+    rows = tokens.numel()
+    if not 1 <= rows <= step.max_rows:
         raise ValueError(f"tokens: of 1 to {step.max_rows} rows")
-    _flat(tokens, torch.int32, tokens.shape, "tokens", dev)
-    _flat(targets, torch.int32, tokens.shape, "targets", dev)
+    at, targets_at = _words(tokens, rows, "tokens", dev), _words(targets, rows, "targets", dev)
     if accepted is None:
         accepted = Accepted.empty(b, dev)
-    elif accepted.count.numel() != b or accepted.count.device != dev or accepted._out[3] == step._plan[0]:
+    elif accepted._requests != b or accepted._device != dev or accepted._lengths == step._lengths:
         raise ValueError(f"results of {b} requests on {dev}, apart from the step's own")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return commit(step, tokens, targets, cache, accepted)
-    k, ks = cache.k, cache.k_scale
-    five = k.dim() == 5
-    K._check(_entry("b2_tree_commit", "p" * 9 + "lppl" + "pppp" + "i" * 8 + "p")(
-        step._plan[0], step._rows[0], step._plan[5], tokens.data_ptr(), targets.data_ptr(), *step._tables, *cache._kv, k.stride(0) * k.element_size() if five else 0,
-        *cache._scales, ks.stride(0) if five and ks is not None else 0, *accepted._out, b, step.block_table.shape[1], step.tree_table.shape[1], cache.layers, cache.pages,
-        cache.heads, cache.d * k.element_size(), tokens.numel(), _stream(dev)), "tree_commit")
+    K._check(_fn()["commit"](step._at, cache._at, accepted._at, at, targets_at, rows, _stream(dev)), "tree_commit")
     return accepted
