@@ -54,7 +54,7 @@ struct Form {
   static constexpr int NDK = NDK_, NW = NW_, D = NDK_ * 64;
   static constexpr bool I8 = I8_;
   static constexpr int T_BYTES = BK * NDK * 128;                 // a K or V tile: [64-dim blocks][64 keys][128 bytes]
-  static constexpr int KS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 6 : 4) * (3 - NDK_), VS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 7 : 5) * (3 - NDK_);     // operand tiles
+  static constexpr int KS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 6 : 4) * (3 - NDK_), VS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 6 : 5) * (3 - NDK_);     // operand tiles
   static constexpr int RS = I8_ ? 5 * (3 - NDK_) : 0;                                                     // stages of bytes
   static constexpr int S_BYTES = 2 * BK * D + 2 * BK * 4;        // keys, values, their scales
   static constexpr int Q_BYTES = NW == 1 ? 0 : NW * BQ * NDK * 128;
@@ -62,6 +62,10 @@ struct Form {
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + KS * T_BYTES, OFF_ST = OFF_V + VS * T_BYTES, OFF_SC = OFF_ST + RS * S_BYTES,
                        OFF_X = OFF_SC + (I8_ ? 4 * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * 2 * BQ * 4, OFF_BAR = OFF_CUM + (kMaxReq + 8) * 4,
                        SMEM = OFF_BAR + 1024 + 1024;
+  // Copies end in any order.  Where the groups take every other tile, a place's tiles have to be one group's: at a place of both, the group that is
+  // ahead would wait for a phase while the one before it is still open, and a parity says no more than that the one before that is over.  (The 8-bit
+  // form's places are filled in order.)
+  static_assert(I8_ || NW_ == 2 || (KS % 2 == 0 && VS % 2 == 0), "places of one group");
   static_assert(SMEM <= 227 * 1024 && KS <= 14 && VS <= 14 && RS <= 14, "shared memory");
 };
 
@@ -94,12 +98,48 @@ __device__ __forceinline__ void ld_16(uint32_t taddr, uint32_t* r) {
                : "r"(taddr)
                : "memory");
 }
+// Bounded waits of a whole warp.  The vote is inside the loop: a warp never comes apart at a wait, which everything behind it that is a warp's
+// (tensor memory, named barriers, operands in uniform registers) takes for granted.
+__device__ __forceinline__ bool warp_wait_inline(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < 256; ++i)
+    if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+  const long long t0 = clock64();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 256; ++i)
+      if (__all_sync(0xffffffffu, mbar_try(bar, parity))) return true;
+    if (__any_sync(0xffffffffu, clock64() - t0 > kWaitCycles)) {
+      if ((threadIdx.x & 31) == 0) record_error(ERR_ATTN_WAIT, (blockIdx.x << 8) | (threadIdx.x >> 5));
+      __syncwarp();
+      return false;
+    }
+  }
+}
+__device__ __noinline__ bool warp_wait_long(uint32_t bar, uint32_t parity) { return warp_wait_inline(bar, parity); }
+// The first look inline, for warps whose phase usually is over; the call is the whole warp's.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, ok != 0) || warp_wait_long(bar, parity);
+}
 __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {      // a look that never waits
   uint32_t ok;
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+// One lane of a warp that is together.  The issuing warps stay together around it, with every operand the same in all lanes, so that operands are
+// in uniform registers: a lone lane pays for moving each of them there.
+__device__ __forceinline__ bool elect() {
+  __syncwarp();
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+__device__ __forceinline__ void pair_sync(int id) {
+  __syncwarp();
+  asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
+}
 
 __device__ __forceinline__ uint32_t bytes_bf16(uint32_t w) {      // even bytes as integers in bf16: 128 + (b & 127) less 128, or 256 where the sign is set
   uint32_t lo = (w & 0x007f007fu) | 0x43004300u, hi = (w & 0x00800080u) | 0x43004300u, d;
@@ -167,7 +207,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto b_scale = [&](int g) { return bars + 744 + (g & 3) * 8; };
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gen + F::OFF_BAR + 776);
   int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 784);      // [warps]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) {
@@ -199,6 +239,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
   }
   if (warp == F::kMma) {
+    __syncwarp();
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
@@ -231,7 +272,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   // tensor memory: queries 64 columns (NW 1), scores 2 x 64, weights 2 x 32, accumulators 2 x D
   const uint32_t t_q = tmem_base;
   auto t_s = [&](int w) { return tmem_base + 64 + (uint32_t)w * 64; };
@@ -289,45 +330,45 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         int page[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) page[x] = __shfl_sync(0xffffffffu, tree ? tree_ids : ids, tree ? x : pi - at + x);
-        if (lane == 0) {
-          if (g >= kd) ok = mbar_wait(empty0 + 8 * s, par ^ 1, ERR_ATTN_WAIT);
-          if (ok) {
-            const uint32_t full = full0 + 8 * s;
-            if constexpr (F::I8) {
-              int pages = 0;
+        if (g >= kd) ok = warp_wait_inline(empty0 + 8 * s, par ^ 1);
+        if (!ok) break;
+        const uint32_t full = full0 + 8 * s;
+        if constexpr (F::I8) {
+          if (elect()) {
+            int pages = 0;
 #pragma unroll
-              for (int x = 0; x < 4; ++x) pages += page[x] >= 0;
-              mbar_expect_tx(full, pages * (kPage * D + kPage * 4));
-              const uint32_t st = st_s0 + s * F::S_BYTES + (is_v ? BK * D : 0), sc = st_s0 + s * F::S_BYTES + 2 * BK * D + (is_v ? BK * 4 : 0);
-              const int8_t* data = is_v ? p.v8 : p.k8;
-              const float* scale = is_v ? p.v_scale : p.k_scale;
+            for (int x = 0; x < 4; ++x) pages += page[x] >= 0;
+            mbar_expect_tx(full, pages * (kPage * D + kPage * 4));
+            const uint32_t st = st_s0 + s * F::S_BYTES + (is_v ? BK * D : 0), sc = st_s0 + s * F::S_BYTES + 2 * BK * D + (is_v ? BK * 4 : 0);
+            const int8_t* data = is_v ? p.v8 : p.k8;
+            const float* scale = is_v ? p.v_scale : p.k_scale;
 #pragma unroll
-              for (int x = 0; x < 4; ++x)
-                if (page[x] >= 0) {
-                  const long long row = ((long long)page[x] * p.n_kv + k.h) * kPage;
-                  bulk_g2s(st + x * (kPage * D), data + row * D, kPage * D, full);
-                  bulk_g2s(sc + x * (kPage * 4), scale + row, kPage * 4, full);
-                }
-            } else {
-              mbar_expect_tx(full, F::T_BYTES);
-              const uint32_t dst = (is_v ? v_s0 : k_s0) + s * F::T_BYTES;
-              const CUtensorMap* map = is_v ? &map_v : &map_k;
-#pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                const int row = (page[x] >= 0 ? page[x] * p.n_kv + k.h : p.num_pages * p.n_kv) * kPage;
-#pragma unroll
-                for (int c = 0; c < NDK; ++c) tma_load_2d(dst + c * (BK * 128) + x * (kPage * 128), map, c * 64, row, full);
+            for (int x = 0; x < 4; ++x)
+              if (page[x] >= 0) {
+                const long long row = ((long long)page[x] * p.n_kv + k.h) * kPage;
+                bulk_g2s(st + x * (kPage * D), data + row * D, kPage * D, full);
+                bulk_g2s(sc + x * (kPage * 4), scale + row, kPage * 4, full);
               }
+          }
+        } else {
+          const uint32_t dst = (is_v ? v_s0 : k_s0) + s * F::T_BYTES;
+          const CUtensorMap* map = is_v ? &map_v : &map_k;
+          if (elect()) {
+            mbar_expect_tx(full, F::T_BYTES);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const int row = (page[x] >= 0 ? page[x] * p.n_kv + k.h : p.num_pages * p.n_kv) * kPage;
+#pragma unroll
+              for (int c = 0; c < NDK; ++c) tma_load_2d(dst + c * (BK * 128) + x * (kPage * 128), map, c * 64, row, full);
             }
           }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
+        __syncwarp();
         if (++s == kd) { s = 0; par ^= 1; }
       }
     }
-    if (!ok && lane == 0)      // copies in flight end before the CTA does
-      for (int i = max(0, g - kd); i < g; ++i) mbar_wait(full0 + 8 * (i % kd), (i / kd) & 1, ERR_ATTN_WAIT);
+    if (!ok)      // copies in flight end before the CTA does
+      for (int i = max(0, g - kd); i < g; ++i) warp_wait_inline(full0 + 8 * (i % kd), (i / kd) & 1);
   } else if (warp < F::kSoft) {
     // ---------------------------------------------------------- products of group w
     const int w = warp - F::kMma;
@@ -336,51 +377,45 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const uint32_t hi_k = (uint32_t)(make_desc_sw128(0) >> 32), hi_v = (uint32_t)(make_desc_v(0) >> 32);
     const uint32_t ql = (uint32_t)make_desc_sw128(q_s + w * (BQ * NDK * 128)), k_lo = (uint32_t)make_desc_sw128(k_s0), v_lo = (uint32_t)make_desc_v(v_s0);
     bool ok = true, live = true;
-    int g0 = 0, j = 0, seg = 0;      // tiles of all segments before, this group's tiles so far
+    int g0 = 0, j = 0, seg = 0, last = -1;      // tiles of all segments before, this group's tiles so far, the last one
+    auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait_inline(bar, parity); };
     auto issue_qk = [&](int g, int jj) -> bool {
       const int ks = g % KS;
-      if (!mbar_wait(b_kfull + 8 * ks, (g / KS) & 1, ERR_ATTN_WAIT)) return false;
-      if (jj >= 1 && !mbar_wait(b_sfree(w), (jj - 1) & 1, ERR_ATTN_WAIT)) return false;      // the scores before are in registers
+      if (!wait(b_kfull + 8 * ks, (g / KS) & 1)) return false;
+      if (jj >= 1 && !wait(b_sfree(w), (jj - 1) & 1)) return false;      // the scores before are in registers
       tc_fence_after();
       const uint32_t kl = k_lo + ks * (F::T_BYTES >> 4);
-      if (live) {
+      if (elect()) {
+        if (live) {
 #pragma unroll
-        for (int x = 0; x < 4 * NDK; ++x) {
-          const uint32_t kx = kl + (((x >> 2) * (BK * 128) + (x & 3) * 32) >> 4);
-          if constexpr (NW == 1) umma_f16_ts_w(t_s(w), t_q + 8 * x, kx, hi_k, idesc_qk, x != 0);
-          else umma_f16_w(t_s(w), ql + (((x >> 2) * (BQ * 128) + (x & 3) * 32) >> 4), hi_k, kx, hi_k, idesc_qk, x != 0);
+          for (int x = 0; x < 4 * NDK; ++x) {
+            const uint32_t kx = kl + (((x >> 2) * (BK * 128) + (x & 3) * 32) >> 4);
+            if constexpr (NW == 1) umma_f16_ts_w(t_s(w), t_q + 8 * x, kx, hi_k, idesc_qk, x != 0);
+            else umma_f16_w(t_s(w), ql + (((x >> 2) * (BQ * 128) + (x & 3) * 32) >> 4), hi_k, kx, hi_k, idesc_qk, x != 0);
+          }
         }
+        tc_commit(b_sfull(w));
+        tc_commit(b_kempty + 8 * ks);
       }
-      tc_commit(b_sfull(w));
-      tc_commit(b_kempty + 8 * ks);
+      __syncwarp();
       return true;
     };
     while (ok && next_segment<F>(p, s_cum, k)) {
       live = NW == 1 || w * BQ < k.tok * p.gqa;      // (a second query tile without rows only hands tiles back)
       const int i0 = NW == 1 ? (w - g0) & 1 : 0;
-      if (lane == 0) {
-        ok = mbar_wait(b_q, seg & 1, ERR_ATTN_WAIT);
-        if (ok && i0 < k.count) ok = issue_qk(g0 + i0, j);
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
+      ok = wait(b_q, seg & 1);
+      if (ok && i0 < k.count) ok = issue_qk(g0 + i0, j);
       for (int i = i0; i < k.count && ok; i += kStep, ++j) {
         const int g = g0 + i, vs = g % VS, valid = keys_of(k.ts + i);
-        const bool tail = !F::I8 && (valid & 15) != 0;
-        bool ahead = false;      // the next scores' product is issued
-        if (lane == 0) {
-          // the next scores first, if their keys are here; else not before this tile's product, which their place may be waiting for
-          if (i + kStep < k.count && mbar_test(b_kfull + 8 * ((g + kStep) % KS), ((g + kStep) / KS) & 1)) {
-            ok = issue_qk(g + kStep, j + 1);
-            ahead = true;
-          }
-          if (ok) ok = mbar_wait(b_pfull(w), j & 1, ERR_ATTN_WAIT);
-          if (ok) ok = mbar_wait(b_vfull + 8 * vs, (g / VS) & 1, ERR_ATTN_WAIT);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        // the next scores first, if their keys are here; else not before this tile's product, which their place may be waiting for
+        const bool more = i + kStep < k.count;
+        const bool ahead = more && __all_sync(0xffffffffu, mbar_test(b_kfull + 8 * ((g + kStep) % KS), ((g + kStep) / KS) & 1));
+        if (ahead) ok = issue_qk(g + kStep, j + 1);
+        if (ok) ok = wait(b_pfull(w), j & 1);
+        if (ok) ok = wait(b_vfull + 8 * vs, (g / VS) & 1);
         if (!ok) break;
-        if (tail) {
+        if (!F::I8 && (valid & 15) != 0) {
           // values behind the last key's are anything: their weights are 0, but 0 x infinity is not
-          mbar_wait(b_vfull + 8 * vs, (g / VS) & 1, ERR_ATTN_WAIT);      // (over: every lane sees the copies)
           const int end = (valid + 15) & ~15;
           for (int x = lane; x < (end - valid) * NDK * 8; x += 32) {
             const int row = valid + x / (NDK * 8), c = x % (NDK * 8);
@@ -389,9 +424,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           fence_proxy_async_smem();
           __syncwarp();
         }
-        if (lane == 0) {
-          tc_fence_after();
-          const uint32_t vl = v_lo + vs * (F::T_BYTES >> 4);
+        tc_fence_after();
+        const uint32_t vl = v_lo + vs * (F::T_BYTES >> 4);
+        if (elect()) {
           if (live) {
 #pragma unroll
             for (int x = 0; x < 4; ++x)      // 16 keys a step; P in tensor memory, 8 columns of pairs
@@ -399,13 +434,16 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           }
           tc_commit(b_odone(w));
           tc_commit(b_vempty + 8 * vs);
-          if (!ahead && i + kStep < k.count) ok = issue_qk(g + kStep, j + 1);
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        __syncwarp();
+        if (more && !ahead) ok = issue_qk(g + kStep, j + 1);
+        last = g;
       }
       g0 += k.count;
       ++seg;
     }
+    // the last arrival that a product makes: none is on its way when the CTA ends
+    if (ok && last >= 0) wait(b_vempty + 8 * (last % VS), (last / VS) & 1);
   } else if (warp < F::kConv) {
     // ---------------------------------------------------------- softmax: two threads per query row of group w
     constexpr float kLazy = 6.f;
@@ -417,7 +455,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     // once a wait has run out no other is made, but every barrier is still come to
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {
-      if (ok) ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, ERR_ATTN_WAIT));
+      if (ok) ok = warp_wait(bar, parity);
     };
     int g0 = 0, j = 0, seg = 0;
     while (next_segment<F>(p, s_cum, k)) {
@@ -440,6 +478,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             x[c] = make_uint4(__byte_perm(x[c].x, x[c].y, 0x5410), __byte_perm(x[c].x, x[c].y, 0x7632), __byte_perm(x[c].z, x[c].w, 0x5410), __byte_perm(x[c].z, x[c].w, 0x7632));
         }
         if constexpr (NW == 1) {
+          __syncwarp();      // (tensor memory is a whole warp's: lanes whose ways parted meet again first, here and below)
           if constexpr (NV == 4) st_16(t_q + lane_addr + c0 * 4, reinterpret_cast<const uint32_t*>(x));
           else st_8(t_q + lane_addr + c0 * 4, reinterpret_cast<const uint32_t*>(x));
           tmem_st_wait();
@@ -477,6 +516,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         }
         tc_fence_after();
         uint32_t v[32];
+        __syncwarp();
         B2_TMEM_LD_32(t_s(w) + lane_addr + half * 32, v);
         uint32_t vis = half ? (uint32_t)(mask >> 32) : (uint32_t)mask;
         if (t != k.r.nt - 1) {
@@ -561,6 +601,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll 1
             for (int c = 0; c < 2 * NDK; ++c) {      // this thread's half of the row
               uint32_t o[16];
+              __syncwarp();
               ld_16(t_o(w) + lane_addr + half * (D / 2) + c * 16, o);
               tmem_ld_wait();
 #pragma unroll
@@ -569,6 +610,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             }
           }
         }
+        __syncwarp();
         st_16(t_p(w) + lane_addr + half * 16, pk);
         tmem_st_wait();
         tc_fence_before();
@@ -586,6 +628,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (half == 0) x_mine[((j & 1) ^ 1) * (2 * BQ)] = mref;      // read by the other group, at this group's parity
         else x_mine[((j & 1) ^ 1) * (2 * BQ)] = l;
       }
+      __syncwarp();
       asm volatile("bar.sync 9, 512;" ::: "memory");
       tc_fence_after();
       const bool whole = k.count == k.r.nt;
@@ -611,6 +654,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll 1
         for (int c = 0; c < NC; ++c) {
           uint32_t o[16], o1[16];
+          __syncwarp();
           if constexpr (NW == 1) {
             ld_16(t_o(0) + lane_addr + c0 + c * 16, o);
             ld_16(t_o(1) + lane_addr + c0 + c * 16, o1);
@@ -624,7 +668,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * inv);
           }
-          if (!row_ok) continue;
           if constexpr (F::I8) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
@@ -633,19 +676,20 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
               o[e + 2] = t2;
             }
           }
-          if (whole) {
+          if (row_ok && whole) {
 #pragma unroll
             for (int e = 0; e < 2; ++e)
               *reinterpret_cast<uint4*>(dst + c * 16 + 8 * e) = make_uint4(
                   pack_bf16(__uint_as_float(o[8 * e]), __uint_as_float(o[8 * e + 1])), pack_bf16(__uint_as_float(o[8 * e + 2]), __uint_as_float(o[8 * e + 3])),
                   pack_bf16(__uint_as_float(o[8 * e + 4]), __uint_as_float(o[8 * e + 5])), pack_bf16(__uint_as_float(o[8 * e + 6]), __uint_as_float(o[8 * e + 7])));
-          } else {
+          } else if (row_ok) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(part + c * 16 + 4 * e) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
         if (!whole && row_ok && half == 0 && (NW == 2 || w == 0)) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(best, sum);
       }
+      __syncwarp();
       tc_fence_before();
       g0 += k.count;
     }
@@ -682,8 +726,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       for (int i = 0; i < k.count; ++i, ++g) {
         const int rs = g % RS, ks = g % KS, vs = g % VS;
         const uint32_t st = st_s0 + rs * F::S_BYTES;
-        ok = mbar_wait(b_rfull + 8 * rs, (g / RS) & 1, ERR_ATTN_WAIT);
-        if (ok && g >= KS) ok = mbar_wait(b_kempty + 8 * ks, ((g / KS) & 1) ^ 1, ERR_ATTN_WAIT);
+        ok = warp_wait(b_rfull + 8 * rs, (g / RS) & 1);
+        if (ok && g >= KS) ok = warp_wait(b_kempty + 8 * ks, ((g / KS) & 1) ^ 1);
         if (!ok) break;
         // the scales of tile g - 4 are read: the places of the values of tiles g - 2 and g - 1 came free with the products of tiles g - 2 - VS and
         // g - 1 - VS, the same group's or a later one's.  Behind the last key they are anything, and made 0: what a place holds that nobody sees must not reach a sum.
@@ -694,16 +738,18 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         }
         expand(st, k_s0 + ks * F::T_BYTES);
         mbar_arrive(b_kfull + 8 * ks);
-        if (g >= VS) ok = mbar_wait(b_vempty + 8 * vs, ((g / VS) & 1) ^ 1, ERR_ATTN_WAIT);
+        if (g >= VS) ok = warp_wait(b_vempty + 8 * vs, ((g / VS) & 1) ^ 1);
         if (!ok) break;
         expand(st + BK * D, v_s0 + vs * F::T_BYTES);
         mbar_arrive(b_vfull + 8 * vs);
         mbar_arrive(b_rempty + 8 * rs);
       }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == F::kMma) {
+    __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
