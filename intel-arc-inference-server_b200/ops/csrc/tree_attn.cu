@@ -136,6 +136,11 @@ __device__ __forceinline__ bool elect() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
   return ok != 0;
 }
+// One arrival for a warp: 32 lanes that arrive at one barrier are served one after another.
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
 __device__ __forceinline__ void pair_sync(int id) {
   __syncwarp();
   asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
@@ -211,25 +216,25 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) {
-      mbar_init(b_kfull + 8 * i, F::I8 ? F::kConvThreads : 1);
+      mbar_init(b_kfull + 8 * i, F::I8 ? F::kConvThreads / 32 : 1);
       mbar_init(b_kempty + 8 * i, NW);
     }
     for (int i = 0; i < VS; ++i) {
-      mbar_init(b_vfull + 8 * i, F::I8 ? F::kConvThreads : 1);
+      mbar_init(b_vfull + 8 * i, F::I8 ? F::kConvThreads / 32 : 1);
       mbar_init(b_vempty + 8 * i, NW);
     }
     if (F::I8) {
       for (int i = 0; i < RS; ++i) {
         mbar_init(b_rfull + 8 * i, 2);
-        mbar_init(b_rempty + 8 * i, F::kConvThreads);
+        mbar_init(b_rempty + 8 * i, F::kConvThreads / 32);
       }
-      for (int i = 0; i < 4; ++i) mbar_init(b_scale(i), 128);
+      for (int i = 0; i < 4; ++i) mbar_init(b_scale(i), 4);
     }
-    mbar_init(b_q, 512);
+    mbar_init(b_q, 16);
     for (int w = 0; w < 2; ++w) {
       mbar_init(b_sfull(w), 1);
-      mbar_init(b_sfree(w), 256);
-      mbar_init(b_pfull(w), 256);
+      mbar_init(b_sfree(w), 8);
+      mbar_init(b_pfull(w), 8);
       mbar_init(b_odone(w), 1);
     }
     mbar_fence_init();
@@ -489,7 +494,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             *reinterpret_cast<uint4*>(gen + w * (BQ * NDK * 128) + ((c0 + c) >> 3) * (BQ * 128) + r * 128 + ((((c0 + c) & 7) ^ (r & 7)) << 4)) = x[c];
           fence_proxy_async_smem();
         }
-        mbar_arrive(b_q);
+        warp_arrive(b_q);
       }
       wait(b_q, seg & 1);      // (all threads are done with the segment before)
       ++seg;
@@ -509,9 +514,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         wait(b_sfull(w), j & 1);
         if (F::I8) wait(b_scale(g), (g >> 2) & 1);
         if (!warp_ok) {      // rows of nobody: the products take what is there
-          mbar_arrive(b_sfree(w));
+          warp_arrive(b_sfree(w));
           if (i != i0) wait(b_odone(w), (j - 1) & 1);
-          mbar_arrive(b_pfull(w));
+          warp_arrive(b_pfull(w));
           continue;
         }
         tc_fence_after();
@@ -527,7 +532,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         const bool whole_tile = __all_sync(0xffffffffu, vis == 0xffffffffu);
         tmem_ld_wait();
         tc_fence_before();
-        mbar_arrive(b_sfree(w));
+        warp_arrive(b_sfree(w));
         const float* sc = s_scale + (g & 3) * (2 * BK) + half * 32;
         if constexpr (F::I8) {
 #pragma unroll
@@ -569,6 +574,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         asm("mov.b64 %0, {%1, %1};" : "=l"(sc2) : "f"(factor));
         asm("mov.b64 %0, {%1, %1};" : "=l"(nm2) : "f"(nm));
         uint32_t pk[16];
+        ulonglong2 vsc = {0, 0};
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
           unsigned long long xy;
@@ -584,8 +590,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           if (c & 1) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc1) : "l"(ee));
           else asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc0) : "l"(ee));
           if constexpr (F::I8) {
-            const unsigned long long f = *reinterpret_cast<const unsigned long long*>(sc + BK + 2 * c);
-            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(ee) : "l"(f));
+            if (!(c & 1)) vsc = *reinterpret_cast<const ulonglong2*>(sc + BK + 2 * c);
+            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(ee) : "l"(c & 1 ? vsc.y : vsc.x));
             asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(ee));
           }
           pk[c] = pack_bf16(e0, e1);
@@ -614,7 +620,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         st_16(t_p(w) + lane_addr + half * 16, pk);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(b_pfull(w));
+        warp_arrive(b_pfull(w));
       }
       // ---- the segment's sums, once its last product is done
       if (i0 < k.count) wait(b_odone(w), (j - 1) & 1);
@@ -698,27 +704,23 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const int ct = tid - F::kConv * 32;
     bool ok = true;
     int g = 0;
+    // Eight threads in a row take four pieces of a key's half (64 dims) and four of the other half of the next key: their loads, and their stores
+    // to the swizzled tile, meet eight different groups of banks.  The second round takes the other halves.
+    const int cl = ct & 3, odd = (ct >> 2) & 1, row = 2 * (ct >> 3) + odd;
+    const uint32_t src0 = row * D + (NDK == 2 ? odd * 64 : 0) + cl * 16, dst0 = (NDK == 2 ? odd * (BK * 128) : 0) + row * 128 + (((2 * cl) ^ (row & 7)) << 4);
     auto expand = [&](uint32_t src, uint32_t dst) {
 #pragma unroll
-      for (int u = 0; u < BK * D / 16 / F::kConvThreads; ++u) {
-        const int x = ct + F::kConvThreads * u, row = x / (D / 16), c = x % (D / 16);
+      for (int u = 0; u < NDK; ++u) {
         uint32_t ww[4], o[8];
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ww[0]), "=r"(ww[1]), "=r"(ww[2]), "=r"(ww[3]) : "r"(src + x * 16));
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ww[0]), "=r"(ww[1]), "=r"(ww[2]), "=r"(ww[3]) : "r"(src + (src0 ^ (u * 64))));
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
           o[2 * y] = bytes_bf16(ww[y]);
           o[2 * y + 1] = bytes_bf16(ww[y] >> 8);
         }
-        // (the second 64 dims' pieces go the other way round, so that eight threads' stores meet eight banks of 16 bytes)
-        const uint32_t to = dst + (c >> 2) * (BK * 128) + row * 128;
-        const int c0 = (2 * c) & 7, turn = (c >> 2) & 1;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int y = e ^ turn;
-          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to + (((c0 + y) ^ (row & 7)) << 4)), "r"(y ? o[4] : o[0]), "r"(y ? o[5] : o[1]), "r"(y ? o[6] : o[2]),
-                       "r"(y ? o[7] : o[3])
-                       : "memory");
-        }
+        const uint32_t to = dst + (dst0 ^ (u * (BK * 128)));
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to ^ 16), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
       }
       fence_proxy_async_smem();
     };
@@ -734,15 +736,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (ct < 2 * BK) {
           const float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + ct * 4);
           s_scale[(g & 3) * (2 * BK) + ct] = (ct & (BK - 1)) >= keys_of(k.ts + i) ? 0.f : ct < BK ? f * p.scale_log2 : f;
-          mbar_arrive(b_scale(g));
+          warp_arrive(b_scale(g));
         }
         expand(st, k_s0 + ks * F::T_BYTES);
-        mbar_arrive(b_kfull + 8 * ks);
+        warp_arrive(b_kfull + 8 * ks);
         if (g >= VS) ok = warp_wait(b_vempty + 8 * vs, ((g / VS) & 1) ^ 1);
         if (!ok) break;
         expand(st + BK * D, v_s0 + vs * F::T_BYTES);
-        mbar_arrive(b_vfull + 8 * vs);
-        mbar_arrive(b_rempty + 8 * rs);
+        warp_arrive(b_vfull + 8 * vs);
+        warp_arrive(b_rempty + 8 * rs);
       }
   }
   __syncwarp();

@@ -307,6 +307,14 @@ def test_attention(name, heads, i8):
 
 @gpu
 @pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("heads,nodes", [((8, 8, 128), 13), ((32, 8, 128), 64), ((8, 8, 64), 30), ((40, 8, 64), 64), ((64, 4, 128), 40)])
+def test_attention_long_parts(heads, nodes, i8):
+    """Tens of tiles to a CTA, of several requests: rings go round, segments end in them, requests of a few tiles lie between long ones."""
+    run_attention(State([9000, 40, 5003, 64, 0, 8200, 700, 6111], [nodes, 1, nodes // 2, nodes, 3, nodes, nodes, 5]), heads, i8)
+
+
+@gpu
+@pytest.mark.parametrize("i8", [False, True])
 @pytest.mark.parametrize("window", [1, 2, 15, 64, 100, 100000])
 def test_attention_window(window, i8):
     run_attention(State([0, 3, 64, 777, 130], [5, 20, 64, 9, 1], spread=2), (8, 2, 128), i8, window)
