@@ -13,8 +13,9 @@
 // begins and ends inside a request as a rule: what it has of one is a segment.  A segment that is all of a request's key head writes results;
 // the others leave unnormalised sums against their running maximum, and a second kernel adds them up in the order of the keys.
 //
-// A CTA: two threads copy (tiled TMA, 16 keys x 64 dims a box, 128-byte swizzle; pages behind the end are asked for outside the tensor and
-// come as zeros); two threads issue products and two groups of 256 threads do softmax, two threads to a query row of which each has 32 of a
+// A CTA: two warps copy (tiled TMA, 16 keys x 64 dims a box, 128-byte swizzle; pages behind the end are asked for outside the tensor and
+// come as zeros), one issues the products for scores and one those of P V, each waiting for a ring's places in their order (a parity wait that could be
+// more than one phase ahead would return at once); two groups of 256 threads do softmax, two threads to a query row of which each has 32 of a
 // tile's 64 keys.  Scores come from tensor memory into registers once, and their place is free for the next ones; P goes back to tensor memory
 // as the A operand of P V; the accumulator is rescaled only where a row's maximum grew by more than 2^6.
 //   up to 128 query rows (NW 1): both groups have the same rows and take every other tile, each with its own maxima, sums and accumulator, which
@@ -54,7 +55,7 @@ struct Form {
   static constexpr int NDK = NDK_, NW = NW_, D = NDK_ * 64;
   static constexpr bool I8 = I8_;
   static constexpr int T_BYTES = BK * NDK * 128;                 // a K or V tile: [64-dim blocks][64 keys][128 bytes]
-  static constexpr int KS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 6 : 4) * (3 - NDK_), VS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 6 : 5) * (3 - NDK_);     // operand tiles
+  static constexpr int KS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 6 : 4) * (3 - NDK_), VS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 7 : 5) * (3 - NDK_);     // operand tiles
   static constexpr int RS = I8_ ? 5 * (3 - NDK_) : 0;                                                     // stages of bytes
   static constexpr int S_BYTES = 2 * BK * D + 2 * BK * 4;        // keys, values, their scales
   static constexpr int Q_BYTES = NW == 1 ? 0 : NW * BQ * NDK * 128;
@@ -62,10 +63,6 @@ struct Form {
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + KS * T_BYTES, OFF_ST = OFF_V + VS * T_BYTES, OFF_SC = OFF_ST + RS * S_BYTES,
                        OFF_X = OFF_SC + (I8_ ? 4 * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * 2 * BQ * 4, OFF_BAR = OFF_CUM + (kMaxReq + 8) * 4,
                        SMEM = OFF_BAR + 1024 + 1024;
-  // Copies end in any order.  Where the groups take every other tile, a place's tiles have to be one group's: at a place of both, the group that is
-  // ahead would wait for a phase while the one before it is still open, and a parity says no more than that the one before that is over.  (The 8-bit
-  // form's places are filled in order.)
-  static_assert(I8_ || NW_ == 2 || (KS % 2 == 0 && VS % 2 == 0), "places of one group");
   static_assert(SMEM <= 227 * 1024 && KS <= 14 && VS <= 14 && RS <= 14, "shared memory");
 };
 
@@ -123,11 +120,6 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) {
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, ok != 0) || warp_wait_long(bar, parity);
 }
-__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {      // a look that never waits
-  uint32_t ok;
-  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-  return ok != 0;
-}
 // One lane of a warp that is together.  The issuing warps stay together around it, with every operand the same in all lanes, so that operands are
 // in uniform registers: a lone lane pays for moving each of them there.
 __device__ __forceinline__ bool elect() {
@@ -146,11 +138,15 @@ __device__ __forceinline__ void pair_sync(int id) {
   asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
 }
 
-__device__ __forceinline__ uint32_t bytes_bf16(uint32_t w) {      // even bytes as integers in bf16: 128 + (b & 127) less 128, or 256 where the sign is set
-  uint32_t lo = (w & 0x007f007fu) | 0x43004300u, hi = (w & 0x00800080u) | 0x43004300u, d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(lo), "r"(hi));
+// Four bytes, their sign bits turned over (u = b + 128), as bf16 pairs b / 64: up to 255 the bits of a bf16 are an integer times 2^-133 (subnormal
+// or not), so one multiply-add makes u 2^-133 2^127 - 2 = (u - 128) / 64.  Three logic instructions a word; the logic pipe is what the expansion of
+// an 8-bit cache is bound by (with a mantissa trick for either sign, nine: 404 cycles for 8 KB, more than their way from HBM).
+__device__ __forceinline__ uint32_t scaled_bf16(uint32_t pair) {
+  uint32_t d;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(pair), "r"(0x7f007f00u), "r"(0xc000c000u));
   return d;
 }
+constexpr float kByteScale = 64.f;      // what the scales make good
 
 // A request as the roles see it.
 struct Req {
@@ -217,11 +213,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) {
       mbar_init(b_kfull + 8 * i, F::I8 ? F::kConvThreads / 32 : 1);
-      mbar_init(b_kempty + 8 * i, NW);
+      mbar_init(b_kempty + 8 * i, 1);
     }
     for (int i = 0; i < VS; ++i) {
       mbar_init(b_vfull + 8 * i, F::I8 ? F::kConvThreads / 32 : 1);
-      mbar_init(b_vempty + 8 * i, NW);
+      mbar_init(b_vempty + 8 * i, 1);
     }
     if (F::I8) {
       for (int i = 0; i < RS; ++i) {
@@ -374,52 +370,55 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (!ok)      // copies in flight end before the CTA does
       for (int i = max(0, g - kd); i < g; ++i) warp_wait_inline(full0 + 8 * (i % kd), (i / kd) & 1);
-  } else if (warp < F::kSoft) {
-    // ---------------------------------------------------------- products of group w
-    const int w = warp - F::kMma;
+  } else if (warp == F::kMma) {
+    // ---------------------------------------------------------- scores: S = Q K^T of every tile, as its keys come and its group's place is free
     constexpr uint32_t idesc_qk = make_idesc(1, 1, BQ, BK);
-    constexpr uint32_t idesc_pv = make_idesc(1, 1, BQ, D) | (1u << 16);      // V is MN-major
-    const uint32_t hi_k = (uint32_t)(make_desc_sw128(0) >> 32), hi_v = (uint32_t)(make_desc_v(0) >> 32);
-    const uint32_t ql = (uint32_t)make_desc_sw128(q_s + w * (BQ * NDK * 128)), k_lo = (uint32_t)make_desc_sw128(k_s0), v_lo = (uint32_t)make_desc_v(v_s0);
-    bool ok = true, live = true;
-    int g0 = 0, j = 0, seg = 0, last = -1;      // tiles of all segments before, this group's tiles so far, the last one
-    auto wait = [&](uint32_t bar, uint32_t parity) { return warp_wait_inline(bar, parity); };
-    auto issue_qk = [&](int g, int jj) -> bool {
-      const int ks = g % KS;
-      if (!wait(b_kfull + 8 * ks, (g / KS) & 1)) return false;
-      if (jj >= 1 && !wait(b_sfree(w), (jj - 1) & 1)) return false;      // the scores before are in registers
-      tc_fence_after();
-      const uint32_t kl = k_lo + ks * (F::T_BYTES >> 4);
-      if (elect()) {
-        if (live) {
-#pragma unroll
-          for (int x = 0; x < 4 * NDK; ++x) {
-            const uint32_t kx = kl + (((x >> 2) * (BK * 128) + (x & 3) * 32) >> 4);
-            if constexpr (NW == 1) umma_f16_ts_w(t_s(w), t_q + 8 * x, kx, hi_k, idesc_qk, x != 0);
-            else umma_f16_w(t_s(w), ql + (((x >> 2) * (BQ * 128) + (x & 3) * 32) >> 4), hi_k, kx, hi_k, idesc_qk, x != 0);
-          }
-        }
-        tc_commit(b_sfull(w));
-        tc_commit(b_kempty + 8 * ks);
-      }
-      __syncwarp();
-      return true;
-    };
+    const uint32_t hi_k = (uint32_t)(make_desc_sw128(0) >> 32);
+    const uint32_t q_lo = (uint32_t)make_desc_sw128(q_s), k_lo = (uint32_t)make_desc_sw128(k_s0);
+    bool ok = true;
+    int g = 0, seg = 0, ks = 0, par = 0, j[2] = {0, 0};      // tiles so far, of all and of either group
     while (ok && next_segment<F>(p, s_cum, k)) {
-      live = NW == 1 || w * BQ < k.tok * p.gqa;      // (a second query tile without rows only hands tiles back)
-      const int i0 = NW == 1 ? (w - g0) & 1 : 0;
-      ok = wait(b_q, seg & 1);
-      if (ok && i0 < k.count) ok = issue_qk(g0 + i0, j);
-      for (int i = i0; i < k.count && ok; i += kStep, ++j) {
-        const int g = g0 + i, vs = g % VS, valid = keys_of(k.ts + i);
-        // the next scores first, if their keys are here; else not before this tile's product, which their place may be waiting for
-        const bool more = i + kStep < k.count;
-        const bool ahead = more && __all_sync(0xffffffffu, mbar_test(b_kfull + 8 * ((g + kStep) % KS), ((g + kStep) / KS) & 1));
-        if (ahead) ok = issue_qk(g + kStep, j + 1);
-        if (ok) ok = wait(b_pfull(w), j & 1);
-        if (ok) ok = wait(b_vfull + 8 * vs, (g / VS) & 1);
-        if (!ok) break;
-        if (!F::I8 && (valid & 15) != 0) {
+      ok = warp_wait_inline(b_q, seg & 1);
+      for (int i = 0; i < k.count && ok; ++i, ++g) {
+        ok = warp_wait_inline(b_kfull + 8 * ks, par);
+        const uint32_t kl = k_lo + ks * (F::T_BYTES >> 4);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (NW == 1 && w != (g & 1)) continue;
+          if (ok && j[w] >= 1) ok = warp_wait_inline(b_sfree(w), (j[w] - 1) & 1);      // the scores before are in registers
+          if (!ok) break;
+          ++j[w];
+          const bool live = NW == 1 || w * BQ < k.tok * p.gqa;      // (a second query tile without rows only hands tiles back)
+          tc_fence_after();
+          if (elect()) {
+            if (live) {
+#pragma unroll
+              for (int x = 0; x < 4 * NDK; ++x) {
+                const uint32_t kx = kl + (((x >> 2) * (BK * 128) + (x & 3) * 32) >> 4);
+                if constexpr (NW == 1) umma_f16_ts_w(t_s(w), t_q + 8 * x, kx, hi_k, idesc_qk, x != 0);
+                else umma_f16_w(t_s(w), q_lo + ((w * (BQ * NDK * 128) + (x >> 2) * (BQ * 128) + (x & 3) * 32) >> 4), hi_k, kx, hi_k, idesc_qk, x != 0);
+              }
+            }
+            tc_commit(b_sfull(w));
+            if (NW == 1 || w == 1) tc_commit(b_kempty + 8 * ks);
+          }
+          __syncwarp();
+        }
+        if (++ks == KS) { ks = 0; par ^= 1; }
+      }
+      ++seg;
+    }
+  } else if (warp < F::kSoft) {
+    // ---------------------------------------------------------- results: O += P V
+    constexpr uint32_t idesc_pv = make_idesc(1, 1, BQ, D) | (1u << 16);      // V is MN-major
+    const uint32_t hi_v = (uint32_t)(make_desc_v(0) >> 32), v_lo = (uint32_t)make_desc_v(v_s0);
+    bool ok = true;
+    int g = 0, vs = 0, par = 0, j[2] = {0, 0};
+    while (ok && next_segment<F>(p, s_cum, k)) {
+      for (int i = 0; i < k.count && ok; ++i, ++g) {
+        const int valid = keys_of(k.ts + i);
+        ok = warp_wait_inline(b_vfull + 8 * vs, par);
+        if (!F::I8 && ok && (valid & 15) != 0) {
           // values behind the last key's are anything: their weights are 0, but 0 x infinity is not
           const int end = (valid + 15) & ~15;
           for (int x = lane; x < (end - valid) * NDK * 8; x += 32) {
@@ -429,26 +428,32 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           fence_proxy_async_smem();
           __syncwarp();
         }
-        tc_fence_after();
         const uint32_t vl = v_lo + vs * (F::T_BYTES >> 4);
-        if (elect()) {
-          if (live) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x)      // 16 keys a step; P in tensor memory, 8 columns of pairs
-              umma_f16_ts_w(t_o(w), t_p(w) + 8 * x, vl + ((x * 16 * 128) >> 4), hi_v, idesc_pv, i != i0 || x != 0);
+        for (int w = 0; w < 2; ++w) {
+          if (NW == 1 && w != (g & 1)) continue;
+          if (ok) ok = warp_wait_inline(b_pfull(w), j[w] & 1);
+          if (!ok) break;
+          ++j[w];
+          const bool live = NW == 1 || w * BQ < k.tok * p.gqa;
+          const bool first = i < kStep;      // the group's first tile of the segment
+          tc_fence_after();
+          if (elect()) {
+            if (live) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x)      // 16 keys a step; P in tensor memory, 8 columns of pairs
+                umma_f16_ts_w(t_o(w), t_p(w) + 8 * x, vl + ((x * 16 * 128) >> 4), hi_v, idesc_pv, !first || x != 0);
+            }
+            tc_commit(b_odone(w));
+            if (NW == 1 || w == 1) tc_commit(b_vempty + 8 * vs);
           }
-          tc_commit(b_odone(w));
-          tc_commit(b_vempty + 8 * vs);
+          __syncwarp();
         }
-        __syncwarp();
-        if (more && !ahead) ok = issue_qk(g + kStep, j + 1);
-        last = g;
+        if (++vs == VS) { vs = 0; par ^= 1; }
       }
-      g0 += k.count;
-      ++seg;
     }
     // the last arrival that a product makes: none is on its way when the CTA ends
-    if (ok && last >= 0) wait(b_vempty + 8 * (last % VS), (last / VS) & 1);
+    if (ok && g > 0) warp_wait_inline(b_vempty + 8 * ((g - 1) % VS), ((g - 1) / VS) & 1);
   } else if (warp < F::kConv) {
     // ---------------------------------------------------------- softmax: two threads per query row of group w
     constexpr float kLazy = 6.f;
@@ -715,8 +720,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ww[0]), "=r"(ww[1]), "=r"(ww[2]), "=r"(ww[3]) : "r"(src + (src0 ^ (u * 64))));
 #pragma unroll
         for (int y = 0; y < 4; ++y) {
-          o[2 * y] = bytes_bf16(ww[y]);
-          o[2 * y + 1] = bytes_bf16(ww[y] >> 8);
+          const uint32_t x = ww[y] ^ 0x80808080u;
+          o[2 * y] = scaled_bf16(x & 0x00ff00ffu);
+          o[2 * y + 1] = scaled_bf16(__byte_perm(x, 0u, 0x4341));
         }
         const uint32_t to = dst + (dst0 ^ (u * (BK * 128)));
         asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
@@ -735,7 +741,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         // g - 1 - VS, the same group's or a later one's.  Behind the last key they are anything, and made 0: what a place holds that nobody sees must not reach a sum.
         if (ct < 2 * BK) {
           const float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + ct * 4);
-          s_scale[(g & 3) * (2 * BK) + ct] = (ct & (BK - 1)) >= keys_of(k.ts + i) ? 0.f : ct < BK ? f * p.scale_log2 : f;
+          s_scale[(g & 3) * (2 * BK) + ct] = (ct & (BK - 1)) >= keys_of(k.ts + i) ? 0.f : f * (ct < BK ? p.scale_log2 * kByteScale : kByteScale);
           warp_arrive(b_scale(g));
         }
         expand(st, k_s0 + ks * F::T_BYTES);
@@ -776,35 +782,39 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p,
   const int c0 = (int)(a / each), c1 = (int)((e - 1) / each);
   if (c0 == c1) return;      // one segment: its CTA wrote the result
   auto slot = [&](int c) { return (((size_t)z * columns + c) * 2 + (a > c * each)) * slot_rows + rr; };
-  float best = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) best = fmaxf(best, p.part_ml[slot(c) * 2]);
-  best = warp_max(best);
-  float sum = 0.f, acc[E] = {};
-  for (int c = c0; c <= c1; c += 32) {
-    float f = 0.f;
-    if (c + lane <= c1) {
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(c + lane) * 2);
-      f = ml.x == -INFINITY ? 0.f : exp2f(ml.x - best);
-      sum += f * ml.y;
-    }
-    const int n = min(32, c1 - c + 1);
-    for (int j = 0; j < n; j += 8) {
-      float x[8][E];
+  // four segments at a time, their sums and their maxima on the way together; rescaled as the running maximum grows
+  constexpr int U = 4;
+  float best = -INFINITY, sum = 0.f, acc[E] = {};
+  for (int c = c0; c <= c1; c += U) {
+    float x[U][E];
+    float2 ml[U];
 #pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        const float* src = p.part_o + slot(min(c + j + y, c1)) * D + lane * E;
+    for (int y = 0; y < U; ++y) {
+      ml[y] = make_float2(-INFINITY, 0.f);
+      if (c + y <= c1) {
+        const size_t at = slot(c + y);
+        ml[y] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+        const float* src = p.part_o + at * D + lane * E;
         if constexpr (E == 4) *reinterpret_cast<float4*>(x[y]) = *reinterpret_cast<const float4*>(src);
         else *reinterpret_cast<float2*>(x[y]) = *reinterpret_cast<const float2*>(src);
       }
+    }
+    float m = best;
 #pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        const float fy = __shfl_sync(0xffffffffu, f, (j + y) & 31);
+    for (int y = 0; y < U; ++y) m = fmaxf(m, ml[y].x);
+    const float old = best == -INFINITY ? 0.f : exp2f(best - m);
+    best = m;
+    sum *= old;
 #pragma unroll
-        for (int d = 0; d < E; ++d) acc[d] += j + y < n && fy > 0.f ? fy * x[y][d] : 0.f;
-      }
+    for (int d = 0; d < E; ++d) acc[d] *= old;
+#pragma unroll
+    for (int y = 0; y < U; ++y) {
+      const float f = ml[y].x == -INFINITY ? 0.f : exp2f(ml[y].x - best);
+      sum += f * ml[y].y;
+#pragma unroll
+      for (int d = 0; d < E; ++d) acc[d] += f > 0.f ? f * x[y][d] : 0.f;
     }
   }
-  sum = warp_sum(sum);
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   __nv_bfloat16* dst = p.out + row * p.ldo + head * D + lane * E;
   if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
