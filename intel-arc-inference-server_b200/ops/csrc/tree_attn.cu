@@ -33,6 +33,7 @@ namespace {
 
 constexpr int kPage = kTreePage, kMaxNodes = kTreeNodes, kMaxReq = kTreeRequests;
 constexpr int BQ = 128, BK = 64;
+constexpr int kScales = 8;       // tiles whose scales are kept
 
 struct TreeAttnParams {
   const __nv_bfloat16* q;
@@ -61,7 +62,7 @@ struct Form {
   static constexpr int Q_BYTES = NW == 1 ? 0 : NW * BQ * NDK * 128;
   static constexpr int kMma = 2, kSoft = 4, kConv = kSoft + 16, kConvThreads = 256, kWarps = kConv + (I8_ ? kConvThreads / 32 : 0), kThreads = kWarps * 32;
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + KS * T_BYTES, OFF_ST = OFF_V + VS * T_BYTES, OFF_SC = OFF_ST + RS * S_BYTES,
-                       OFF_X = OFF_SC + (I8_ ? 4 * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * 2 * BQ * 4, OFF_BAR = OFF_CUM + (kMaxReq + 8) * 4,
+                       OFF_X = OFF_SC + (I8_ ? kScales * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * 2 * BQ * 4, OFF_BAR = OFF_CUM + (kMaxReq + 8) * 4,
                        SMEM = OFF_BAR + 1024 + 1024;
   static_assert(SMEM <= 227 * 1024 && KS <= 14 && VS <= 14 && RS <= 14, "shared memory");
 };
@@ -198,25 +199,25 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t q_s = base, k_s0 = base + F::OFF_K, v_s0 = base + F::OFF_V, st_s0 = base + F::OFF_ST, bars = base + F::OFF_BAR;
   int* const s_cum = reinterpret_cast<int*>(gen + F::OFF_CUM);
-  float* const s_scale = reinterpret_cast<float*>(gen + F::OFF_SC);       // [4][K, V][64]
+  float* const s_scale = reinterpret_cast<float*>(gen + F::OFF_SC);       // [kScales][K, V][64]
   float* const s_x = reinterpret_cast<float*>(gen + F::OFF_X);            // [group][parity][half][128]
   const uint32_t b_kfull = bars, b_kempty = bars + 112, b_vfull = bars + 224, b_vempty = bars + 336, b_rfull = bars + 448, b_rempty = bars + 560, b_q = bars + 672;
   auto b_sfull = [&](int w) { return bars + 680 + w * 8; };
   auto b_sfree = [&](int w) { return bars + 696 + w * 8; };
   auto b_pfull = [&](int w) { return bars + 712 + w * 8; };
   auto b_odone = [&](int w) { return bars + 728 + w * 8; };
-  auto b_scale = [&](int g) { return bars + 744 + (g & 3) * 8; };
-  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gen + F::OFF_BAR + 776);
-  int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 784);      // [warps]
+  auto b_scale = [&](int g) { return bars + 744 + (g % kScales) * 8; };
+  uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gen + F::OFF_BAR + 808);
+  int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 816);      // [warps]
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) {
-      mbar_init(b_kfull + 8 * i, F::I8 ? F::kConvThreads / 32 : 1);
+      mbar_init(b_kfull + 8 * i, F::I8 ? F::kConvThreads / 64 : 1);
       mbar_init(b_kempty + 8 * i, 1);
     }
     for (int i = 0; i < VS; ++i) {
-      mbar_init(b_vfull + 8 * i, F::I8 ? F::kConvThreads / 32 : 1);
+      mbar_init(b_vfull + 8 * i, F::I8 ? F::kConvThreads / 64 : 1);
       mbar_init(b_vempty + 8 * i, 1);
     }
     if (F::I8) {
@@ -224,7 +225,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         mbar_init(b_rfull + 8 * i, 2);
         mbar_init(b_rempty + 8 * i, F::kConvThreads / 32);
       }
-      for (int i = 0; i < 4; ++i) mbar_init(b_scale(i), 4);
+      for (int i = 0; i < kScales; ++i) mbar_init(b_scale(i), 4);
     }
     mbar_init(b_q, 16);
     for (int w = 0; w < 2; ++w) {
@@ -517,7 +518,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       for (int i = i0; i < k.count; i += kStep, ++j) {
         const int g = g0 + i, t = k.ts + i;
         wait(b_sfull(w), j & 1);
-        if (F::I8) wait(b_scale(g), (g >> 2) & 1);
+        if (F::I8) wait(b_scale(g), (g / kScales) & 1);
         if (!warp_ok) {      // rows of nobody: the products take what is there
           warp_arrive(b_sfree(w));
           if (i != i0) wait(b_odone(w), (j - 1) & 1);
@@ -538,7 +539,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         tmem_ld_wait();
         tc_fence_before();
         warp_arrive(b_sfree(w));
-        const float* sc = s_scale + (g & 3) * (2 * BK) + half * 32;
+        const float* sc = s_scale + (g % kScales) * (2 * BK) + half * 32;
         if constexpr (F::I8) {
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
@@ -705,52 +706,53 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       g0 += k.count;
     }
   } else if constexpr (F::I8) {
-    // ---------------------------------------------------------- bytes to integers in bf16: a thread's piece is 16 bytes of a key
-    const int ct = tid - F::kConv * 32;
-    bool ok = true;
-    int g = 0;
+    // ---------------------------------------------------------- bytes to bf16: four warps for keys, four for values; a thread's piece is 16 bytes of a key
+    const int ct = (tid - F::kConv * 32) & 127;
+    const bool is_v = warp >= F::kConv + 4;
     // Eight threads in a row take four pieces of a key's half (64 dims) and four of the other half of the next key: their loads, and their stores
     // to the swizzled tile, meet eight different groups of banks.  The second round takes the other halves.
     const int cl = ct & 3, odd = (ct >> 2) & 1, row = 2 * (ct >> 3) + odd;
     const uint32_t src0 = row * D + (NDK == 2 ? odd * 64 : 0) + cl * 16, dst0 = (NDK == 2 ? odd * (BK * 128) : 0) + row * 128 + (((2 * cl) ^ (row & 7)) << 4);
-    auto expand = [&](uint32_t src, uint32_t dst) {
-#pragma unroll
-      for (int u = 0; u < NDK; ++u) {
-        uint32_t ww[4], o[8];
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ww[0]), "=r"(ww[1]), "=r"(ww[2]), "=r"(ww[3]) : "r"(src + (src0 ^ (u * 64))));
-#pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const uint32_t x = ww[y] ^ 0x80808080u;
-          o[2 * y] = scaled_bf16(x & 0x00ff00ffu);
-          o[2 * y + 1] = scaled_bf16(__byte_perm(x, 0u, 0x4341));
-        }
-        const uint32_t to = dst + (dst0 ^ (u * (BK * 128)));
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
-        asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to ^ 16), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
-      }
-      fence_proxy_async_smem();
-    };
+    const uint32_t full0 = is_v ? b_vfull : b_kfull, empty0 = is_v ? b_vempty : b_kempty, tile0 = is_v ? v_s0 : k_s0;
+    constexpr int PL = F::KS;
+    static_assert(!F::I8 || F::KS == F::VS, "places of keys and values");
+    bool ok = true;
+    int g = 0, rs = 0, rpar = 0, ps = 0, ppar = 1;
     while (ok && next_segment<F>(p, s_cum, k))
       for (int i = 0; i < k.count; ++i, ++g) {
-        const int rs = g % RS, ks = g % KS, vs = g % VS;
-        const uint32_t st = st_s0 + rs * F::S_BYTES;
-        ok = warp_wait(b_rfull + 8 * rs, (g / RS) & 1);
-        if (ok && g >= KS) ok = warp_wait(b_kempty + 8 * ks, ((g / KS) & 1) ^ 1);
+        const uint32_t st = st_s0 + rs * F::S_BYTES + (is_v ? BK * D : 0), dst = tile0 + ps * F::T_BYTES;
+        ok = warp_wait(b_rfull + 8 * rs, rpar);
+        if (ok && g >= PL) ok = warp_wait(empty0 + 8 * ps, ppar);
         if (!ok) break;
-        // the scales of tile g - 4 are read: the places of the values of tiles g - 2 and g - 1 came free with the products of tiles g - 2 - VS and
-        // g - 1 - VS, the same group's or a later one's.  Behind the last key they are anything, and made 0: what a place holds that nobody sees must not reach a sum.
-        if (ct < 2 * BK) {
-          const float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + ct * 4);
-          s_scale[(g & 3) * (2 * BK) + ct] = (ct & (BK - 1)) >= keys_of(k.ts + i) ? 0.f : f * (ct < BK ? p.scale_log2 * kByteScale : kByteScale);
+        // the scales of tile g - kScales are read: this place came free with a product of tile g - PL, and those of a tile's scores wait for the
+        // scores of the group's tile before to be in registers.  Behind the last key scales are anything, and made 0: what a place holds that nobody sees must
+        // not reach a sum.
+        static_assert(kScales >= F::KS + 4, "scales of tiles under way");
+        if (ct < BK) {
+          const float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + (is_v ? BK * 4 : 0) + ct * 4);
+          s_scale[(g % kScales) * (2 * BK) + (is_v ? BK : 0) + ct] = ct >= keys_of(k.ts + i) ? 0.f : f * (is_v ? kByteScale : p.scale_log2 * kByteScale);
           warp_arrive(b_scale(g));
         }
-        expand(st, k_s0 + ks * F::T_BYTES);
-        warp_arrive(b_kfull + 8 * ks);
-        if (g >= VS) ok = warp_wait(b_vempty + 8 * vs, ((g / VS) & 1) ^ 1);
-        if (!ok) break;
-        expand(st + BK * D, v_s0 + vs * F::T_BYTES);
-        warp_arrive(b_vfull + 8 * vs);
+#pragma unroll
+        for (int u = 0; u < 2 * NDK; ++u) {      // two halves of rows 0 to 31, of rows 32 to 63
+          const int up = u & (NDK - 1), low = u / NDK;
+          uint32_t ww[4], o[8];
+          asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(ww[0]), "=r"(ww[1]), "=r"(ww[2]), "=r"(ww[3]) : "r"(st + (src0 ^ (up * 64)) + low * (32 * D)));
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            const uint32_t x = ww[y] ^ 0x80808080u;
+            o[2 * y] = scaled_bf16(x & 0x00ff00ffu);
+            o[2 * y + 1] = scaled_bf16(__byte_perm(x, 0u, 0x4341));
+          }
+          const uint32_t to = dst + (dst0 ^ (up * (BK * 128))) + low * (32 * 128);
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to ^ 16), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]) : "memory");
+        }
+        fence_proxy_async_smem();
+        warp_arrive(full0 + 8 * ps);
         warp_arrive(b_rempty + 8 * rs);
+        if (++rs == RS) { rs = 0; rpar ^= 1; }
+        if (++ps == PL) { ps = 0; ppar ^= 1; }
       }
   }
   __syncwarp();
