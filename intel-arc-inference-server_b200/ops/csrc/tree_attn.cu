@@ -34,6 +34,7 @@ namespace {
 constexpr int kPage = kTreePage, kMaxNodes = kTreeNodes, kMaxReq = kTreeRequests;
 constexpr int BQ = 128, BK = 64;
 constexpr int kScales = 8;       // tiles whose scales are kept
+constexpr int kKept = 256;       // requests whose lengths and rows are kept in shared memory
 
 struct TreeAttnParams {
   const __nv_bfloat16* q;
@@ -47,8 +48,8 @@ struct TreeAttnParams {
   float scale_log2;
   __nv_bfloat16* out;
   long long ldo;
-  float *part_o, *part_ml;         // [group][column][2][NW x 128 rows][D], and maximum and sum
-  int* sched;                      // tiles a column, then the requests' first tiles (of one key head)
+  float *part_o, *part_ml;         // [group][column][2][D / 4][NW x 128 rows][4], and [...][rows] maximum and sum
+  int* sched;                      // places a column, the requests' first places (of one key head), their tiles
 };
 
 template <int NDK_, bool I8_, int NW_>
@@ -57,12 +58,12 @@ struct Form {
   static constexpr bool I8 = I8_;
   static constexpr int T_BYTES = BK * NDK * 128;                 // a K or V tile: [64-dim blocks][64 keys][128 bytes]
   static constexpr int KS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 6 : 4) * (3 - NDK_), VS = I8_ ? (NW_ == 1 ? 3 : 2) : (NW_ == 1 ? 7 : 5) * (3 - NDK_);     // operand tiles
-  static constexpr int RS = I8_ ? 5 * (3 - NDK_) : 0;                                                     // stages of bytes
+  static constexpr int RS = I8_ ? (NW_ == 1 ? 5 : 4) * (3 - NDK_) : 0;                                                     // stages of bytes
   static constexpr int S_BYTES = 2 * BK * D + 2 * BK * 4;        // keys, values, their scales
   static constexpr int Q_BYTES = NW == 1 ? 0 : NW * BQ * NDK * 128;
   static constexpr int kMma = 2, kSoft = 4, kConv = kSoft + 16, kConvThreads = 256, kWarps = kConv + (I8_ ? kConvThreads / 32 : 0), kThreads = kWarps * 32;
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + KS * T_BYTES, OFF_ST = OFF_V + VS * T_BYTES, OFF_SC = OFF_ST + RS * S_BYTES,
-                       OFF_X = OFF_SC + (I8_ ? kScales * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * 2 * BQ * 4, OFF_BAR = OFF_CUM + (kMaxReq + 8) * 4,
+                       OFF_X = OFF_SC + (I8_ ? kScales * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * 2 * BQ * 4, OFF_REQ = OFF_CUM + (kMaxReq + 8) * 4, OFF_BAR = OFF_REQ + 3 * kKept * 4,
                        SMEM = OFF_BAR + 1024 + 1024;
   static_assert(SMEM <= 227 * 1024 && KS <= 14 && VS <= 14 && RS <= 14, "shared memory");
 };
@@ -160,7 +161,7 @@ __device__ __forceinline__ int nodes_of(const TreeAttnParams& p, int b, int& r0)
   return max(0, min(min(p.row_start[b + 1], p.rows) - r0, kMaxNodes));
 }
 
-// The segments of a CTA's part [u, u1) of the line of tiles.
+// The segments of a CTA's part [u, u1) of the line of tiles.  A request's tiles of one key head take s_cum[b + 1] - s_cum[b] places of it.
 struct Walk {
   long long u, u0, u1;
   int b;
@@ -168,22 +169,34 @@ struct Walk {
   int h, ts, count, tok;       // key head, first tile and tiles of the segment, nodes of the CTA's group
 };
 
+// s_req: tiles, cached positions and first row of up to kKept requests
 template <class F>
-__device__ __forceinline__ bool next_segment(const TreeAttnParams& p, const int* s_cum, Walk& k) {
+__device__ __forceinline__ bool next_segment(const TreeAttnParams& p, const int* s_cum, const int* s_req, Walk& k) {
   for (;;) {
     if (k.u >= k.u1) return false;
     while ((long long)s_cum[k.b + 1] * p.n_kv <= k.u) ++k.b;
-    const int nt = s_cum[k.b + 1] - s_cum[k.b];
+    const int places = s_cum[k.b + 1] - s_cum[k.b];
     const long long rel = k.u - (long long)s_cum[k.b] * p.n_kv;
-    k.h = (int)(rel / nt);
-    k.ts = (int)(rel - (long long)k.h * nt);
-    k.count = (int)min((long long)(nt - k.ts), k.u1 - k.u);
-    k.u += k.count;
+    k.h = (int)(rel / places);
+    k.ts = (int)(rel - (long long)k.h * places);
     k.r.b = k.b;
-    k.r.n = nodes_of(p, k.b, k.r.r0);
-    k.r.length = p.lengths[k.b];
+    if (p.B <= kKept) {
+      k.r.length = s_req[kKept + k.b];
+      const int rn = s_req[2 * kKept + k.b];
+      k.r.r0 = rn >> 7;
+      k.r.n = rn & 127;
+    } else {
+      k.r.n = nodes_of(p, k.b, k.r.r0);
+      k.r.length = p.lengths[k.b];
+    }
     k.r.first = first_tile(p, k.r.length);
-    k.r.nt = nt;
+    k.r.nt = (k.r.length + BK - 1) / BK - k.r.first + 1;
+    if (k.ts >= k.r.nt) {      // places behind the last tile
+      k.u += places - k.ts;
+      continue;
+    }
+    k.count = (int)min((long long)(k.r.nt - k.ts), k.u1 - k.u);
+    k.u += k.count;
     k.tok = min(p.group_tokens, k.r.n - (int)blockIdx.y * p.group_tokens);
     if (k.tok > 0) return true;
   }
@@ -199,6 +212,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   uint8_t* const gen = smem_raw + (base - smem_u32(smem_raw));
   const uint32_t q_s = base, k_s0 = base + F::OFF_K, v_s0 = base + F::OFF_V, st_s0 = base + F::OFF_ST, bars = base + F::OFF_BAR;
   int* const s_cum = reinterpret_cast<int*>(gen + F::OFF_CUM);
+  int* const s_req = reinterpret_cast<int*>(gen + F::OFF_REQ);
   float* const s_scale = reinterpret_cast<float*>(gen + F::OFF_SC);       // [kScales][K, V][64]
   float* const s_x = reinterpret_cast<float*>(gen + F::OFF_X);            // [group][parity][half][128]
   const uint32_t b_kfull = bars, b_kempty = bars + 112, b_vfull = bars + 224, b_vempty = bars + 336, b_rfull = bars + 448, b_rempty = bars + 560, b_q = bars + 672;
@@ -208,7 +222,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto b_odone = [&](int w) { return bars + 728 + w * 8; };
   auto b_scale = [&](int g) { return bars + 744 + (g % kScales) * 8; };
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gen + F::OFF_BAR + 808);
-  int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 816);      // [warps]
+  int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 816);      // [32], [8]
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
@@ -256,6 +270,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const int length = p.lengths[b], n = nodes_of(p, b, r0);
       const int nt = n > 0 ? (length + BK - 1) / BK - first_tile(p, length) + 1 : 0;
       s_cum[b + 1] = mine += nt;
+      if (b < kKept) {
+        s_req[b] = nt;
+        s_req[kKept + b] = length;
+        s_req[2 * kKept + b] = r0 << 7 | n;
+      }
     }
     int x = mine;
 #pragma unroll
@@ -281,9 +300,53 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto t_p = [&](int w) { return tmem_base + 192 + (uint32_t)w * 32; };
   auto t_o = [&](int w) { return tmem_base + 256 + (uint32_t)w * D; };
 
-  const long long total = (long long)s_cum[p.B] * p.n_kv, each = (total + gridDim.x - 1) / gridDim.x;
+  long long total = (long long)s_cum[p.B] * p.n_kv, each = (total + gridDim.x - 1) / gridDim.x;
+  // Where there are columns enough for every request's key head, a request's tiles can begin a column: then a CTA has one segment, whose start and
+  // end cost as much as four or five tiles.  Eight column lengths from the least on are looked at, by a warp each; the first that fits is taken.
+  // (One request of 4100 positions, 8 key heads: 66 tiles in 16.5 columns of 4, or 17 of 4.)
+  if (p.B * p.n_kv <= (int)gridDim.x && total > 0) {
+    if (warp < 8) {
+      const int len = (int)each + warp;
+      int sum = 0;
+      for (int b = lane; b < p.B; b += 32) sum += (s_req[b] + len - 1) / len;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) s_sums[32 + warp] = sum;
+    }
+    __syncthreads();
+    int take = -1;
+#pragma unroll
+    for (int c = 7; c >= 0; --c)
+      if (s_sums[32 + c] * p.n_kv <= (int)gridDim.x) take = c;
+    if (take >= 0) {
+      each += take;
+      if (warp == 0) {      // the line again, in whole columns
+        int before = 0;
+        for (int b0 = 0; b0 < p.B; b0 += 32) {
+          const int b = b0 + lane, mine = b < p.B ? (int)((s_req[b] + each - 1) / each * each) : 0;
+          int x = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+          }
+          if (b < p.B) s_cum[b + 1] = before + x;
+          before += __shfl_sync(0xffffffffu, x, 31);
+        }
+      }
+      __syncthreads();
+      total = (long long)s_cum[p.B] * p.n_kv;
+    }
+  }
   if (blockIdx.x == 0 && blockIdx.y == 0) {
-    for (int b = tid; b <= p.B; b += F::kThreads) p.sched[b + 1] = s_cum[b];
+    for (int b = tid; b <= p.B; b += F::kThreads) {
+      p.sched[b + 1] = s_cum[b];
+      if (b < p.B) {
+        int r0;
+        const int length = p.lengths[b];
+        p.sched[p.B + 2 + b] = nodes_of(p, b, r0) > 0 ? (length + BK - 1) / BK - first_tile(p, length) + 1 : 0;
+      }
+    }
     if (tid == 0) p.sched[0] = (int)each;
   }
   Walk k;
@@ -309,7 +372,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const int kd = F::I8 ? RS : is_v ? VS : KS;      // depth of this warp's ring
     const uint32_t full0 = F::I8 ? b_rfull : is_v ? b_vfull : b_kfull, empty0 = F::I8 ? b_rempty : is_v ? b_vempty : b_kempty;
     int s = 0, par = 0;
-    while (ok && next_segment<F>(p, s_cum, k)) {
+    while (ok && next_segment<F>(p, s_cum, s_req, k)) {
       const int limit = min((k.r.length + kPage - 1) / kPage, p.max_blocks), tree_pages = (k.r.n + kPage - 1) / kPage;
       const int* bt = p.block_table + (size_t)k.r.b * p.max_blocks;
       auto entry = [&](int i) {      // (what names no page reads as page 0, which is nobody's; behind the end there is none)
@@ -378,7 +441,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const uint32_t q_lo = (uint32_t)make_desc_sw128(q_s), k_lo = (uint32_t)make_desc_sw128(k_s0);
     bool ok = true;
     int g = 0, seg = 0, ks = 0, par = 0, j[2] = {0, 0};      // tiles so far, of all and of either group
-    while (ok && next_segment<F>(p, s_cum, k)) {
+    while (ok && next_segment<F>(p, s_cum, s_req, k)) {
       ok = warp_wait_inline(b_q, seg & 1);
       for (int i = 0; i < k.count && ok; ++i, ++g) {
         ok = warp_wait_inline(b_kfull + 8 * ks, par);
@@ -415,7 +478,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     const uint32_t hi_v = (uint32_t)(make_desc_v(0) >> 32), v_lo = (uint32_t)make_desc_v(v_s0);
     bool ok = true;
     int g = 0, vs = 0, par = 0, j[2] = {0, 0};
-    while (ok && next_segment<F>(p, s_cum, k)) {
+    while (ok && next_segment<F>(p, s_cum, s_req, k)) {
       for (int i = 0; i < k.count && ok; ++i, ++g) {
         const int valid = keys_of(k.ts + i);
         ok = warp_wait_inline(b_vfull + 8 * vs, par);
@@ -469,7 +532,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       if (ok) ok = warp_wait(bar, parity);
     };
     int g0 = 0, j = 0, seg = 0;
-    while (next_segment<F>(p, s_cum, k)) {
+    while (next_segment<F>(p, s_cum, s_req, k)) {
       const int rr = (NW == 1 ? 0 : w * BQ) + r, live_rows = k.tok * p.gqa;
       const bool row_ok = rr < live_rows, warp_ok = rr - lane < live_rows;
       const int node = blockIdx.y * p.group_tokens + rr / p.gqa, head = k.h * p.gqa + rr % p.gqa, row = k.r.r0 + node;
@@ -662,7 +725,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         constexpr int NC = NW == 1 ? NDK : 2 * NDK;      // pieces of 16 columns that this thread writes: a quarter of the row, or half
         const int c0 = NW == 1 ? (w * 2 + half) * NC * 16 : half * NC * 16;
         __nv_bfloat16* dst = p.out + row * p.ldo + head * D + c0;
-        float* part = p.part_o + slot * D + c0;
+        float* part = p.part_o + (slot - rr) * D + (size_t)(c0 / 4) * (NW * BQ * 4) + rr * 4;      // [D / 4][rows][4]: lanes next to one another
 #pragma unroll 1
         for (int c = 0; c < NC; ++c) {
           uint32_t o[16], o1[16];
@@ -696,7 +759,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
                   pack_bf16(__uint_as_float(o[8 * e + 4]), __uint_as_float(o[8 * e + 5])), pack_bf16(__uint_as_float(o[8 * e + 6]), __uint_as_float(o[8 * e + 7])));
           } else if (row_ok) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(part + c * 16 + 4 * e) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(part + (size_t)(c * 4 + e) * (NW * BQ * 4)) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
         if (!whole && row_ok && half == 0 && (NW == 2 || w == 0)) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(best, sum);
@@ -718,7 +781,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     static_assert(!F::I8 || F::KS == F::VS, "places of keys and values");
     bool ok = true;
     int g = 0, rs = 0, rpar = 0, ps = 0, ppar = 1;
-    while (ok && next_segment<F>(p, s_cum, k))
+    while (ok && next_segment<F>(p, s_cum, s_req, k))
       for (int i = 0; i < k.count; ++i, ++g) {
         const uint32_t st = st_s0 + rs * F::S_BYTES + (is_v ? BK * D : 0), dst = tile0 + ps * F::T_BYTES;
         ok = warp_wait(b_rfull + 8 * rs, rpar);
@@ -765,40 +828,41 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   }
 }
 
-// Segments of a row's head, added up in the order of the keys: a warp per row and head.
+// Segments of a request's key head, added up in the order of the keys: a CTA takes 32 query rows x 32 columns, a lane a row.  128 threads and few
+// registers, so that it finds room beside a CTA of the attention and is there when that ends.
 template <int D>
-__global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p, int columns, int slot_rows) {
-  constexpr int E = D / 32;
+__global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttnParams p, int columns, int slot_rows, int groups) {
+  constexpr int PARTS = D / 32;
+  __shared__ uint32_t s_out[32][17];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_launch_dependents();
-  const int item = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int row = item / p.n_q, head = item - row * p.n_q;
-  if (row >= p.rows) return;
-  const int b = p.row_req[row];
-  if (b < 0 || b >= p.B) return;
+  const int item = blockIdx.x, z = item % groups, h = item / groups % p.n_kv, b = item / groups / p.n_kv;
+  const int rr0 = blockIdx.y / PARTS * 32, c0 = blockIdx.y % PARTS * 32;
   const long long each = p.sched[0];
-  const int before = p.sched[1 + b], nt = p.sched[2 + b] - before;
-  const int h = head / p.gqa, node = row - p.row_start[b], z = node / p.group_tokens, rr = (node - z * p.group_tokens) * p.gqa + head % p.gqa;
-  if (nt < 1 || node < 0 || node >= kMaxNodes) return;
-  const long long a = (long long)before * p.n_kv + (long long)h * nt, e = a + nt;
-  const int c0 = (int)(a / each), c1 = (int)((e - 1) / each);
-  if (c0 == c1) return;      // one segment: its CTA wrote the result
-  auto slot = [&](int c) { return (((size_t)z * columns + c) * 2 + (a > c * each)) * slot_rows + rr; };
-  // four segments at a time, their sums and their maxima on the way together; rescaled as the running maximum grows
+  const int before = p.sched[1 + b], places = p.sched[2 + b] - before, nt = p.sched[p.B + 2 + b];
+  int r0;
+  const int n = nodes_of(p, b, r0), rows = (min(p.group_tokens, n - z * p.group_tokens)) * p.gqa;
+  if (nt < 1 || rr0 >= rows) return;
+  const long long a = (long long)before * p.n_kv + (long long)h * places;
+  const int first = (int)(a / each), last = (int)((a + nt - 1) / each);
+  if (first == last) return;      // one segment: its CTA wrote the result
+  const int rr = min(rr0 + lane, slot_rows - 1);
+  auto slot = [&](int c) { return (((size_t)z * columns + c) * 2 + (a > c * each)) * slot_rows; };
   constexpr int U = 4;
-  float best = -INFINITY, sum = 0.f, acc[E] = {};
-  for (int c = c0; c <= c1; c += U) {
-    float x[U][E];
+  float best = -INFINITY, sum = 0.f, acc[2][4] = {};
+  for (int c = first; c <= last; c += U) {
+    float4 x[U][2];
     float2 ml[U];
 #pragma unroll
     for (int y = 0; y < U; ++y) {
       ml[y] = make_float2(-INFINITY, 0.f);
-      if (c + y <= c1) {
+      if (c + y <= last) {
         const size_t at = slot(c + y);
-        ml[y] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-        const float* src = p.part_o + at * D + lane * E;
-        if constexpr (E == 4) *reinterpret_cast<float4*>(x[y]) = *reinterpret_cast<const float4*>(src);
-        else *reinterpret_cast<float2*>(x[y]) = *reinterpret_cast<const float2*>(src);
+        ml[y] = *reinterpret_cast<const float2*>(p.part_ml + (at + rr) * 2);
+        const float* src = p.part_o + at * D + (size_t)(c0 / 4 + 2 * warp) * (slot_rows * 4) + rr * 4;
+        x[y][0] = *reinterpret_cast<const float4*>(src);
+        x[y][1] = *reinterpret_cast<const float4*>(src + slot_rows * 4);
       }
     }
     float m = best;
@@ -808,19 +872,32 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(const TreeAttnParams p,
     best = m;
     sum *= old;
 #pragma unroll
-    for (int d = 0; d < E; ++d) acc[d] *= old;
+    for (int d = 0; d < 8; ++d) acc[d >> 2][d & 3] *= old;
 #pragma unroll
     for (int y = 0; y < U; ++y) {
       const float f = ml[y].x == -INFINITY ? 0.f : exp2f(ml[y].x - best);
-      sum += f * ml[y].y;
+      if (f > 0.f) {
+        sum += f * ml[y].y;
 #pragma unroll
-      for (int d = 0; d < E; ++d) acc[d] += f > 0.f ? f * x[y][d] : 0.f;
+        for (int e = 0; e < 2; ++e) {
+          acc[e][0] += f * x[y][e].x; acc[e][1] += f * x[y][e].y; acc[e][2] += f * x[y][e].z; acc[e][3] += f * x[y][e].w;
+        }
+      }
     }
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
-  __nv_bfloat16* dst = p.out + row * p.ldo + head * D + lane * E;
-  if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(acc[0] * inv, acc[1] * inv), pack_bf16(acc[2] * inv, acc[3] * inv));
-  else *reinterpret_cast<uint32_t*>(dst) = pack_bf16(acc[0] * inv, acc[1] * inv);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    s_out[lane][4 * warp + 2 * e] = pack_bf16(acc[e][0] * inv, acc[e][1] * inv);
+    s_out[lane][4 * warp + 2 * e + 1] = pack_bf16(acc[e][2] * inv, acc[e][3] * inv);
+  }
+  __syncthreads();
+  // 64 bytes of a row: four threads
+  const int row = threadIdx.x >> 2, piece = threadIdx.x & 3, q = rr0 + row;
+  if (q >= rows) return;
+  const int node = z * p.group_tokens + q / p.gqa, head = h * p.gqa + q % p.gqa;
+  *reinterpret_cast<uint4*>(p.out + (r0 + node) * p.ldo + head * D + c0 + 8 * piece) =
+      make_uint4(s_out[row][4 * piece], s_out[row][4 * piece + 1], s_out[row][4 * piece + 2], s_out[row][4 * piece + 3]);
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -884,8 +961,9 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const TreeAttnParams& p
   }
   const int rc = b2_launch(tree_attn_kernel<F>, dim3(s.columns, s.groups), dim3(F::kThreads), F::SMEM, st, true, mk, mv, p);
   if (rc) return rc;
-  const long long items = (long long)p.rows * p.n_q;
-  return b2_launch(tree_merge_kernel<F::D>, dim3((unsigned)((items + 7) / 8)), dim3(256), 0, st, true, p, s.columns, s.nw * BQ);
+  const int most = s.tokens * p.gqa;
+  return b2_launch(tree_merge_kernel<F::D>, dim3((unsigned)(p.B * p.n_kv * s.groups), (unsigned)((most + 31) / 32 * (F::D / 32))), dim3(128), 0, st, true, p, s.columns,
+                   s.nw * BQ, s.groups);
 }
 
 }  // namespace
@@ -901,7 +979,7 @@ extern "C" int b2_tree_cache(B2TreeCache* c) {
 // fp32 words of workspace for b2_tree_attention on the current device
 extern "C" long long b2_tree_attention_work(const B2TreeStep* t, int n_q, int n_kv, int D) {
   const Shape s = shape_of(t->requests, t->max_blocks, n_kv, n_q / n_kv, t->max_nodes);
-  return 2ll * s.groups * s.columns * s.nw * BQ * (D + 2) + (t->requests + 2 + 3) / 4 * 4;
+  return 2ll * s.groups * s.columns * s.nw * BQ * (D + 2) + (2 * t->requests + 2 + 3) / 4 * 4;
 }
 
 extern "C" int b2_tree_attention(const B2TreeStep* step, const B2TreeCache* cache, const void* q, long long ldq, void* out, long long ldo, float* work, int rows,
