@@ -45,6 +45,7 @@ struct TreeAttnParams {
   const unsigned long long* masks;
   int B, max_blocks, tree_blocks, num_pages, rows, n_q, n_kv, gqa, window;
   int group_tokens;                // nodes to a CTA's query tiles
+  int single;                      // > 0: places of a request's key head, each a column of its own
   float scale_log2;
   __nv_bfloat16* out;
   long long ldo;
@@ -156,6 +157,8 @@ struct Req {
 };
 
 __device__ __forceinline__ int first_tile(const TreeAttnParams& p, int length) { return p.window > 0 ? max(0, length - p.window + 1) / BK : 0; }
+__device__ __forceinline__ int tiles_of(const TreeAttnParams& p, int length) { return (length + BK - 1) / BK - first_tile(p, length) + 1; }
+__device__ __forceinline__ int length_of(const TreeAttnParams& p, int b) { return max(0, min(p.lengths[b], p.max_blocks * kPage)); }
 __device__ __forceinline__ int nodes_of(const TreeAttnParams& p, int b, int& r0) {
   r0 = p.row_start[b];
   return max(0, min(min(p.row_start[b + 1], p.rows) - r0, kMaxNodes));
@@ -163,8 +166,7 @@ __device__ __forceinline__ int nodes_of(const TreeAttnParams& p, int b, int& r0)
 
 // The segments of a CTA's part [u, u1) of the line of tiles.  A request's tiles of one key head take s_cum[b + 1] - s_cum[b] places of it.
 struct Walk {
-  long long u, u0, u1;
-  int b;
+  int u, u0, u1, b;
   Req r;
   int h, ts, count, tok;       // key head, first tile and tiles of the segment, nodes of the CTA's group
 };
@@ -174,11 +176,10 @@ template <class F>
 __device__ __forceinline__ bool next_segment(const TreeAttnParams& p, const int* s_cum, const int* s_req, Walk& k) {
   for (;;) {
     if (k.u >= k.u1) return false;
-    while ((long long)s_cum[k.b + 1] * p.n_kv <= k.u) ++k.b;
-    const int places = s_cum[k.b + 1] - s_cum[k.b];
-    const long long rel = k.u - (long long)s_cum[k.b] * p.n_kv;
-    k.h = (int)(rel / places);
-    k.ts = (int)(rel - (long long)k.h * places);
+    while (s_cum[k.b + 1] * p.n_kv <= k.u) ++k.b;
+    const int places = s_cum[k.b + 1] - s_cum[k.b], rel = k.u - s_cum[k.b] * p.n_kv;
+    k.h = rel / places;
+    k.ts = rel - k.h * places;
     k.r.b = k.b;
     if (p.B <= kKept) {
       k.r.length = s_req[kKept + k.b];
@@ -187,15 +188,15 @@ __device__ __forceinline__ bool next_segment(const TreeAttnParams& p, const int*
       k.r.n = rn & 127;
     } else {
       k.r.n = nodes_of(p, k.b, k.r.r0);
-      k.r.length = p.lengths[k.b];
+      k.r.length = length_of(p, k.b);
     }
     k.r.first = first_tile(p, k.r.length);
-    k.r.nt = (k.r.length + BK - 1) / BK - k.r.first + 1;
+    k.r.nt = tiles_of(p, k.r.length);
     if (k.ts >= k.r.nt) {      // places behind the last tile
       k.u += places - k.ts;
       continue;
     }
-    k.count = (int)min((long long)(k.r.nt - k.ts), k.u1 - k.u);
+    k.count = min(k.r.nt - k.ts, k.u1 - k.u);
     k.u += k.count;
     k.tok = min(p.group_tokens, k.r.n - (int)blockIdx.y * p.group_tokens);
     if (k.tok > 0) return true;
@@ -267,8 +268,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     int mine = 0;
     for (int b = b0; b < min(b0 + per, p.B); ++b) {
       int r0;
-      const int length = p.lengths[b], n = nodes_of(p, b, r0);
-      const int nt = n > 0 ? (length + BK - 1) / BK - first_tile(p, length) + 1 : 0;
+      const int length = length_of(p, b), n = nodes_of(p, b, r0);
+      const int nt = n > 0 ? tiles_of(p, length) : 0;
       s_cum[b + 1] = mine += nt;
       if (b < kKept) {
         s_req[b] = nt;
@@ -300,31 +301,31 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto t_p = [&](int w) { return tmem_base + 192 + (uint32_t)w * 32; };
   auto t_o = [&](int w) { return tmem_base + 256 + (uint32_t)w * D; };
 
-  long long total = (long long)s_cum[p.B] * p.n_kv, each = (total + gridDim.x - 1) / gridDim.x;
+  int total = s_cum[p.B] * p.n_kv, each = p.single ? p.single : (total + gridDim.x - 1) / gridDim.x;
   // Where there are columns enough for every request's key head, a request's tiles can begin a column: then a CTA has one segment, whose start and
-  // end cost as much as four or five tiles.  Eight column lengths from the least on are looked at, by a warp each; the first that fits is taken.
-  // (One request of 4100 positions, 8 key heads: 66 tiles in 16.5 columns of 4, or 17 of 4.)
-  if (p.B * p.n_kv <= (int)gridDim.x && total > 0) {
-    if (warp < 8) {
-      const int len = (int)each + warp;
-      int sum = 0;
-      for (int b = lane; b < p.B; b += 32) sum += (s_req[b] + len - 1) / len;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (lane == 0) s_sums[32 + warp] = sum;
-    }
-    __syncthreads();
-    int take = -1;
-#pragma unroll
-    for (int c = 7; c >= 0; --c)
-      if (s_sums[32 + c] * p.n_kv <= (int)gridDim.x) take = c;
-    if (take >= 0) {
-      each += take;
-      if (warp == 0) {      // the line again, in whole columns
+  // end cost as much as four or five tiles.  Eight column lengths from the least on are looked at; the first that fits is taken.
+  // (One request of 4100 positions, 8 key heads, 66 tiles: 17 columns of 4 instead of 16.5; 21.2 -> 16.7 us with the merge.)
+  // single: tables so short that a request's key head is one column in any case, and nothing is left to merge.
+  if (p.single || p.B * p.n_kv <= (int)gridDim.x) {
+    if (warp == 0) {
+      bool fits = p.single > 0;
+#pragma unroll 1
+      for (int c = 0; c < 8 && !fits; ++c) {
+        const int len = each + c;
+        int sum = 0;
+#pragma unroll 1
+        for (int b = lane; b < p.B; b += 32) sum += (s_req[b] + len - 1) / max(len, 1);
+        fits = __reduce_add_sync(0xffffffffu, sum) * p.n_kv <= (int)gridDim.x;
+        if (fits) each = len;
+      }
+      if (fits && each > 0) {      // the line again, in whole columns
         int before = 0;
+#pragma unroll 1
         for (int b0 = 0; b0 < p.B; b0 += 32) {
-          const int b = b0 + lane, mine = b < p.B ? (int)((s_req[b] + each - 1) / each * each) : 0;
-          int x = mine;
+          const int b = b0 + lane;
+          int r0, nt = 0;
+          if (b < p.B) nt = p.single ? (nodes_of(p, b, r0) > 0 ? 1 : 0) : s_req[b];
+          int x = (nt + each - 1) / each * each;
 #pragma unroll
           for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, x, o);
@@ -334,29 +335,30 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           before += __shfl_sync(0xffffffffu, x, 31);
         }
       }
-      __syncthreads();
-      total = (long long)s_cum[p.B] * p.n_kv;
+      if (lane == 0) s_sums[32] = each;
     }
+    __syncthreads();
+    each = s_sums[32];
+    total = s_cum[p.B] * p.n_kv;
   }
-  if (blockIdx.x == 0 && blockIdx.y == 0) {
+  if (!p.single && blockIdx.x == 0 && blockIdx.y == 0) {
     for (int b = tid; b <= p.B; b += F::kThreads) {
       p.sched[b + 1] = s_cum[b];
       if (b < p.B) {
         int r0;
-        const int length = p.lengths[b];
-        p.sched[p.B + 2 + b] = nodes_of(p, b, r0) > 0 ? (length + BK - 1) / BK - first_tile(p, length) + 1 : 0;
+        p.sched[p.B + 2 + b] = p.B <= kKept ? s_req[b] : nodes_of(p, b, r0) > 0 ? tiles_of(p, length_of(p, b)) : 0;
       }
     }
-    if (tid == 0) p.sched[0] = (int)each;
+    if (tid == 0) p.sched[0] = each;
   }
   Walk k;
-  k.u0 = k.u = min(total, blockIdx.x * each);
+  k.u0 = k.u = min(total, (int)blockIdx.x * each);
   k.u1 = min(total, k.u0 + each);
   {
     int lo = 0, hi = p.B - 1;      // the last request that begins at or before u0
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if ((long long)s_cum[mid] * p.n_kv <= k.u0) lo = mid; else hi = mid - 1;
+      if (s_cum[mid] * p.n_kv <= k.u0) lo = mid; else hi = mid - 1;
     }
     k.b = lo;
   }
@@ -839,13 +841,11 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttnParams p,
   pdl_launch_dependents();
   const int item = blockIdx.x, z = item % groups, h = item / groups % p.n_kv, b = item / groups / p.n_kv;
   const int rr0 = blockIdx.y / PARTS * 32, c0 = blockIdx.y % PARTS * 32;
-  const long long each = p.sched[0];
-  const int before = p.sched[1 + b], places = p.sched[2 + b] - before, nt = p.sched[p.B + 2 + b];
+  const int each = p.sched[0], before = p.sched[1 + b], places = p.sched[2 + b] - before, nt = p.sched[p.B + 2 + b];
   int r0;
   const int n = nodes_of(p, b, r0), rows = (min(p.group_tokens, n - z * p.group_tokens)) * p.gqa;
   if (nt < 1 || rr0 >= rows) return;
-  const long long a = (long long)before * p.n_kv + (long long)h * places;
-  const int first = (int)(a / each), last = (int)((a + nt - 1) / each);
+  const int a = before * p.n_kv + h * places, first = a / each, last = (a + nt - 1) / each;
   if (first == last) return;      // one segment: its CTA wrote the result
   const int rr = min(rr0 + lane, slot_rows - 1);
   auto slot = [&](int c) { return (((size_t)z * columns + c) * 2 + (a > c * each)) * slot_rows; };
@@ -933,9 +933,12 @@ int sm_count() {
   return n;
 }
 
+// Places on the line of tiles are 32-bit numbers.
+bool too_long(const B2TreeStep& t, int n_kv) { return (long long)t.requests * n_kv * (t.max_blocks / 4 + 2) >= 1ll << 30; }
+
 // Query tiles of a CTA, nodes to a CTA, CTAs over the same keys, columns of CTAs.
 struct Shape {
-  int nw, tokens, groups, columns;
+  int nw, tokens, groups, columns, single;
 };
 Shape shape_of(int B, int max_blocks, int n_kv, int gqa, int max_nodes) {
   Shape s;
@@ -943,7 +946,14 @@ Shape shape_of(int B, int max_blocks, int n_kv, int gqa, int max_nodes) {
   const int most = s.nw * BQ / gqa;
   s.groups = (max_nodes + most - 1) / most;
   s.tokens = (max_nodes + s.groups - 1) / s.groups;
-  const long long units = (long long)B * n_kv * (max_blocks / 4 + 2);      // tiles there can be
+  // A table of few pages (up to four tiles and the tree's): a request's key head is one CTA's, and the second launch is spared.
+  const int most_tiles = max_blocks / 4 + 2;
+  s.single = most_tiles <= 6 && (long long)B * n_kv < 65536 ? most_tiles : 0;
+  if (s.single) {
+    s.columns = B * n_kv;
+    return s;
+  }
+  const long long units = (long long)B * n_kv * most_tiles;      // tiles there can be
   const long long c = (long long)sm_count() / s.groups;
   s.columns = (int)(c < 1 ? 1 : c < units ? c : units);
   return s;
@@ -960,7 +970,7 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const TreeAttnParams& p
     configured[dev & 63] = true;
   }
   const int rc = b2_launch(tree_attn_kernel<F>, dim3(s.columns, s.groups), dim3(F::kThreads), F::SMEM, st, true, mk, mv, p);
-  if (rc) return rc;
+  if (rc || s.single) return rc;
   const int most = s.tokens * p.gqa;
   return b2_launch(tree_merge_kernel<F::D>, dim3((unsigned)(p.B * p.n_kv * s.groups), (unsigned)((most + 31) / 32 * (F::D / 32))), dim3(128), 0, st, true, p, s.columns,
                    s.nw * BQ, s.groups);
@@ -979,7 +989,7 @@ extern "C" int b2_tree_cache(B2TreeCache* c) {
 // fp32 words of workspace for b2_tree_attention on the current device
 extern "C" long long b2_tree_attention_work(const B2TreeStep* t, int n_q, int n_kv, int D) {
   const Shape s = shape_of(t->requests, t->max_blocks, n_kv, n_q / n_kv, t->max_nodes);
-  return 2ll * s.groups * s.columns * s.nw * BQ * (D + 2) + (2 * t->requests + 2 + 3) / 4 * 4;
+  return (s.single ? 0 : 2ll * s.groups * s.columns * s.nw * BQ * (D + 2)) + (2 * t->requests + 2 + 3) / 4 * 4;
 }
 
 extern "C" int b2_tree_attention(const B2TreeStep* step, const B2TreeCache* cache, const void* q, long long ldq, void* out, long long ldo, float* work, int rows,
@@ -987,7 +997,7 @@ extern "C" int b2_tree_attention(const B2TreeStep* step, const B2TreeCache* cach
   const B2TreeStep& t = *step;
   const B2TreeCache& c = *cache;
   if (rows < 1 || t.requests < 1 || t.requests > kMaxReq || n_q < 1 || c.heads < 1 || n_q % c.heads || n_q / c.heads > 64 || (c.d != 64 && c.d != 128) || t.max_nodes < 1 ||
-      t.max_nodes > kMaxNodes || c.pages < 1)
+      t.max_nodes > kMaxNodes || c.pages < 1 || too_long(t, c.heads))
     return -1;
   if (((uintptr_t)q | (uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)out | (uintptr_t)work | (uintptr_t)c.k_scale | (uintptr_t)c.v_scale) % 16 || ldq % 8 || ldo % 8) return -2;
   const Shape s = shape_of(t.requests, t.max_blocks, c.heads, n_q / c.heads, t.max_nodes);
@@ -997,7 +1007,8 @@ extern "C" int b2_tree_attention(const B2TreeStep* step, const B2TreeCache* cach
   p.masks = t.masks; p.B = t.requests; p.max_blocks = t.max_blocks; p.tree_blocks = t.tree_blocks; p.num_pages = c.pages; p.rows = rows;
   p.n_q = n_q; p.n_kv = c.heads; p.gqa = n_q / c.heads; p.window = window; p.group_tokens = s.tokens; p.scale_log2 = scale * 1.4426950408889634f;
   p.out = (__nv_bfloat16*)out; p.ldo = ldo;
-  const size_t slots = 2ull * s.groups * s.columns * s.nw * BQ;
+  const size_t slots = s.single ? 0 : 2ull * s.groups * s.columns * s.nw * BQ;
+  p.single = s.single;
   p.part_o = work; p.part_ml = work + slots * c.d; p.sched = reinterpret_cast<int*>(work + slots * (c.d + 2));
   const CUtensorMap &mk = c.map_k, &mv = c.map_v;
   const cudaStream_t st = (cudaStream_t)stream;

@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) tree_rope_kernel(const TreeRopeParams p) 
   for (int c = 0; c < HC; ++c) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[c][e] = 0.f;
-    if (!live || h0 + c >= heads) continue;
+    if (h0 + c >= heads) continue;      // (a row without a slot is read all the same: its number is not waited for)
     if constexpr (F32) {
       const float* src = reinterpret_cast<const float*>(p.qkv) + row * p.ld + (h0 + c) * D;
       const float4 a = *reinterpret_cast<const float4*>(src + off_a), b = *reinterpret_cast<const float4*>(src + off_b);
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(256) tree_rope_kernel(const TreeRopeParams p) 
     for (int s = 1; s < p.slices; ++s) {
 #pragma unroll
       for (int c = 0; c < HC; ++c) {
-        if (!live || h0 + c >= heads) continue;
+        if (h0 + c >= heads) continue;
         const float* src = reinterpret_cast<const float*>(p.qkv) + s * p.slice + row * p.ld + (h0 + c) * D;
         const float4 a = *reinterpret_cast<const float4*>(src + off_a), b = *reinterpret_cast<const float4*>(src + off_b);
         x[c][0] += a.x; x[c][1] += a.y; x[c][2] += a.z; x[c][3] += a.w; x[c][4] += b.x; x[c][5] += b.y; x[c][6] += b.z; x[c][7] += b.w;

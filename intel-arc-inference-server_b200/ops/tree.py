@@ -25,7 +25,7 @@ from typing import Optional
 import torch
 
 from . import lib as K
-from .logprob import _elsewhere, _rows_of, _stream
+from .logprob import _elsewhere, _stream
 
 PAGE = 16
 MAX_NODES = 64          # nodes of a tree: an ancestor mask is one 64-bit word
@@ -84,6 +84,27 @@ def _flat(t: torch.Tensor, dtype, shape, what: str, device=None) -> torch.Tensor
     return t
 
 
+def _matrix(t: torch.Tensor, dtype, what: str, device, dims: int = 2) -> tuple:
+    """(rows, columns, elements from row to row, address) of a matrix whose rows begin at multiples of 16 bytes, or of the first of several
+    (``dims`` 3: their number and the elements from one to the next behind it)."""
+    if t.dtype is not dtype or t.dim() != dims or t.get_device() != device.index:
+        raise ValueError(f"{what}: rows of {dtype} on {device}, not {t.dtype} {list(t.shape)} on {t.device}")
+    more = ()
+    if dims == 2:
+        (m, n), (ld, step) = t.shape, t.stride()
+    else:
+        (s, m, n), (apart, ld, step) = t.shape, t.stride()
+        if s < 1 or apart * dtype.itemsize % 16:
+            raise ValueError(f"{what}: one slice at least, slices at multiples of 16 bytes")
+        more = (s, apart)
+    at = t.data_ptr()
+    if m < 2:
+        ld = (n + 15) // 16 * 16      # (a lone row's stride says nothing)
+    if n > 1 and step != 1 or ld < n or (at | ld * dtype.itemsize) % 16:
+        raise ValueError(f"{what}: one element after another, rows that do not overlap and begin at multiples of 16 bytes")
+    return (m, n, ld, at) + more
+
+
 def _words(t: torch.Tensor, n: int, what: str, device) -> int:
     """Address of ``n`` int32 numbers."""
     if t.dtype is not torch.int32 or t.dim() != 1 or t.numel() != n or t.get_device() != device.index or not t.is_contiguous():
@@ -100,7 +121,7 @@ class PagePool:
         self.free, self.n_free = free, _flat(n_free, torch.int32, (1,), "number of free pages", free.device)
         self.held = _flat(held, torch.int32, (held.numel(),), "pages of the requests", free.device)
         self._c = _Pool(free.data_ptr(), n_free.data_ptr(), held.data_ptr(), free.numel())
-        self._at, self._requests, self._device = ctypes.addressof(self._c), held.numel(), free.device
+        self._at, self._requests, self._index = ctypes.addressof(self._c), held.numel(), free.device.index
 
 
 class TreeCache:
@@ -129,6 +150,7 @@ class TreeCache:
         self.device, self.i8 = k.device, i8
         if i8 and (k_scale.data_ptr() | v_scale.data_ptr() | (k_scale.stride(0) * 4 if k.dim() == 5 else 0)) % 16:
             raise ValueError("a layer's scales begin at multiples of 16 bytes")
+        self._index = k.device.index
         self._c, self._at = _aligned(_Cache)
         c, five = self._c, k.dim() == 5
         c.k, c.v, c.layers, c.pages, c.heads, c.d = k.data_ptr(), v.data_ptr(), self.layers, self.pages, self.heads, self.d
@@ -172,7 +194,7 @@ class TreeStep:
         self._c = _Step(*(t.data_ptr() for t in (block_table, tree_table, self.lengths, self.row_start, self.row_req, self.row_pos, self.slots, self.parents, self.masks,
                                                  self.status)), b, block_table.shape[1], tree_table.shape[1], max_rows, max_nodes, num_pages)
         self._at, self._lengths, self._work = ctypes.addressof(self._c), self.lengths.data_ptr(), {}
-        self._floats = torch.empty(0, device=dev)
+        self._floats, self._index = torch.empty(0, device=dev), dev.index
 
     def check(self):
         """Waits for the last plan and raises where it could not be made."""
@@ -190,7 +212,7 @@ class Accepted:
         self.path, self.count = _flat(path, torch.int32, (b, MAX_NODES), "accepted path", dev), _flat(count, torch.int32, (b,), "accepted nodes")
         self.next_token, self.lengths = _flat(next_token, torch.int32, (b,), "next tokens", dev), _flat(lengths, torch.int32, (b,), "lengths", dev)
         self._c = _Accepted(path.data_ptr(), count.data_ptr(), next_token.data_ptr(), lengths.data_ptr())
-        self._at, self._requests, self._device, self._lengths = ctypes.addressof(self._c), b, dev, lengths.data_ptr()
+        self._at, self._requests, self._index, self._lengths = ctypes.addressof(self._c), b, dev.index, lengths.data_ptr()
 
     @staticmethod
     def empty(requests: int, device) -> "Accepted":
@@ -214,7 +236,7 @@ def plan(step: TreeStep, lengths: torch.Tensor, counts: torch.Tensor, parents: O
         parents_at = _words(parents, rows, "parents", dev)
         if rows > step.max_rows:
             raise ValueError(f"parents: of up to {step.max_rows} rows, not {rows}")
-    if pool._requests != b or after._requests != b or pool._device != dev or after._c.free != pool._c.free:
+    if pool._requests != b or after._requests != b or pool._index != step._index or after._c.free != pool._c.free:
         raise ValueError(f"pools of {b} requests on {dev}, over the same free pages")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
@@ -227,7 +249,7 @@ def plan(step: TreeStep, lengths: torch.Tensor, counts: torch.Tensor, parents: O
 def _check_cache(step: TreeStep, cache: TreeCache, layers: bool):
     if step.tree is None:
         raise ValueError("the step has no plan yet")
-    if cache.device != step.device or cache.pages < step.num_pages or cache.layers > 1 and not layers:
+    if cache._index != step._index or cache.pages < step.num_pages or cache.layers > 1 and not layers:
         raise ValueError(f"{'a' if layers else 'one layer of a'} cache of at least {step.num_pages} pages on {step.device}")
 
 
@@ -238,30 +260,33 @@ def rope_append(step: TreeStep, qkv: torch.Tensor, rope: tuple, q: torch.Tensor,
     ``interleaved`` 2 i and 2 i + 1.  Scaled positions and factors are the tables' (``models.config.Rotary``).  Rows behind the step's are left."""
     _check_cache(step, cache, False)
     dev, d, n_kv = step.device, cache.d, cache.heads
-    slices, slice_elems, x = 0, 0, qkv
-    if qkv.dtype is torch.float32:
-        slices = 1
-        if qkv.dim() == 3:
-            slices, slice_elems, x = qkv.shape[0], qkv.stride(0), qkv[0] if qkv.shape[0] else qkv
-    rows, n, ld, at = _rows_of(x, qkv.dtype, "rows", 16 if slices else 8)
-    if qkv.dtype not in (torch.bfloat16, torch.float32) or x.device != dev or not 1 <= rows <= step.max_rows or at % 16 or slice_elems % 4:
-        raise ValueError(f"rows: 1 to {step.max_rows} of bf16 or fp32 on {dev}, slices and the first row at multiples of 16 bytes")
+    if qkv.dtype is torch.bfloat16:
+        slices, slice_elems = 0, 0
+        rows, n, ld, at = _matrix(qkv, torch.bfloat16, "rows", dev)
+    elif qkv.dim() == 3:
+        rows, n, ld, at, slices, slice_elems = _matrix(qkv, torch.float32, "rows", dev, 3)
+    else:
+        slices, slice_elems = 1, 0
+        rows, n, ld, at = _matrix(qkv, torch.float32, "rows", dev)
+    if not 1 <= rows <= step.max_rows:
+        raise ValueError(f"rows: 1 to {step.max_rows}, not {rows}")
     n_q, rest = divmod(n, d)
     n_q -= 2 * n_kv
     if rest or n_q < 1 or n_q % n_kv:
         raise ValueError(f"rows of {n} columns: heads of {d}, {n_kv} of keys and of values")
-    mq, cols, ldq, pq = _rows_of(q, torch.bfloat16, "queries", 8)
-    if mq != rows or cols != n_q * d or q.device != dev or pq % 16:
-        raise ValueError(f"queries: {rows} rows of {n_q * d} on {dev}")
+    mq, cols, ldq, pq = _matrix(q, torch.bfloat16, "queries", dev)
+    if mq != rows or cols != n_q * d:
+        raise ValueError(f"queries: {rows} rows of {n_q * d}")
     cos, sin = rope
-    if cos.dim() != 2 or cos.shape[0] < 1 or cos.shape[1] % 4 or 2 * cos.shape[1] > d or (cos.data_ptr() | sin.data_ptr()) % 16:
-        raise ValueError(f"rotation: tables of positions x pairs, a multiple of 4 up to {d // 2}")
-    _flat(cos, torch.float32, cos.shape, "cosines", dev)
-    _flat(sin, torch.float32, cos.shape, "sines", dev)
+    positions, pairs = cos.shape if cos.dim() == 2 else (0, 0)
+    cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+    if positions < 1 or pairs % 4 or 2 * pairs > d or sin.shape != cos.shape or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or (cos_at | sin_at) % 16 \
+            or cos.get_device() != dev.index or sin.get_device() != dev.index or not cos.is_contiguous() or not sin.is_contiguous():
+        raise ValueError(f"rotation: two contiguous fp32 tables of positions x pairs on {dev}, pairs a multiple of 4 up to {d // 2}")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return rope_append(step, qkv, rope, q, cache, interleaved)
-    K._check(_fn()["rope"](step._at, cache._at, at, ld, slice_elems, slices, rows, cos.data_ptr(), sin.data_ptr(), cos.shape[1], cos.shape[0], int(interleaved), n_q, pq, ldq,
+    K._check(_fn()["rope"](step._at, cache._at, at, ld, slice_elems, slices, rows, cos_at, sin_at, pairs, positions, bool(interleaved), n_q, pq, ldq,
                            _stream(dev)), "tree_rope")
     return q
 
@@ -274,14 +299,14 @@ def attention(step: TreeStep, q: torch.Tensor, cache: TreeCache, out: torch.Tens
     dev, d, n_kv = step.device, cache.d, cache.heads
     if not step.tree:
         raise ValueError("the step's rows are no trees'")
-    rows, n, ldq, pq = _rows_of(q, torch.bfloat16, "queries", 16)
-    mo, no, ldo, po = _rows_of(out, torch.bfloat16, "outputs", 16)
+    rows, n, ldq, pq = _matrix(q, torch.bfloat16, "queries", dev)
+    mo, no, ldo, po = _matrix(out, torch.bfloat16, "outputs", dev)
     n_q = n // d
-    if n != n_q * d or n_q < 1 or n_q % n_kv or n_q // n_kv > MAX_GROUP or not 1 <= rows <= step.max_rows or q.device != dev:
+    if n != n_q * d or n_q < 1 or n_q % n_kv or n_q // n_kv > MAX_GROUP or not 1 <= rows <= step.max_rows:
         raise ValueError(f"queries: 1 to {step.max_rows} rows of heads of {d}, 1 to {MAX_GROUP} to each of {n_kv} key heads, on {dev}")
-    if mo != rows or no != n or out.device != dev:
+    if mo != rows or no != n:
         raise ValueError(f"outputs: {rows} rows of {n} on {dev}")
-    if window < 0 or not 0 < scale < float("inf"):
+    if not 0 <= window < 1 << 31 or not 0 < scale < float("inf"):
         raise ValueError("a window of 0 (none) or more positions, a scale above 0")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
@@ -291,7 +316,7 @@ def attention(step: TreeStep, q: torch.Tensor, cache: TreeCache, out: torch.Tens
         room = step._work[n_q, n_kv, d] = _fn()["attention_work"](step._at, n_q, n_kv, d)
     work = step._floats.new_empty(room)      # this call's own: calls of one step on several streams share nothing
     K._check(_fn()["attention"](step._at, cache._at, pq, ldq, po, ldo, work.data_ptr(), rows, n_q, window, scale, _stream(dev)), "tree_attention")
-    K.launch_count += 1      # segments added up
+    K.launch_count += 1      # segments added up (of tables of some length)
     return out
 
 
@@ -313,7 +338,7 @@ def commit(step: TreeStep, tokens: torch.Tensor, targets: torch.Tensor, cache: T
     at, targets_at = _words(tokens, rows, "tokens", dev), _words(targets, rows, "targets", dev)
     if accepted is None:
         accepted = Accepted.empty(b, dev)
-    elif accepted._requests != b or accepted._device != dev or accepted._lengths == step._lengths:
+    elif accepted._requests != b or accepted._index != step._index or accepted._lengths == step._lengths:
         raise ValueError(f"results of {b} requests on {dev}, apart from the step's own")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
