@@ -309,14 +309,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   if (p.single || p.B * p.n_kv <= (int)gridDim.x) {
     if (warp == 0) {
       bool fits = p.single > 0;
-#pragma unroll 1
-      for (int c = 0; c < 8 && !fits; ++c) {
-        const int len = each + c;
+      if (!fits && each > 0) {      // lanes: eight lengths x four parts of the requests
+        const int len = each + (lane & 7);
         int sum = 0;
-#pragma unroll 1
-        for (int b = lane; b < p.B; b += 32) sum += (s_req[b] + len - 1) / max(len, 1);
-        fits = __reduce_add_sync(0xffffffffu, sum) * p.n_kv <= (int)gridDim.x;
-        if (fits) each = len;
+        for (int b = lane >> 3; b < p.B; b += 4) sum += (s_req[b] + len - 1) / len;
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const unsigned good = __ballot_sync(0xffffffffu, sum * p.n_kv <= (int)gridDim.x) & 0xff;
+        fits = good != 0;
+        if (fits) each += __ffs(good) - 1;
       }
       if (fits && each > 0) {      // the line again, in whole columns
         int before = 0;

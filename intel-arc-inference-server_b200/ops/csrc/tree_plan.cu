@@ -5,7 +5,7 @@
 //   commit  the accepted path of every tree (node 0, then the child whose token is its parent's target, as long as there is one); the
 //           path's keys and values move from the tree's pages to the request's positions, in all layers
 //
-// Plan is one CTA of 1024 threads: everything hangs on three prefix sums over the requests, and a launch is all that a call costs.
+// Plan is one CTA, or one cluster of eight: everything hangs on three prefix sums over the requests, and a launch is all that a call costs.
 #include "tree.cuh"
 
 using namespace b2;
@@ -13,6 +13,7 @@ using namespace b2;
 namespace {
 
 constexpr int kPage = kTreePage, kMaxNodes = kTreeNodes, kMaxReq = kTreeRequests;
+constexpr int kUpRows = 8192;      // rows whose parents are kept in shared memory
 
 enum : int { PLAN_POOL = 1, PLAN_TABLE = 2, PLAN_ROWS = 4, PLAN_COUNT = 8, PLAN_PARENT = 16, PLAN_LENGTH = 32, PLAN_PAGE = 64 };
 
@@ -30,42 +31,55 @@ struct TreePlanParams {
 };
 
 // Exclusive prefix sums of one number per thread over the CTA; the total in `total`.
-__device__ __forceinline__ long long scan_1024(long long v, long long* warp_sums, long long& total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long x = v;
+template <typename T>
+__device__ __forceinline__ T scan_cta(T v, long long* warp_sums, T& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  T x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, x, o);
+    const T y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
   __syncthreads();
   if (lane == 31) warp_sums[warp] = x;
   __syncthreads();
-  if (warp == 0) {
-    long long w = warp_sums[lane];
+  T w = lane < warps ? (T)warp_sums[lane] : 0;      // every warp for itself
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    warp_sums[lane] = w;
+  for (int o = 1; o < 32; o <<= 1) {
+    const T y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
-  __syncthreads();
-  total = warp_sums[31];
-  return x - v + (warp ? warp_sums[warp - 1] : 0);
+  total = __shfl_sync(0xffffffffu, w, 31);
+  const T before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+  return x - v + (warp ? before : 0);
 }
 
-__global__ void __launch_bounds__(1024) tree_plan_kernel(const TreePlanParams p) {
+__device__ __forceinline__ int cluster_rank() { int r; asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ int cluster_size() { int r; asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// A cluster of one CTA, or of eight where there are more rows than one CTA's threads: each does the sums for itself (there is nothing to wait for
+// that way), the first one keeps the pages, all of them write rows.  A request a thread.
+__global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams p) {
   __shared__ long long sums[32];
   __shared__ int s_start[kMaxReq + 1], s_need[kMaxReq], s_held[kMaxReq], s_first[kMaxReq], s_len[kMaxReq];
+  __shared__ int8_t s_up[kUpRows];
   __shared__ int s_status;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, rank = cluster_rank(), ranks = cluster_size();
   pdl_wait();
   pdl_launch_dependents();
-  const bool tree = p.parents != nullptr, mine = tid < p.B;
+  const bool tree = p.parents != nullptr, mine = tid < p.B, up_here = tree && p.rows <= kUpRows;
   if (tid == 0) s_status = 0;
   const int count = mine ? p.counts[tid] : 0, held = mine ? p.held[tid] : 0, n_free = *p.n_free;
   const int length = mine && count >= 0 ? p.lengths[tid] : 0;
+  if (up_here)
+    for (int r = tid; r < p.rows; r += threads) {
+      const int up = p.parents[r];
+      s_up[r] = up >= -1 && up < kMaxNodes ? (int8_t)up : (int8_t)127;      // (127: before no node)
+    }
+  auto parent = [&](int r) { return up_here ? (int)s_up[r] : p.parents[r]; };
   __syncthreads();
   if (mine) {
     int bad = 0;
@@ -75,25 +89,25 @@ __global__ void __launch_bounds__(1024) tree_plan_kernel(const TreePlanParams p)
     if (n_free < 0 || n_free > p.free_cap) bad |= PLAN_POOL;
     if (bad) atomicOr(&s_status, bad);
   }
-  long long total;
-  const long long start = scan_1024(max(count, 0), sums, total);
+  int total;
+  const int start = scan_cta(min(max(count, 0), p.rows + 1), sums, total);      // (at most 2^20 + 1 each)
   if (total > p.rows && tid == 0) atomicOr(&s_status, PLAN_ROWS);
   if (mine) {
-    s_start[tid] = (int)min(start, (long long)p.rows);
+    s_start[tid] = min(start, p.rows);
     s_need[tid] = tree ? 0 : max(count, 0);
     s_held[tid] = held;
     s_len[tid] = length;
   }
-  if (tid == 0) s_start[p.B] = (int)min(total, (long long)p.rows);
+  if (tid == 0) s_start[p.B] = min(total, p.rows);
   __syncthreads();
   if (s_status == 0 && tree) {
     // ---- a warp per tree: ancestors by walking up (a node's parent stands before it, so every walk ends)
-    for (int b = warp; b < p.B; b += 32) {
+    for (int b = warp; b < p.B; b += threads >> 5) {
       const int r0 = s_start[b], n = s_start[b + 1] - r0;
       int deepest = 0;
       bool bad = false;
       for (int i = lane; i < n; i += 32) {
-        const int up = p.parents[r0 + i];
+        const int up = parent(r0 + i);
         bad |= up < -1 || up >= i;
       }
       bad = __any_sync(0xffffffffu, bad);
@@ -102,12 +116,11 @@ __global__ void __launch_bounds__(1024) tree_plan_kernel(const TreePlanParams p)
         continue;
       }
       for (int i = lane; i < n; i += 32) {
-        unsigned long long mask = 0;
-        for (int at = i; at >= 0; at = p.parents[r0 + at]) mask |= 1ull << at;
-        const int depth = __popcll(mask);
+        int depth = 0;
+        for (int at = i; at >= 0; at = parent(r0 + at)) ++depth;
         deepest = max(deepest, depth);
       }
-      for (int o = 16; o > 0; o >>= 1) deepest = max(deepest, __shfl_xor_sync(0xffffffffu, deepest, o));
+      deepest = __reduce_max_sync(0xffffffffu, deepest);
       if (lane == 0) s_need[b] = deepest;
     }
     __syncthreads();
@@ -118,32 +131,38 @@ __global__ void __launch_bounds__(1024) tree_plan_kernel(const TreePlanParams p)
   const bool left = mine && count < 0;
   if (mine && !left && want > p.max_blocks) atomicOr(&s_status, PLAN_TABLE);
   long long back, take;
-  const long long back0 = scan_1024(left ? held : 0, sums, back);
-  const long long take0 = scan_1024(mine && !left ? want - held : 0, sums, take);
+  const long long back0 = scan_cta(left ? (long long)held : 0ll, sums, back);
+  const long long take0 = scan_cta(mine && !left ? want - held : 0ll, sums, take);
   if (mine) s_first[tid] = (int)take0;
   if (tid == 0 && ((long long)n_free + back > p.free_cap || take > (long long)n_free + back)) atomicOr(&s_status, PLAN_POOL);
   __syncthreads();
   const int status = s_status;
-  if (status == 0 && left)
+  if (rank == 0 && tid == 0) p.status[0] = status;
+  if (ranks > 1) cluster_barrier();      // everyone has read what the first CTA now writes
+  const long long top = (long long)n_free + back - 1;     // the page that is taken first
+  if (rank == 0 && status == 0 && left)
     for (int i = 0; i < held; ++i) {
       int* at = p.block_table + (size_t)tid * p.max_blocks + i;
       p.free[n_free + back0 + i] = *at;
       *at = 0;
     }
-  __syncthreads();
-  const long long top = (long long)n_free + back - 1;     // the page that is taken first
-  if (status == 0 && mine && !left)
-    for (int i = 0; i < (int)(want - held); ++i) p.block_table[(size_t)tid * p.max_blocks + held + i] = p.free[top - take0 - i];
-  if (mine) {
-    p.held_out[tid] = status ? held : left ? 0 : (int)want;
-    p.out_lengths[tid] = status ? 0 : length;
+  if (back > 0) {      // pages that came back may be taken at once
+    if (ranks > 1) cluster_barrier();
+    else __syncthreads();
   }
-  if (tid == 0) p.n_free_out[0] = status ? n_free : (int)(n_free + back - take);
-  for (int b = tid; b <= p.B; b += 1024) p.row_start[b] = status ? 0 : s_start[b];
+  if (rank == 0) {
+    if (status == 0 && mine && !left)
+      for (int i = 0; i < (int)(want - held); ++i) p.block_table[(size_t)tid * p.max_blocks + held + i] = p.free[top - take0 - i];
+    if (mine) {
+      p.held_out[tid] = status ? held : left ? 0 : (int)want;
+      p.out_lengths[tid] = status ? 0 : length;
+    }
+    if (tid == 0) p.n_free_out[0] = status ? n_free : (int)(n_free + back - take);
+    for (int b = tid; b <= p.B; b += threads) p.row_start[b] = status ? 0 : s_start[b];
+  }
   // ---- rows
   const int rows = status ? 0 : s_start[p.B];
-  bool bad_page = false;
-  for (int r = tid; r < p.max_rows; r += 1024) {
+  for (int r = rank * threads + tid; r < p.max_rows; r += ranks * threads) {
     int req = -1, pos = -1, slot = -1, up = -1;
     unsigned long long mask = 0;
     if (r < rows) {
@@ -156,10 +175,10 @@ __global__ void __launch_bounds__(1024) tree_plan_kernel(const TreePlanParams p)
       const int i = r - s_start[req];
       int page;
       if (tree) {
-        up = p.parents[r];
-        for (int at = i; at >= 0; at = p.parents[s_start[req] + at]) mask |= 1ull << at;
-        pos = s_len[req] + __popcll(mask) - 1;
         page = p.tree_table[(size_t)req * p.tree_blocks + i / kPage];
+        up = parent(r);
+        for (int at = i; at >= 0; at = parent(s_start[req] + at)) mask |= 1ull << at;
+        pos = s_len[req] + __popcll(mask) - 1;
         slot = i % kPage;
       } else {
         pos = s_len[req] + i;
@@ -168,7 +187,7 @@ __global__ void __launch_bounds__(1024) tree_plan_kernel(const TreePlanParams p)
         slot = pos % kPage;
       }
       if (page < 0 || page >= p.num_pages) {
-        bad_page = true;
+        atomicOr(&s_status, PLAN_PAGE);
         slot = -1;
       } else {
         slot += page * kPage;
@@ -182,8 +201,10 @@ __global__ void __launch_bounds__(1024) tree_plan_kernel(const TreePlanParams p)
       p.out_parents[r] = up;
     }
   }
-  const int any_bad = __syncthreads_or(bad_page);
-  if (tid == 0) p.status[0] = status | (any_bad ? PLAN_PAGE : 0);
+  __syncthreads();
+  if (s_status != status) {      // pages that are not there
+    if (tid == 0) atomicOr(p.status, PLAN_PAGE);
+  }
 }
 
 struct TreeCommitParams {
@@ -281,7 +302,20 @@ extern "C" int b2_tree_plan(const B2TreeStep* step, const B2TreePool* pool, cons
   p.row_req = t.row_req; p.row_pos = t.row_pos; p.slots = t.slots; p.out_parents = t.parents; p.masks = t.masks; p.status = t.status;
   p.B = t.requests; p.max_blocks = t.max_blocks; p.tree_blocks = t.tree_blocks; p.free_cap = pool->capacity; p.max_rows = t.max_rows; p.max_nodes = t.max_nodes;
   p.num_pages = t.num_pages; p.rows = rows;
-  return b2_launch(tree_plan_kernel, dim3(1), dim3(1024), 0, (cudaStream_t)stream, true, p);
+  const int threads = t.requests <= 256 && t.max_rows <= 512 ? 256 : 1024, ctas = t.max_rows > 1024 ? 8 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = b2_no_pdl() ? 1 : 2;
+  return (int)cudaLaunchKernelEx(&cfg, tree_plan_kernel, p);
 }
 
 extern "C" int b2_tree_commit(const B2TreeStep* step, const B2TreeCache* cache, const B2TreeAccepted* accepted, const int* tokens, const int* targets, int rows,

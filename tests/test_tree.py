@@ -113,6 +113,9 @@ PLANS = {
     "rows": dict(lengths=[0, 5, 16, 4000], counts=[33, 1, 0, 17], tree=False),
     "rows of a long prompt": dict(lengths=[3, 70000], counts=[5001, 700], tree=False, reserve=9),
     "rows, leaving": dict(lengths=[50, 20], counts=[-1, 50], tree=False),
+    "rows of many requests": dict(lengths=[(997 * i) % 3001 for i in range(300)], counts=[(37 * i) % 53 for i in range(300)], tree=False, reserve=2000),
+    "pages that came back, many rows": dict(lengths=[30000, 5, 700], counts=[-1, 9000, 20000], tree=False, free=3),
+    "many trees": dict(lengths=[(997 * i) % 3001 for i in range(200)], counts=[1 + (37 * i) % 64 for i in range(200)], spread=2),
     "thirty-two nodes a tree": dict(lengths=[33, 8], counts=[32, 9], tree_blocks=2),
 }
 
@@ -159,6 +162,7 @@ FAULTS = {
     "length": (dict(lengths=[-1, 4], counts=[2, 2]), 32),
     "page": (dict(lengths=[4, 4], counts=[2, 2]), 64),
     "rows": (dict(lengths=[4, 4], counts=[2, 2]), 4),
+    "pool, many rows": (dict(lengths=[16, 3], counts=[2000, 2000], tree=False, free=100), 1),
     "number of free pages": (dict(lengths=[4], counts=[2]), 1),
     "held": (dict(lengths=[4], counts=[2]), 2),
 }
