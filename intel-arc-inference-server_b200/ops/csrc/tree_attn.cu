@@ -15,7 +15,7 @@
 //
 // A CTA: two warps copy (tiled TMA, 16 keys x 64 dims a box, 128-byte swizzle; pages behind the end are asked for outside the tensor and
 // come as zeros), one issues the products for scores and one those of P V, each waiting for a ring's places in their order (a parity wait that could be
-// more than one phase ahead would return at once); two groups of 256 threads do softmax, two threads to a query row of which each has 32 of a
+// more than one phase ahead would return at once); two groups of 256 threads do softmax, four threads to two query rows of a
 // tile's 64 keys.  Scores come from tensor memory into registers once, and their place is free for the next ones; P goes back to tensor memory
 // as the A operand of P V; the accumulator is rescaled only where a row's maximum grew by more than 2^6.
 //   up to 128 query rows (NW 1): both groups have the same rows and take every other tile, each with its own maxima, sums and accumulator, which
@@ -64,7 +64,7 @@ struct Form {
   static constexpr int Q_BYTES = NW == 1 ? 0 : NW * BQ * NDK * 128;
   static constexpr int kMma = 2, kSoft = 4, kConv = kSoft + 16, kConvThreads = 256, kWarps = kConv + (I8_ ? kConvThreads / 32 : 0), kThreads = kWarps * 32;
   static constexpr int OFF_K = Q_BYTES, OFF_V = OFF_K + KS * T_BYTES, OFF_ST = OFF_V + VS * T_BYTES, OFF_SC = OFF_ST + RS * S_BYTES,
-                       OFF_X = OFF_SC + (I8_ ? kScales * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * 2 * BQ * 4, OFF_REQ = OFF_CUM + (kMaxReq + 8) * 4, OFF_BAR = OFF_REQ + 3 * kKept * 4,
+                       OFF_X = OFF_SC + (I8_ ? kScales * 2 * BK * 4 : 0), OFF_CUM = OFF_X + 2 * 2 * BQ * 4, OFF_REQ = OFF_CUM + (kMaxReq + 8) * 4, OFF_BAR = OFF_REQ + 3 * kKept * 4,
                        SMEM = OFF_BAR + 1024 + 1024;
   static_assert(SMEM <= 227 * 1024 && KS <= 14 && VS <= 14 && RS <= 14, "shared memory");
 };
@@ -83,6 +83,33 @@ __device__ __forceinline__ uint64_t make_desc_v(uint32_t smem_addr) {
 // columns of the thread's row between registers and tensor memory
 __device__ __forceinline__ void st_16(uint32_t taddr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+               : "memory");
+}
+// 16 rows x 64 columns: the thread has rows t / 4 (registers 4 b, 4 b + 1) and t / 4 + 8 (4 b + 2, 4 b + 3), columns 8 b + 2 (t % 4) and the next
+#define TREE_LD_16x64(taddr, r)                                                                                                      \
+  asm volatile(                                                                                                                      \
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 "                                                                                      \
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, "    \
+      "[%32];"                                                                                                                       \
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),       \
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),          \
+        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),          \
+        "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])                                                                           \
+      : "r"(taddr)                                                                                                                   \
+      : "memory")
+#define TREE_ST_16x64(taddr, r)                                                                                                      \
+  asm volatile(                                                                                                                      \
+      "tcgen05.st.sync.aligned.16x256b.x8.b32 [%32], "                                                                               \
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::  \
+          "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),   \
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]),         \
+      "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]),         \
+      "r"(r[31]), "r"(taddr)                                                                                                         \
+      : "memory")
+// 16 rows x 32 columns: rows t / 4 (register 2 b) and t / 4 + 8 (2 b + 1), column 4 b + t % 4
+__device__ __forceinline__ void st_16x32(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x8.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
                "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
                : "memory");
 }
@@ -135,10 +162,6 @@ __device__ __forceinline__ bool elect() {
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
-}
-__device__ __forceinline__ void pair_sync(int id) {
-  __syncwarp();
-  asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory");
 }
 
 // Four bytes, their sign bits turned over (u = b + 128), as bf16 pairs b / 64: up to 255 the bits of a bf16 are an integer times 2^-133 (subnormal
@@ -215,7 +238,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   int* const s_cum = reinterpret_cast<int*>(gen + F::OFF_CUM);
   int* const s_req = reinterpret_cast<int*>(gen + F::OFF_REQ);
   float* const s_scale = reinterpret_cast<float*>(gen + F::OFF_SC);       // [kScales][K, V][64]
-  float* const s_x = reinterpret_cast<float*>(gen + F::OFF_X);            // [group][parity][half][128]
+  float* const s_x = reinterpret_cast<float*>(gen + F::OFF_X);            // [group][maximum, sum][128]
   const uint32_t b_kfull = bars, b_kempty = bars + 112, b_vfull = bars + 224, b_vempty = bars + 336, b_rfull = bars + 448, b_rempty = bars + 560, b_q = bars + 672;
   auto b_sfull = [&](int w) { return bars + 680 + w * 8; };
   auto b_sfree = [&](int w) { return bars + 696 + w * 8; };
@@ -526,9 +549,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     constexpr float kLazy = 6.f;
     const int sw = warp - F::kSoft, w = sw >> 3, half = (sw >> 2) & 1, quarter = warp & 3, r = quarter * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-    const int pair = 1 + w * 4 + quarter;      // named barrier of the row's two warps
-    float* const x_mine = s_x + (w * 4 + half) * BQ + r;       // [parity 0]; parity 1 is 2 BQ further
-    float* const x_other = s_x + (w * 4 + (half ^ 1)) * BQ + r;
+    // scores: 16 rows of the quarter's 32 to a warp, half a row's 64 columns to four threads that pass maxima on by shuffles (with the
+    // columns cut between two warps they had to meet at a barrier in every tile); queries and results: a row to a lane, columns cut
+    const int mr = quarter * 32 + half * 16 + (lane >> 2), mc = 2 * (lane & 3);      // this thread's rows mr and mr + 8, its first column
+    const uint32_t half_addr = (uint32_t)(quarter * 32 + half * 16) << 16;
     // once a wait has run out no other is made, but every barrier is still come to
     bool ok = true;
     auto wait = [&](uint32_t bar, uint32_t parity) {
@@ -570,22 +594,35 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       }
       wait(b_q, seg & 1);      // (all threads are done with the segment before)
       ++seg;
-      const int lo = row_ok && p.window > 0 ? p.row_pos[row] - p.window + 1 : 0;      // the first position that is seen
-      unsigned long long mask = 0;
-      if (row_ok && k.ts + k.count == k.r.nt) {
-        mask = p.masks[row];
-        if (k.r.n < 64) mask &= (1ull << k.r.n) - 1;
-        if (lo > k.r.length)
-          for (int i = 0; i < k.r.n; ++i)
-            if (p.row_pos[k.r.r0 + i] < lo) mask &= ~(1ull << i);
+      const bool some = (NW == 1 ? 0 : w * BQ) + quarter * 32 + half * 16 < live_rows;      // rows of a request in this warp's scores
+      int lo[2] = {0, 0};                            // the first position that is seen
+      unsigned long long mask[2] = {0, 0};
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const int qr = (NW == 1 ? 0 : w * BQ) + mr + 8 * y;
+        if (qr >= live_rows) continue;
+        const int at = k.r.r0 + blockIdx.y * p.group_tokens + qr / p.gqa;
+        if (p.window > 0) lo[y] = p.row_pos[at] - p.window + 1;
+        if (k.ts + k.count == k.r.nt) {
+          mask[y] = p.masks[at];
+          if (k.r.n < 64) mask[y] &= (1ull << k.r.n) - 1;
+          if (lo[y] > k.r.length)
+            for (int i = 0; i < k.r.n; ++i)
+              if (p.row_pos[k.r.r0 + i] < lo[y]) mask[y] &= ~(1ull << i);
+        }
       }
-      float mref = -INFINITY, l = 0.f;
+      // tiles that all of the warp's rows see all of: plain0 <= t < plain1
+      const int plain1 = min(k.r.length / BK - k.r.first, k.r.nt - 1);
+      const int plain0 = p.window > 0 ? (max(0, __reduce_max_sync(0xffffffffu, max(lo[0], lo[1]))) + BK - 1) / BK - k.r.first : 0;
+      // the reference that scores are taken against, negative (0 before the first key: 2^s of a row without any is not used); sums of this thread's columns
+      float mref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+      unsigned long long nm2[2] = {0ull, 0ull};
       const int i0 = NW == 1 ? (w - g0) & 1 : 0;
       for (int i = i0; i < k.count; i += kStep, ++j) {
         const int g = g0 + i, t = k.ts + i;
         wait(b_sfull(w), j & 1);
         if (F::I8) wait(b_scale(g), (g / kScales) & 1);
-        if (!warp_ok) {      // rows of nobody: the products take what is there
+        if (!some) {      // rows of nobody: the products take what is there
           warp_arrive(b_sfree(w));
           if (i != i0) wait(b_odone(w), (j - 1) & 1);
           warp_arrive(b_pfull(w));
@@ -594,135 +631,152 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         tc_fence_after();
         uint32_t v[32];
         __syncwarp();
-        B2_TMEM_LD_32(t_s(w) + lane_addr + half * 32, v);
-        uint32_t vis = half ? (uint32_t)(mask >> 32) : (uint32_t)mask;
-        if (t != k.r.nt - 1) {
-          const int key0 = (k.r.first + t) * BK + half * 32, end = min(32, k.r.length - key0), begin = max(0, lo - key0);
-          vis = end >= 32 ? 0xffffffffu : end > 0 ? (1u << end) - 1 : 0u;
-          if (begin > 0) vis = begin >= 32 ? 0u : vis & (0xffffffffu << begin);
-        }
-        const bool whole_tile = __all_sync(0xffffffffu, vis == 0xffffffffu);
+        TREE_LD_16x64(t_s(w) + half_addr, v);
         tmem_ld_wait();
         tc_fence_before();
         warp_arrive(b_sfree(w));
-        const float* sc = s_scale + (g % kScales) * (2 * BK) + half * 32;
+        // v[4 c + 2 y + e]: row mr + 8 y, column 8 c + mc + e
+        const float* sc = s_scale + (g % kScales) * (2 * BK) + mc;
         if constexpr (F::I8) {
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const ulonglong2 f = *reinterpret_cast<const ulonglong2*>(sc + c);
-            unsigned long long a, b;
-            asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "r"(v[c]), "r"(v[c + 1]));
-            asm("mov.b64 %0, {%1, %2};" : "=l"(b) : "r"(v[c + 2]), "r"(v[c + 3]));
-            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(f.x));
-            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(b) : "l"(f.y));
-            asm("mov.b64 {%0, %1}, %2;" : "=r"(v[c]), "=r"(v[c + 1]) : "l"(a));
-            asm("mov.b64 {%0, %1}, %2;" : "=r"(v[c + 2]), "=r"(v[c + 3]) : "l"(b));
+          for (int c = 0; c < 8; ++c) {
+            const unsigned long long f = *reinterpret_cast<const unsigned long long*>(sc + 8 * c);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              unsigned long long a;
+              asm("mov.b64 %0, {%1, %2};" : "=l"(a) : "r"(v[4 * c + 2 * y]), "r"(v[4 * c + 2 * y + 1]));
+              asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(a) : "l"(f));
+              asm("mov.b64 {%0, %1}, %2;" : "=r"(v[4 * c + 2 * y]), "=r"(v[4 * c + 2 * y + 1]) : "l"(a));
+            }
           }
         }
-        if (!whole_tile) {
+        if (t < plain0 || t >= plain1) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!(vis >> c & 1)) v[c] = 0xff800000u;
-        }
-        float ma = __uint_as_float(v[0]), mb = __uint_as_float(v[1]);
+          for (int y = 0; y < 2; ++y) {
+            unsigned long long vis = mask[y];
+            if (t != k.r.nt - 1) {
+              const int key0 = (k.r.first + t) * BK, end = min(BK, k.r.length - key0), begin = lo[y] - key0;
+              vis = end >= BK ? ~0ull : (1ull << end) - 1;
+              vis = begin <= 0 ? vis : begin >= BK ? 0ull : vis & (~0ull << begin);
+            }
+            vis >>= mc;
+            const uint32_t part[2] = {(uint32_t)vis, (uint32_t)(vis >> 32)};
 #pragma unroll
-        for (int c = 2; c < 32; c += 4) {
-          asm("max.f32 %0, %0, %1, %2;" : "+f"(ma) : "f"(__uint_as_float(v[c])), "f"(__uint_as_float(v[c + 1])));
-          if (c + 3 < 32) asm("max.f32 %0, %0, %1, %2;" : "+f"(mb) : "f"(__uint_as_float(v[c + 2])), "f"(__uint_as_float(v[c + 3])));
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+              for (int e = 0; e < 2; ++e)
+                if (!(part[c >> 2] >> (8 * (c & 3) + e) & 1)) v[4 * c + 2 * y + e] = 0xff800000u;
+          }
         }
-        float tmax = fmaxf(ma, mb);
-        x_mine[(j & 1) * (2 * BQ)] = tmax;
-        pair_sync(pair);
-        tmax = fmaxf(tmax, x_other[(j & 1) * (2 * BQ)]);
         const float factor = F::I8 ? 1.f : p.scale_log2;
-        tmax *= factor;
-        float alpha = 1.f;
-        if (tmax > mref + kLazy || (mref == -INFINITY && tmax > -INFINITY)) {
-          alpha = exp2f(mref - tmax);      // 0 at the row's first key
-          mref = tmax;
-        }
-        const float nm = mref == -INFINITY ? 0.f : -mref;
-        unsigned long long sc2, nm2, acc0 = 0ull, acc1 = 0ull;
-        asm("mov.b64 %0, {%1, %1};" : "=l"(sc2) : "f"(factor));
-        asm("mov.b64 %0, {%1, %1};" : "=l"(nm2) : "f"(nm));
-        uint32_t pk[16];
-        ulonglong2 vsc = {0, 0};
+        float top[2];
 #pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          unsigned long long xy;
-          asm("mov.b64 %0, {%1, %2};" : "=l"(xy) : "r"(v[2 * c]), "r"(v[2 * c + 1]));
-          if (F::I8) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(xy) : "l"(nm2));
-          else asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(xy) : "l"(sc2), "l"(nm2));
-          float x0, x1, e0, e1;
-          asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(xy));
-          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(x0));
-          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(x1));
-          unsigned long long ee;
-          asm("mov.b64 %0, {%1, %2};" : "=l"(ee) : "f"(e0), "f"(e1));
-          if (c & 1) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc1) : "l"(ee));
-          else asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc0) : "l"(ee));
-          if constexpr (F::I8) {
-            if (!(c & 1)) vsc = *reinterpret_cast<const ulonglong2*>(sc + BK + 2 * c);
-            asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(ee) : "l"(c & 1 ? vsc.y : vsc.x));
-            asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(ee));
-          }
-          pk[c] = pack_bf16(e0, e1);
+        for (int y = 0; y < 2; ++y) {
+          top[y] = fmaxf(__uint_as_float(v[2 * y]), __uint_as_float(v[2 * y + 1]));
+#pragma unroll
+          for (int c = 1; c < 8; ++c) asm("max.f32 %0, %0, %1, %2;" : "+f"(top[y]) : "f"(__uint_as_float(v[4 * c + 2 * y])), "f"(__uint_as_float(v[4 * c + 2 * y + 1])));
         }
-        float a0, a1, a2, a3;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(acc0));
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(a2), "=f"(a3) : "l"(acc1));
-        l = l * alpha + ((a0 + a1) + (a2 + a3));
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          const float a = __shfl_xor_sync(0xffffffffu, top[0], o), b = __shfl_xor_sync(0xffffffffu, top[1], o);
+          top[0] = fmaxf(top[0], a);
+          top[1] = fmaxf(top[1], b);
+        }
+        top[0] *= factor;
+        top[1] *= factor;
+        // a row whose maximum grew by more than 2^kLazy gets a new reference: rare, and all of the warp goes that way
+        const bool grown = __any_sync(0xffffffffu, top[0] > mref[0] + kLazy || top[1] > mref[1] + kLazy);
+        float alpha[2] = {1.f, 1.f};
+        if (grown) {
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            if (top[y] > mref[y] + kLazy) {
+              alpha[y] = exp2f(mref[y] - top[y]);      // 0 at the row's first key
+              mref[y] = top[y];
+              l[y] *= alpha[y];
+              asm("mov.b64 %0, {%1, %1};" : "=l"(nm2[y]) : "f"(-top[y]));
+            }
+        }
+        unsigned long long sc2, acc[2] = {0ull, 0ull};
+        asm("mov.b64 %0, {%1, %1};" : "=l"(sc2) : "f"(factor));
+        uint32_t pk[16];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          unsigned long long f = 0;
+          if constexpr (F::I8) f = *reinterpret_cast<const unsigned long long*>(sc + BK + 8 * c);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            unsigned long long xy;
+            asm("mov.b64 %0, {%1, %2};" : "=l"(xy) : "r"(v[4 * c + 2 * y]), "r"(v[4 * c + 2 * y + 1]));
+            if (F::I8) asm("add.rn.f32x2 %0, %0, %1;" : "+l"(xy) : "l"(nm2[y]));
+            else asm("fma.rn.f32x2 %0, %0, %1, %2;" : "+l"(xy) : "l"(sc2), "l"(nm2[y]));
+            float x0, x1, e0, e1;
+            asm("mov.b64 {%0, %1}, %2;" : "=f"(x0), "=f"(x1) : "l"(xy));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(x0));
+            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(x1));
+            unsigned long long ee;
+            asm("mov.b64 %0, {%1, %2};" : "=l"(ee) : "f"(e0), "f"(e1));
+            asm("add.rn.f32x2 %0, %0, %1;" : "+l"(acc[y]) : "l"(ee));
+            if constexpr (F::I8) {
+              asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(ee) : "l"(f));
+              asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(ee));
+            }
+            pk[2 * c + y] = pack_bf16(e0, e1);
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          float a0, a1;
+          asm("mov.b64 {%0, %1}, %2;" : "=f"(a0), "=f"(a1) : "l"(acc[y]));
+          l[y] += a0 + a1;
+        }
         if (i != i0) {      // the product before has read its weights, and the accumulator is whole
           wait(b_odone(w), (j - 1) & 1);
           tc_fence_after();
-          if (__any_sync(0xffffffffu, alpha != 1.f)) {
+          if (grown) {
 #pragma unroll 1
-            for (int c = 0; c < 2 * NDK; ++c) {      // this thread's half of the row
-              uint32_t o[16];
+            for (int c = 0; c < NDK; ++c) {
               __syncwarp();
-              ld_16(t_o(w) + lane_addr + half * (D / 2) + c * 16, o);
+              TREE_LD_16x64(t_o(w) + half_addr + c * 64, v);
               tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              st_16(t_o(w) + lane_addr + half * (D / 2) + c * 16, o);
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * alpha[e >> 1 & 1]);
+              TREE_ST_16x64(t_o(w) + half_addr + c * 64, v);
             }
           }
         }
         __syncwarp();
-        st_16(t_p(w) + lane_addr + half * 16, pk);
+        st_16x32(t_p(w) + half_addr, pk);
         tmem_st_wait();
         tc_fence_before();
         warp_arrive(b_pfull(w));
       }
       // ---- the segment's sums, once its last product is done
       if (i0 < k.count) wait(b_odone(w), (j - 1) & 1);
-      // sums of the halves meet in the slots of the parity that the group's last tile did not use; maxima (one group's, for the other) in
-      // those that it used, behind the barrier that all threads come to
-      x_mine[(j & 1) * (2 * BQ)] = l;
-      pair_sync(pair);
-      l += x_other[(j & 1) * (2 * BQ)];
-      tc_fence_before();
-      if (NW == 1) {
-        if (half == 0) x_mine[((j & 1) ^ 1) * (2 * BQ)] = mref;      // read by the other group, at this group's parity
-        else x_mine[((j & 1) ^ 1) * (2 * BQ)] = l;
+      // maxima and sums of all rows, for the lanes that have the results (written anew behind the next segment's start, which all threads come to)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
+        l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+        if ((lane & 3) == 0) {
+          s_x[(w * 2) * BQ + mr + 8 * y] = mref[y];
+          s_x[(w * 2 + 1) * BQ + mr + 8 * y] = l[y];
+        }
       }
+      tc_fence_before();
       __syncwarp();
       asm volatile("bar.sync 9, 512;" ::: "memory");
       tc_fence_after();
       const bool whole = k.count == k.r.nt;
       const size_t slot = (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (k.u - k.count != k.u0)) * (NW * BQ) + rr;
       if (warp_ok) {
-        float f[2] = {1.f, 0.f}, best = mref, sum = l;
+        float f0 = 1.f, f1 = 1.f, best = s_x[(w * 2) * BQ + r], sum = s_x[(w * 2 + 1) * BQ + r];
         if constexpr (NW == 1) {
-          // tiles of the other group so far: its parity
-          const int other_j = (w == 0) ? (g0 + k.count) / 2 : (g0 + k.count + 1) / 2;
-          const float* xo = s_x + (w ^ 1) * 4 * BQ + ((other_j & 1) ^ 1) * (2 * BQ) + r;
-          const float mo = xo[0], lo2 = xo[BQ];
-          best = fmaxf(mref, mo);
-          const float fm = mref == -INFINITY ? 0.f : exp2f(mref - best), fo = mo == -INFINITY ? 0.f : exp2f(mo - best);
-          sum = l * fm + lo2 * fo;
-          f[w] = fm;
-          f[w ^ 1] = fo;
+          const float m0 = s_x[r], m1 = s_x[2 * BQ + r];
+          best = fmaxf(m0, m1);
+          f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - best);
+          f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - best);
+          sum = s_x[BQ + r] * f0 + s_x[3 * BQ + r] * f1;
         }
         const float inv = whole ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
         constexpr int NC = NW == 1 ? NDK : 2 * NDK;      // pieces of 16 columns that this thread writes: a quarter of the row, or half
@@ -739,7 +793,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              o[e] = __float_as_uint(((f[0] > 0.f ? f[0] * __uint_as_float(o[e]) : 0.f) + (f[1] > 0.f ? f[1] * __uint_as_float(o1[e]) : 0.f)) * inv);
+              o[e] = __float_as_uint(((f0 > 0.f ? f0 * __uint_as_float(o[e]) : 0.f) + (f1 > 0.f ? f1 * __uint_as_float(o1[e]) : 0.f)) * inv);
           } else {
             ld_16(t_o(w) + lane_addr + c0 + c * 16, o);
             tmem_ld_wait();
