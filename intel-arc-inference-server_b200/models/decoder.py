@@ -23,6 +23,7 @@ import torch
 
 from ..ops import lib as K
 from ..ops import logprob as LP
+from ..ops import tree as T
 from .config import ModelConfig, SandwichBlock
 from .oracle import rope_tables
 from .weights import ModelWeights, LayerWeights, QLinear
@@ -200,6 +201,7 @@ class DecoderModel:
         self.device = weights.embed.device
         self.max_rows = max_rows
         self.nsplit_attn = nsplit_attn
+        self.tree = None            # ``runtime.trees.TreeVerifier`` while the rows are nodes of token trees
         self.listed = None
         if cfg.layer_specs:
             from .listed import ListedLayers
@@ -340,11 +342,24 @@ class DecoderModel:
         else:
             K.resid_norm(0, m, cfg.hidden, lw.input_norm, cfg.rms_eps, b.resid, b.x, embed=self.w.embed, ctrl=ctrl, vocab=cfg.vocab, flag=b.flag)
 
+    def _rope_append(self, part, s: int, m: int, ctrl, block_table, max_blocks, kv: KVCache, li: int):
+        """The rows' qkv partial sums turned by their positions: queries into ``buf.q``, keys and values of layer ``li`` to their places."""
+        cfg, b = self.cfg, self.buf
+        if self.tree is not None:
+            T.rope_append(self.tree.step, part.view(-1)[: s * m * cfg.qkv_dim].view(s, m, cfg.qkv_dim), (self.cos_t, self.sin_t), b.q[:m], self.tree.caches[li])
+            return
+        kc, vc, ks, vs = kv.layer(li)
+        K.rope_append(part, m * cfg.qkv_dim, s, m, ctrl, block_table, max_blocks, self.cos_t, self.sin_t,
+                      cfg.n_q_heads, cfg.n_kv_heads, cfg.head_dim, b.q, kc, vc, ks, vs, kv.kv_int8)
+
     def _attention(self, m: int, ctrl, block_table, max_blocks, kv: KVCache, kc, vc, ks, vs, window: int = 0,
-                   quant_out: bool = False) -> bool:
+                   quant_out: bool = False, li: int = -1) -> bool:
         """Split-KV attention of the step's rows into ``buf.attn_out``.  Head size 128 (bf16 or int8 KV) goes to the
         tensor-core kernel that serves a request's consecutive rows together; the rest to the per-row kernel."""
         cfg, b = self.cfg, self.buf
+        if self.tree is not None:
+            T.attention(self.tree.step, b.q[:m], self.tree.caches[li], b.attn_out[:m], self.scale, max(window, 0))
+            return False
         if window == -1 and (cfg.head_dim != 128 or self.nsplit_attn > 64 or cfg.gqa > 16):
             raise NotImplementedError("block rows need the multi-row attention kernel (head size 128)")
         if self._attn_rows_ok(m) or window == -1:
@@ -390,9 +405,8 @@ class DecoderModel:
         cfg, b = self.cfg, self.buf
         part, s = self._gemv("qkv", lw.qkv, b.x, m)
         kc, vc, ks, vs = kv.layer(li)
-        K.rope_append(part, m * cfg.qkv_dim, s, m, ctrl, block_table, max_blocks, self.cos_t, self.sin_t,
-                      cfg.n_q_heads, cfg.n_kv_heads, cfg.head_dim, b.q, kc, vc, ks, vs, kv.kv_int8)
-        self._attention(m, ctrl, block_table, max_blocks, kv, kc, vc, ks, vs, self._window(li))
+        self._rope_append(part, s, m, ctrl, block_table, max_blocks, kv, li)
+        self._attention(m, ctrl, block_table, max_blocks, kv, kc, vc, ks, vs, self._window(li), li=li)
         return self._gemv("o", lw.o, b.attn_out, m)
 
     def ffn_block(self, lw: LayerWeights, m: int):
@@ -456,17 +470,16 @@ class DecoderModel:
         ``buf.ssq`` do."""
         cfg, b = self.cfg, self.buf
         kc, vc, ks, vs = kv.layer(li)
-        if self.rope_fold and not kv.kv_int8 and cfg.head_dim == 128 and lw.qkv.n == cfg.qkv_dim:
+        if self.rope_fold and self.tree is None and not kv.kv_int8 and cfg.head_dim == 128 and lw.qkv.n == cfg.qkv_dim:
             self._qkv_rope(lw, m, ctrl, block_table, max_blocks, kc, vc, x_ready)
         else:
             if x_ready:
                 part, s = self._gemv("qkv", lw.qkv, b.x, m)
             else:
                 part, s = self._gemv_fused("qkv", lw.qkv, b.resid, m, norm_w=lw.input_norm, x_mode=2)
-            K.rope_append(part, m * cfg.qkv_dim, s, m, ctrl, block_table, max_blocks, self.cos_t, self.sin_t,
-                          cfg.n_q_heads, cfg.n_kv_heads, cfg.head_dim, b.q, kc, vc, ks, vs, kv.kv_int8)
+            self._rope_append(part, s, m, ctrl, block_table, max_blocks, kv, li)
         q8 = self._attention(m, ctrl, block_table, max_blocks, kv, kc, vc, ks, vs, self._window(li),
-                             quant_out=lw.o.k == cfg.n_q_heads * 128)
+                             quant_out=lw.o.k == cfg.n_q_heads * 128, li=li)
         self._gemv_fused("o", lw.o, b.attn_out, m, fold=True, prequantised=q8)
         gu, s_gu = self._gemv_fused("gate_up", lw.gate_up, b.resid, m, norm_w=lw.post_norm, x_mode=2)
         self._gemv_fused("down", lw.down, gu, m, fold=True, x_mode=1, s_in=s_gu, x_slice=m * 2 * cfg.ffn)
@@ -497,17 +510,16 @@ class DecoderModel:
         from . import moe as _moe
         cfg, b = self.cfg, self.buf
         kc, vc, ks, vs = kv.layer(li)
-        if self.rope_fold and not kv.kv_int8 and cfg.head_dim == 128 and lw.qkv.n == cfg.qkv_dim:
+        if self.rope_fold and self.tree is None and not kv.kv_int8 and cfg.head_dim == 128 and lw.qkv.n == cfg.qkv_dim:
             self._qkv_rope(lw, m, ctrl, block_table, max_blocks, kc, vc, x_ready)
         else:
             if x_ready:
                 part, s = self._gemv("qkv", lw.qkv, b.x, m)
             else:
                 part, s = self._gemv_fused("qkv", lw.qkv, b.resid, m, norm_w=lw.input_norm, x_mode=2)
-            K.rope_append(part, m * cfg.qkv_dim, s, m, ctrl, block_table, max_blocks, self.cos_t, self.sin_t,
-                          cfg.n_q_heads, cfg.n_kv_heads, cfg.head_dim, b.q, kc, vc, ks, vs, kv.kv_int8)
+            self._rope_append(part, s, m, ctrl, block_table, max_blocks, kv, li)
         q8 = self._attention(m, ctrl, block_table, max_blocks, kv, kc, vc, ks, vs, self._window(li),
-                             quant_out=lw.o.k == cfg.n_q_heads * 128)
+                             quant_out=lw.o.k == cfg.n_q_heads * 128, li=li)
         self._gemv_fused("o", lw.o, b.attn_out, m, fold=True, prequantised=q8)
         # the experts and the router read normalised rows
         K.resid_norm(1, m, cfg.hidden, lw.post_norm, cfg.rms_eps, b.resid, b.x, resid_in=b.resid, splits=0)

@@ -51,8 +51,9 @@ class Engine:
     def __init__(self, weights: ModelWeights, max_seqs: int = 1, max_len: int = 4096, kv_dtype: str = "bf16",
                  max_rows: int = 64, use_graphs: bool = True, int8_head: bool = False, num_pages: Optional[int] = None,
                  nsplit_attn: int = 0, prefill_backend: str = "auto", tp=None, nccl=None,
-                 extra_kv_layers: int = 0):
-        """``tp``: wires of a tensor-parallel group; every rank builds the same Engine over its weight shard and
+                 extra_kv_layers: int = 0, tree_nodes: int = 0):
+        """``tree_nodes``: the slots have pages for trees of so many drafted tokens (``verify_trees``), out of ``num_pages`` where that is given.
+        ``tp``: wires of a tensor-parallel group; every rank builds the same Engine over its weight shard and
         is driven with the same calls (same rows, same order) -- the step's kernels do the crossings."""
         self.cfg = cfg = weights.cfg
         self.tp = tp if tp is not None and tp.world > 1 else None
@@ -61,8 +62,9 @@ class Engine:
         if cfg.layer_specs and weights.embed.dtype == torch.float32:
             kv_dtype = "f32"        # a model served in 32-bit keeps its cache in 32-bit
         self.max_blocks = (max_len + PAGE - 1) // PAGE
+        tree_blocks = (tree_nodes + PAGE - 1) // PAGE
         if num_pages is None:
-            num_pages = max_seqs * self.max_blocks + 1
+            num_pages = max_seqs * (self.max_blocks + tree_blocks) + 1
         if not nsplit_attn:     # sized for contexts near the longest one the engine holds
             nsplit_attn = attn_splits(cfg.n_kv_heads, max_len)
         self.model = DecoderModel(weights, max_rows=max_rows, max_pos=max_len, nsplit_attn=nsplit_attn,
@@ -70,7 +72,7 @@ class Engine:
         self.kv = KVCache(cfg, cfg.n_layers + extra_kv_layers, num_pages, self.device, kv_dtype,   # + draft-head layers
                           n_slots=max_seqs)
         self.kv_dtype = kv_dtype
-        self.pool = KvPool(num_pages, max_seqs, self.max_blocks)
+        self.pool = KvPool(num_pages, max_seqs * (2 if tree_nodes else 1), max(self.max_blocks, tree_blocks))      # (a slot's tree: ``max_seqs`` further)
         self.ctrl = torch.zeros(K.CTRL_WORDS, dtype=torch.int32, device=self.device)
         # pinned staging rings: a queued non-blocking copy may run long after the host moved on (see utils/staging.py)
         self.ctrl_stage = Staged((K.CTRL_WORDS,), torch.int32)
@@ -95,6 +97,10 @@ class Engine:
             from .buffer_registry import audit
             audit(self.model.buf, self.kv, cfg, kv_dtype, max_seqs)
         self._batch = None          # runner of mixed batches (models that list their layers)
+        self.trees = None
+        if tree_nodes:
+            from .trees import TreeVerifier
+            self.trees = TreeVerifier(self, tree_nodes)
         self.launches_per_step: Dict[Tuple[int, bool, bool], int] = {}
 
     def close(self):
@@ -468,6 +474,15 @@ class Engine:
         buf = ScoreBuffer(len(tokens), top, self.device)
         LP.token_logprobs(lg, torch.tensor(tokens, dtype=torch.int32).to(self.device), out=buf.out)
         return buf.read()
+
+    def verify_trees(self, trees: Dict[int, Tuple[Sequence[int], Sequence[int]]]) -> dict:
+        """One step over a tree of drafted tokens per slot (slot -> tokens, parents; node 0 is the slot's next token, with parent -1): slot ->
+        ``runtime.trees.Verified``, the greedy path through the tree and the token behind it.  Drafts that plain decoding would not make leave no trace;
+        to sample, ``trees.forward`` gives the rows' logits and ``trees.commit`` takes the drawn tokens."""
+        if self.trees is None:
+            raise ValueError("an engine without pages for trees: Engine(tree_nodes=...)")
+        self.trees.forward(trees)
+        return self.trees.commit()
 
     def decode_begin(self, slots: Sequence[int], tokens: Sequence[int]):
         """Arm plain decode: one row per slot, starting with ``tokens`` at each slot's current length."""

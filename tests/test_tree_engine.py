@@ -1,0 +1,139 @@
+"""Token trees through the engine: their step, settled, against plain decoding of the same models."""
+import random
+
+import pytest
+import torch
+
+from b200serve.models import config as C
+from b200serve.models.weights import random_weights
+from b200serve.runtime.engine import Engine, Row
+
+gpu = pytest.mark.gpu
+
+
+def engine(name, weights, **kw):
+    return Engine(weights, max_len=512, use_graphs=False, **kw)
+
+
+def make_tree(chain, vocab, rng, wrong=2):
+    """The chain's tokens with wrong ones beside them, in an order in which parents come first."""
+    tokens, parents, at = [chain[0]], [-1], 0
+    for t in chain[1:]:
+        places = [None] * wrong + [t]
+        rng.shuffle(places)
+        here = at
+        for x in places:
+            tokens.append(rng.randrange(vocab) if x is None else x)
+            parents.append(here)
+            if x is not None:
+                at = len(tokens) - 1
+    return tokens, parents
+
+
+def path_to(parents, i):
+    out = []
+    while i >= 0:
+        out.append(i)
+        i = parents[i]
+    return out[::-1]
+
+
+MODELS = {"tiny-dense": C.tiny_dense, "small-dense": C.small_dense, "small-windowed": C.small_windowed, "small-moe": C.small_moe}
+
+
+@gpu
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("name", MODELS)
+def test_logits_of_every_node(name, kv):
+    """A node's logits are those of its path decoded row by row (the same rows but for the order of sums: tolerance of the other step kernels)."""
+    cfg = MODELS[name]()
+    w = random_weights(cfg, device="cuda", seed=1)
+    rng = random.Random(5)
+    prompt = [rng.randrange(cfg.vocab) for _ in range(61)]
+    tree = ([rng.randrange(cfg.vocab) for _ in range(11)], [-1, 0, 0, 1, 1, 2, 3, 3, 6, 6, 9])
+    eng = engine(name, w, max_seqs=2, kv_dtype=kv, tree_nodes=16)
+    eng.prefill(1, prompt)
+    got = eng.trees.forward({1: tree}).clone()
+    assert eng.seq_len == [0, 61]
+    plain = engine(name, w, max_seqs=1, kv_dtype=kv)
+    plain.prefill(0, prompt)
+    for i in (0, 4, 5, 7, 10):
+        path = path_to(tree[1], i)
+        plain.truncate(0, len(prompt))
+        plain.forward_rows([Row(0, len(prompt) + d, tree[0][n]) for d, n in enumerate(path)])
+        want = plain.logits(len(path))
+        for d, n in enumerate(path):
+            # both sides round each layer's activations to bf16 from sums in other orders
+            assert (got[n] - want[d]).norm() <= 0.02 * want[d].norm(), (i, n)
+
+
+@gpu
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+@pytest.mark.parametrize("name", ["tiny-dense", "small-dense", "small-moe"])
+def test_decoding_with_trees(name, kv):
+    """Several requests decoded by trees that hold the right continuation, part of it or none: the tokens are those of plain decoding as long as that
+    has no near ties, and the positions count up by the accepted paths."""
+    cfg = MODELS[name]()
+    w = random_weights(cfg, device="cuda", seed=2)
+    rng = random.Random(9)
+    prompts = [[rng.randrange(cfg.vocab) for _ in range(n)] for n in (40, 7, 129)]
+    plain = engine(name, w, max_seqs=1, kv_dtype=kv)
+    want, clear = [], []
+    for p in prompts:
+        plain.reset(0)
+        tokens, sure = [plain.prefill(0, p)], [True]
+        for _ in range(24):
+            tokens.append(plain.forward_rows([Row(0, plain.seq_len[0], tokens[-1])])[0])
+            top = plain.logits(1)[0].topk(2).values
+            sure.append(bool(top[0] - top[1] > 0.05 * top[0].abs()))
+        want.append(tokens)
+        clear.append(sure)
+    eng = engine(name, w, max_seqs=4, kv_dtype=kv, tree_nodes=20)
+    out = {s: [eng.prefill(s, p)] for s, p in enumerate(prompts)}
+    follow = {s: out[s][0] == want[s][0] for s in out}
+    for round_ in range(5):
+        trees = {}
+        for s in out:
+            n = len(out[s])
+            ahead = want[s][n - 1: n + 3] if follow[s] else [out[s][-1]]
+            ahead[0] = out[s][-1]
+            keep = rng.choice((len(ahead), len(ahead), 1, 2))
+            trees[s] = make_tree(ahead[:keep], cfg.vocab, rng)
+        before = list(eng.seq_len)
+        got = eng.verify_trees(trees)
+        for s, v in got.items():
+            tokens, parents = trees[s]
+            assert v.path[0] == 0 and all(parents[b] == a for a, b in zip(v.path, v.path[1:]))
+            assert v.tokens == [tokens[i] for i in v.path] and eng.seq_len[s] == before[s] + len(v.path)
+            assert len(eng.pool.table(s)) == -(-eng.seq_len[s] // 16)
+            out[s] += v.tokens[1:] + [v.next_token]
+    checked = 0
+    for s in out:
+        for i, (a, b) in enumerate(zip(out[s], want[s])):
+            if not all(clear[s][: i + 1]):
+                break
+            assert a == b, (s, i)
+            checked += 1
+    assert checked >= 6       # (a seed whose first tokens are clear)
+
+
+@gpu
+def test_refusals():
+    cfg = C.tiny_dense()
+    w = random_weights(cfg, device="cuda", seed=1)
+    eng = engine("", w, max_seqs=2, tree_nodes=8)
+    with pytest.raises(ValueError, match="no trees"):
+        eng.trees.commit()
+    for bad in ({0: ([1, 2], [-1])}, {0: ([1, 2], [0, 0])}, {0: ([1, 2], [-1, 1])}, {0: ([1] * 9, [-1] + [0] * 8)}, {2: ([1], [-1])}, {0: ([], [])}, {}, {0: ([5000], [-1])}):
+        with pytest.raises(ValueError):
+            eng.verify_trees(bad)
+    assert eng.seq_len == [0, 0]
+    with pytest.raises(ValueError, match="pages for trees"):
+        engine("", w, max_seqs=1).verify_trees({0: ([1], [-1])})
+    hybrid = random_weights(C.small_hybrid(), device="cuda", seed=1)
+    with pytest.raises(ValueError, match="attention layers"):
+        engine("", hybrid, max_seqs=1, tree_nodes=8)
+    # a tree of one node on an empty slot
+    v = eng.verify_trees({1: ([3], [-1])})
+    assert v[1].path == [0] and v[1].tokens == [3] and eng.seq_len == [0, 1]
+    torch.cuda.synchronize()
