@@ -618,3 +618,167 @@ def test_refusals():
     no(T.commit, r.step, i32(8), i32(8), make_cache(r.pages, 2, 128, False))
     torch.cuda.synchronize()
     K.check_status()
+
+
+# ------------------------------------------------------------------ a run of them together
+class Loop:
+    """Requests that decode by trees, everything on the device: plan, one layer's append and attention, commit, lengths and pages carried from step
+    to step."""
+
+    def __init__(self, seed, i8=False, spare=40):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        self.b, self.nodes, self.n_q, self.n_kv, self.d = 3, 7, 4, 2, 64
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")       # noqa: E731
+        held = [2, 1, 0]
+        pages = 1 + 3 + 3 + spare
+        self.table = torch.zeros(3, 12, dtype=torch.int32, device="cuda")
+        self.table[0, :2], self.table[1, :1] = i32([1, 2]), i32([3])
+        self.pool = T.PagePool(torch.arange(7, 7 + spare, dtype=torch.int32, device="cuda"), i32([spare]), i32(held))
+        self.step = T.TreeStep(self.table, i32([[4], [5], [6]]), 3 * self.nodes, pages, self.nodes)
+        self.lengths, self.counts = i32([20, 16, 0]), i32([self.nodes, 3, self.nodes])
+        self.cache = make_cache(pages, self.n_kv, self.d, i8, seed)
+        self.accepted = T.Accepted(i32([[0] * 64] * 3), i32([0] * 3), i32([0] * 3), self.lengths)
+        rows = 2 * self.nodes + 3
+        self.parents, self.tokens, self.targets = i32([0] * rows), i32([0] * rows), i32([0] * rows)
+        self.qkv = torch.zeros(rows, (self.n_q + 2 * self.n_kv) * self.d, dtype=torch.bfloat16, device="cuda")
+        self.q, self.out = (torch.zeros(rows, self.n_q * self.d, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        angle = torch.arange(200, device="cuda")[:, None] * torch.tensor([0.3 ** i for i in range(32)], device="cuda")
+        self.rope = (angle.cos(), angle.sin())
+        self.g = g
+
+    def draw(self, rng):
+        one = [p for n in (self.nodes, 3, self.nodes) for p in tree_parents(n, rng, 2)]
+        i32 = lambda x: torch.tensor(x, dtype=torch.int32)       # noqa: E731
+        self.parents.copy_(i32(one))
+        self.tokens.copy_(i32([rng.randrange(2) for _ in one]))
+        self.targets.copy_(i32([rng.randrange(2) for _ in one]))
+        self.qkv.copy_(torch.randn(self.qkv.shape, device="cuda", generator=self.g))
+
+    def run(self):
+        T.plan(self.step, self.lengths, self.counts, self.parents, self.pool)
+        T.rope_append(self.step, self.qkv, self.rope, self.q, self.cache)
+        T.attention(self.step, self.q, self.cache, self.out, 0.125)
+        T.commit(self.step, self.tokens, self.targets, self.cache, self.accepted)
+
+    def state(self):
+        return [t.clone() for t in (self.lengths, self.table, self.pool.n_free, self.pool.held, self.out, self.cache.k, self.cache.v, self.accepted.path, self.accepted.next_token)]
+
+
+@gpu
+@pytest.mark.parametrize("i8", [False, True])
+def test_loop_in_a_graph(i8):
+    """Steps replayed from a CUDA graph, which no host number enters, are the steps run one by one; and those are right: what is in the cache at the
+    end is what attention over plain rows at the requests' positions sees."""
+    a, b = Loop(1, i8), Loop(1, i8)
+    ra, rb = random.Random(4), random.Random(4)
+    for _ in range(2):
+        a.draw(ra), b.draw(rb), a.run(), b.run()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        b.run()
+    total = 0
+    for _ in range(12):
+        a.draw(ra), b.draw(rb)
+        a.run()
+        graph.replay()
+        torch.cuda.synchronize()
+        a.step.check(), b.step.check()
+        K.check_status()
+        for x, y in zip(a.state(), b.state()):
+            assert torch.equal(x, y)
+        assert 3 <= a.accepted.count.sum().item() <= 17
+        total += a.accepted.count.sum().item()
+    assert a.lengths.sum().item() >= 36 + total
+    held, table = a.pool.held.tolist(), a.table.tolist()
+    used = [p for r in range(3) for p in table[r][: held[r]]]
+    assert len(set(used)) == len(used) and 0 not in used
+    assert all(h * PAGE >= n for h, n in zip(held, a.lengths.tolist()))
+
+
+@gpu
+def test_keys_after_commits():
+    """Keys that a loop of steps left at a request's positions are the accepted nodes' rows, turned by those positions."""
+    a, rng = Loop(2), random.Random(8)
+    want = {r: [] for r in range(3)}
+    start = a.lengths.tolist()
+    for _ in range(6):
+        a.draw(rng)
+        before, rows = a.lengths.tolist(), a.qkv.clone()
+        a.run()
+        path, count, first = a.accepted.path.tolist(), a.accepted.count.tolist(), a.step.row_start.tolist()
+        for r in range(3):
+            for i in range(count[r]):
+                want[r].append((before[r] + i, rows[first[r] + path[r][i]]))
+    table = a.table.tolist()
+    freq = torch.tensor([0.3 ** i for i in range(32)], device="cuda")
+    for r in range(3):
+        assert [p for p, _ in want[r]] == list(range(start[r], a.lengths[r].item()))
+        for pos, row in want[r]:
+            key = row.reshape(-1, a.d)[a.n_q: a.n_q + a.n_kv]
+            turned = rope_reference(key[None], torch.tensor([pos], device="cuda"), freq.double(), False)[0]
+            got = a.cache.k[table[r][pos // PAGE], :, pos % PAGE].double()
+            # tables of fp32 angles: off by 2^-24 of an angle up to 200, and the rounding to bf16
+            assert ((got - turned).abs() <= HALF * turned.abs() + 200 * 2.0 ** -23 * key.double().abs().amax(-1, keepdim=True)).all()
+            assert torch.equal(a.cache.v[table[r][pos // PAGE], :, pos % PAGE], row.reshape(-1, a.d)[a.n_q + a.n_kv:])
+
+
+@gpu
+def test_two_calls_at_once():
+    """Layers of one step on two streams, and steps of their own, share nothing."""
+    s = State([3000, 700, 64, 5], [16, 9, 30, 2]).cuda()
+    s.plan()
+    caches = [make_cache(s.pages, 8, 128, i8, seed) for seed, i8 in ((1, False), (2, True), (3, False), (4, False))]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = [torch.randn(s.max_rows, 40 * 128, device="cuda", generator=g).bfloat16() for _ in caches]
+    want, got = [torch.empty_like(x) for x in q], [torch.empty_like(x) for x in q]
+    for x, c, o in zip(q, caches, want):
+        T.attention(s.step, x, c, o, 0.09)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in caches]
+    for _ in range(20):
+        for x, c, o, st in zip(q, caches, got, streams):
+            with torch.cuda.stream(st):
+                T.attention(s.step, x, c, o, 0.09)
+    torch.cuda.synchronize()
+    K.check_status()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("i8", [False, True])
+def test_far_pages(i8):
+    """Pages whose elements lie beyond 2^32 bytes, and beyond 2^31 elements of a layer, from its beginning."""
+    pages, n_kv, d = 150000, 8, 128
+    s = State([200, 33], [20, 7])
+    near = s.pages
+    move = lambda p: p and p + pages - near       # noqa: E731  (the same pages at the end of a large cache)
+    s.table, s.tree_table, s.free = [[move(p) for p in t] for t in s.table], [[move(p) for p in t] for t in s.tree_table], [move(p) for p in s.free]
+    s.pages = pages
+    small = make_cache(near, n_kv, d, i8, 7)
+    dtype = torch.int8 if i8 else torch.bfloat16
+    k, v = (torch.zeros(pages, n_kv, PAGE, d, dtype=dtype, device="cuda") for _ in range(2))
+    k[pages - near:], v[pages - near:] = small.k, small.v
+    if i8:
+        ks, vs = (torch.ones(pages, n_kv, PAGE, device="cuda") for _ in range(2))
+        ks[pages - near:], vs[pages - near:] = small.k_scale, small.v_scale
+    cache = T.TreeCache(k, v, ks, vs) if i8 else T.TreeCache(k, v)
+    run_attention(s, (16, n_kv, d), i8, cache=cache)
+    rows = s.rows
+    qkv = torch.randn(rows, (16 + 2 * n_kv) * d, device="cuda")
+    q = torch.empty(rows, 16 * d, dtype=torch.bfloat16, device="cuda")
+    table = torch.ones(400, 64, device="cuda"), torch.zeros(400, 64, device="cuda")
+    T.rope_append(s.step, qkv, table, q, cache)
+    slots = s.step.slots[:rows].long()
+    y = qkv.reshape(rows, -1, d)[:, 16: 16 + n_kv]
+    if not i8:
+        assert torch.equal(cache.k[slots // PAGE, :, slots % PAGE], y.bfloat16())
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")       # noqa: E731
+    was = cache.v[slots[0] // PAGE, :, slots[0] % PAGE].clone()
+    got = T.commit(s.step, i32([1] * rows), i32([0] * rows), cache)
+    assert got.count.tolist() == [1, 1]
+    page = s.t_table[0, 200 // PAGE].item()
+    assert page > pages - near and torch.equal(cache.v[page, :, 200 % PAGE], was)
+    K.check_status()
