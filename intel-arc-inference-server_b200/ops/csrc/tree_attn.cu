@@ -676,26 +676,24 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 #pragma unroll
           for (int c = 1; c < 8; ++c) asm("max.f32 %0, %0, %1, %2;" : "+f"(top[y]) : "f"(__uint_as_float(v[4 * c + 2 * y])), "f"(__uint_as_float(v[4 * c + 2 * y + 1])));
         }
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-          const float a = __shfl_xor_sync(0xffffffffu, top[0], o), b = __shfl_xor_sync(0xffffffffu, top[1], o);
-          top[0] = fmaxf(top[0], a);
-          top[1] = fmaxf(top[1], b);
-        }
         top[0] *= factor;
         top[1] *= factor;
-        // a row whose maximum grew by more than 2^kLazy gets a new reference: rare, and all of the warp goes that way
+        // A row whose maximum grew by more than 2^kLazy gets a new reference: rare, and all of the warp goes that way.  (Only there do a row's four
+        // threads ask one another.)
         const bool grown = __any_sync(0xffffffffu, top[0] > mref[0] + kLazy || top[1] > mref[1] + kLazy);
         float alpha[2] = {1.f, 1.f};
         if (grown) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
+          for (int y = 0; y < 2; ++y) {
+            top[y] = fmaxf(top[y], __shfl_xor_sync(0xffffffffu, top[y], 1));
+            top[y] = fmaxf(top[y], __shfl_xor_sync(0xffffffffu, top[y], 2));
             if (top[y] > mref[y] + kLazy) {
               alpha[y] = exp2f(mref[y] - top[y]);      // 0 at the row's first key
               mref[y] = top[y];
               l[y] *= alpha[y];
               asm("mov.b64 %0, {%1, %1};" : "=l"(nm2[y]) : "f"(-top[y]));
             }
+          }
         }
         unsigned long long sc2, acc[2] = {0ull, 0ull};
         asm("mov.b64 %0, {%1, %1};" : "=l"(sc2) : "f"(factor));
