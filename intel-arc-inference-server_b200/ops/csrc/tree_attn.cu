@@ -226,9 +226,44 @@ __device__ __forceinline__ bool next_segment(const TreeAttnParams& p, const int*
   }
 }
 
+// Tiles that some rows may see less of than others: the tree's, and with a window those that it begins in for any of the tree's rows.
+__device__ __forceinline__ bool uneven(const TreeAttnParams& p, const Req& r, int t) {
+  return t == r.nt - 1 || (p.window > 0 && (r.first + t) * BK < r.length + r.n - p.window);
+}
+
+// Values that are no numbers, in uneven tiles: a product with a weight of 0 would give them to rows that do not see them, so the tile has zeros
+// there, and the rows that see them get them here, behind their results (`out`, or the partial sums `part`, `apart` floats from one four columns to
+// the next).  Such a value decides its sum whatever its weight is.
+template <class F>
+__device__ __noinline__ void add_no_numbers(const TreeAttnParams& p, const Req r, int h, int ts, int count, int row, int c0, int columns, __nv_bfloat16* out, float* part,
+                                            int apart) {
+  const int lo = p.window > 0 ? p.row_pos[row] - p.window + 1 : 0;
+  const unsigned long long mask = p.masks[row];
+  for (int t = ts; t < ts + count; ++t) {
+    if (!uneven(p, r, t)) continue;
+    const bool tree = t == r.nt - 1;
+    const int key0 = (r.first + t) * BK, keys = tree ? r.n : min(BK, r.length - key0);
+    for (int x = 0; x < keys; ++x) {
+      const int i = (tree ? x : key0 + x) / kPage;
+      if (tree ? !(mask >> x & 1) || (p.window > 0 && p.row_pos[r.r0 + x] < lo) : key0 + x < lo) continue;
+      int page = tree ? i < p.tree_blocks ? p.tree_table[(size_t)r.b * p.tree_blocks + i] : 0 : p.block_table[(size_t)r.b * p.max_blocks + i];
+      if (page < 0 || page >= p.num_pages) page = 0;
+      const long long at = ((long long)page * p.n_kv + h) * kPage + x % kPage;
+      for (int c = 0; c < columns; ++c) {
+        float f;
+        if (F::I8) f = (float)p.v8[at * F::D + c0 + c] * p.v_scale[at];
+        else f = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.v8)[at * F::D + c0 + c]);
+        if (f - f == 0.f) continue;
+        if (out) out[c] = __float2bfloat16(__bfloat162float(out[c]) + f);
+        else part[(c >> 2) * apart + (c & 3)] += f;
+      }
+    }
+  }
+}
+
 template <class F>
 __global__ void __launch_bounds__(F::kThreads, 1)
-tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const TreeAttnParams p) {
+tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeAttnParams p) {
   constexpr int NDK = F::NDK, NW = F::NW, KS = F::KS, VS = F::VS, D = F::D, RS = F::I8 ? F::RS : 1;
   constexpr int kStep = NW == 1 ? 2 : 1;      // a group's next tile
   extern __shared__ uint8_t smem_raw[];
@@ -247,8 +282,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto b_scale = [&](int g) { return bars + 744 + (g % kScales) * 8; };
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gen + F::OFF_BAR + 808);
   int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 816);      // [32], [8]
+  volatile int* const s_odd = s_sums + 40;         // [8]: the segment's number, where its uneven tiles have values that are no numbers
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
+  if (tid < 8) s_odd[tid] = 0;
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) {
       mbar_init(b_kfull + 8 * i, F::I8 ? F::kConvThreads / 64 : 1);
@@ -620,6 +657,34 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const int i0 = NW == 1 ? (w - g0) & 1 : 0;
       for (int i = i0; i < k.count; i += kStep, ++j) {
         const int g = g0 + i, t = k.ts + i;
+        if (!F::I8 && uneven(p, k.r, t)) {
+          // the tile's values while its scores are made (the place's values before were used: two tiles of the group ago at the latest)
+          static_assert(F::I8 || VS >= 4, "places of values");
+          wait(b_vfull + 8 * (g % VS), (g / VS) & 1);
+          const int pieces = keys_of(t) * (NDK * 8);
+          bool odd = false;
+          for (int x = tid - (F::kSoft + 8 * w) * 32; x < pieces; x += 256) {
+            const uint32_t at = v_s0 + (g % VS) * F::T_BYTES + (x & (NDK - 1)) * (BK * 128) + (x >> (NDK - 1)) * 16;
+            uint32_t u[4], any = 0;
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(at));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7fff7fffu) + 0x00800080u;      // the sign bit: an exponent of ones
+            if (any & 0x80008000u) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((u[e] & 0x7f80u) == 0x7f80u) u[e] &= 0xffff0000u;
+                if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0xffffu;
+              }
+              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+              odd = true;
+            }
+          }
+          if (odd) {
+            s_odd[seg & 7] = seg;
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+        }
         wait(b_sfull(w), j & 1);
         if (F::I8) wait(b_scale(g), (g / kScales) & 1);
         if (!some) {      // rows of nobody: the products take what is there
@@ -756,6 +821,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       for (int y = 0; y < 2; ++y) {
         l[y] += __shfl_xor_sync(0xffffffffu, l[y], 1);
         l[y] += __shfl_xor_sync(0xffffffffu, l[y], 2);
+        if (l[y] != l[y]) mref[y] = INFINITY;      // (no number as a score: what is made of the row is none either)
         if ((lane & 3) == 0) {
           s_x[(w * 2) * BQ + mr + 8 * y] = mref[y];
           s_x[(w * 2 + 1) * BQ + mr + 8 * y] = l[y];
@@ -776,7 +842,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - best);
           sum = s_x[BQ + r] * f0 + s_x[3 * BQ + r] * f1;
         }
-        const float inv = whole ? (sum > 0.f ? 1.f / sum : 0.f) : 1.f;
+        const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
         constexpr int NC = NW == 1 ? NDK : 2 * NDK;      // pieces of 16 columns that this thread writes: a quarter of the row, or half
         const int c0 = NW == 1 ? (w * 2 + half) * NC * 16 : half * NC * 16;
         __nv_bfloat16* dst = p.out + row * p.ldo + head * D + c0;
@@ -791,7 +857,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-              o[e] = __float_as_uint(((f0 > 0.f ? f0 * __uint_as_float(o[e]) : 0.f) + (f1 > 0.f ? f1 * __uint_as_float(o1[e]) : 0.f)) * inv);
+              o[e] = __float_as_uint(((f0 != 0.f ? f0 * __uint_as_float(o[e]) : 0.f) + (f1 != 0.f ? f1 * __uint_as_float(o1[e]) : 0.f)) * inv);
           } else {
             ld_16(t_o(w) + lane_addr + c0 + c * 16, o);
             tmem_ld_wait();
@@ -817,6 +883,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(part + (size_t)(c * 4 + e) * (NW * BQ * 4)) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
+        if (row_ok && s_odd[seg & 7] == seg)
+          add_no_numbers<F>(p, k.r, k.h, k.ts, k.count, row, c0, NC * 16, whole ? dst : nullptr, part, NW * BQ * 4);
         if (!whole && row_ok && half == 0 && (NW == 2 || w == 0)) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(best, sum);
       }
       __syncwarp();
@@ -835,8 +903,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     constexpr int PL = F::KS;
     static_assert(!F::I8 || F::KS == F::VS, "places of keys and values");
     bool ok = true;
-    int g = 0, rs = 0, rpar = 0, ps = 0, ppar = 1;
-    while (ok && next_segment<F>(p, s_cum, s_req, k))
+    int g = 0, seg = 0, rs = 0, rpar = 0, ps = 0, ppar = 1;      // (fewer than eight tiles ahead of the softmax: `s_odd`)
+    while (ok && next_segment<F>(p, s_cum, s_req, k)) {
+      ++seg;
       for (int i = 0; i < k.count; ++i, ++g) {
         const uint32_t st = st_s0 + rs * F::S_BYTES + (is_v ? BK * D : 0), dst = tile0 + ps * F::T_BYTES;
         ok = warp_wait(b_rfull + 8 * rs, rpar);
@@ -847,7 +916,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         // not reach a sum.
         static_assert(kScales >= F::KS + 4, "scales of tiles under way");
         if (ct < BK) {
-          const float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + (is_v ? BK * 4 : 0) + ct * 4);
+          float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + (is_v ? BK * 4 : 0) + ct * 4);
+          if (is_v && f - f != 0.f && ct < keys_of(k.ts + i) && uneven(p, k.r, k.ts + i)) {      // (add_no_numbers)
+            f = 0.f;
+            s_odd[seg & 7] = seg;
+          }
           s_scale[(g % kScales) * (2 * BK) + (is_v ? BK : 0) + ct] = ct >= keys_of(k.ts + i) ? 0.f : f * (is_v ? kByteScale : p.scale_log2 * kByteScale);
           warp_arrive(b_scale(g));
         }
@@ -872,6 +945,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (++rs == RS) { rs = 0; rpar ^= 1; }
         if (++ps == PL) { ps = 0; ppar ^= 1; }
       }
+    }
   }
   __syncwarp();
   tc_fence_before();
@@ -929,7 +1003,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttnParams p,
 #pragma unroll
     for (int y = 0; y < U; ++y) {
       const float f = ml[y].x == -INFINITY ? 0.f : exp2f(ml[y].x - best);
-      if (f > 0.f) {
+      if (f != 0.f) {
         sum += f * ml[y].y;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
@@ -938,7 +1012,7 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttnParams p,
       }
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < 2; ++e) {
     s_out[lane][4 * warp + 2 * e] = pack_bf16(acc[e][0] * inv, acc[e][1] * inv);

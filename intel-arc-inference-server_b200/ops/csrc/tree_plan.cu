@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
   const bool tree = p.parents != nullptr, mine = tid < p.B, up_here = tree && p.rows <= kUpRows;
   if (tid == 0) s_status = 0;
   const int count = mine ? p.counts[tid] : 0, held = mine ? p.held[tid] : 0, n_free = *p.n_free;
-  const int length = mine && count >= 0 ? p.lengths[tid] : 0;
+  const int given = mine ? p.lengths[tid] : 0, length = count >= 0 ? given : 0;
   if (up_here)
     for (int r = tid; r < p.rows; r += threads) {
       const int up = p.parents[r];
@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
       for (int i = 0; i < (int)(want - held); ++i) p.block_table[(size_t)tid * p.max_blocks + held + i] = p.free[top - take0 - i];
     if (mine) {
       p.held_out[tid] = status ? held : left ? 0 : (int)want;
-      p.out_lengths[tid] = status ? 0 : length;
+      p.out_lengths[tid] = status ? given : length;
     }
     if (tid == 0) p.n_free_out[0] = status ? n_free : (int)(n_free + back - take);
     for (int b = tid; b <= p.B; b += threads) p.row_start[b] = status ? 0 : s_start[b];

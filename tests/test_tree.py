@@ -190,6 +190,7 @@ def test_plan_that_cannot_be_made(name):
     if bit != 64:
         assert all(torch.equal(a, b) for a, b in zip(before, (s.t_table, s.t_held, s.t_n, s.t_free)))
         assert s.step.row_start.tolist() == [0] * (s.b + 1) and set(s.step.slots.tolist()) == {-1}
+        assert torch.equal(s.step.lengths, s.t_lengths)      # (what commit says behind it, too)
     else:
         assert s.step.slots.tolist()[2:] == [-1, -1] and min(s.step.slots.tolist()[:2]) >= 0
 
@@ -278,7 +279,7 @@ ATTENTIONS = {
 HEADS = {"gqa5": (10, 2, 128), "gqa1": (3, 3, 128), "gqa4 d64": (8, 2, 64), "gqa16": (16, 1, 128), "gqa7 d64": (7, 1, 64)}
 
 
-def run_attention(s, heads, i8, window=0, scale=None, seed=0, masks=None, cache=None, pad=0, qscale=1.5):
+def run_attention(s, heads, i8, window=0, scale=None, seed=0, masks=None, cache=None, pad=0, qscale=1.5, clean=None, special=None):
     n_q, n_kv, d = heads
     s.cuda()
     s.plan()
@@ -293,9 +294,13 @@ def run_attention(s, heads, i8, window=0, scale=None, seed=0, masks=None, cache=
     T.attention(s.step, q, cache, out, scale, window)
     torch.cuda.synchronize()
     K.check_status()
-    want, tol = attention_reference(s, q, cache, scale, window, masks)
+    want, tol = attention_reference(s, q, clean or cache, scale, window, masks)
     got = out.double().reshape(want.shape)
-    bad = (got - want).abs()[: s.rows] > tol[: s.rows]
+    if special is not None:      # no numbers where a sum has one, numbers elsewhere
+        odd = ~torch.isfinite(special)
+        assert torch.equal(got[odd].nan_to_num(-7.0, 1e30, -1e30), special[odd].nan_to_num(-7.0, 1e30, -1e30))
+        got = torch.where(odd, want, got)
+    bad = ~((got - want).abs()[: s.rows] <= tol[: s.rows])
     assert not bad.any(), ((got - want).abs()[: s.rows] - tol[: s.rows]).max()
     assert (out[s.rows:] == 7.0).all()
     return q, cache, out
@@ -347,6 +352,101 @@ def test_attention_places_that_nobody_sees(value, i8):
     for name in ("k", "v") + (("k_scale", "v_scale") if i8 else ()):
         getattr(cache, name)[at // PAGE, :, at % PAGE] = getattr(whole, name)[at // PAGE, :, at % PAGE]
     run_attention(s, (6, 2, 128), i8, cache=cache)
+
+
+MIXED = {      # requests of one tile and of many, one part and several
+    "short": dict(lengths=[37, 0, 64, 130], counts=[5, 3, 17, 64]),
+    "long tables": dict(lengths=[37, 0, 64, 130, 2100], counts=[5, 3, 17, 64, 30], blocks=200),
+}
+
+
+@gpu
+@pytest.mark.parametrize("window", [0, 20, 70])
+@pytest.mark.parametrize("heads", [(6, 2, 128), (8, 1, 64), (5, 5, 64), (16, 2, 128)])
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("name", MIXED)
+def test_attention_values_that_some_rows_see(name, i8, heads, window):
+    """Infinities and NaN among the values of a node, or of a position at a window's edge, are theirs alone who see it."""
+    n_q, n_kv, d = heads
+    s = State(**MIXED[name])
+    cache, clean = (make_cache(s.pages, n_kv, d, i8, 5) for _ in range(2))
+    special = torch.zeros(s.rows, n_q, d, dtype=torch.float64, device="cuda")
+    row = 0
+    for r, (length, c) in enumerate(zip(s.lengths, s.counts)):
+        at, (mask, depth) = slots_of(s, r, s.table), ancestors(s.parents[r])
+        near = [j for j in range(length) if window and j >= length - window - 1]
+        for j in s.rng.sample(near, min(3, len(near))) + [length + x for x in s.rng.sample(range(c), min(c, 4))]:
+            page, place, h, value = at[j] // PAGE, at[j] % PAGE, s.rng.randrange(n_kv), s.rng.choice([INF, -INF, NAN])
+            if i8:
+                cache.v_scale[page, h, place], clean.v_scale[page, h, place] = value, 0.0
+                v = cache.v[page, h, place].double() * value
+            else:
+                dims = s.rng.sample(range(d), 5)
+                cache.v[page, h, place, dims], clean.v[page, h, place, dims] = value, 0.0
+                v = torch.zeros(d, dtype=torch.float64, device="cuda")
+                v[dims] = value
+            for i in range(c):
+                pos, sees = j if j < length else length + depth[j - length], j < length or mask[i] >> (j - length) & 1
+                if sees and (not window or pos > length + depth[i] - window):
+                    special[row + i, h * (n_q // n_kv): (h + 1) * (n_q // n_kv)] += v
+        row += c
+    run_attention(s, heads, i8, window, cache=cache, clean=clean, special=special)
+
+
+@gpu
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("name", MIXED)
+def test_attention_scores_that_are_no_numbers(name, i8):
+    """A query with a NaN, a key with an infinity: no numbers in the rows that they belong to or that see them, all others as ever."""
+    s = State(**MIXED[name]).cuda()
+    s.plan()
+    s.step.check()
+    cache = make_cache(s.pages, 2, 128, i8, 5)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(s.rows, 6 * 128, device="cuda", generator=g).bfloat16()
+    want, got = torch.empty_like(q), torch.empty_like(q)
+    T.attention(s.step, q, cache, want, 0.1)
+    odd = torch.zeros(s.rows, 6, dtype=torch.bool, device="cuda")
+    q[2, 130], q[4, 0] = NAN, INF      # heads 1 and 0
+    odd[2, 1] = odd[4, 0] = True
+    row = 0
+    for r, c in enumerate(s.counts):
+        slot, mask = slots_of(s, r, s.table)[s.lengths[r] + c - 2], ancestors(s.parents[r])[0]
+        if i8:
+            cache.k_scale[slot // PAGE, 1, slot % PAGE] = INF
+        else:
+            cache.k[slot // PAGE, 1, slot % PAGE, 9] = INF
+        for i in range(c):
+            odd[row + i, 3:] |= bool(mask[i] >> (c - 2) & 1)
+        row += c
+    T.attention(s.step, q, cache, got, 0.1)
+    torch.cuda.synchronize()
+    K.check_status()
+    got, want = got.reshape(s.rows, 6, 128), want.reshape(s.rows, 6, 128)
+    # (an infinite score above all others, or a NaN: every weight is NaN; one below all others: its weight is 0)
+    x = torch.isnan(got).all(2)
+    assert not (x & ~odd).any() and torch.equal(got[~odd], want[~odd])
+    assert x[2, 1] and x[4, 0]
+    numbers = torch.isfinite(got).all(2)
+    assert (numbers | x).all() and x[odd].sum() > odd.sum() // 4
+
+
+@gpu
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("heads", [(10, 2, 128), (7, 1, 64)])
+@pytest.mark.parametrize("name", ATTENTIONS)
+def test_attention_long_tables(name, heads, i8):
+    """Tables far longer than what is in them: parts over requests instead of a CTA for each."""
+    run_attention(State(**ATTENTIONS[name], blocks=400), heads, i8)
+
+
+@gpu
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("blocks", [20, 100])
+@pytest.mark.parametrize("heads,window", [((2, 2, 64), 0), ((12, 2, 128), 0), ((4, 1, 128), 33)])
+def test_attention_many_requests(heads, window, blocks, i8):
+    """More requests than a CTA keeps the numbers of."""
+    run_attention(State([(91 * i) % 270 for i in range(700)], [(5 * i) % 7 - (i % 9 == 0) if (5 * i) % 7 else 0 for i in range(700)], blocks=blocks), heads, i8, window)
 
 
 @gpu
