@@ -158,6 +158,9 @@ __device__ __forceinline__ bool elect() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
   return ok != 0;
 }
+__device__ __forceinline__ void ld_shared(uint32_t at, uint32_t* r) {
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at));
+}
 // One arrival for a warp: 32 lanes that arrive at one barrier are served one after another.
 __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   __syncwarp();
@@ -193,6 +196,17 @@ struct Walk {
   Req r;
   int h, ts, count, tok;       // key head, first tile and tiles of the segment, nodes of the CTA's group
 };
+
+__device__ __forceinline__ void begin_walk(const TreeAttnParams& p, const int* s_cum, int total, int each, Walk& k) {
+  k.u0 = k.u = min(total, (int)blockIdx.x * each);
+  k.u1 = min(total, k.u0 + each);
+  int lo = 0, hi = p.B - 1;      // the last request that begins at or before u0
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (s_cum[mid] * p.n_kv <= k.u0) lo = mid; else hi = mid - 1;
+  }
+  k.b = lo;
+}
 
 // s_req: tiles, cached positions and first row of up to kKept requests
 template <class F>
@@ -231,31 +245,47 @@ __device__ __forceinline__ bool uneven(const TreeAttnParams& p, const Req& r, in
   return t == r.nt - 1 || (p.window > 0 && (r.first + t) * BK < r.length + r.n - p.window);
 }
 
-// Values that are no numbers, in uneven tiles: a product with a weight of 0 would give them to rows that do not see them, so the tile has zeros
-// there, and the rows that see them get them here, behind their results (`out`, or the partial sums `part`, `apart` floats from one four columns to
-// the next).  Such a value decides its sum whatever its weight is.
+// Values that are no numbers, in uneven tiles: a product with a weight of 0 would give them to rows that do not see them, so such a tile has zeros
+// there, and where that was so the CTA goes through its segments once more when all is done, and adds them to the results (or partial sums) of the
+// rows that see them.  Such a value decides its sum whatever its weight is.
 template <class F>
-__device__ __noinline__ void add_no_numbers(const TreeAttnParams& p, const Req r, int h, int ts, int count, int row, int c0, int columns, __nv_bfloat16* out, float* part,
-                                            int apart) {
-  const int lo = p.window > 0 ? p.row_pos[row] - p.window + 1 : 0;
-  const unsigned long long mask = p.masks[row];
-  for (int t = ts; t < ts + count; ++t) {
-    if (!uneven(p, r, t)) continue;
-    const bool tree = t == r.nt - 1;
-    const int key0 = (r.first + t) * BK, keys = tree ? r.n : min(BK, r.length - key0);
-    for (int x = 0; x < keys; ++x) {
-      const int i = (tree ? x : key0 + x) / kPage;
-      if (tree ? !(mask >> x & 1) || (p.window > 0 && p.row_pos[r.r0 + x] < lo) : key0 + x < lo) continue;
-      int page = tree ? i < p.tree_blocks ? p.tree_table[(size_t)r.b * p.tree_blocks + i] : 0 : p.block_table[(size_t)r.b * p.max_blocks + i];
-      if (page < 0 || page >= p.num_pages) page = 0;
-      const long long at = ((long long)page * p.n_kv + h) * kPage + x % kPage;
-      for (int c = 0; c < columns; ++c) {
-        float f;
-        if (F::I8) f = (float)p.v8[at * F::D + c0 + c] * p.v_scale[at];
-        else f = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.v8)[at * F::D + c0 + c]);
-        if (f - f == 0.f) continue;
-        if (out) out[c] = __float2bfloat16(__bfloat162float(out[c]) + f);
-        else part[(c >> 2) * apart + (c & 3)] += f;
+__device__ __noinline__ void add_no_numbers(const TreeAttnParams& p, const int* s_cum, const int* s_req, int each) {
+  constexpr int C = 8, D = F::D, R = F::NW * BQ;
+  Walk k;
+  begin_walk(p, s_cum, s_cum[p.B] * p.n_kv, each, k);
+  while (next_segment<F>(p, s_cum, s_req, k)) {
+    const Req& r = k.r;
+    for (int item = threadIdx.x; item < k.tok * p.gqa * (D / C); item += F::kThreads) {
+      const int rr = item / (D / C), c0 = item % (D / C) * C, row = r.r0 + (int)blockIdx.y * p.group_tokens + rr / p.gqa, head = k.h * p.gqa + rr % p.gqa;
+      const int lo = p.window > 0 ? p.row_pos[row] - p.window + 1 : 0;
+      const unsigned long long mask = p.masks[row];
+      float more[C] = {};
+      for (int t = k.ts; t < k.ts + k.count; ++t) {
+        if (!uneven(p, r, t)) continue;
+        const bool tree = t == r.nt - 1;
+        const int key0 = (r.first + t) * BK, keys = tree ? r.n : min(BK, r.length - key0);
+        for (int x = 0; x < keys; ++x) {
+          const int i = (tree ? x : key0 + x) / kPage;
+          if (tree ? !(mask >> x & 1) || (p.window > 0 && p.row_pos[r.r0 + x] < lo) : key0 + x < lo) continue;
+          int page = tree ? i < p.tree_blocks ? p.tree_table[(size_t)r.b * p.tree_blocks + i] : 0 : p.block_table[(size_t)r.b * p.max_blocks + i];
+          if (page < 0 || page >= p.num_pages) page = 0;
+          const long long at = ((long long)page * p.n_kv + k.h) * kPage + x % kPage;
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            float f;
+            if (F::I8) f = (float)p.v8[at * D + c0 + c] * p.v_scale[at];
+            else f = __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.v8)[at * D + c0 + c]);
+            if (f - f != 0.f) more[c] += f;
+          }
+        }
+      }
+      const size_t slot = (((size_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + (k.u - k.count != k.u0)) * R;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        if (more[c] == 0.f) continue;
+        __nv_bfloat16* o = p.out + row * p.ldo + head * D + c0 + c;
+        if (k.count == r.nt) *o = __float2bfloat16(__bfloat162float(*o) + more[c]);
+        else p.part_o[slot * D + (size_t)((c0 + c) / 4) * (R * 4) + rr * 4 + (c & 3)] += more[c];
       }
     }
   }
@@ -282,10 +312,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   auto b_scale = [&](int g) { return bars + 744 + (g % kScales) * 8; };
   uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(gen + F::OFF_BAR + 808);
   int* const s_sums = reinterpret_cast<int*>(gen + F::OFF_BAR + 816);      // [32], [8]
-  volatile int* const s_odd = s_sums + 40;         // [8]: the segment's number, where its uneven tiles have values that are no numbers
+  volatile int* const s_odd = s_sums + 40;         // an uneven tile had values that are no numbers; places a column
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
-  if (tid < 8) s_odd[tid] = 0;
+  if (tid == 0) *s_odd = 0;
   if (tid == 0) {
     for (int i = 0; i < KS; ++i) {
       mbar_init(b_kfull + 8 * i, F::I8 ? F::kConvThreads / 64 : 1);
@@ -412,17 +442,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (tid == 0) p.sched[0] = each;
   }
+  if (tid == 0) s_odd[1] = each;
   Walk k;
-  k.u0 = k.u = min(total, (int)blockIdx.x * each);
-  k.u1 = min(total, k.u0 + each);
-  {
-    int lo = 0, hi = p.B - 1;      // the last request that begins at or before u0
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (s_cum[mid] * p.n_kv <= k.u0) lo = mid; else hi = mid - 1;
-    }
-    k.b = lo;
-  }
+  begin_walk(p, s_cum, total, each, k);
   // keys of tile t of the walk's request
   auto keys_of = [&](int t) { return t == k.r.nt - 1 ? k.r.n : min(BK, k.r.length - (k.r.first + t) * BK); };
 
@@ -555,6 +577,36 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           fence_proxy_async_smem();
           __syncwarp();
         }
+        if (!F::I8 && ok && uneven(p, k.r, k.ts + i)) {
+          // x 0 is 0 of numbers alone
+          const int pieces = valid * (NDK * 8);
+          auto piece = [&](int x) { return v_s0 + vs * F::T_BYTES + (x & (NDK - 1)) * (BK * 128) + (x >> (NDK - 1)) * 16; };
+          uint32_t zero[4] = {0, 0, 0, 0};
+#pragma unroll 1
+          for (int x0 = lane; x0 < pieces + lane; x0 += 256)
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+              uint32_t u[4];
+              ld_shared(piece(min(x0 + 32 * y, pieces - 1)), u);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(zero[e]) : "r"(u[e]), "r"(0));
+            }
+          if (__any_sync(0xffffffffu, ((zero[0] | zero[1] | zero[2] | zero[3]) & 0x7fff7fffu) != 0)) {
+            for (int x = lane; x < pieces; x += 32) {
+              uint32_t u[4];
+              ld_shared(piece(x), u);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((u[e] & 0x7f80u) == 0x7f80u) u[e] &= 0xffff0000u;
+                if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0xffffu;
+              }
+              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(piece(x)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
+            }
+            *s_odd = 1;
+            fence_proxy_async_smem();
+          }
+          __syncwarp();
+        }
         const uint32_t vl = v_lo + vs * (F::T_BYTES >> 4);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
@@ -657,34 +709,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const int i0 = NW == 1 ? (w - g0) & 1 : 0;
       for (int i = i0; i < k.count; i += kStep, ++j) {
         const int g = g0 + i, t = k.ts + i;
-        if (!F::I8 && uneven(p, k.r, t)) {
-          // the tile's values while its scores are made (the place's values before were used: two tiles of the group ago at the latest)
-          static_assert(F::I8 || VS >= 4, "places of values");
-          wait(b_vfull + 8 * (g % VS), (g / VS) & 1);
-          const int pieces = keys_of(t) * (NDK * 8);
-          bool odd = false;
-          for (int x = tid - (F::kSoft + 8 * w) * 32; x < pieces; x += 256) {
-            const uint32_t at = v_s0 + (g % VS) * F::T_BYTES + (x & (NDK - 1)) * (BK * 128) + (x >> (NDK - 1)) * 16;
-            uint32_t u[4], any = 0;
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]) : "r"(at));
-#pragma unroll
-            for (int e = 0; e < 4; ++e) any |= (u[e] & 0x7fff7fffu) + 0x00800080u;      // the sign bit: an exponent of ones
-            if (any & 0x80008000u) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((u[e] & 0x7f80u) == 0x7f80u) u[e] &= 0xffff0000u;
-                if ((u[e] & 0x7f800000u) == 0x7f800000u) u[e] &= 0xffffu;
-              }
-              asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]) : "memory");
-              odd = true;
-            }
-          }
-          if (odd) {
-            s_odd[seg & 7] = seg;
-            fence_proxy_async_smem();
-          }
-          __syncwarp();
-        }
         wait(b_sfull(w), j & 1);
         if (F::I8) wait(b_scale(g), (g / kScales) & 1);
         if (!some) {      // rows of nobody: the products take what is there
@@ -883,8 +907,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             for (int e = 0; e < 4; ++e) *reinterpret_cast<uint4*>(part + (size_t)(c * 4 + e) * (NW * BQ * 4)) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           }
         }
-        if (row_ok && s_odd[seg & 7] == seg)
-          add_no_numbers<F>(p, k.r, k.h, k.ts, k.count, row, c0, NC * 16, whole ? dst : nullptr, part, NW * BQ * 4);
         if (!whole && row_ok && half == 0 && (NW == 2 || w == 0)) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(best, sum);
       }
       __syncwarp();
@@ -903,9 +925,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     constexpr int PL = F::KS;
     static_assert(!F::I8 || F::KS == F::VS, "places of keys and values");
     bool ok = true;
-    int g = 0, seg = 0, rs = 0, rpar = 0, ps = 0, ppar = 1;      // (fewer than eight tiles ahead of the softmax: `s_odd`)
-    while (ok && next_segment<F>(p, s_cum, s_req, k)) {
-      ++seg;
+    int g = 0, rs = 0, rpar = 0, ps = 0, ppar = 1;
+    while (ok && next_segment<F>(p, s_cum, s_req, k))
       for (int i = 0; i < k.count; ++i, ++g) {
         const uint32_t st = st_s0 + rs * F::S_BYTES + (is_v ? BK * D : 0), dst = tile0 + ps * F::T_BYTES;
         ok = warp_wait(b_rfull + 8 * rs, rpar);
@@ -919,7 +940,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           float f = *reinterpret_cast<const float*>(gen + F::OFF_ST + rs * F::S_BYTES + 2 * BK * D + (is_v ? BK * 4 : 0) + ct * 4);
           if (is_v && f - f != 0.f && ct < keys_of(k.ts + i) && uneven(p, k.r, k.ts + i)) {      // (add_no_numbers)
             f = 0.f;
-            s_odd[seg & 7] = seg;
+            *s_odd = 1;
           }
           s_scale[(g % kScales) * (2 * BK) + (is_v ? BK : 0) + ct] = ct >= keys_of(k.ts + i) ? 0.f : f * (is_v ? kByteScale : p.scale_log2 * kByteScale);
           warp_arrive(b_scale(g));
@@ -945,7 +966,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (++rs == RS) { rs = 0; rpar ^= 1; }
         if (++ps == PL) { ps = 0; ppar ^= 1; }
       }
-    }
   }
   __syncwarp();
   tc_fence_before();
@@ -955,6 +975,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
+  if (*s_odd) add_no_numbers<F>(p, s_cum, s_req, s_odd[1]);
 }
 
 // Segments of a request's key head, added up in the order of the keys: a CTA takes 32 query rows x 32 columns, a lane a row.  128 threads and few
