@@ -13,7 +13,7 @@
 // begins and ends inside a request as a rule: what it has of one is a segment.  A segment that is all of a request's key head writes results;
 // the others leave unnormalised sums against their running maximum, and a second kernel adds them up in the order of the keys.
 //
-// A CTA: two warps copy (tiled TMA, 16 keys x 64 dims a box, 128-byte swizzle; pages behind the end are asked for outside the tensor and
+// A CTA, one to an SM: two warps copy (tiled TMA, 16 keys x 64 dims a box, 128-byte swizzle; pages behind the end are asked for outside the tensor and
 // come as zeros), one issues the products for scores and one those of P V, each waiting for a ring's places in their order (a parity wait that could be
 // more than one phase ahead would return at once); two groups of 256 threads do softmax, four threads to two query rows of a
 // tile's 64 keys.  Scores come from tensor memory into registers once, and their place is free for the next ones; P goes back to tensor memory
@@ -22,9 +22,15 @@
 //     meet at the segment's end; the queries are in tensor memory.  One softmax takes longer than its tile's bytes, two at a time do not.
 //   up to 256 (NW 2): a group has a query tile of its own and both share every K / V tile; the queries are in shared memory.
 // More rows take further CTAs (blockIdx.y) over the same keys.
-// An 8-bit cache comes in as bytes (bulk copies, scales with them), eight warps make integers in bf16 of them, which are exact; K's scale goes on
-// the scores and V's on the weights, both in fp32.  Of four dimensions the second and the third change places on the way (pairs come apart that
+// An 8-bit cache comes in as bytes (bulk copies, scales with them); four warps for keys and four for values make b / 64 in bf16 of them, which is
+// exact; K's scale goes on the scores and V's on the weights, both in fp32.  Of four dimensions the second and the third change places on the way (pairs come apart that
 // way), which the queries follow and the results undo.
+//
+// What bounds it.  bf16 with one query tile: the cache's bytes (32 requests of 2000 to 33000 positions, 40 heads on 8 of 128: 2.3 GB in 391 us, 5.9 TB/s of
+// the 6.5 that a copy reaches).  Two query tiles: the softmax, a chain of about 2000 cycles a tile whose four warps to a scheduler hide half of it, and the
+// scores' product, which reads Q from shared memory (16 requests of up to 9000 positions, 40 to 64 nodes, 16 heads on 4: 173 MB in 66 us).  8 bits: instructions, about 5000 a tile and SM, of
+// which the expansion is a third (12 requests of up to 65000 positions, 24 nodes, 40 heads on 8: 1.09 GB in 405 us).  One request: a segment's start and end, about four tiles' time, and
+// the second launch (4100 positions: 18 us).  Full tables of many short requests: the same, a request at a time.
 #include "tree.cuh"
 
 using namespace b2;
@@ -978,8 +984,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   if (*s_odd) add_no_numbers<F>(p, s_cum, s_req, s_odd[1]);
 }
 
-// Segments of a request's key head, added up in the order of the keys: a CTA takes 32 query rows x 32 columns, a lane a row.  128 threads and few
-// registers, so that it finds room beside a CTA of the attention and is there when that ends.
+// Segments of a request's key head, added up in the order of the keys: a CTA takes 32 query rows x 32 columns, a lane a row (partial sums stand with
+// their rows next to one another for that), four segments' loads on their way together.  Bound by its launch and two ways to memory: 4 us behind one
+// request of 17 segments.  (Two segments at a time in half the registers, which finds room beside a CTA of the attention: 18.0 -> 20.7 us; eight: no change.)
 template <int D>
 __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttnParams p, int columns, int slot_rows, int groups) {
   constexpr int PARTS = D / 32;
@@ -1090,13 +1097,17 @@ struct Shape {
 };
 Shape shape_of(int B, int max_blocks, int n_kv, int gqa, int max_nodes) {
   Shape s;
+  // One query tile on two groups in turn, or two query tiles.  64 nodes x 4 heads as 256 rows of one CTA / as 128 of
+  // two CTAs over the same keys: 66 / 78 us; 16 nodes x 5 heads, 80 rows, with the second group idle: 394 -> 466, in 8 bits (24 x 5) 406 -> 608.
   s.nw = max_nodes * gqa <= BQ ? 1 : 2;
   const int most = s.nw * BQ / gqa;
   s.groups = (max_nodes + most - 1) / most;
   s.tokens = (max_nodes + s.groups - 1) / s.groups;
-  // A table of few pages (up to four tiles and the tree's): a request's key head is one CTA's, and the second launch is spared.
+  // Short tables of few requests: a request's key head is one CTA's, and the second launch is spared.  Full tables, 32 heads on 8, one CTA / parts
+  // that are added up, us: 1 request 9.7 / 10.4 at 6 tiles, 11.8 / 11.4 at 10; 16 requests 11.1 / 13.6 and 14.9 / 16.9; 32 requests (256 CTAs)
+  // 22.6 / 28.0 and 29.4 / 33.9, at 18 39.9 / 43.2 and 1 request 15.7 / 15.4; 48 requests 28.9 / 25.5 at 3 tiles, 128 requests 82 / 62 at 6.
   const int most_tiles = max_blocks / 4 + 2;
-  s.single = most_tiles <= 6 && (long long)B * n_kv < 65536 ? most_tiles : 0;
+  s.single = most_tiles <= 10 && (long long)B * n_kv * s.groups <= 2 * sm_count() ? most_tiles : 0;
   if (s.single) {
     s.columns = B * n_kv;
     return s;

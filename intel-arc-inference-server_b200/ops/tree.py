@@ -11,8 +11,9 @@ token, which is not in the cache yet.  Nodes stand in pages of their own (``tree
 
 ``plan`` without parents lays out rows at consecutive positions (prompt portions, decode rows) for ``rope_append``: their slots are the
 request's own.  Everything happens on the current stream, nothing waits for the host: lengths, tables and the list of free pages stay on the
-device, and a step can be captured into a CUDA graph.  What only the device knows is checked there; a plan that cannot be made leaves pages
-and tables as they are and no rows (``TreeStep.check``).
+device, and a step can be captured into a CUDA graph.  What only the device knows is checked there; a plan that cannot be made leaves pages,
+tables and lengths as they are and no rows (``TreeStep.check``); a row whose table names a page that is not there has slot -1 and is not stored.
+A step's buffers are one plan's at a time: calls that read them may run on several streams, the next plan belongs behind them.
 
 Caches are ``KVCache`` planes: ``[page][kv head][16][D]`` with D 64 or 128, bf16, or int8 with fp32 scales ``[page][kv head][16]``.
 """
@@ -194,6 +195,7 @@ class TreeStep:
         self._c = _Step(*(t.data_ptr() for t in (block_table, tree_table, self.lengths, self.row_start, self.row_req, self.row_pos, self.slots, self.parents, self.masks,
                                                  self.status)), b, block_table.shape[1], tree_table.shape[1], max_rows, max_nodes, num_pages)
         self._at, self._lengths, self._work = ctypes.addressof(self._c), self.lengths.data_ptr(), {}
+        self._small = (2 * b + 2 + 3) // 4 * 4          # fp32 words of workspace of an attention that leaves no segments
         self._floats, self._index = torch.empty(0, device=dev), dev.index
 
     def check(self):
@@ -294,7 +296,7 @@ def rope_append(step: TreeStep, qkv: torch.Tensor, rope: tuple, q: torch.Tensor,
 def attention(step: TreeStep, q: torch.Tensor, cache: TreeCache, out: torch.Tensor, scale: float, window: int = 0) -> torch.Tensor:
     """Rows ``q`` ``[rows][n_q D]`` bf16 over one layer's cache into ``out`` (the same shape, bf16): softmax in fp32 over the request's cached
     positions and the nodes of the row's mask, ``window`` > 0: those less than ``window`` positions before the row.  A row that sees nothing is
-    0, whatever the places hold that it does not see; rows behind the step's are left."""
+    0, whatever the places hold that it does not see (infinities and NaN too); rows behind the step's are left.  ``out`` may be ``q``."""
     _check_cache(step, cache, False)
     dev, d, n_kv = step.device, cache.d, cache.heads
     if not step.tree:
@@ -316,7 +318,8 @@ def attention(step: TreeStep, q: torch.Tensor, cache: TreeCache, out: torch.Tens
         room = step._work[n_q, n_kv, d] = _fn()["attention_work"](step._at, n_q, n_kv, d)
     work = step._floats.new_empty(room)      # this call's own: calls of one step on several streams share nothing
     K._check(_fn()["attention"](step._at, cache._at, pq, ldq, po, ldo, work.data_ptr(), rows, n_q, window, scale, _stream(dev)), "tree_attention")
-    K.launch_count += 1      # segments added up (of tables of some length)
+    if room > step._small:
+        K.launch_count += 1      # segments added up
     return out
 
 

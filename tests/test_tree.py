@@ -461,6 +461,15 @@ def test_attention_strides():
 
 
 @gpu
+@pytest.mark.parametrize("name", MIXED)
+def test_attention_over_its_queries(name):
+    s = State(**MIXED[name])
+    q, cache, out = run_attention(s, (6, 2, 128), False)
+    T.attention(s.step, q, cache, q, 128 ** -0.5)
+    assert torch.equal(q[: s.rows], out[: s.rows])
+
+
+@gpu
 def test_attention_pages_that_are_not_there():
     """A table that names pages outside the cache: they are nobody's, and nothing is read."""
     s = State([100], [4]).cuda()
