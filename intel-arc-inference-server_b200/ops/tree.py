@@ -235,7 +235,7 @@ def plan(step: TreeStep, lengths: torch.Tensor, counts: torch.Tensor, parents: O
     rows, parents_at = step.max_rows, None
     if parents is not None:
         rows = parents.numel()
-        parents_at = _words(parents, rows, "parents", dev)
+        parents_at = _words(parents, rows, "parents", dev) or at      # (an empty tensor has no address, and no parents are something else)
         if rows > step.max_rows:
             raise ValueError(f"parents: of up to {step.max_rows} rows, not {rows}")
     if pool._requests != b or after._requests != b or pool._index != step._index or after._c.free != pool._c.free:

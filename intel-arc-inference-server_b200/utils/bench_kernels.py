@@ -3,6 +3,7 @@
     python -m b200serve.utils.bench_kernels gemv            # W4A16 weight-streaming kernel, 27B shapes
     python -m b200serve.utils.bench_kernels gemm            # tcgen05 GEMMs, 27B prefill shapes
     python -m b200serve.utils.bench_kernels logprob         # log probabilities: rows of logits, rows through both heads
+    python -m b200serve.utils.bench_kernels tree            # steps over token trees: attention over paged caches, in bf16 and 8 bits
 
 Weights rotate through enough copies to exceed the 126 MB L2 between launches, so
 every launch streams from HBM.  Fractions are of the measured peaks in
@@ -114,6 +115,35 @@ def bench_gemm():
     K.check_status()
 
 
+def bench_tree():
+    """Tree attention over full caches of 40 query heads on 8 of 128, two caches in turn."""
+    from ..ops import tree as T
+    hbm, _, src = peaks()
+    for b, length, nodes, i8 in ((1, 4100, 16, False), (8, 16384, 16, False), (32, 4096, 16, False), (16, 5000, 48, False), (8, 32768, 24, True)):
+        n_kv, d, group, blocks = 8, 128, 5, -(-length // 16) + 4
+        pages = 1 + b * (blocks + 4)
+        at = torch.arange(1, pages, dtype=torch.int32, device="cuda").view(b, blocks + 4)
+        step = T.TreeStep(at[:, :blocks].contiguous(), at[:, blocks:].contiguous(), b * nodes, pages, nodes)
+        i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")         # noqa: E731
+        T.plan(step, i32(*[length] * b), i32(*[nodes] * b), i32(*([-1] + [i // 2 for i in range(nodes - 1)]) * b), T.PagePool(i32(0), i32(0), i32(*[blocks] * b)))
+        step.check()
+        shape = (pages, n_kv, 16, d)
+        if i8:
+            caches = [T.TreeCache(*(torch.randint(-127, 128, shape, dtype=torch.int8, device="cuda") for _ in range(2)),
+                                  *(torch.rand(shape[:-1], device="cuda") * 0.01 for _ in range(2))) for _ in range(2)]
+        else:
+            caches = [T.TreeCache(*(torch.randn(shape, device="cuda").bfloat16() for _ in range(2))) for _ in range(2)]
+        q = torch.randn(b * nodes, n_kv * group * d, device="cuda").bfloat16()
+        out = torch.empty_like(q)
+
+        def run():
+            for c in caches:
+                T.attention(step, q, c, out, d ** -0.5)
+        us = time_ms(run) * 1e3 / len(caches)
+        size = b * (length + nodes) * n_kv * 2 * (d + 4 if i8 else 2 * d) + 4 * q.numel()
+        print(f"tree attention, {b} x {length} positions, {nodes} nodes, {'int8' if i8 else 'bf16'}: {us:.1f} us, {size / us / 1e3 / hbm:.2f} of {src} copy")
+
+
 def bench_logprob():
     """Rows of 151,936 logits in a graph (small calls are shorter than the host's part of them), and prompts through the 27B shape's heads."""
     from ..ops import logprob as LP
@@ -204,4 +234,4 @@ if __name__ == "__main__":
     elif what == "gemv-graph":  # back-to-back launches inside a CUDA graph
         bench_gemv((1, 4, 8), graph=True)
     else:
-        {"gemv": bench_gemv, "gemm": bench_gemm, "logprob": bench_logprob}[what]()
+        {"gemv": bench_gemv, "gemm": bench_gemm, "logprob": bench_logprob, "tree": bench_tree}[what]()

@@ -152,6 +152,19 @@ def test_plan_beside_its_pool():
     assert s.t_held.tolist() == s.held and s.t_n.tolist() == [s.n_free]
 
 
+@gpu
+def test_plan_of_no_parents():
+    """An empty tensor of parents is a step of trees without nodes, not one of consecutive rows."""
+    s = State([40, 7], [3, 2]).cuda()
+    s.plan()
+    assert s.step.masks.tolist()[0] == 1
+    T.plan(s.step, s.t_lengths, torch.zeros_like(s.t_counts), s.t_parents[:0], s.pool)
+    s.step.check()
+    assert s.step.masks.tolist() == [0] * 5 and s.step.parents.tolist() == [-1] * 5 and s.step.row_start.tolist() == [0, 0, 0]
+    T.plan(s.step, s.t_lengths, s.t_counts, s.t_parents[:0], s.pool)
+    assert s.step.status.item() == 4
+
+
 FAULTS = {
     "pool": (dict(lengths=[16, 3], counts=[20, 2], spread=1, free=1), 1),
     "table": (dict(lengths=[60], counts=[20], spread=1, blocks=4), 2),
