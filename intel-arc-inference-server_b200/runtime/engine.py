@@ -80,6 +80,7 @@ class Engine:
         self.out_host = torch.zeros(K.CTRL_WORDS, dtype=torch.int32).pin_memory()
         self.block_table = torch.zeros(max_seqs, self.max_blocks, dtype=torch.int32, device=self.device)
         self.seq_len = [0] * max_seqs
+        self.trees = None           # steps over token trees (``tree_nodes``)
         self._snap = None           # (rows, {slot: recurrent state before them}) of the last step of a recurrent model
         self.use_graphs = use_graphs
         self.graphs: Dict[Tuple[int, bool, bool], torch.cuda.CUDAGraph] = {}
@@ -97,7 +98,6 @@ class Engine:
             from .buffer_registry import audit
             audit(self.model.buf, self.kv, cfg, kv_dtype, max_seqs)
         self._batch = None          # runner of mixed batches (models that list their layers)
-        self.trees = None
         if tree_nodes:
             from .trees import TreeVerifier
             self.trees = TreeVerifier(self, tree_nodes)
@@ -121,10 +121,14 @@ class Engine:
             self.pool.release(s)
             self.seq_len[s] = 0
             self.kv.reset_slot(s)       # recurrent state
+            if self.trees is not None:
+                self.trees.forget(s)
 
     def truncate(self, slot: int, length: int):
         """Drop everything after ``length`` positions (rejected draft rows)."""
         assert length <= self.seq_len[slot]
+        if self.trees is not None:
+            self.trees.forget(slot)
         replay = rest = None
         if length == 0 < self.seq_len[slot]:
             self.kv.reset_slot(slot)

@@ -46,9 +46,11 @@ class TreeVerifier:
         scales = (kv.k_scale[:n], kv.v_scale[:n]) if kv.kv_int8 else ()
         self.all = T.TreeCache(kv.k[:n], kv.v[:n], *scales)
         i32 = lambda *s: torch.zeros(s, dtype=torch.int32, device=eng.device)         # noqa: E731
-        self.inputs = i32(3 * b + eng.max_rows)      # lengths, rows, held pages, parents
-        self.staging = torch.zeros(3 * b + eng.max_rows, dtype=torch.int32).pin_memory()
-        lengths, self.counts, held, self.parents = self.inputs.split([b, b, b, eng.max_rows])
+        self.inputs = i32(3 * b + 2 * eng.max_rows)      # lengths, rows, held pages, parents, tokens
+        self.staging = torch.zeros(3 * b + 2 * eng.max_rows, dtype=torch.int32).pin_memory()
+        lengths, self.counts, held, self.parents, self.tokens = self.inputs.split([b, b, b, eng.max_rows, eng.max_rows])
+        self.best = i32(eng.max_rows)       # arg-max of the rows: the engine's own words are the next step's, whoever makes it
+        self.at_lengths: List[int] = []
         self.lengths = lengths
         self.pool = T.PagePool(i32(1), i32(1), held)       # (the host's pool has given the pages: nothing is taken here)
         self.accepted = T.Accepted.empty(b, eng.device)
@@ -56,7 +58,7 @@ class TreeVerifier:
 
     def forward(self, trees: Dict[int, Tuple[Sequence[int], Sequence[int]]]) -> torch.Tensor:
         """Runs the nodes of ``trees`` (slot -> tokens, parents; node 0's parent is -1); fp32 logits of all rows, slots in order, nodes in theirs
-        (valid until the next step).  The requests' positions are as they were until ``commit``."""
+        (valid until the next step).  The requests' positions are as they were until ``commit``; other slots may prefill and step in between."""
         from .engine import Row
         eng = self.eng
         rows, todo, self.rows = [], [], []
@@ -76,7 +78,6 @@ class TreeVerifier:
         eng.require_ok()
         for slot, _, _, deepest in todo:
             eng._ensure_pages(slot, eng.seq_len[slot] + deepest)
-        self.rows = [t[:3] for t in todo]
         b, host = eng.max_seqs, self.staging.numpy()
         torch.cuda.current_stream(eng.device).synchronize()       # (the staging of a step before is read)
         host[:b] = eng.seq_len
@@ -86,6 +87,7 @@ class TreeVerifier:
         for slot, tokens, parents, _ in todo:
             host[b + slot] = len(tokens)
             host[at: at + len(parents)] = parents
+            host[at + eng.max_rows: at + eng.max_rows + len(tokens)] = tokens
             at += len(parents)
         self.inputs.copy_(self.staging, non_blocking=True)
         eng._write_rows(rows)
@@ -97,17 +99,26 @@ class TreeVerifier:
             model.step_rows(m, eng.ctrl, eng.block_table, eng.max_blocks, eng.kv, False)
         finally:
             model.tree = None
+        self.best[:m].copy_(eng.ctrl[K.CTRL_OUT_TOKEN: K.CTRL_OUT_TOKEN + m])
+        self.rows, self.at_lengths = [t[:3] for t in todo], [eng.seq_len[t[0]] for t in todo]
         return eng.logits(m)
+
+    def forget(self, slot: int):
+        """The slot's positions are no longer those that the last ``forward`` saw: it cannot be settled."""
+        if any(s == slot for s, _, _ in self.rows):
+            self.rows = []
 
     def commit(self, targets: Optional[torch.Tensor] = None) -> Dict[int, Verified]:
         """Settles the last ``forward``: ``targets`` int32, the token behind every row (a draw from its logits; None: the arg-max).  The accepted
-        nodes' keys and values become the requests' next positions."""
+        nodes' keys and values become the requests' next positions.  Refused where one of the trees' slots has been reset, cut or run further since."""
         eng, m = self.eng, sum(len(t) for _, t, _ in self.rows)
+        if [eng.seq_len[s] for s, _, _ in self.rows] != self.at_lengths[: len(self.rows)]:
+            m, self.rows = 0, []
         if not m:
             raise ValueError("no trees to settle")
         if targets is None:
-            targets = eng.ctrl[K.CTRL_OUT_TOKEN: K.CTRL_OUT_TOKEN + m]
-        got = T.commit(self.step, eng.ctrl[K.CTRL_CUR_TOKEN: K.CTRL_CUR_TOKEN + m], targets, self.all, self.accepted)
+            targets = self.best[:m]
+        got = T.commit(self.step, self.tokens[:m], targets, self.all, self.accepted)
         path, count, following = got.path.tolist(), got.count.tolist(), got.next_token.tolist()      # (waits)
         rows, self.rows = self.rows, []
         self.step.check()

@@ -137,3 +137,47 @@ def test_refusals():
     v = eng.verify_trees({1: ([3], [-1])})
     assert v[1].path == [0] and v[1].tokens == [3] and eng.seq_len == [0, 1]
     torch.cuda.synchronize()
+
+
+@gpu
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+def test_other_slots_run_between_a_step_and_its_settling(kv):
+    """A step of trees is settled with its own tokens and arg-maxes, whatever other slots have run since."""
+    cfg = C.small_dense()
+    w = random_weights(cfg, device="cuda", seed=1)
+    rng = random.Random(9)
+    prompt, other = [rng.randrange(cfg.vocab) for _ in range(45)], [rng.randrange(cfg.vocab) for _ in range(20)]
+    alone, shared = (engine("", w, max_seqs=2, kv_dtype=kv, tree_nodes=16) for _ in range(2))
+    first = [e.prefill(0, prompt) for e in (alone, shared)]
+    assert first[0] == first[1]
+    chain = [first[0]]
+    for _ in range(3):      # drafts: what the model itself goes on with
+        chain.append(alone.verify_trees({0: ([chain[-1]], [-1])})[0].next_token)
+    alone.truncate(0, len(prompt))
+    tree = make_tree(chain, cfg.vocab, rng)
+    want = alone.verify_trees({0: tree})[0]
+    shared.trees.forward({0: tree})
+    token = shared.prefill(1, other)
+    shared.forward_rows([Row(1, len(other), token)])
+    got = shared.trees.commit()
+    assert got == {0: want} and len(want.path) > 1
+    assert shared.seq_len == [len(prompt) + len(want.path), len(other) + 1]
+
+
+@gpu
+def test_trees_of_a_slot_that_changed_are_not_settled():
+    cfg = C.tiny_dense()
+    eng = engine("", random_weights(cfg, device="cuda", seed=1), max_seqs=2, tree_nodes=8)
+    prompt, tree = [1, 2, 3, 4, 5], ([3, 4], [-1, 0])
+    for change in (lambda: eng.truncate(0, 4), lambda: (eng.reset(0), eng.prefill(0, prompt)), lambda: eng.forward_rows([Row(0, 5, 7)])):
+        eng.reset()
+        eng.prefill(0, prompt)
+        eng.trees.forward({0: tree})
+        change()
+        held = list(eng.seq_len)
+        with pytest.raises(ValueError, match="no trees"):
+            eng.trees.commit()
+        assert eng.seq_len == held
+    eng.trees.forward({1: tree})        # another slot's changes are not this one's
+    eng.truncate(0, 2)
+    assert 1 in eng.trees.commit()
