@@ -64,16 +64,18 @@ __device__ __forceinline__ void cluster_barrier() {
 
 // A cluster of one CTA, or of eight where there are more rows than one CTA's threads: each does the sums for itself (there is nothing to wait for
 // that way), the first one keeps the pages, all of them write rows.  A request a thread.
+// A parent that is none goes into a word of its own, and the barrier behind the trees is everyone's: what threads look at to go into a block with
+// barriers must not change while others still look.
 __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams p) {
   __shared__ long long sums[32];
   __shared__ int s_start[kMaxReq + 1], s_need[kMaxReq], s_held[kMaxReq], s_first[kMaxReq], s_len[kMaxReq];
   __shared__ int8_t s_up[kUpRows];
-  __shared__ int s_status;
+  __shared__ int s_status, s_trees;
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, rank = cluster_rank(), ranks = cluster_size();
   pdl_wait();
   pdl_launch_dependents();
   const bool tree = p.parents != nullptr, mine = tid < p.B, up_here = tree && p.rows <= kUpRows;
-  if (tid == 0) s_status = 0;
+  if (tid == 0) s_status = s_trees = 0;
   const int count = mine ? p.counts[tid] : 0, held = mine ? p.held[tid] : 0, n_free = *p.n_free;
   const int given = mine ? p.lengths[tid] : 0, length = count >= 0 ? given : 0;
   if (up_here)
@@ -114,7 +116,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
       }
       bad = __any_sync(0xffffffffu, bad);
       if (bad) {
-        if (lane == 0) atomicOr(&s_status, PLAN_PARENT);
+        if (lane == 0) s_trees = PLAN_PARENT;
         continue;
       }
       for (int i = lane; i < n; i += 32) {
@@ -125,10 +127,10 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
       deepest = __reduce_max_sync(0xffffffffu, deepest);
       if (lane == 0) s_need[b] = deepest;
     }
-    __syncthreads();
   }
+  __syncthreads();
   // ---- pages: those of requests that left go back, then what is missing comes off the end of the list
-  const int need = mine && s_status == 0 ? s_need[tid] : 0;
+  const int need = mine && (s_status | s_trees) == 0 ? s_need[tid] : 0;
   const long long want = need > 0 ? max((long long)held, ((long long)length + need + kPage - 1) / kPage) : held;
   const bool left = mine && count < 0;
   if (mine && !left && want > p.max_blocks) atomicOr(&s_status, PLAN_TABLE);
@@ -138,7 +140,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
   if (mine) s_first[tid] = (int)take0;
   if (tid == 0 && ((long long)n_free + back > p.free_cap || take > (long long)n_free + back)) atomicOr(&s_status, PLAN_POOL);
   __syncthreads();
-  const int status = s_status;
+  const int status = s_status | s_trees;
   if (rank == 0 && tid == 0) p.status[0] = status;
   if (ranks > 1) cluster_barrier();      // everyone has read what the first CTA now writes
   const long long top = (long long)n_free + back - 1;     // the page that is taken first
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
     }
   }
   __syncthreads();
-  if (s_status != status) {      // pages that are not there
+  if ((s_status | s_trees) != status) {      // pages that are not there
     if (tid == 0) atomicOr(p.status, PLAN_PAGE);
   }
 }

@@ -208,6 +208,32 @@ def test_plan_that_cannot_be_made(name):
         assert s.step.slots.tolist()[2:] == [-1, -1] and min(s.step.slots.tolist()[:2]) >= 0
 
 
+def unchanged(s, before):
+    """A plan that could not be made left nothing."""
+    assert all(torch.equal(a, b) for a, b in zip(before, (s.t_table, s.t_held, s.t_n, s.t_free)))
+    assert s.step.row_start.tolist() == [0] * (s.b + 1) and set(s.step.slots.tolist()) == {-1}
+    assert torch.equal(s.step.lengths, s.t_lengths)
+
+
+@gpu
+@pytest.mark.parametrize("at", [0, 5, 199])
+@pytest.mark.parametrize("nodes", [3, 41])
+def test_plan_with_a_bad_parent_among_many_trees(nodes, at):
+    """One warp finds it while others have not come to the trees yet, in one CTA and in a cluster: all of them go the same way, so that nothing but the
+    parent is at fault, and every barrier is everyone's."""
+    s = State([(37 * i) % 301 for i in range(200)], [1 + (nodes - 1) * (i % 3 == 0 or i == at) for i in range(200)])
+    s.parents[at][1] = 1
+    s.cuda()
+    before = [t.clone() for t in (s.t_table, s.t_held, s.t_n, s.t_free)]
+    for _ in range(5):
+        s.plan()
+        assert s.step.status.item() == 16
+        unchanged(s, before)
+    s.t_parents[sum(s.counts[:at]) + 1] = s.parents[at][1] = 0
+    s.plan()
+    same_plan(s)
+
+
 # ------------------------------------------------------------------ caches
 def make_cache(pages, n_kv, d, i8, seed=0, layers=None, fill=None):
     g = torch.Generator(device="cuda").manual_seed(seed)
