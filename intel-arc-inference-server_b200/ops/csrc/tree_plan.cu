@@ -64,18 +64,18 @@ __device__ __forceinline__ void cluster_barrier() {
 
 // A cluster of one CTA, or of eight where there are more rows than one CTA's threads: each does the sums for itself (there is nothing to wait for
 // that way), the first one keeps the pages, all of them write rows.  A request a thread.
-// A parent that is none goes into a word of its own, and the barrier behind the trees is everyone's: what threads look at to go into a block with
-// barriers must not change while others still look.
+// What is at fault with the numbers, with the trees and with the pages are three words: each is written up to a barrier that is everyone's and only
+// looked at behind it, since what threads go by must not change while others still look.
 __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams p) {
   __shared__ long long sums[32];
   __shared__ int s_start[kMaxReq + 1], s_need[kMaxReq], s_held[kMaxReq], s_first[kMaxReq], s_len[kMaxReq];
   __shared__ int8_t s_up[kUpRows];
-  __shared__ int s_status, s_trees;
+  __shared__ int s_numbers, s_trees, s_pages;
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, rank = cluster_rank(), ranks = cluster_size();
   pdl_wait();
   pdl_launch_dependents();
   const bool tree = p.parents != nullptr, mine = tid < p.B, up_here = tree && p.rows <= kUpRows;
-  if (tid == 0) s_status = s_trees = 0;
+  if (tid == 0) s_numbers = s_trees = s_pages = 0;
   const int count = mine ? p.counts[tid] : 0, held = mine ? p.held[tid] : 0, n_free = *p.n_free;
   const int given = mine ? p.lengths[tid] : 0, length = count >= 0 ? given : 0;
   if (up_here)
@@ -91,11 +91,11 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
     if (held < 0 || held > p.max_blocks) bad |= PLAN_TABLE;
     if (tree && count > p.max_nodes) bad |= PLAN_COUNT;
     if (n_free < 0 || n_free > p.free_cap) bad |= PLAN_POOL;
-    if (bad) atomicOr(&s_status, bad);
+    if (bad) atomicOr(&s_numbers, bad);
   }
   int total;
   const int start = scan_cta(min(max(count, 0), p.rows + 1), sums, total);      // (at most 2^20 + 1 each)
-  if (total > p.rows && tid == 0) atomicOr(&s_status, PLAN_ROWS);
+  if (total > p.rows && tid == 0) atomicOr(&s_numbers, PLAN_ROWS);
   if (mine) {
     s_start[tid] = min(start, p.rows);
     s_need[tid] = tree ? 0 : max(count, 0);
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
   }
   if (tid == 0) s_start[p.B] = min(total, p.rows);
   __syncthreads();
-  if (s_status == 0 && tree) {
+  if (s_numbers == 0 && tree) {
     // ---- a warp per tree: ancestors by walking up (a node's parent stands before it, so every walk ends)
     for (int b = warp; b < p.B; b += threads >> 5) {
       const int r0 = s_start[b], n = s_start[b + 1] - r0;
@@ -130,17 +130,17 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
   }
   __syncthreads();
   // ---- pages: those of requests that left go back, then what is missing comes off the end of the list
-  const int need = mine && (s_status | s_trees) == 0 ? s_need[tid] : 0;
+  const int need = mine && (s_numbers | s_trees) == 0 ? s_need[tid] : 0;
   const long long want = need > 0 ? max((long long)held, ((long long)length + need + kPage - 1) / kPage) : held;
   const bool left = mine && count < 0;
-  if (mine && !left && want > p.max_blocks) atomicOr(&s_status, PLAN_TABLE);
+  if (mine && !left && want > p.max_blocks) atomicOr(&s_pages, PLAN_TABLE);
   long long back, take;
   const long long back0 = scan_cta(left ? (long long)held : 0ll, sums, back);
   const long long take0 = scan_cta(mine && !left ? want - held : 0ll, sums, take);
   if (mine) s_first[tid] = (int)take0;
-  if (tid == 0 && ((long long)n_free + back > p.free_cap || take > (long long)n_free + back)) atomicOr(&s_status, PLAN_POOL);
+  if (tid == 0 && ((long long)n_free + back > p.free_cap || take > (long long)n_free + back)) atomicOr(&s_pages, PLAN_POOL);
   __syncthreads();
-  const int status = s_status | s_trees;
+  const int status = s_numbers | s_trees | s_pages;
   if (rank == 0 && tid == 0) p.status[0] = status;
   if (ranks > 1) cluster_barrier();      // everyone has read what the first CTA now writes
   const long long top = (long long)n_free + back - 1;     // the page that is taken first
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
         slot = pos % kPage;
       }
       if (page < 0 || page >= p.num_pages) {
-        atomicOr(&s_status, PLAN_PAGE);
+        atomicOr(&s_pages, PLAN_PAGE);
         slot = -1;
       } else {
         slot += page * kPage;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
     }
   }
   __syncthreads();
-  if ((s_status | s_trees) != status) {      // pages that are not there
+  if ((s_numbers | s_trees | s_pages) != status) {      // pages that are not there
     if (tid == 0) atomicOr(p.status, PLAN_PAGE);
   }
 }

@@ -234,6 +234,21 @@ def test_plan_with_a_bad_parent_among_many_trees(nodes, at):
     same_plan(s)
 
 
+@gpu
+@pytest.mark.parametrize("blocks,free,status", [(40, 1000, 1), (3, 1100, 2), (3, 1000, 3)])
+@pytest.mark.parametrize("tree", [True, False])
+def test_plan_of_many_requests_whose_pages_do_not_suffice(tree, blocks, free, status):
+    """A request's table that is too short does not change what the others need: the pool is found short or not by all of their pages."""
+    s = State([16] * 1024, [1] * 1023 + [40], tree=tree, spread=1, blocks=40, free=free)
+    s.table, s.blocks = [t[:blocks] for t in s.table], blocks
+    s.cuda()
+    before = [t.clone() for t in (s.t_table, s.t_held, s.t_n, s.t_free)]
+    for _ in range(20):
+        s.plan()
+        assert s.step.status.item() == status
+    unchanged(s, before)
+
+
 # ------------------------------------------------------------------ caches
 def make_cache(pages, n_kv, d, i8, seed=0, layers=None, fill=None):
     g = torch.Generator(device="cuda").manual_seed(seed)
