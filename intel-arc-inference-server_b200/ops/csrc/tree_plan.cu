@@ -64,18 +64,18 @@ __device__ __forceinline__ void cluster_barrier() {
 
 // A cluster of one CTA, or of eight where there are more rows than one CTA's threads: each does the sums for itself (there is nothing to wait for
 // that way), the first one keeps the pages, all of them write rows.  A request a thread.
-// What is at fault with the numbers, with the trees and with the pages are three words: each is written up to a barrier that is everyone's and only
+// What is at fault with the numbers, the trees, the pages and the rows are four words: each is written up to a barrier that is everyone's and only
 // looked at behind it, since what threads go by must not change while others still look.
 __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams p) {
   __shared__ long long sums[32];
   __shared__ int s_start[kMaxReq + 1], s_need[kMaxReq], s_held[kMaxReq], s_first[kMaxReq], s_len[kMaxReq];
   __shared__ int8_t s_up[kUpRows];
-  __shared__ int s_numbers, s_trees, s_pages;
+  __shared__ int s_numbers, s_trees, s_pages, s_rows;
   const int tid = threadIdx.x, threads = blockDim.x, lane = tid & 31, warp = tid >> 5, rank = cluster_rank(), ranks = cluster_size();
   pdl_wait();
   pdl_launch_dependents();
   const bool tree = p.parents != nullptr, mine = tid < p.B, up_here = tree && p.rows <= kUpRows;
-  if (tid == 0) s_numbers = s_trees = s_pages = 0;
+  if (tid == 0) s_numbers = s_trees = s_pages = s_rows = 0;
   const int count = mine ? p.counts[tid] : 0, held = mine ? p.held[tid] : 0, n_free = *p.n_free;
   const int given = mine ? p.lengths[tid] : 0, length = count >= 0 ? given : 0;
   if (up_here)
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
         slot = pos % kPage;
       }
       if (page < 0 || page >= p.num_pages) {
-        atomicOr(&s_pages, PLAN_PAGE);
+        s_rows = PLAN_PAGE;
         slot = -1;
       } else {
         slot += page * kPage;
@@ -206,9 +206,7 @@ __global__ void __launch_bounds__(1024, 1) tree_plan_kernel(const TreePlanParams
     }
   }
   __syncthreads();
-  if ((s_numbers | s_trees | s_pages) != status) {      // pages that are not there
-    if (tid == 0) atomicOr(p.status, PLAN_PAGE);
-  }
+  if (tid == 0 && s_rows) atomicOr(p.status, s_rows);      // pages that are not there
 }
 
 struct TreeCommitParams {

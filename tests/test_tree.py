@@ -249,6 +249,29 @@ def test_plan_of_many_requests_whose_pages_do_not_suffice(tree, blocks, free, st
     unchanged(s, before)
 
 
+@gpu
+@pytest.mark.parametrize("requests", [40, 500])
+@pytest.mark.parametrize("bad", [0, 17, 39])
+def test_plan_with_tree_pages_that_are_not_there(requests, bad):
+    """Rows in such pages have no slots, and that is all: the requests' new pages, the pool and the numbers are those of the plan, whichever warps met
+    them first."""
+    s = State([16 * (1 + i % 3) for i in range(requests)], [1 + i % 2 for i in range(requests)])
+    s.cuda()
+    s.t_tree[bad, 0] = s.pages + 7
+    after = T.PagePool(s.t_free, torch.empty_like(s.t_n), torch.empty_like(s.t_held))
+    want, table = s.want(), s.t_table.clone()
+    lost = [r == bad for r in want["row_req"]]
+    slots = [-1 if gone else slot for slot, gone in zip(want["slots"], lost)]
+    assert any(lost) and sum(h > -(-n // PAGE) for h, n in zip(want["held"], s.lengths)) == requests
+    for _ in range(20):
+        s.t_table.copy_(table)
+        s.plan(after)
+        assert s.step.status.item() == 64
+        assert s.step.slots.tolist() == slots and s.step.row_pos.tolist() == want["row_pos"] and s.step.masks.tolist() == want["masks"]
+        assert s.t_table.tolist() == want["table"] and after.held.tolist() == want["held"] and after.n_free.tolist() == [len(want["free"])]
+        assert s.step.lengths.tolist() == s.lengths and s.step.row_start.tolist() == want["row_start"]
+
+
 # ------------------------------------------------------------------ caches
 def make_cache(pages, n_kv, d, i8, seed=0, layers=None, fill=None):
     g = torch.Generator(device="cuda").manual_seed(seed)
