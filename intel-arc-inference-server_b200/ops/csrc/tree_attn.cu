@@ -201,6 +201,11 @@ __device__ __noinline__ void zero_no_numbers(uint32_t at, int rows) {
   fence_proxy_async_smem();
 }
 
+// The weight of a part of a row's keys whose maximum is m beside others' of up to `best`: 0 only where the row saw nothing of the part (what such a part
+// holds is not looked at), else 2^-126 at least.  That is nothing beside a sum of numbers, but leaves a part that is no number what it is, wherever the
+// row's keys were cut (a weight of 0 in 32 bits would drop it or make it NaN).
+__device__ __forceinline__ float part_weight(float m, float best) { return m == -INFINITY ? 0.f : fmaxf(exp2f(m - best), 1.17549435e-38f); }
+
 // A request as the roles see it.
 struct Req {
   int b, r0, n, length, first, nt;      // first row, nodes, cached positions, first tile of the cache that is read, tiles (the tree's is the last)
@@ -875,8 +880,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if constexpr (NW == 1) {
           const float m0 = s_x[r], m1 = s_x[2 * BQ + r];
           best = fmaxf(m0, m1);
-          f0 = m0 == -INFINITY ? 0.f : exp2f(m0 - best);
-          f1 = m1 == -INFINITY ? 0.f : exp2f(m1 - best);
+          f0 = part_weight(m0, best);
+          f1 = part_weight(m1, best);
           sum = s_x[BQ + r] * f0 + s_x[3 * BQ + r] * f1;
         }
         const float inv = whole ? (sum == 0.f ? 0.f : 1.f / sum) : 1.f;
@@ -1030,14 +1035,14 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(const TreeAttnParams p,
     float m = best;
 #pragma unroll
     for (int y = 0; y < U; ++y) m = fmaxf(m, ml[y].x);
-    const float old = best == -INFINITY ? 0.f : exp2f(best - m);
+    const float old = part_weight(best, m);
     best = m;
     sum *= old;
 #pragma unroll
     for (int d = 0; d < 8; ++d) acc[d >> 2][d & 3] *= old;
 #pragma unroll
     for (int y = 0; y < U; ++y) {
-      const float f = ml[y].x == -INFINITY ? 0.f : exp2f(ml[y].x - best);
+      const float f = part_weight(ml[y].x, best);
       if (f != 0.f) {
         sum += f * ml[y].y;
 #pragma unroll

@@ -471,6 +471,60 @@ def test_attention_values_that_some_rows_see(name, i8, heads, window):
 
 
 @gpu
+@pytest.mark.parametrize("blocks", [None, 400])
+@pytest.mark.parametrize("heads", [(6, 2, 128), (16, 2, 128), (5, 5, 64)])
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("where", ["node", "position"])
+def test_attention_values_of_no_weight_that_are_no_numbers(where, i8, heads, blocks):
+    """A value that is no number decides the sums of the rows that see it, also where its key's score lies hundreds of powers of two below others: in one
+    CTA (short tables) as in parts that are added up.  (The last request's tiles of little weight are every other one: those of a softmax group.)"""
+    n_q, n_kv, d = heads
+    s = State([300, 130, 100], [20, 9, 7], blocks=blocks)
+    g = torch.Generator(device="cuda").manual_seed(11)
+    sign = torch.randint(0, 2, (n_kv, d), device="cuda", generator=g) * 2.0 - 1
+    cache, clean = (make_cache(s.pages, n_kv, d, i8, 5) for _ in range(2))
+    special, row = torch.zeros(s.rows, n_q, d, dtype=torch.float64, device="cuda"), 0
+    for r, (length, c) in enumerate(zip(s.lengths, s.counts)):
+        at, mask = slots_of(s, r, s.table), ancestors(s.parents[r])[0]
+        low = [j for j in range(length + c) if (j >= length if where == "node" else j < 64 or (j >= length and r == 2))]
+        for j, slot in enumerate(at):      # keys along the queries, or against them
+            way = -sign if j in low else sign
+            noise = torch.randn(n_kv, d, device="cuda", generator=g)
+            for t in (cache, clean):
+                t.k[slot // PAGE, :, slot % PAGE] = (way * 100 + noise * 3).round().to(torch.int8) if i8 else (way * 12 + noise * 0.3).bfloat16()
+                if i8:
+                    t.k_scale[slot // PAGE, :, slot % PAGE] = 0.12
+        j = length + 2 if where == "node" else 10
+        page, place, h = at[j] // PAGE, at[j] % PAGE, r % n_kv
+        if i8:
+            cache.v_scale[page, h, place], clean.v_scale[page, h, place] = INF, 0.0
+            v = cache.v[page, h, place].double() * INF
+        else:
+            dims = torch.tensor([3, 40, d - 1], device="cuda")
+            v = torch.zeros(d, dtype=torch.float64, device="cuda")
+            v[dims] = torch.tensor([INF, -INF, NAN], dtype=torch.float64, device="cuda")
+            cache.v[page, h, place, dims], clean.v[page, h, place, dims] = v[dims].bfloat16(), 0.0
+        for i in range(c):
+            if j < length or mask[i] >> (j - length) & 1:
+                special[row + i, h * (n_q // n_kv): (h + 1) * (n_q // n_kv)] += v
+        row += c
+    s.cuda()
+    s.plan()
+    s.step.check()
+    q = (sign.repeat_interleave(n_q // n_kv, 0) * (1 + torch.rand(s.rows, n_q, d, device="cuda", generator=g) / 2)).bfloat16().flatten(1)
+    out = torch.empty_like(q)
+    T.attention(s.step, q, cache, out, d ** -0.5)
+    torch.cuda.synchronize()
+    K.check_status()
+    want, tol = attention_reference(s, q, clean, d ** -0.5, 0)
+    got, odd = out.double().reshape(want.shape), ~torch.isfinite(special)
+    assert odd.any() and not torch.isfinite(got[odd]).any()
+    if where == "node":      # (where all rows see a position, 0 times what is none is NaN)
+        assert torch.equal(got[odd].nan_to_num(-7.0, 1e30, -1e30), special[odd].nan_to_num(-7.0, 1e30, -1e30))
+    assert ((got - want).abs() <= tol)[~odd].all()
+
+
+@gpu
 @pytest.mark.parametrize("i8", [False, True])
 @pytest.mark.parametrize("name", MIXED)
 def test_attention_scores_that_are_no_numbers(name, i8):
