@@ -82,6 +82,8 @@ class EngineKV:
         for pg in pages:
             e.pool.unpin(pg)
         e.seq_len[slot] = length
+        if getattr(e, "trees", None) is not None:
+            e.trees.forget(slot)        # (its length may be the same)
         self._sync_table(slot)
 
     def grow(self, slot: int, n_pages: int) -> List[int]:

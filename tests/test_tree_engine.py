@@ -181,3 +181,23 @@ def test_trees_of_a_slot_that_changed_are_not_settled():
     eng.trees.forward({1: tree})        # another slot's changes are not this one's
     eng.truncate(0, 2)
     assert 1 in eng.trees.commit()
+
+
+@gpu
+def test_trees_of_a_slot_with_other_pages_are_not_settled():
+    """A slot that the prefix store gave other pages is not the one whose tree has run, though it is as long."""
+    from b200serve.server.prefix import EngineKV
+    eng = engine("", random_weights(C.tiny_dense(), device="cuda", seed=1), max_seqs=3, tree_nodes=8)
+    store, tree = EngineKV(eng), ([3, 4], [-1, 0])
+    eng.prefill(0, list(range(1, 33)))
+    eng.prefill(1, list(range(41, 73)))
+    for slot, pages in ((0, eng.pool.table(1)), (2, [])):
+        eng.trees.forward({slot: tree})
+        store.set_slot(slot, list(pages), eng.seq_len[slot])
+        held = eng.kv.k.clone(), list(eng.seq_len)
+        with pytest.raises(ValueError, match="no trees"):
+            eng.trees.commit()
+        assert torch.equal(eng.kv.k, held[0]) and eng.seq_len == held[1]
+    eng.trees.forward({0: tree})
+    store.set_slot(2, list(eng.pool.table(1)), 32)      # another slot's
+    assert 0 in eng.trees.commit()
