@@ -322,12 +322,23 @@ extern "C" int b2_tree_plan(const B2TreeStep* step, const B2TreePool* pool, cons
   return (int)cudaLaunchKernelEx(&cfg, tree_plan_kernel, p);
 }
 
+// -3: results that overlap what is read (a request's CTAs, one per layer, each read everything, and one of them writes the results)
 extern "C" int b2_tree_commit(const B2TreeStep* step, const B2TreeCache* cache, const B2TreeAccepted* accepted, const int* tokens, const int* targets, int rows,
                               void* stream) {
   const B2TreeStep& t = *step;
   const B2TreeCache& c = *cache;
   const int row_bytes = c.d * (c.k_scale ? 1 : 2);
   if (t.requests < 1 || t.requests > kMaxReq || c.layers < 1 || row_bytes % 16 || ((uintptr_t)c.k | (uintptr_t)c.v | (uintptr_t)c.layer_bytes) % 16) return -1;
+  const auto meet = [](const void* a, long long na, const void* b, long long nb) {
+    return (uintptr_t)a < (uintptr_t)b + 4 * nb && (uintptr_t)b < (uintptr_t)a + 4 * na;
+  };
+  const long long B = t.requests;
+  const struct { const void* at; long long n; } read[] = {{tokens, rows}, {targets, rows}, {t.lengths, B}, {t.row_start, B + 1}, {t.parents, t.max_rows},
+                                                          {t.block_table, B * t.max_blocks}, {t.tree_table, B * t.tree_blocks}};
+  for (const auto& r : read)
+    if (meet(r.at, r.n, accepted->path, B * kMaxNodes) || meet(r.at, r.n, accepted->count, B) || meet(r.at, r.n, accepted->next_token, B) ||
+        meet(r.at, r.n, accepted->lengths, B))
+      return -3;
   TreeCommitParams p;
   p.lengths = t.lengths; p.row_start = t.row_start; p.parents = t.parents; p.tokens = tokens; p.targets = targets; p.block_table = t.block_table;
   p.tree_table = t.tree_table; p.B = t.requests; p.max_blocks = t.max_blocks; p.tree_blocks = t.tree_blocks; p.planes = c.layers; p.num_pages = c.pages;

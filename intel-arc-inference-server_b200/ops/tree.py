@@ -194,7 +194,7 @@ class TreeStep:
         self.tree: Optional[bool] = None       # the last plan's rows are trees'
         self._c = _Step(*(t.data_ptr() for t in (block_table, tree_table, self.lengths, self.row_start, self.row_req, self.row_pos, self.slots, self.parents, self.masks,
                                                  self.status)), b, block_table.shape[1], tree_table.shape[1], max_rows, max_nodes, num_pages)
-        self._at, self._lengths, self._work = ctypes.addressof(self._c), self.lengths.data_ptr(), {}
+        self._at, self._work = ctypes.addressof(self._c), {}
         self._small = (2 * b + 2 + 3) // 4 * 4          # fp32 words of workspace of an attention that leaves no segments
         self._floats, self._index = torch.empty(0, device=dev), dev.index
 
@@ -214,7 +214,7 @@ class Accepted:
         self.path, self.count = _flat(path, torch.int32, (b, MAX_NODES), "accepted path", dev), _flat(count, torch.int32, (b,), "accepted nodes")
         self.next_token, self.lengths = _flat(next_token, torch.int32, (b,), "next tokens", dev), _flat(lengths, torch.int32, (b,), "lengths", dev)
         self._c = _Accepted(path.data_ptr(), count.data_ptr(), next_token.data_ptr(), lengths.data_ptr())
-        self._at, self._requests, self._index, self._lengths = ctypes.addressof(self._c), b, dev.index, lengths.data_ptr()
+        self._at, self._requests, self._index = ctypes.addressof(self._c), b, dev.index
 
     @staticmethod
     def empty(requests: int, device) -> "Accepted":
@@ -330,7 +330,7 @@ def commit(step: TreeStep, tokens: torch.Tensor, targets: torch.Tensor, cache: T
     """Settles a step.  ``tokens``: the rows' tokens; ``targets``: the token that the model gives behind each row (its arg-max, or a draw), int32
     ``[rows]``.  The path begins at a tree's node 0 and goes on with the child whose token is its parent's target, of equal ones the first.
     Its keys and values move from the tree's pages to the request's positions in every layer of ``cache``; nothing else is touched.
-    ``accepted.lengths`` may be the tensor that the next ``plan`` reads."""
+    ``accepted.lengths`` may be the tensor that the next ``plan`` reads; no result may share memory with ``tokens``, ``targets`` or the step."""
     _check_cache(step, cache, True)
     dev, b = step.device, step.requests
     if not step.tree:
@@ -341,10 +341,13 @@ def commit(step: TreeStep, tokens: torch.Tensor, targets: torch.Tensor, cache: T
     at, targets_at = _words(tokens, rows, "tokens", dev), _words(targets, rows, "targets", dev)
     if accepted is None:
         accepted = Accepted.empty(b, dev)
-    elif accepted._requests != b or accepted._index != step._index or accepted._lengths == step._lengths:
-        raise ValueError(f"results of {b} requests on {dev}, apart from the step's own")
+    elif accepted._requests != b or accepted._index != step._index:
+        raise ValueError(f"results of {b} requests on {dev}")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return commit(step, tokens, targets, cache, accepted)
-    K._check(_fn()["commit"](step._at, cache._at, accepted._at, at, targets_at, rows, _stream(dev)), "tree_commit")
+    rc = _fn()["commit"](step._at, cache._at, accepted._at, at, targets_at, rows, _stream(dev))
+    if rc == -3:
+        raise ValueError("results apart from the tokens, the targets and the step's own")
+    K._check(rc, "tree_commit")
     return accepted

@@ -775,6 +775,28 @@ def test_commit(name, chance, layers, n_kv, d, i8):
         assert torch.equal(getattr(cache, n), want[n]), n
 
 
+@gpu
+def test_commit_results_apart_from_what_it_reads():
+    """Results over the tokens, the targets or the step would be written while other layers' walks still read: refused."""
+    s = State([20, 5], [7, 4]).cuda()
+    s.plan()
+    cache = make_cache(s.pages, 1, 64, False, layers=3)
+    i32 = lambda n: torch.zeros(n, dtype=torch.int32, device="cuda")       # noqa: E731
+    tokens, targets, room = i32(11), i32(11), i32(200)
+    for count, following, lengths in ((tokens[9:], i32(2), i32(2)), (i32(2), tokens[:2], i32(2)), (i32(2), targets[3: 5], i32(2)), (i32(2), i32(2), targets[:2]),
+                                      (s.step.lengths, i32(2), i32(2)), (i32(2), i32(2), s.step.lengths), (i32(2), s.step.row_start[1:], i32(2)),
+                                      (i32(2), s.step.parents[8: 10], i32(2)), (s.t_table.view(-1)[1: 3], i32(2), i32(2)), (i32(2), s.t_tree.view(-1)[3: 5], i32(2))):
+        with pytest.raises(ValueError, match="apart from"):
+            T.commit(s.step, tokens, targets, cache, T.Accepted(i32(128).view(2, 64), count, following, lengths))
+    with pytest.raises(ValueError, match="apart from"):
+        T.commit(s.step, room[120: 131], targets, cache, T.Accepted(room[:128].view(2, 64), i32(2), i32(2), i32(2)))
+    want = T.commit(s.step, tokens, targets, cache)
+    got = T.commit(s.step, room[128: 139], targets, cache, T.Accepted(room[:128].view(2, 64), room[139: 141], room[141: 143], s.t_lengths))
+    for name in ("path", "count", "next_token", "lengths"):
+        assert torch.equal(getattr(want, name), getattr(got, name))
+    K.check_status()
+
+
 # ------------------------------------------------------------------ refusals
 def test_refusals_on_the_host():
     """What is not on a CUDA device is refused before the library is asked."""
