@@ -32,6 +32,7 @@ PAGE = 16
 MAX_NODES = 64          # nodes of a tree: an ancestor mask is one 64-bit word
 MAX_REQUESTS = 1024
 MAX_ROWS = 1 << 20
+MAX_BLOCKS = 1 << 27    # of a table, one too many: positions are 32-bit numbers
 
 _FAULTS = {1: "the pool has not enough pages, or no room for those that come back", 2: "a block table is too short, or a request holds more pages than its table has",
            4: "more rows than the step has room for", 8: "a tree of too many nodes", 16: "a parent that does not stand before its child",
@@ -165,8 +166,8 @@ class TreeCache:
 class TreeStep:
     """What ``plan`` leaves of a step, for up to ``max_rows`` rows: ``lengths`` ``[requests]`` and ``row_start`` ``[requests + 1]``; of every row
     its request ``row_req``, position ``row_pos``, cache slot ``slots`` (page x 16 + place), parent ``parents`` and, 64 bits, ancestors ``masks``
-    (bit j: node j of its tree, itself among them; a program may clear or set bits before ``attention``).  Rows behind the last request's
-    are -1 (masks 0).
+    (bit j: node j of its tree, itself among them; a program may clear or set bits before ``attention``; a plan without parents leaves these two as
+    they were).  Rows behind the last request's are -1 (masks 0).
 
     ``block_table`` int32 ``[requests][blocks]``: pages of the requests' positions, filled up by ``plan``.  ``tree_table`` int32
     ``[requests][blocks]``: pages of their trees.  ``num_pages``: pages that tables may name.  ``max_nodes``: of a tree, at most."""
@@ -175,8 +176,8 @@ class TreeStep:
         b, dev = block_table.shape[0], block_table.device
         _flat(block_table, torch.int32, (b, block_table.shape[-1]), "block table")
         _flat(tree_table, torch.int32, (b, tree_table.shape[-1]), "tree table", dev)
-        if not 1 <= b <= MAX_REQUESTS or block_table.shape[1] < 1:
-            raise ValueError(f"a step of 1 to {MAX_REQUESTS} requests, whose tables hold a page at least")
+        if not 1 <= b <= MAX_REQUESTS or not 1 <= block_table.shape[1] < MAX_BLOCKS:
+            raise ValueError(f"a step of 1 to {MAX_REQUESTS} requests, whose tables hold 1 to {MAX_BLOCKS - 1} pages")
         if not 1 <= max_rows <= MAX_ROWS:
             raise ValueError(f"a step of 1 to {MAX_ROWS} rows")
         if not 1 <= max_nodes <= min(MAX_NODES, PAGE * tree_table.shape[1]):

@@ -882,6 +882,14 @@ def test_refusals():
     K.check_status()
 
 
+@gpu
+def test_tables_whose_positions_pass_32_bits_are_refused():
+    table, tree = torch.zeros(1, 1 << 27, dtype=torch.int32, device="cuda"), torch.zeros(1, 4, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="pages"):
+        T.TreeStep(table, tree, 8, 100)
+    T.TreeStep(table[:, : (1 << 27) - 1], tree, 8, 100)
+
+
 # ------------------------------------------------------------------ a run of them together
 class Loop:
     """Requests that decode by trees, everything on the device: plan, one layer's append and attention, commit, lengths and pages carried from step
