@@ -617,6 +617,59 @@ def test_attention_pages_that_are_not_there():
     assert torch.isfinite(out).all() and not torch.equal(out, want)
 
 
+@gpu
+@pytest.mark.parametrize("blocks", [None, 400])
+@pytest.mark.parametrize("heads", [(6, 2, 128), (16, 2, 64)])
+@pytest.mark.parametrize("i8", [False, True])
+def test_attention_pages_that_are_not_there_read_as_page_0(i8, heads, blocks):
+    """Entries of either table that name no page of the cache, in one CTA and in parts: page 0 in their place, and nothing else changes."""
+    n_q, n_kv, d = heads
+    s = State([100, 37, 200], [4, 20, 40], blocks=blocks).cuda()
+    s.plan()
+    s.step.check()
+    cache = make_cache(s.pages, n_kv, d, i8, 9)
+    q = torch.randn(s.rows, n_q * d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(2)).bfloat16()
+    for r, table, at, page in ((0, "table", 4, 1 << 30), (0, "table", 5, -5), (1, "table", 0, s.pages), (2, "table", 12, -(1 << 31)), (1, "tree_table", 1, s.pages + 3), (2, "tree_table", 0, -1)):
+        getattr(s, table)[r][at] = 0
+        (s.t_table if table == "table" else s.t_tree)[r, at] = page
+    out = torch.empty_like(q)
+    T.attention(s.step, q, cache, out, d ** -0.5)
+    torch.cuda.synchronize()
+    K.check_status()
+    want, tol = attention_reference(s, q, cache, d ** -0.5, 0)
+    assert ((out.double().reshape(want.shape) - want).abs() <= tol).all()
+
+
+@gpu
+@pytest.mark.parametrize("blocks", [None, 400])
+@pytest.mark.parametrize("rows", [1, 3, 4, 17, 24, 63])
+@pytest.mark.parametrize("i8", [False, True])
+def test_fewer_rows_than_the_step_has(i8, rows, blocks):
+    """Calls with the first of a step's rows: those rows' results, their keys and values, and nothing behind them."""
+    s = State([100, 37, 200], [4, 20, 40], blocks=blocks).cuda()
+    s.plan()
+    s.step.check()
+    cache = make_cache(s.pages, 2, 128, i8, 9)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    qkv, rope = torch.randn(s.rows, 10 * 128, device="cuda", generator=g), (torch.rand(300, 64, device="cuda", generator=g), torch.rand(300, 64, device="cuda", generator=g))
+    q, part = (torch.full((s.rows, 6 * 128), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    whole = T.TreeCache(*(None if t is None else t.clone() for t in (cache.k, cache.v, cache.k_scale, cache.v_scale)))
+    T.rope_append(s.step, qkv, rope, q, whole)
+    T.rope_append(s.step, qkv[:rows], rope, part[:rows], cache)
+    assert torch.equal(part[:rows], q[:rows]) and (part[rows:] == 7.0).all()
+    at = s.step.slots.long()
+    for name in ("k", "v") + (("k_scale", "v_scale") if i8 else ()):
+        a, b = getattr(cache, name)[at // PAGE, :, at % PAGE], getattr(whole, name)[at // PAGE, :, at % PAGE]
+        assert torch.equal(a[:rows], b[:rows]) and not (a[rows:] == b[rows:]).flatten(1).all(1).any()
+    out = torch.full_like(q, 7.0)
+    T.attention(s.step, q[:rows], whole, out[:rows], 0.1)
+    torch.cuda.synchronize()
+    K.check_status()
+    assert (out[rows:] == 7.0).all()
+    want, tol = attention_reference(s, q, whole, 0.1, 0)
+    assert ((out.double().reshape(want.shape) - want).abs() <= tol)[:rows].all()
+
+
 # ------------------------------------------------------------------ rotation and append
 def rope_reference(x, pos, freq, interleaved):
     """Turned heads [rows][heads][d] in 64 bits."""

@@ -201,3 +201,30 @@ def test_trees_of_a_slot_with_other_pages_are_not_settled():
     eng.trees.forward({0: tree})
     store.set_slot(2, list(eng.pool.table(1)), 32)      # another slot's
     assert 0 in eng.trees.commit()
+
+
+@gpu
+@pytest.mark.parametrize("kv", ["bf16", "int8"])
+def test_trees_beside_decoding_from_graphs(kv):
+    """Steps of trees between decode steps that are replayed: the same tokens as those steps by themselves."""
+    cfg = C.small_dense()
+    w = random_weights(cfg, device="cuda", seed=1)
+    prompts = [list(range(1, 46)), list(range(60, 80))]
+    got = []
+    for graphs in (False, True):
+        eng = Engine(w, max_len=512, use_graphs=graphs, max_seqs=2, tree_nodes=40, kv_dtype=kv)
+        last = [eng.prefill(s, p) for s, p in enumerate(prompts)]
+        tokens = [[], []]
+        for step in range(6):
+            eng.decode_begin([0, 1], last)
+            for _ in range(2):
+                last = eng.decode_step()
+                for s in (0, 1):
+                    tokens[s].append(last[s])
+            rng = random.Random(step)
+            trees = {s: make_tree([last[s], rng.randrange(cfg.vocab), rng.randrange(cfg.vocab)], cfg.vocab, rng, 1 + step) for s in (0, 1)}
+            for s, v in eng.verify_trees(trees).items():
+                tokens[s] += v.tokens[1:] + [v.next_token]
+                last[s] = v.next_token
+        got.append((tokens, list(eng.seq_len)))
+    assert got[0] == got[1]
