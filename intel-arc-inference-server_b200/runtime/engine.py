@@ -303,6 +303,8 @@ class Engine:
         self.require_ok()
         for r in rows:
             self._ensure_pages(r.slot, r.pos + 1)
+            if self.trees is not None:
+                self.trees.forget(r.slot)       # (a row may stand at a position that is there already: the length says nothing)
         self._snapshot(rows)
         self._write_rows(rows)
         self._run(len(rows), advance)

@@ -228,3 +228,19 @@ def test_trees_beside_decoding_from_graphs(kv):
                 last[s] = v.next_token
         got.append((tokens, list(eng.seq_len)))
     assert got[0] == got[1]
+
+
+@gpu
+def test_trees_of_a_slot_whose_position_was_run_again_are_not_settled():
+    """A row at a position that the slot has already replaces what the tree's rows have seen, and the slot stays as long as it was."""
+    eng = engine("", random_weights(C.tiny_dense(), device="cuda", seed=1), max_seqs=2, tree_nodes=8)
+    for s in (0, 1):
+        eng.prefill(s, [1, 2, 3, 4, 5])
+    eng.trees.forward({0: ([3, 4], [-1, 0])})
+    eng.forward_rows([Row(0, 2, 9)])
+    assert eng.seq_len == [5, 5]
+    with pytest.raises(ValueError, match="no trees"):
+        eng.trees.commit()
+    eng.trees.forward({0: ([3, 4], [-1, 0])})
+    eng.forward_rows([Row(1, 2, 9)])
+    assert 0 in eng.trees.commit()
