@@ -33,7 +33,7 @@ class TreeVerifier:
 
     def __init__(self, eng, nodes: int):
         cfg = eng.cfg
-        if cfg.layer_specs or cfg.n_gdn_layers or cfg.head_dim not in (64, 128) or eng.tp is not None or eng.model.nccl is not None:
+        if cfg.layer_specs or cfg.n_gdn_layers or cfg.head_dim not in (64, 128) or not eng.can_score:      # (a pipeline's stage has a part of the layers)
             raise ValueError("token trees: attention layers with heads of 64 or 128 on one GPU")
         self.eng, blocks = eng, -(-nodes // PAGE)
         b = eng.max_seqs
@@ -61,6 +61,8 @@ class TreeVerifier:
         (valid until the next step).  The requests' positions are as they were until ``commit``; other slots may prefill and step in between."""
         from .engine import Row
         eng = self.eng
+        if eng.model.ep is not None:
+            raise ValueError("token trees: experts on one GPU")
         rows, todo, self.rows = [], [], []
         for slot in sorted(trees):
             tokens, parents = list(trees[slot][0]), list(trees[slot][1])

@@ -244,3 +244,20 @@ def test_trees_of_a_slot_whose_position_was_run_again_are_not_settled():
     eng.trees.forward({0: ([3, 4], [-1, 0])})
     eng.forward_rows([Row(1, 2, 9)])
     assert 0 in eng.trees.commit()
+
+
+@gpu
+def test_models_over_several_gpus_are_refused():
+    """A pipeline's stage has some of the layers, experts of other ranks are others' steps: no step over trees."""
+    from b200serve.parallel.pp import PipelineEngine
+    w = random_weights(C.small_moe(), device="cuda", seed=1)
+    with pytest.raises(ValueError, match="one GPU"):
+        PipelineEngine(w, 0, 2, max_len=128, tree_nodes=8)
+    PipelineEngine(w, 0, 2, max_len=128)
+    eng = engine("", w, max_seqs=1, tree_nodes=8)
+    eng.prefill(0, [1, 2, 3])
+    eng.model.ep = object()
+    with pytest.raises(ValueError, match="one GPU"):
+        eng.verify_trees({0: ([3, 4], [-1, 0])})
+    eng.model.ep = None
+    assert eng.seq_len == [3] and 0 in eng.verify_trees({0: ([3, 4], [-1, 0])})
