@@ -26,11 +26,13 @@
 // exact; K's scale goes on the scores and V's on the weights, both in fp32.  Of four dimensions the second and the third change places on the way (pairs come apart that
 // way), which the queries follow and the results undo.
 //
-// What bounds it.  bf16 with one query tile: the cache's bytes (32 requests of 2000 to 33000 positions, 40 heads on 8 of 128: 2.3 GB in 391 us, 5.9 TB/s of
-// the 6.5 that a copy reaches).  Two query tiles: the softmax, a chain of about 2000 cycles a tile whose four warps to a scheduler hide half of it, and the
-// scores' product, which reads Q from shared memory (16 requests of up to 9000 positions, 40 to 64 nodes, 16 heads on 4: 173 MB in 66 us).  8 bits: instructions, about 5000 a tile and SM, of
-// which the expansion is a third (12 requests of up to 65000 positions, 24 nodes, 40 heads on 8: 1.09 GB in 405 us).  One request: a segment's start and end, about four tiles' time, and
-// the second launch (4100 positions: 18 us).  Full tables of many short requests: the same, a request at a time.
+// What bounds it (times of twenty calls in a graph; in long streams of calls the power cap adds a tenth and more to the large ones).  bf16 with one query
+// tile: the cache's bytes (32 requests of 2000 to 33000 positions, 40 heads on 8 of 128: 2.3 GB in 383 us, 6.0 TB/s of the 6.5 that a copy reaches; 424 in a
+// stream).  Two query tiles: the softmax, a chain of about 2000 cycles a tile whose four warps to a scheduler hide half of it, and the scores' product, which
+// reads Q from shared memory (16 requests of up to 9000 positions, 40 to 64 nodes, 16 heads on 4: 173 MB in 66 us).  8 bits: instructions, 4600 a tile in 71 % of
+// the issue slots, of which the expansion is about 800 and the arithmetic of the scores about 1200 by the code; the rest, 140 bytes of spills
+// in it, has not been taken apart (12 requests of up to 65000 positions, 24 nodes, 40 heads on 8: 1.09 GB in 404 us; 471 in a stream).  One request: a segment's
+// start and end, about four tiles' time, and the second launch (4100 positions: 18 us).  Full tables of many short requests: the same, a request at a time.
 #include "tree.cuh"
 
 using namespace b2;
@@ -47,7 +49,7 @@ struct TreeAttnParams {
   long long ldq;
   const int8_t *k8, *v8;           // 8-bit form
   const float *k_scale, *v_scale;
-  const int *lengths, *row_start, *row_req, *row_pos, *block_table, *tree_table;
+  const int *lengths, *row_start, *row_pos, *block_table, *tree_table;
   const unsigned long long* masks;
   int B, max_blocks, tree_blocks, num_pages, rows, n_q, n_kv, gqa, window;
   int group_tokens;                // nodes to a CTA's query tiles
@@ -423,7 +425,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   int total = s_cum[p.B] * p.n_kv, each = p.single ? p.single : (total + gridDim.x - 1) / gridDim.x;
   // Where there are columns enough for every request's key head, a request's tiles can begin a column: then a CTA has one segment, whose start and
   // end cost as much as four or five tiles.  Eight column lengths from the least on are looked at; the first that fits is taken.
-  // (One request of 4100 positions, 8 key heads, 66 tiles: 17 columns of 4 instead of 16.5; 21.2 -> 16.7 us with the merge.)
+  // (One request of 4100 positions, 8 key heads, 66 tiles: 17 columns of 4 instead of 16.5; 21.2 -> 16.7 us with the merge, before values were looked at, 18.0 now.)
   // single: tables so short that a request's key head is one column in any case, and nothing is left to merge.
   if (p.single || p.B * p.n_kv <= (int)gridDim.x) {
     if (warp == 0) {
@@ -1103,7 +1105,9 @@ int sm_count() {
 // Places on the line of tiles are 32-bit numbers.
 bool too_long(const B2TreeStep& t, int n_kv) { return (long long)t.requests * n_kv * (t.max_blocks / 4 + 2) >= 1ll << 30; }
 
-// Query tiles of a CTA, nodes to a CTA, CTAs over the same keys, columns of CTAs.
+// Query tiles of a CTA, nodes to a CTA, CTAs over the same keys, columns of CTAs.  The host knows what a step can hold, not what it holds, and a step
+// made for more pays for it: 32 requests of 16 nodes, 40 heads on 8, in a step for trees of 16 / of 64 nodes 382 / 880 us (groups without rows, the second
+// query tile empty), one request 18.0 / 20.2; one of 300 positions in a table of that / of 8192 positions 11.2 / 12.3.
 struct Shape {
   int nw, tokens, groups, columns, single;
 };
@@ -1118,6 +1122,7 @@ Shape shape_of(int B, int max_blocks, int n_kv, int gqa, int max_nodes) {
   // Short tables of few requests: a request's key head is one CTA's, and the second launch is spared.  Full tables, 32 heads on 8, one CTA / parts
   // that are added up, us: 1 request 9.7 / 10.4 at 6 tiles, 11.8 / 11.4 at 10; 16 requests 11.1 / 13.6 and 14.9 / 16.9; 32 requests (256 CTAs)
   // 22.6 / 28.0 and 29.4 / 33.9, at 18 39.9 / 43.2 and 1 request 15.7 / 15.4; 48 requests 28.9 / 25.5 at 3 tiles, 128 requests 82 / 62 at 6.
+  // (A bound, not the best of both everywhere: 8 to 32 requests at 18 tiles lose 5 to 10 % by it, 1 request at 10 and 32 at 3 tiles 2 to 3 %.)
   const int most_tiles = max_blocks / 4 + 2;
   s.single = most_tiles <= 10 && (long long)B * n_kv * s.groups <= 2 * sm_count() ? most_tiles : 0;
   if (s.single) {
@@ -1174,7 +1179,7 @@ extern "C" int b2_tree_attention(const B2TreeStep* step, const B2TreeCache* cach
   const Shape s = shape_of(t.requests, t.max_blocks, c.heads, n_q / c.heads, t.max_nodes);
   TreeAttnParams p;
   p.q = (const __nv_bfloat16*)q; p.ldq = ldq; p.k8 = (const int8_t*)c.k; p.v8 = (const int8_t*)c.v; p.k_scale = c.k_scale; p.v_scale = c.v_scale;
-  p.lengths = t.lengths; p.row_start = t.row_start; p.row_req = t.row_req; p.row_pos = t.row_pos; p.block_table = t.block_table; p.tree_table = t.tree_table;
+  p.lengths = t.lengths; p.row_start = t.row_start; p.row_pos = t.row_pos; p.block_table = t.block_table; p.tree_table = t.tree_table;
   p.masks = t.masks; p.B = t.requests; p.max_blocks = t.max_blocks; p.tree_blocks = t.tree_blocks; p.num_pages = c.pages; p.rows = rows;
   p.n_q = n_q; p.n_kv = c.heads; p.gqa = n_q / c.heads; p.window = window; p.group_tokens = s.tokens; p.scale_log2 = scale * 1.4426950408889634f;
   p.out = (__nv_bfloat16*)out; p.ldo = ldo;

@@ -11,7 +11,8 @@
 // other thread, and cosines and sines are read once for the row's heads.  All of a thread's loads are in flight together, and stay as they came
 // until their turn.  5000 rows of 32 + 8 + 8 heads, bf16: 24.3 us (5.2 TB/s) with four heads a thread and five CTAs an SM; 26.0 with as many
 // registers as it likes, 28.1 / 29.0 with two / eight heads; unpacked as they come 33 to 36, which leaves half the bytes under way.
-// 16 rows, four slices: 2.2 us with a head a thread.
+// 16 rows, four slices: 2.1 us with a head a thread.  1008 rows of 16 + 4 + 4 heads into 8 bits: 7.4 us (18 MB, 2.8 us of bytes; what the rest is was not
+// measured: heads of queries come by the scales' shuffles too, and 8-bit values leave four at a time).
 #include "tree.cuh"
 
 using namespace b2;

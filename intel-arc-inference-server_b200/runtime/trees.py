@@ -1,8 +1,8 @@
 """Token trees on the engine: several drafted continuations of each request, verified in one step (``ops/tree.py``).
 
 A request's tree is its next token (node 0, which is not in the cache yet) and drafts behind it, each with the node it follows.  One step runs
-all nodes of all trees; the longest path whose tokens are what the model gives behind their parents is kept -- greedily, the tokens that
-plain decoding would have made, one by one -- and the rest leaves no trace.  The engine keeps pages for the trees of every slot
+all nodes of all trees; the path is kept that goes on, from node 0, with the child whose token is what the model gives behind its parent (of
+equal children the first, whichever path is the longer) -- greedily, the tokens that plain decoding would have made, one by one -- and the rest leaves no trace.  The engine keeps pages for the trees of every slot
 (``Engine(tree_nodes=...)``).
 """
 from __future__ import annotations
