@@ -323,7 +323,7 @@ extern "C" int b2_tree_plan(const B2TreeStep* step, const B2TreePool* pool, cons
   return (int)cudaLaunchKernelEx(&cfg, tree_plan_kernel, p);
 }
 
-// -3: results that overlap what is read (a request's CTAs, one per layer, each read everything, and one of them writes the results)
+// -3: results that overlap what is read (a request's CTAs, one per layer, each read everything, and one of them writes the results), or the step's other numbers
 extern "C" int b2_tree_commit(const B2TreeStep* step, const B2TreeCache* cache, const B2TreeAccepted* accepted, const int* tokens, const int* targets, int rows,
                               void* stream) {
   const B2TreeStep& t = *step;
@@ -335,7 +335,8 @@ extern "C" int b2_tree_commit(const B2TreeStep* step, const B2TreeCache* cache, 
   };
   const long long B = t.requests;
   const struct { const void* at; long long n; } read[] = {{tokens, rows}, {targets, rows}, {t.lengths, B}, {t.row_start, B + 1}, {t.parents, t.max_rows},
-                                                          {t.block_table, B * t.max_blocks}, {t.tree_table, B * t.tree_blocks}};
+                                                          {t.block_table, B * t.max_blocks}, {t.tree_table, B * t.tree_blocks}, {t.row_req, t.max_rows},
+                                                          {t.row_pos, t.max_rows}, {t.slots, t.max_rows}, {t.masks, 2ll * t.max_rows}, {t.status, 1}};
   for (const auto& r : read)
     if (meet(r.at, r.n, accepted->path, B * kMaxNodes) || meet(r.at, r.n, accepted->count, B) || meet(r.at, r.n, accepted->next_token, B) ||
         meet(r.at, r.n, accepted->lengths, B))

@@ -838,7 +838,8 @@ def test_commit_results_apart_from_what_it_reads():
     tokens, targets, room = i32(11), i32(11), i32(200)
     for count, following, lengths in ((tokens[9:], i32(2), i32(2)), (i32(2), tokens[:2], i32(2)), (i32(2), targets[3: 5], i32(2)), (i32(2), i32(2), targets[:2]),
                                       (s.step.lengths, i32(2), i32(2)), (i32(2), i32(2), s.step.lengths), (i32(2), s.step.row_start[1:], i32(2)),
-                                      (i32(2), s.step.parents[8: 10], i32(2)), (s.t_table.view(-1)[1: 3], i32(2), i32(2)), (i32(2), s.t_tree.view(-1)[3: 5], i32(2))):
+                                      (i32(2), s.step.parents[8: 10], i32(2)), (s.step.slots[:2], i32(2), i32(2)), (s.step.row_pos[9:], i32(2), i32(2)),
+                                      (i32(2), s.step.row_req[4: 6], i32(2)), (i32(2), i32(2), s.step.masks.view(torch.int32)[20:]), (s.t_table.view(-1)[1: 3], i32(2), i32(2)), (i32(2), s.t_tree.view(-1)[3: 5], i32(2))):
         with pytest.raises(ValueError, match="apart from"):
             T.commit(s.step, tokens, targets, cache, T.Accepted(i32(128).view(2, 64), count, following, lengths))
     with pytest.raises(ValueError, match="apart from"):
