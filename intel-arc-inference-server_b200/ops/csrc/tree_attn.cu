@@ -828,6 +828,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
               asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(ee) : "l"(f));
               asm("mov.b64 {%0, %1}, %2;" : "=f"(e0), "=f"(e1) : "l"(ee));
             }
+            // (to bf16, since the product's operands are of one type, V's; the sum is of the weights as they were.  Results are 0.19 to 0.25 % from
+            // those in 64 bits, 0.17 of it their own rounding)
             pk[2 * c + y] = pack_bf16(e0, e1);
           }
         }
